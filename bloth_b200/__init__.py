@@ -26,6 +26,7 @@ from .kernels import (  # noqa: F401
     apply_rope_qk,
     apply_rotary_pos_emb,
     fused_add_rms_norm,
+    fused_attention,
     fused_norm_rope,
     fused_qk_norm_rope,
 )
@@ -54,6 +55,7 @@ __all__ = [
     "fused_add_rms_norm",
     "fused_norm_rope",
     "fused_qk_norm_rope",
+    "fused_attention",
     "BlothQKNormRoPE",
     "rope_embedding",
     "apply_rope",

@@ -1,0 +1,177 @@
+// Attention over [B, S, H, D] head tensors, forward and backward: the
+// arguments, the sequences they describe and the tiles of a sequence that see
+// one another, shared by every attention kernel.
+//
+// Mathematics, per query row i and the keys j it sees (see_keys below):
+//   s_ij = scale * q_i . k_j,  lse_i = log sum_j exp(s_ij),
+//   p_ij = exp(s_ij - lse_i),  o_i = sum_j p_ij v_j;
+// backward, which recomputes p from lse instead of reading it:
+//   delta_i = do_i . o_i,  dp_ij = do_i . v_j,  ds_ij = p_ij (dp_ij - delta_i),
+//   dv_j = sum_i p_ij do_i,  dq_i = scale sum_j ds_ij k_j,
+//   dk_j = scale sum_i ds_ij q_i.
+// A row that sees no key has o = 0, lse = -inf and no gradient. Query heads
+// h of a group of G = Hq / Hk share key head h / G, whose gradients sum over
+// the group inside one CTA, in a fixed order: no atomics anywhere.
+#pragma once
+
+#include "common.cuh"
+#include "heads_impl.cuh"
+
+namespace bloth {
+
+struct AttnArgs {
+  HT q, k, v, o, dout, dq, dk, dv;
+  float* lse;         // [B, Hq, Sq] natural logarithm (forward writes, backward reads)
+  float* lse2;        // backward workspace: [Hq, R] lse * log2(e), +inf where nothing is seen
+  float* delta;       // backward workspace: [Hq, R]
+  int64_t R;          // rows per head of lse2 and delta (attn_stat_rows)
+  const void* qseq;   // dense: [B] query lengths or NULL; packed: [n + 1] offsets
+  const void* kseq;   // the same for keys
+  int seq_dt;
+  int packed;         // 0: dense, else the number of packed sequences n
+  int B, Sq, Sk, Hq, Hk, G;
+  float scale, scale_log2;
+  int causal;
+  int window;         // 0: none
+  unsigned int* fault;
+};
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// One sequence: its rows in the tensors and its lengths.
+struct AttnSeq {
+  int b;           // batch row of the tensors
+  int q0, qlen;    // first query row and their number
+  int k0, klen;
+  int64_t stat0;   // first row of its lse2 and delta rows
+  int tile;        // tile of the sequence this CTA works on; < 0: none
+};
+
+__device__ __forceinline__ int seq_at(const void* p, int dt, int i, int limit) {
+  const int64_t v = dt == BLOTH_I64 ? __ldg(reinterpret_cast<const long long*>(p) + i)
+                                    : (int64_t)__ldg(reinterpret_cast<const int*>(p) + i);
+  return (int)(v < 0 ? 0 : (v > limit ? limit : v));
+}
+
+// Rows of lse2 and delta a packed sequence starts at: 16-byte units, and room
+// for its last tile of 128 rows in full.
+__host__ __device__ __forceinline__ int64_t attn_stat_base(int64_t cu, int64_t s) {
+  return (cu + 3) / 4 * 4 + 132 * s;
+}
+inline int64_t attn_stat_rows(int64_t B, int64_t Sq, int64_t packed) {
+  return packed ? attn_stat_base(Sq, packed + 2) + 128 : B * ((Sq + 127) / 128 * 128);
+}
+// Tiles of `tile` rows that cover every sequence, at most (the offsets of
+// packed sequences are known on the device only). The rows before the first
+// sequence and those past the last are two more, which see nothing.
+inline int64_t attn_tiles(int64_t S, int64_t packed, int tile) {
+  return (S + tile - 1) / tile + (packed ? packed + 2 : 0);
+}
+
+// The sequence and tile of flat tile index `t` (BY_Q: tiles of query rows,
+// else of key rows). Called by whole warps; every warp finds the same.
+// Packed offsets are clamped to the tensors and to be non-decreasing, so no
+// content of the offsets leads outside of them.
+template <bool BY_Q>
+__device__ __forceinline__ AttnSeq find_seq(const AttnArgs& a, int b, int t, int tile) {
+  AttnSeq s;
+  if (!a.packed) {
+    s.b = b;
+    s.q0 = s.k0 = 0;
+    s.qlen = a.qseq ? seq_at(a.qseq, a.seq_dt, b, a.Sq) : a.Sq;
+    s.klen = a.kseq ? seq_at(a.kseq, a.seq_dt, b, a.Sk) : a.Sk;
+    s.stat0 = (int64_t)b * ((a.Sq + 127) / 128 * 128);
+    s.tile = t;
+    return s;
+  }
+  s.b = 0;
+  s.tile = -1;
+  const int lane = threadIdx.x & 31;
+  const int n = a.packed;
+  int before = 0;
+  int last_q = 0, last_k = 0;  // ends of the pieces before this step of 32
+  for (int base = 0; base <= n + 1; base += 32) {
+    // piece i = base + lane ends at offset i: the rows before the first
+    // sequence, the n sequences, the rows past the last one
+    const int i = base + lane;
+    int q1 = i <= n ? seq_at(a.qseq, a.seq_dt, i, a.Sq) : a.Sq;
+    int k1 = i <= n ? seq_at(a.kseq, a.seq_dt, i, a.Sk) : a.Sk;
+    q1 = max(q1, last_q);
+    k1 = max(k1, last_k);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {  // running maxima: non-decreasing ends
+      const int uq = __shfl_up_sync(0xffffffffu, q1, o), uk = __shfl_up_sync(0xffffffffu, k1, o);
+      if (lane >= o) {
+        q1 = max(q1, uq);
+        k1 = max(k1, uk);
+      }
+    }
+    int q0 = __shfl_up_sync(0xffffffffu, q1, 1), k0 = __shfl_up_sync(0xffffffffu, k1, 1);
+    if (lane == 0) {
+      q0 = last_q;
+      k0 = last_k;
+    }
+    const int rows = BY_Q ? q1 - q0 : k1 - k0;
+    int tiles = i <= n + 1 ? (rows + tile - 1) / tile : 0;
+    int upto = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += u;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, t < before + upto);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      s.q0 = __shfl_sync(0xffffffffu, q0, src);
+      s.qlen = __shfl_sync(0xffffffffu, q1, src) - s.q0;
+      s.k0 = __shfl_sync(0xffffffffu, k0, src);
+      s.klen = __shfl_sync(0xffffffffu, k1, src) - s.k0;
+      s.tile = t - before - __shfl_sync(0xffffffffu, upto - tiles, src);
+      s.stat0 = attn_stat_base(s.q0, base + src);
+      // rows outside of the sequences: nothing is seen from or by them
+      if (base + src == 0 || base + src == n + 1) (BY_Q ? s.klen : s.qlen) = 0;
+      return s;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+    last_q = __shfl_sync(0xffffffffu, q1, 31);
+    last_k = __shfl_sync(0xffffffffu, k1, 31);
+  }
+  return s;
+}
+
+// Query i of a sequence sees key j when j < klen and, causal, j <= i + klen -
+// qlen (the last query sees the last key), and, with a window, j > i + klen -
+// qlen - window.
+__device__ __forceinline__ bool see_keys(const AttnArgs& a, const AttnSeq& s, int i, int j) {
+  const int at = i + s.klen - s.qlen;
+  return i < s.qlen && j < s.klen && (!a.causal || j <= at) && (!a.window || j > at - a.window);
+}
+
+// Keys [lo, hi) seen by any of the query rows [m0, m1) (m1 <= qlen).
+__device__ __forceinline__ void key_range(const AttnArgs& a, const AttnSeq& s, int m0, int m1,
+                                          int& lo, int& hi) {
+  const int off = s.klen - s.qlen;
+  hi = a.causal ? min(s.klen, m1 + off) : s.klen;
+  lo = a.window ? max(0, m0 + off - a.window + 1) : 0;
+  if (m1 <= m0 || hi <= lo) lo = hi = 0;
+}
+
+// Queries [lo, hi) that see any of the key rows [n0, n1) (n1 <= klen).
+__device__ __forceinline__ void query_range(const AttnArgs& a, const AttnSeq& s, int n0, int n1,
+                                            int& lo, int& hi) {
+  const int off = s.klen - s.qlen;
+  lo = a.causal ? max(0, n0 - off) : 0;
+  hi = a.window ? min(s.qlen, n1 - off + a.window - 1) : s.qlen;
+  if (n1 <= n0 || hi <= lo) lo = hi = 0;
+}
+
+// Host launchers (attn_simt_<type>.cu, attn_stat.cu).
+template <typename T>
+int attn_simt_fwd(const AttnArgs& a, int D, cudaStream_t st);
+template <typename T>
+int attn_simt_bwd(const AttnArgs& a, int D, cudaStream_t st);
+template <typename T>
+int attn_stats(const AttnArgs& a, int D, cudaStream_t st);
+
+}  // namespace bloth

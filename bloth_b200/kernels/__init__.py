@@ -8,6 +8,7 @@ the RoPE-only ops.
 from .rms_norm import bloth_rms_norm, rms_norm  # noqa: F401
 from .add_rms_norm import fused_add_rms_norm  # noqa: F401
 from .fused_norm_qkv_rope import fused_norm_rope, fused_qk_norm_rope  # noqa: F401
+from .attention import fused_attention  # noqa: F401
 from .rope import apply_rope, apply_rope_qk, apply_rotary_pos_emb, rope_embedding  # noqa: F401
 
 __all__ = [
@@ -16,6 +17,7 @@ __all__ = [
     "fused_add_rms_norm",
     "fused_norm_rope",
     "fused_qk_norm_rope",
+    "fused_attention",
     "apply_rope",
     "apply_rope_qk",
     "apply_rotary_pos_emb",

@@ -1,0 +1,205 @@
+"""Attention over head tensors, with autograd, on the sm_100a kernels.
+
+``fused_attention(q, k, v, ...)`` takes the [B, S, H, D] tensors that
+``fused_qk_norm_rope``, ``fused_qk_norm_mrope`` and ``apply_rope_qk`` return:
+whole sequences, a chunk of new tokens over a longer cache, single tokens,
+padded batches (``q_lens``, ``k_lens``) and packed documents
+(``cu_seqlens``). Its backward recomputes the probabilities from the saved row
+statistics. The reference has no attention of its own.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from .. import _lib
+from .fused_norm_qkv_rope import _head_strides, _heads
+
+
+def _addressable(t):
+    """_heads, with tensors that repeat a row of memory written out (a tensor
+    map cannot describe a stride of 0)."""
+    if t is not None and any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+        t = t.contiguous()
+    return _heads(t)
+
+
+def _sequence_arg(x, n: int, device, name: str):
+    """Lengths [n] or offsets [n] as a contiguous int32 or int64 tensor."""
+    if x is None:
+        return None
+    if x.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"[Bloth] {name} must be int32 or int64, got {x.dtype}")
+    if x.dim() != 1 or (n is not None and x.numel() != n):
+        raise ValueError(f"[Bloth] {name} must have shape [{'n + 1' if n is None else n}], got "
+                         f"{tuple(x.shape)}")
+    if x.device != device:
+        raise ValueError(f"[Bloth] {name} must be on {device}, got {x.device}")
+    return x.contiguous()
+
+
+def _sequences(q4, k4, q_lens, k_lens, cu_q, cu_k):
+    """(q_seq, k_seq, packed) of the C ABI."""
+    if cu_q is not None or cu_k is not None:
+        if q_lens is not None or k_lens is not None:
+            raise ValueError("[Bloth] give lengths (q_lens, k_lens) or offsets (cu_seqlens), "
+                             "not both")
+        if cu_q is None:
+            raise ValueError("[Bloth] cu_seqlens_k needs cu_seqlens")
+        if q4.shape[0] != 1:
+            raise ValueError("[Bloth] packed sequences take [T, H, D] or [1, T, H, D] tensors")
+        cu_q = _sequence_arg(cu_q, None, q4.device, "cu_seqlens")
+        if cu_q.numel() < 2:
+            raise ValueError("[Bloth] cu_seqlens needs at least two offsets")
+        if cu_k is None:
+            if k4.shape[1] != q4.shape[1]:
+                raise ValueError("[Bloth] q and k differ in length: give cu_seqlens_k too")
+            cu_k = cu_q
+        else:
+            cu_k = _sequence_arg(cu_k, cu_q.numel(), q4.device, "cu_seqlens_k")
+        if cu_k.dtype != cu_q.dtype:
+            cu_k = cu_k.to(cu_q.dtype)
+        return cu_q, cu_k, cu_q.numel() - 1
+    q_lens = _sequence_arg(q_lens, q4.shape[0], q4.device, "q_lens")
+    k_lens = _sequence_arg(k_lens, q4.shape[0], q4.device, "k_lens")
+    if q_lens is not None and k_lens is not None and q_lens.dtype != k_lens.dtype:
+        q_lens, k_lens = q_lens.long(), k_lens.long()
+    return q_lens, k_lens, 0
+
+
+def _seq_dtype(q_seq, k_seq) -> int:
+    t = q_seq if q_seq is not None else k_seq
+    return _lib.I32 if t is None else _lib.dtype_code(t.dtype)
+
+
+def _workspace(entry: str, device, *args):
+    n = _lib.workspace_bytes(entry, device, *args)
+    return (torch.empty(n, dtype=torch.uint8, device=device) if n else None), n
+
+
+def attention_forward(q4, k4, v4, q_seq, k_seq, packed, scale, causal, window, want_lse=True):
+    """(out, lse) of addressable head tensors; lse is None unless wanted."""
+    B, Sq, Hq, D = q4.shape
+    Sk, Hk = k4.shape[1], k4.shape[2]
+    out = torch.empty((B, Sq, Hq, D), dtype=q4.dtype, device=q4.device)
+    lse = torch.empty((B, Hq, Sq), dtype=torch.float32, device=q4.device) if want_lse else None
+    code = _lib.dtype_code(q4.dtype)
+    ws, n = _workspace("bloth_attention_fwd_workspace_bytes", q4.device, B, Sq, Sk, Hq, Hk, D,
+                       packed, code)
+    rc = _lib.call("bloth_attention_fwd", q4, _lib.ptr(q4), _head_strides(q4), _lib.ptr(k4),
+                   _head_strides(k4), _lib.ptr(v4), _head_strides(v4), _lib.ptr(out),
+                   _head_strides(out), _lib.ptr(lse), _lib.ptr(q_seq), _lib.ptr(k_seq),
+                   _seq_dtype(q_seq, k_seq), packed, B, Sq, Sk, Hq, Hk, D, scale, int(causal),
+                   window, code, _lib.ptr(ws), n, _lib.stream_of(q4))
+    _lib.check(rc, "attention forward")
+    return out, lse
+
+
+def attention_backward(do4, q4, k4, v4, out, lse, q_seq, k_seq, packed, scale, causal, window,
+                       want_q=True, want_kv=True):
+    """(dq, dk, dv); None for those not wanted."""
+    B, Sq, Hq, D = q4.shape
+    Sk, Hk = k4.shape[1], k4.shape[2]
+    dq = torch.empty((B, Sq, Hq, D), dtype=q4.dtype, device=q4.device) if want_q else None
+    dk = torch.empty((B, Sk, Hk, D), dtype=q4.dtype, device=q4.device) if want_kv else None
+    dv = torch.empty((B, Sk, Hk, D), dtype=q4.dtype, device=q4.device) if want_kv else None
+    code = _lib.dtype_code(q4.dtype)
+    ws, n = _workspace("bloth_attention_bwd_workspace_bytes", q4.device, B, Sq, Sk, Hq, Hk, D,
+                       packed, code)
+    rc = _lib.call("bloth_attention_bwd", q4, _lib.ptr(do4), _head_strides(do4), _lib.ptr(q4),
+                   _head_strides(q4), _lib.ptr(k4), _head_strides(k4), _lib.ptr(v4),
+                   _head_strides(v4), _lib.ptr(out), _head_strides(out), _lib.ptr(lse),
+                   _lib.ptr(dq), _head_strides(dq), _lib.ptr(dk), _head_strides(dk),
+                   _lib.ptr(dv), _head_strides(dv), _lib.ptr(q_seq), _lib.ptr(k_seq),
+                   _seq_dtype(q_seq, k_seq), packed, B, Sq, Sk, Hq, Hk, D, scale, int(causal),
+                   window, code, _lib.ptr(ws), n, _lib.stream_of(q4))
+    _lib.check(rc, "attention backward")
+    return dq, dk, dv
+
+
+class _AttentionFunction(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, q, k, v, q_seq, k_seq, packed, scale, causal, window, want_lse):
+        q4, k4, v4 = (_addressable(t) for t in (q, k, v))
+        need = any(ctx.needs_input_grad[:3])
+        out, lse = attention_forward(q4, k4, v4, q_seq, k_seq, packed, scale, causal, window,
+                                     need or want_lse)
+        if need:
+            ctx.save_for_backward(q4, k4, v4, out, lse, q_seq, k_seq)
+            ctx.meta = (packed, scale, causal, window, q.shape, k.shape, v.shape)
+        y = out.view(q.shape)
+        if not want_lse:
+            return y
+        rows = lse[0] if q.dim() == 3 else lse
+        ctx.mark_non_differentiable(rows)
+        return y, rows
+
+    @staticmethod
+    def backward(ctx, dout, *_):
+        q4, k4, v4, out, lse, q_seq, k_seq = ctx.saved_tensors
+        packed, scale, causal, window, shape_q, shape_k, shape_v = ctx.meta
+        want_q, want_k, want_v = ctx.needs_input_grad[:3]
+        dq, dk, dv = attention_backward(_addressable(dout.view(q4.shape)), q4, k4, v4, out, lse,
+                                        q_seq, k_seq, packed, scale, causal, window, want_q,
+                                        want_k or want_v)
+        return (dq.view(shape_q) if want_q else None, dk.view(shape_k) if want_k else None,
+                dv.view(shape_v) if want_v else None, None, None, None, None, None, None, None)
+
+
+def fused_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = True,
+                    window: int | None = None, scale: float | None = None,
+                    q_lens: torch.Tensor | None = None, k_lens: torch.Tensor | None = None,
+                    cu_seqlens: torch.Tensor | None = None,
+                    cu_seqlens_k: torch.Tensor | None = None, return_lse: bool = False):
+    """softmax(scale * q k^T) v of q [B, Sq, Hq, D] and k, v [B, Sk, Hk, D].
+
+    Hq is a multiple of Hk (query head h reads key head h // (Hq // Hk)); D is
+    64, 128 or 256; bf16, fp16 or fp32, all three alike. ``scale`` defaults to
+    1/sqrt(D). ``causal``: query i sees keys up to i + klen - qlen, so the last
+    query sees the last key. ``window`` (causal only) leaves it the last
+    ``window`` of those.
+
+    ``q_lens`` and ``k_lens`` [B] (int32 or int64, on the device): the rows in
+    use at the start of each batch row. ``cu_seqlens`` [n + 1]: the offsets of
+    n sequences packed in [T, H, D] (or [1, T, H, D]) tensors;
+    ``cu_seqlens_k`` where the keys have their own. Lengths and offsets are
+    read on the device and clamped to the tensors. Rows outside of every
+    sequence and rows that see no key get zeros, and no gradient; their inputs
+    are never used, whatever they hold. A key that some rows of its sequence
+    see has to be finite for all of them (a probability of 0 times an infinity
+    is not a number).
+
+    Returns out, shaped as q; with ``return_lse`` also the fp32 logarithms of
+    the rows' sums of exponentials [B, Hq, Sq] ([Hq, S] for 3-D tensors), -inf
+    for rows that see nothing, without a gradient.
+    """
+    _lib.require_cuda(q, k, v, q_lens, k_lens, cu_seqlens, cu_seqlens_k)
+    if not (q.dim() == k.dim() == v.dim()) or q.dim() not in (3, 4):
+        raise ValueError("[Bloth] q, k and v must be [B, S, H, D] or [S, H, D]")
+    if not (q.dtype == k.dtype == v.dtype):
+        raise TypeError(f"[Bloth] q, k and v differ in dtype: {q.dtype}, {k.dtype}, {v.dtype}")
+    if q.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise TypeError(f"[Bloth] unsupported dtype {q.dtype}")
+    if not (q.device == k.device == v.device):
+        raise ValueError("[Bloth] q, k and v must be on one device")
+    if k.shape != v.shape or q.shape[-1] != k.shape[-1] or \
+            (q.dim() == 4 and q.shape[0] != k.shape[0]):
+        raise ValueError(f"[Bloth] shapes do not match: q {tuple(q.shape)}, k {tuple(k.shape)}, "
+                         f"v {tuple(v.shape)}")
+    if q.shape[-1] not in (64, 128, 256):
+        raise ValueError(f"[Bloth] head_dim {q.shape[-1]} is not one of 64, 128, 256")
+    if k.shape[-2] == 0 or q.shape[-2] % k.shape[-2] or q.shape[-2] == 0:
+        raise ValueError(f"[Bloth] {q.shape[-2]} query heads over {k.shape[-2]} key heads")
+    if scale is None:
+        scale = 1.0 / math.sqrt(q.shape[-1])
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"[Bloth] scale must be positive and finite, got {scale}")
+    if window is not None and (not causal or window < 1):
+        raise ValueError("[Bloth] window must be at least 1, and needs causal=True")
+    q4 = q if q.dim() == 4 else q.unsqueeze(0)
+    k4 = k if k.dim() == 4 else k.unsqueeze(0)
+    q_seq, k_seq, packed = _sequences(q4, k4, q_lens, k_lens, cu_seqlens, cu_seqlens_k)
+    return _AttentionFunction.apply(q, k, v, q_seq, k_seq, packed, float(scale), bool(causal),
+                                    int(window or 0), bool(return_lse))

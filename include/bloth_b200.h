@@ -264,6 +264,57 @@ int bloth_rope(const void* q, const int64_t* q_strides, void* q_out, const int64
                const void* cos, const void* sin, const int64_t* cs_strides, int64_t cs_rows,
                int cs_dtype, float rope_scale, int64_t B, int64_t S, int64_t Hq, int64_t Hk,
                int64_t D, int transpose, int dtype, void* stream);
+/* ------------------------------------------------------------------------
+ * Attention over head tensors: out = softmax(scale * q k^T) v per query row
+ * over the keys it sees, and its backward, which recomputes the probabilities
+ * from lse. q, out, dout, dq: [B, Sq, Hq, D]; k, v, dk, dv: [B, Sk, Hk, D]
+ * (head convention and strides as above); Hq a multiple of Hk, query head h
+ * reads key head h / (Hq / Hk). D: 64, 128 or 256. lse [B, Hq, Sq] fp32, the
+ * natural logarithm of each row's sum of exponentials.
+ *
+ * Sequences. packed == 0: batch row b holds q_seq[b] query rows and k_seq[b]
+ * key rows at its start (clamped to [0, Sq] and [0, Sk]; NULL: all of them).
+ * packed == n > 0: B must be 1, and q_seq and k_seq are n + 1 offsets each
+ * (clamped to the tensors, and to be non-decreasing): sequence i holds query
+ * rows q_seq[i] .. q_seq[i+1] - 1 and key rows k_seq[i] .. k_seq[i+1] - 1.
+ * seq_dtype: I32 or I64. Both arrays are read on the device.
+ *
+ * With qlen and klen a sequence's lengths, query i sees key j < klen when,
+ * causal, j <= i + klen - qlen (the last query sees the last key) and, with
+ * window > 0 (causal only), also j > i + klen - qlen - window. A row that sees
+ * nothing, and every row outside of the sequences, has out = 0, lse = -inf and
+ * zero gradients; what memory holds outside of the sequences is never used.
+ *
+ * Scores, row statistics, probabilities and all sums are fp32; with 16-bit
+ * tensors probabilities and ds are rounded to the tensors' type where they
+ * enter a matrix product. Results do not depend on scheduling.
+ * No counterpart in the reference, whose path ends at RoPE.
+ * ---------------------------------------------------------------------- */
+size_t bloth_attention_fwd_workspace_bytes(int64_t B, int64_t Sq, int64_t Sk, int64_t Hq,
+                                           int64_t Hk, int64_t D, int64_t packed, int dtype);
+/* lse may be NULL when no backward follows. The workspace may be NULL when the
+   function above reports 0 bytes; its base is aligned to 16 bytes. */
+int bloth_attention_fwd(const void* q, const int64_t* q_strides, const void* k,
+                        const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                        void* out, const int64_t* out_strides, float* lse, const void* q_seq,
+                        const void* k_seq, int seq_dtype, int64_t packed, int64_t B, int64_t Sq,
+                        int64_t Sk, int64_t Hq, int64_t Hk, int64_t D, float scale, int causal,
+                        int64_t window, int dtype, void* workspace, size_t workspace_bytes,
+                        void* stream);
+size_t bloth_attention_bwd_workspace_bytes(int64_t B, int64_t Sq, int64_t Sk, int64_t Hq,
+                                           int64_t Hk, int64_t D, int64_t packed, int dtype);
+/* out and lse are the forward's. dq may be NULL, and dk and dv both (not one
+   of them), when they are not wanted. */
+int bloth_attention_bwd(const void* dout, const int64_t* dout_strides, const void* q,
+                        const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                        const void* v, const int64_t* v_strides, const void* out,
+                        const int64_t* out_strides, const float* lse, void* dq,
+                        const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
+                        const int64_t* dv_strides, const void* q_seq, const void* k_seq,
+                        int seq_dtype, int64_t packed, int64_t B, int64_t Sq, int64_t Sk,
+                        int64_t Hq, int64_t Hk, int64_t D, float scale, int causal,
+                        int64_t window, int dtype, void* workspace, size_t workspace_bytes,
+                        void* stream);
 #ifdef __cplusplus
 }
 #endif
