@@ -110,8 +110,13 @@ int bloth_attention_fwd(const void* q, const int64_t* q_strides, const void* k,
   a.lse = lse;
   (void)workspace;
   (void)workspace_bytes;
-  return by_dtype(dtype,
-                  [&](auto t) { return attn_simt_fwd<decltype(t)>(a, (int)D, as_stream(stream)); });
+  return by_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    if constexpr (sizeof(T) == 2) {
+      if (D <= 128 && Sk > 0) return attn_tc_fwd<T>(a, (int)D, as_stream(stream));
+    }
+    return attn_simt_fwd<T>(a, (int)D, as_stream(stream));
+  });
 }
 
 size_t bloth_attention_bwd_workspace_bytes(int64_t B, int64_t Sq, int64_t Sk, int64_t Hq,

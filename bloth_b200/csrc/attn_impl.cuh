@@ -166,7 +166,9 @@ __device__ __forceinline__ void query_range(const AttnArgs& a, const AttnSeq& s,
   if (n1 <= n0 || hi <= lo) lo = hi = 0;
 }
 
-// Host launchers (attn_simt_<type>.cu, attn_stat.cu).
+// Host launchers. attn_tc_*: 16-bit tensors, head_dim 64 or 128.
+template <typename T>
+int attn_tc_fwd(const AttnArgs& a, int D, cudaStream_t st);
 template <typename T>
 int attn_simt_fwd(const AttnArgs& a, int D, cudaStream_t st);
 template <typename T>

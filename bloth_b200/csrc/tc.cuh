@@ -1,0 +1,190 @@
+// Tensor-core and tensor-copy primitives for sm_100a as inline PTX: tensor
+// maps and tiled bulk copies, tcgen05 matrix products with accumulators in
+// tensor memory, their shared-memory descriptors, and the bounded wait of the
+// kernels that hand tiles between warps.
+//
+// Tiles. A 16-bit operand tile of R rows and D columns lies in shared memory
+// as D / 64 blocks of [R][64] elements (128 bytes a row), each written by one
+// tiled copy with the 128-byte swizzle, 1024-byte aligned. The same tile
+// serves as an operand whose contracted index runs along its columns
+// (desc_k: "K-major") or along its rows (desc_mn: "MN-major").
+#pragma once
+
+#include <cuda.h>
+
+#include "bulk.cuh"
+
+namespace bloth {
+
+// ------------------------------------------------------------------ waits
+// Waits for phase `parity` of `bar`. False once the CTA has given up: when
+// this wait takes longer than kWaitLimitNs (recorded in the fault word), or
+// another thread's did (*stop, in shared memory).
+__device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, volatile int* stop,
+                                        unsigned int* fault) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const unsigned long long t0 = global_ns();
+  while (!mbar_try_wait(bar, parity)) {
+    if (*stop) return false;
+    if (global_ns() - t0 > kWaitLimitNs) {
+      *stop = 1;
+      if (fault != nullptr) atomicOr(fault, kFaultCopyTimeout);
+      return false;
+    }
+  }
+  return true;
+}
+
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
+// ----------------------------------------------------------- tiled copies
+// One box of a 4-D tensor map (column, row, head, batch) into shared memory.
+__device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int col, int row,
+                                         int head, int batch, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_addr(dst)),
+      "l"(map), "r"(col), "r"(row), "r"(head), "r"(batch), "r"(smem_addr(bar))
+      : "memory");
+}
+
+// ------------------------------------------------------------ descriptors
+// Shared-memory operand descriptor: address and offsets in 16-byte units,
+// version 1 (bit 46), 128-byte swizzle (2 in bits 61-63).
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead, uint32_t stride) {
+  return (uint64_t)((addr & 0x3ffff) >> 4) | ((uint64_t)(lead >> 4) << 16) |
+         ((uint64_t)(stride >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// Contracted index along the columns: groups of 8 rows are 1024 bytes apart;
+// a step of 16 columns is 32 bytes inside a 64-column block.
+__device__ __forceinline__ uint64_t desc_k(uint32_t addr) { return smem_desc(addr, 0, 1024); }
+// Contracted index along the rows: groups of 8 rows are 1024 bytes apart, the
+// next 64 columns one block of `block` bytes further.
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t block) {
+  return smem_desc(addr, block, 1024);
+}
+
+// Instruction descriptor: fp32 accumulator, A and B of type T, M x N, B's
+// contracted index along its rows (b_mn) or columns.
+template <typename T>
+__host__ __device__ constexpr uint32_t mma_desc(int m, int n, bool b_mn) {
+  const uint32_t ty = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  return (1u << 4) | (ty << 7) | (ty << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(m >> 4) << 24);
+}
+
+// --------------------------------------------------------- matrix products
+// Tensor memory [d] (+)= A x B for 16 contracted elements; issued by one
+// thread. A in shared memory (mma_ss) or in tensor memory (mma_ts).
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                       bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((int)add)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                       bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((int)add)
+      : "memory");
+}
+// `bar` completes a phase when every product issued so far has completed.
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                   smem_addr(bar))
+               : "memory");
+}
+
+// ----------------------------------------------------------- tensor memory
+// Whole-warp allocation of `cols` columns; the address goes to *dst.
+__device__ __forceinline__ void tmem_alloc(uint32_t* dst, uint32_t cols) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                   smem_addr(dst)),
+               "r"(cols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tc_fence_before() {
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void tc_fence_after() {
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+
+// 32 columns of the warp's 32 lanes: lane l gets row l. The address carries
+// the warp's first lane in its upper half.
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(
+          addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+      "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
+      "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// ------------------------------------------------------------- arithmetic
+// 2^x; 2 ulp, results below the normal range are 0.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Two floats rounded to T in one register, the first in the lower half.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Host: tensor map of a head tensor [B, S, H, D] of 16-bit elements, boxes of
+// `rows` rows x 64 columns of one head, 128-byte swizzle, zeros outside.
+int head_map(CUtensorMap* map, const void* p, int64_t sb, int64_t ss, int64_t sh, int B, int64_t S,
+             int H, int D, int rows, int dtype);
+
+}  // namespace bloth
