@@ -170,6 +170,9 @@ int bloth_attention_bwd(const void* dout, const int64_t* dout_strides, const voi
       const int r = attn_stats<T>(a, (int)D, as_stream(stream));
       if (r != BLOTH_OK) return r;
     }
+    if constexpr (sizeof(T) == 2) {
+      if (D <= 128 && Sq > 0 && Sk > 0) return attn_tc_bwd<T>(a, (int)D, as_stream(stream));
+    }
     return attn_simt_bwd<T>(a, (int)D, as_stream(stream));
   });
 }

@@ -170,6 +170,8 @@ __device__ __forceinline__ void query_range(const AttnArgs& a, const AttnSeq& s,
 template <typename T>
 int attn_tc_fwd(const AttnArgs& a, int D, cudaStream_t st);
 template <typename T>
+int attn_tc_bwd(const AttnArgs& a, int D, cudaStream_t st);
+template <typename T>
 int attn_simt_fwd(const AttnArgs& a, int D, cudaStream_t st);
 template <typename T>
 int attn_simt_bwd(const AttnArgs& a, int D, cudaStream_t st);
