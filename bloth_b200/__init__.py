@@ -22,13 +22,16 @@ __version__ = "0.2.0"
 
 from . import kernels  # noqa: F401
 from .kernels import (  # noqa: F401
+    apply_mrope_qk,
     apply_rope,
     apply_rope_qk,
     apply_rotary_pos_emb,
     fused_add_rms_norm,
     fused_attention,
     fused_norm_rope,
+    fused_qk_norm_mrope,
     fused_qk_norm_rope,
+    mrope_axes,
 )
 from .modules import (  # noqa: F401
     BlothFusedNormQKV,
@@ -55,6 +58,9 @@ __all__ = [
     "fused_add_rms_norm",
     "fused_norm_rope",
     "fused_qk_norm_rope",
+    "fused_qk_norm_mrope",
+    "apply_mrope_qk",
+    "mrope_axes",
     "fused_attention",
     "BlothQKNormRoPE",
     "rope_embedding",

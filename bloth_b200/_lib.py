@@ -75,6 +75,16 @@ _SIGNATURES = {
     "bloth_rope": (_int, [_vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _int, _vp,
                           _vp, _vp, _i64p, _i64, _int, _f32, _i64, _i64, _i64, _i64, _i64, _int,
                           _int, _vp]),
+    "bloth_qk_norm_mrope_fwd": (_int, [_vp, _i64p, _vp, _i64p, _vp, _vp, _f32, _vp, _i64p, _vp,
+                                       _i64p, _vp, _vp, _vp, _i64p, _int, _int, _vp, _vp, _f32,
+                                       _i64, _i64, _i64, _i64, _i64, _f32, _int, _int, _vp]),
+    "bloth_qk_norm_mrope_bwd_workspace_bytes": (_sz, [_i64, _i64, _i64, _int]),
+    "bloth_qk_norm_mrope_bwd": (_int, [_vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _vp,
+                                       _f32, _vp, _vp, _vp, _i64p, _vp, _i64p, _vp, _vp, _vp,
+                                       _i64p, _int, _int, _vp, _vp, _f32, _i64, _i64, _i64, _i64,
+                                       _i64, _int, _int, _vp, _sz, _vp]),
+    "bloth_mrope": (_int, [_vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _int, _int,
+                           _vp, _vp, _f32, _i64, _i64, _i64, _i64, _i64, _int, _int, _vp]),
     "bloth_attention_fwd_workspace_bytes": (_sz, [_i64] * 7 + [_int]),
     "bloth_attention_fwd": (_int, [_vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _vp, _vp,
                                    _int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _int,

@@ -1,6 +1,7 @@
 // extern "C" entry points declared in include/bloth_b200.h: argument
 // validation, element-type dispatch and the choice between the 16-byte vector
 // path and the scalar path of the row kernels.
+#include <algorithm>
 #include <cstring>
 
 #include "common.cuh"
@@ -143,6 +144,192 @@ int fill_rope_source(HeadArgs& a, const void* pos, const int64_t* pos_strides, i
   return BLOTH_OK;
 }
 
+// Axes of positions of several axes; n == 0: one position per token.
+struct Axes {
+  int64_t stride = 0;
+  int n = 0;
+  const unsigned char* of = nullptr;  // axis of each of the D/2 pairs
+};
+
+int fill_axes(HeadArgs& a, const Axes& x, int64_t D) {
+  if (x.n == 0) return BLOTH_OK;
+  if (x.of == nullptr || a.pos == nullptr) return BLOTH_ERR_NULL;
+  if (x.n < 1 || x.n > 4) return BLOTH_ERR_SHAPE;
+  for (int64_t i = 0; i < D / 2; ++i) {
+    if (x.of[i] >= x.n) return BLOTH_ERR_ARG;
+    a.axes[i >> 4] |= (uint32_t)x.of[i] << (2 * (i & 15));
+  }
+  a.n_axes = x.n;
+  a.pos_sa = x.stride;
+  return BLOTH_OK;
+}
+
+// The axes arguments of the *_mrope entry points: pos_strides is [axis,
+// batch, sequence], of which fill_rope_source takes the last two.
+int mrope_axes(Axes& x, const int64_t* pos_strides, int n_axes, const unsigned char* axis_of) {
+  if (pos_strides == nullptr) return BLOTH_ERR_NULL;
+  if (n_axes < 1 || n_axes > 4) return BLOTH_ERR_SHAPE;
+  x.stride = pos_strides[0];
+  x.n = n_axes;
+  x.of = axis_of;
+  return BLOTH_OK;
+}
+
+int qk_norm_rope_fwd(const Axes& ax, const void* q, const int64_t* q_strides, const void* k,
+                     const int64_t* k_strides, const void* wq, const void* wk, float w_offset,
+                     void* q_out, const int64_t* qo_strides, void* k_out,
+                     const int64_t* ko_strides, float* rstd_q, float* rstd_k, const void* pos,
+                     const int64_t* pos_strides, int pos_dtype, const float* inv_freq,
+                     const void* cos, const void* sin, const int64_t* cs_strides,
+                     int64_t cs_rows, int cs_dtype, float rope_scale, int64_t B, int64_t S,
+                     int64_t Hq, int64_t Hk, int64_t D, float eps, int dtype, int w_dtype,
+                     void* stream) {
+  if (!is_float_dt(dtype) || !is_float_dt(w_dtype)) return BLOTH_ERR_DTYPE;
+  if (!head_dim_ok(D) || B < 0 || S < 0 || Hq < 0 || Hk < 0 || Hq + Hk < 1 || Hq > (1 << 20) ||
+      Hk > (1 << 20) || (S > 0 && B >= kMaxTokens / S))
+    return BLOTH_ERR_SHAPE;
+  HeadArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.fault = fault_word();
+  int rc = fill_rope_source(a, pos, pos_strides, pos_dtype, inv_freq, cos, sin, cs_strides,
+                            cs_rows, cs_dtype, rope_scale, dtype, D);
+  if (rc) return rc;
+  if ((rc = fill_axes(a, ax, D))) return rc;
+  if (B * S == 0) return BLOTH_OK;
+  const void* src[2] = {q, k};
+  const int64_t* sst[2] = {q_strides, k_strides};
+  void* dst[2] = {q_out, k_out};
+  const int64_t* dstst[2] = {qo_strides, ko_strides};
+  const void* w[2] = {wq, wk};
+  float* rs[2] = {rstd_q, rstd_k};
+  const int64_t H[2] = {Hq, Hk};
+  for (int t = 0; t < 2; ++t) {
+    if (H[t] == 0) continue;
+    if ((rc = check_heads_tensor(src[t], sst[t], dtype))) return rc;
+    if ((rc = check_heads_tensor(dst[t], dstst[t], dtype))) return rc;
+    if (w[t] == nullptr || rs[t] == nullptr) return BLOTH_ERR_NULL;
+    if (!aligned(w[t], 16)) return BLOTH_ERR_ALIGN;
+    a.src[t] = make_ht(src[t], sst[t]);
+    a.dst[t] = make_ht(dst[t], dstst[t]);
+    a.w[t] = w[t];
+    a.rstd_out[t] = rs[t];
+    a.H[t] = (int)H[t];
+  }
+  a.w_dt = w_dtype;
+  a.w_off = w_offset;
+  a.B = B;
+  a.S = S;
+  a.eps = eps;
+  return dispatch_dtype(dtype, [&](auto t) {
+    return a.n_axes > 1 ? heads_fwd<decltype(t), true>(a, (int)D, true, as_stream(stream))
+                        : heads_fwd<decltype(t)>(a, (int)D, true, as_stream(stream));
+  });
+}
+
+int qk_norm_rope_bwd(const Axes& ax, const void* dq_out, const int64_t* dqo_strides,
+                     const void* dk_out, const int64_t* dko_strides, const void* q,
+                     const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                     const void* wq, const void* wk, float w_offset, const float* rstd_q,
+                     const float* rstd_k, void* dq, const int64_t* dq_strides, void* dk,
+                     const int64_t* dk_strides, void* dwq, void* dwk, const void* pos,
+                     const int64_t* pos_strides, int pos_dtype, const float* inv_freq,
+                     const void* cos, const void* sin, const int64_t* cs_strides,
+                     int64_t cs_rows, int cs_dtype, float rope_scale, int64_t B, int64_t S,
+                     int64_t Hq, int64_t Hk, int64_t D, int dtype, int w_dtype, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  if (!is_float_dt(dtype) || !is_float_dt(w_dtype)) return BLOTH_ERR_DTYPE;
+  if (!head_dim_ok(D) || B < 0 || S < 0 || Hq < 0 || Hk < 0 || Hq + Hk < 1 || Hq > (1 << 20) ||
+      Hk > (1 << 20) || (S > 0 && B >= kMaxTokens / S))
+    return BLOTH_ERR_SHAPE;
+  HeadArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.fault = fault_word();
+  int rc = fill_rope_source(a, pos, pos_strides, pos_dtype, inv_freq, cos, sin, cs_strides,
+                            cs_rows, cs_dtype, rope_scale, dtype, D);
+  if (rc) return rc;
+  if ((rc = fill_axes(a, ax, D))) return rc;
+  const void* g[2] = {dq_out, dk_out};
+  const int64_t* gst[2] = {dqo_strides, dko_strides};
+  const void* x[2] = {q, k};
+  const int64_t* xst[2] = {q_strides, k_strides};
+  void* dst[2] = {dq, dk};
+  const int64_t* dstst[2] = {dq_strides, dk_strides};
+  const void* w[2] = {wq, wk};
+  const float* rs[2] = {rstd_q, rstd_k};
+  void* dw[2] = {dwq, dwk};
+  const int64_t H[2] = {Hq, Hk};
+  for (int t = 0; t < 2; ++t) {
+    if (H[t] == 0) continue;
+    if (w[t] == nullptr || dw[t] == nullptr) return BLOTH_ERR_NULL;
+    if (!aligned(w[t], 16)) return BLOTH_ERR_ALIGN;
+    a.w[t] = w[t];
+    a.H[t] = (int)H[t];
+    if (B * S == 0) continue;
+    if ((rc = check_heads_tensor(g[t], gst[t], dtype))) return rc;
+    if ((rc = check_heads_tensor(x[t], xst[t], dtype))) return rc;
+    if ((rc = check_heads_tensor(dst[t], dstst[t], dtype))) return rc;
+    if (rs[t] == nullptr) return BLOTH_ERR_NULL;
+    a.src[t] = make_ht(g[t], gst[t]);
+    a.x[t] = make_ht(x[t], xst[t]);
+    a.dst[t] = make_ht(dst[t], dstst[t]);
+    a.rstd_in[t] = rs[t];
+  }
+  a.w_dt = w_dtype;
+  a.w_off = w_offset;
+  a.B = B;
+  a.S = S;
+  a.rstd_bulk = (Hq % 4 == 0) && (Hk % 4 == 0) && aligned(rstd_q, 16) &&
+                (Hk == 0 || aligned(rstd_k, 16));
+  return dispatch_dtype(dtype, [&](auto t) {
+    void* const dw1 = Hk > 0 ? dwk : nullptr;
+    return a.n_axes > 1 ? heads_bwd<decltype(t), true>(a, (int)D, workspace, workspace_bytes, dwq,
+                                                       dw1, as_stream(stream))
+                        : heads_bwd<decltype(t)>(a, (int)D, workspace, workspace_bytes, dwq, dw1,
+                                                 as_stream(stream));
+  });
+}
+
+int rope_call(const Axes& ax, const void* q, const int64_t* q_strides, void* q_out,
+              const int64_t* qo_strides, const void* k, const int64_t* k_strides, void* k_out,
+              const int64_t* ko_strides, const void* pos, const int64_t* pos_strides,
+              int pos_dtype, const float* inv_freq, const void* cos, const void* sin,
+              const int64_t* cs_strides, int64_t cs_rows, int cs_dtype, float rope_scale,
+              int64_t B, int64_t S, int64_t Hq, int64_t Hk, int64_t D, int transpose, int dtype,
+              void* stream) {
+  if (!is_float_dt(dtype)) return BLOTH_ERR_DTYPE;
+  if (!head_dim_ok(D) || B < 0 || S < 0 || Hq < 0 || Hk < 0 || Hq + Hk < 1 || Hq > (1 << 20) ||
+      Hk > (1 << 20) || (S > 0 && B >= kMaxTokens / S))
+    return BLOTH_ERR_SHAPE;
+  HeadArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.fault = fault_word();
+  int rc = fill_rope_source(a, pos, pos_strides, pos_dtype, inv_freq, cos, sin, cs_strides,
+                            cs_rows, cs_dtype, rope_scale, dtype, D);
+  if (rc) return rc;
+  if ((rc = fill_axes(a, ax, D))) return rc;
+  if (B * S == 0) return BLOTH_OK;
+  const void* src[2] = {q, k};
+  const int64_t* sst[2] = {q_strides, k_strides};
+  void* dst[2] = {q_out, k_out};
+  const int64_t* dstst[2] = {qo_strides, ko_strides};
+  const int64_t H[2] = {Hq, Hk};
+  for (int t = 0; t < 2; ++t) {
+    if (H[t] == 0) continue;
+    if ((rc = check_heads_tensor(src[t], sst[t], dtype))) return rc;
+    if ((rc = check_heads_tensor(dst[t], dstst[t], dtype))) return rc;
+    a.src[t] = make_ht(src[t], sst[t]);
+    a.dst[t] = make_ht(dst[t], dstst[t]);
+    a.H[t] = (int)H[t];
+  }
+  a.B = B;
+  a.S = S;
+  a.transpose = transpose ? 1 : 0;
+  a.w_dt = BLOTH_F32;
+  return dispatch_dtype(dtype, [&](auto t) {
+    return a.n_axes > 1 ? heads_fwd<decltype(t), true>(a, (int)D, false, as_stream(stream))
+                        : heads_fwd<decltype(t)>(a, (int)D, false, as_stream(stream));
+  });
+}
 }  // namespace
 
 extern "C" {
@@ -383,44 +570,10 @@ int bloth_qk_norm_rope_fwd(const void* q, const int64_t* q_strides, const void* 
                            const int64_t* cs_strides, int64_t cs_rows, int cs_dtype,
                            float rope_scale, int64_t B, int64_t S, int64_t Hq,
                            int64_t Hk, int64_t D, float eps, int dtype, int w_dtype, void* stream) {
-  if (!is_float_dt(dtype) || !is_float_dt(w_dtype)) return BLOTH_ERR_DTYPE;
-  if (!head_dim_ok(D) || B < 0 || S < 0 || Hq < 0 || Hk < 0 || Hq + Hk < 1 || Hq > (1 << 20) ||
-      Hk > (1 << 20) || (S > 0 && B >= kMaxTokens / S))
-    return BLOTH_ERR_SHAPE;
-  HeadArgs a;
-  std::memset(&a, 0, sizeof(a));
-  a.fault = fault_word();
-  int rc = fill_rope_source(a, pos, pos_strides, pos_dtype, inv_freq, cos, sin, cs_strides,
-                            cs_rows, cs_dtype, rope_scale, dtype, D);
-  if (rc) return rc;
-  if (B * S == 0) return BLOTH_OK;
-  const void* src[2] = {q, k};
-  const int64_t* sst[2] = {q_strides, k_strides};
-  void* dst[2] = {q_out, k_out};
-  const int64_t* dstst[2] = {qo_strides, ko_strides};
-  const void* w[2] = {wq, wk};
-  float* rs[2] = {rstd_q, rstd_k};
-  const int64_t H[2] = {Hq, Hk};
-  for (int t = 0; t < 2; ++t) {
-    if (H[t] == 0) continue;
-    if ((rc = check_heads_tensor(src[t], sst[t], dtype))) return rc;
-    if ((rc = check_heads_tensor(dst[t], dstst[t], dtype))) return rc;
-    if (w[t] == nullptr || rs[t] == nullptr) return BLOTH_ERR_NULL;
-    if (!aligned(w[t], 16)) return BLOTH_ERR_ALIGN;
-    a.src[t] = make_ht(src[t], sst[t]);
-    a.dst[t] = make_ht(dst[t], dstst[t]);
-    a.w[t] = w[t];
-    a.rstd_out[t] = rs[t];
-    a.H[t] = (int)H[t];
-  }
-  a.w_dt = w_dtype;
-  a.w_off = w_offset;
-  a.B = B;
-  a.S = S;
-  a.eps = eps;
-  return dispatch_dtype(dtype, [&](auto t) {
-    return heads_fwd<decltype(t)>(a, (int)D, true, as_stream(stream));
-  });
+  return qk_norm_rope_fwd(Axes(), q, q_strides, k, k_strides, wq, wk, w_offset, q_out,
+                          qo_strides, k_out, ko_strides, rstd_q, rstd_k, pos, pos_strides,
+                          pos_dtype, inv_freq, cos, sin, cs_strides, cs_rows, cs_dtype,
+                          rope_scale, B, S, Hq, Hk, D, eps, dtype, w_dtype, stream);
 }
 
 size_t bloth_qk_norm_rope_bwd_workspace_bytes(int64_t B, int64_t S, int64_t D, int dtype) {
@@ -446,52 +599,11 @@ int bloth_qk_norm_rope_bwd(const void* dq_out, const int64_t* dqo_strides, const
                            int64_t Hk, int64_t D,
                            int dtype, int w_dtype, void* workspace, size_t workspace_bytes,
                            void* stream) {
-  if (!is_float_dt(dtype) || !is_float_dt(w_dtype)) return BLOTH_ERR_DTYPE;
-  if (!head_dim_ok(D) || B < 0 || S < 0 || Hq < 0 || Hk < 0 || Hq + Hk < 1 || Hq > (1 << 20) ||
-      Hk > (1 << 20) || (S > 0 && B >= kMaxTokens / S))
-    return BLOTH_ERR_SHAPE;
-  HeadArgs a;
-  std::memset(&a, 0, sizeof(a));
-  a.fault = fault_word();
-  int rc = fill_rope_source(a, pos, pos_strides, pos_dtype, inv_freq, cos, sin, cs_strides,
-                            cs_rows, cs_dtype, rope_scale, dtype, D);
-  if (rc) return rc;
-  const void* g[2] = {dq_out, dk_out};
-  const int64_t* gst[2] = {dqo_strides, dko_strides};
-  const void* x[2] = {q, k};
-  const int64_t* xst[2] = {q_strides, k_strides};
-  void* dst[2] = {dq, dk};
-  const int64_t* dstst[2] = {dq_strides, dk_strides};
-  const void* w[2] = {wq, wk};
-  const float* rs[2] = {rstd_q, rstd_k};
-  void* dw[2] = {dwq, dwk};
-  const int64_t H[2] = {Hq, Hk};
-  for (int t = 0; t < 2; ++t) {
-    if (H[t] == 0) continue;
-    if (w[t] == nullptr || dw[t] == nullptr) return BLOTH_ERR_NULL;
-    if (!aligned(w[t], 16)) return BLOTH_ERR_ALIGN;
-    a.w[t] = w[t];
-    a.H[t] = (int)H[t];
-    if (B * S == 0) continue;
-    if ((rc = check_heads_tensor(g[t], gst[t], dtype))) return rc;
-    if ((rc = check_heads_tensor(x[t], xst[t], dtype))) return rc;
-    if ((rc = check_heads_tensor(dst[t], dstst[t], dtype))) return rc;
-    if (rs[t] == nullptr) return BLOTH_ERR_NULL;
-    a.src[t] = make_ht(g[t], gst[t]);
-    a.x[t] = make_ht(x[t], xst[t]);
-    a.dst[t] = make_ht(dst[t], dstst[t]);
-    a.rstd_in[t] = rs[t];
-  }
-  a.w_dt = w_dtype;
-  a.w_off = w_offset;
-  a.B = B;
-  a.S = S;
-  a.rstd_bulk = (Hq % 4 == 0) && (Hk % 4 == 0) && aligned(rstd_q, 16) &&
-                (Hk == 0 || aligned(rstd_k, 16));
-  return dispatch_dtype(dtype, [&](auto t) {
-    return heads_bwd<decltype(t)>(a, (int)D, workspace, workspace_bytes, dwq,
-                                  Hk > 0 ? dwk : nullptr, as_stream(stream));
-  });
+  return qk_norm_rope_bwd(Axes(), dq_out, dqo_strides, dk_out, dko_strides, q, q_strides, k,
+                          k_strides, wq, wk, w_offset, rstd_q, rstd_k, dq, dq_strides, dk,
+                          dk_strides, dwq, dwk, pos, pos_strides, pos_dtype, inv_freq, cos, sin,
+                          cs_strides, cs_rows, cs_dtype, rope_scale, B, S, Hq, Hk, D, dtype,
+                          w_dtype, workspace, workspace_bytes, stream);
 }
 
 int bloth_rope(const void* q, const int64_t* q_strides, void* q_out, const int64_t* qo_strides,
@@ -500,37 +612,71 @@ int bloth_rope(const void* q, const int64_t* q_strides, void* q_out, const int64
                const void* cos, const void* sin, const int64_t* cs_strides, int64_t cs_rows,
                int cs_dtype, float rope_scale, int64_t B, int64_t S, int64_t Hq, int64_t Hk,
                int64_t D, int transpose, int dtype, void* stream) {
-  if (!is_float_dt(dtype)) return BLOTH_ERR_DTYPE;
-  if (!head_dim_ok(D) || B < 0 || S < 0 || Hq < 0 || Hk < 0 || Hq + Hk < 1 || Hq > (1 << 20) ||
-      Hk > (1 << 20) || (S > 0 && B >= kMaxTokens / S))
-    return BLOTH_ERR_SHAPE;
-  HeadArgs a;
-  std::memset(&a, 0, sizeof(a));
-  a.fault = fault_word();
-  int rc = fill_rope_source(a, pos, pos_strides, pos_dtype, inv_freq, cos, sin, cs_strides,
-                            cs_rows, cs_dtype, rope_scale, dtype, D);
-  if (rc) return rc;
-  if (B * S == 0) return BLOTH_OK;
-  const void* src[2] = {q, k};
-  const int64_t* sst[2] = {q_strides, k_strides};
-  void* dst[2] = {q_out, k_out};
-  const int64_t* dstst[2] = {qo_strides, ko_strides};
-  const int64_t H[2] = {Hq, Hk};
-  for (int t = 0; t < 2; ++t) {
-    if (H[t] == 0) continue;
-    if ((rc = check_heads_tensor(src[t], sst[t], dtype))) return rc;
-    if ((rc = check_heads_tensor(dst[t], dstst[t], dtype))) return rc;
-    a.src[t] = make_ht(src[t], sst[t]);
-    a.dst[t] = make_ht(dst[t], dstst[t]);
-    a.H[t] = (int)H[t];
-  }
-  a.B = B;
-  a.S = S;
-  a.transpose = transpose ? 1 : 0;
-  a.w_dt = BLOTH_F32;
-  return dispatch_dtype(dtype, [&](auto t) {
-    return heads_fwd<decltype(t)>(a, (int)D, false, as_stream(stream));
+  return rope_call(Axes(), q, q_strides, q_out, qo_strides, k, k_strides, k_out, ko_strides, pos,
+                   pos_strides, pos_dtype, inv_freq, cos, sin, cs_strides, cs_rows, cs_dtype,
+                   rope_scale, B, S, Hq, Hk, D, transpose, dtype, stream);
+}
+
+size_t bloth_qk_norm_mrope_bwd_workspace_bytes(int64_t B, int64_t S, int64_t D, int dtype) {
+  if (!is_float_dt(dtype) || !head_dim_ok(D) || B < 0 || S < 0) return 0;
+  size_t bytes = 0;
+  dispatch_dtype(dtype, [&](auto t) {
+    bytes = std::max(heads_bwd_workspace<decltype(t)>(B * S, (int)D),
+                     heads_bwd_workspace<decltype(t), true>(B * S, (int)D));
+    return 0;
   });
+  return bytes;
+}
+
+int bloth_qk_norm_mrope_fwd(const void* q, const int64_t* q_strides, const void* k,
+                            const int64_t* k_strides, const void* wq, const void* wk,
+                            float w_offset, void* q_out, const int64_t* qo_strides, void* k_out,
+                            const int64_t* ko_strides, float* rstd_q, float* rstd_k,
+                            const void* pos, const int64_t* pos_strides, int pos_dtype, int n_axes,
+                            const unsigned char* axis_of, const float* inv_freq, float rope_scale,
+                            int64_t B, int64_t S, int64_t Hq, int64_t Hk, int64_t D, float eps,
+                            int dtype, int w_dtype, void* stream) {
+  Axes ax;
+  const int rc = mrope_axes(ax, pos_strides, n_axes, axis_of);
+  if (rc) return rc;
+  return qk_norm_rope_fwd(ax, q, q_strides, k, k_strides, wq, wk, w_offset, q_out, qo_strides,
+                          k_out, ko_strides, rstd_q, rstd_k, pos, pos_strides + 1, pos_dtype,
+                          inv_freq, nullptr, nullptr, nullptr, 0, 0, rope_scale, B, S, Hq, Hk, D,
+                          eps, dtype, w_dtype, stream);
+}
+
+int bloth_qk_norm_mrope_bwd(const void* dq_out, const int64_t* dqo_strides, const void* dk_out,
+                            const int64_t* dko_strides, const void* q, const int64_t* q_strides,
+                            const void* k, const int64_t* k_strides, const void* wq,
+                            const void* wk, float w_offset, const float* rstd_q,
+                            const float* rstd_k, void* dq, const int64_t* dq_strides, void* dk,
+                            const int64_t* dk_strides, void* dwq, void* dwk, const void* pos,
+                            const int64_t* pos_strides, int pos_dtype, int n_axes,
+                            const unsigned char* axis_of, const float* inv_freq, float rope_scale,
+                            int64_t B, int64_t S, int64_t Hq, int64_t Hk, int64_t D, int dtype,
+                            int w_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  Axes ax;
+  const int rc = mrope_axes(ax, pos_strides, n_axes, axis_of);
+  if (rc) return rc;
+  return qk_norm_rope_bwd(ax, dq_out, dqo_strides, dk_out, dko_strides, q, q_strides, k, k_strides,
+                          wq, wk, w_offset, rstd_q, rstd_k, dq, dq_strides, dk, dk_strides, dwq,
+                          dwk, pos, pos_strides + 1, pos_dtype, inv_freq, nullptr, nullptr,
+                          nullptr, 0, 0, rope_scale, B, S, Hq, Hk, D, dtype, w_dtype, workspace,
+                          workspace_bytes, stream);
+}
+
+int bloth_mrope(const void* q, const int64_t* q_strides, void* q_out, const int64_t* qo_strides,
+                const void* k, const int64_t* k_strides, void* k_out, const int64_t* ko_strides,
+                const void* pos, const int64_t* pos_strides, int pos_dtype, int n_axes,
+                const unsigned char* axis_of, const float* inv_freq, float rope_scale, int64_t B,
+                int64_t S, int64_t Hq, int64_t Hk, int64_t D, int transpose, int dtype,
+                void* stream) {
+  Axes ax;
+  const int rc = mrope_axes(ax, pos_strides, n_axes, axis_of);
+  if (rc) return rc;
+  return rope_call(ax, q, q_strides, q_out, qo_strides, k, k_strides, k_out, ko_strides, pos,
+                   pos_strides + 1, pos_dtype, inv_freq, nullptr, nullptr, nullptr, 0, 0,
+                   rope_scale, B, S, Hq, Hk, D, transpose, dtype, stream);
 }
 
 }  // extern "C"

@@ -48,6 +48,11 @@ struct HeadArgs {
   const void* pos;
   int pos_dt;
   int64_t pos_sb, pos_ss;
+  // positions of several axes (time, height, width): axis x of a token is
+  // x * pos_sa elements on, and pair i is turned by axis axis_of(axes, i)
+  int n_axes;         // 0 or 1: one position per token
+  int64_t pos_sa;
+  uint32_t axes[8];   // 2 bits a pair
   const float* inv_freq;
   const void* cos;
   const void* sin;
@@ -99,22 +104,33 @@ __device__ __forceinline__ void partner(const Pack<T, HG<T, D>::VEC> (&v)[HG<T, 
   unpack(v[0], pf[1]);
 }
 
+// The axis whose position turns pair i.
+__device__ __forceinline__ int axis_of(const HeadArgs& a, int i) {
+  return (int)(a.axes[i >> 4] >> (2 * (i & 15))) & 3;
+}
+
+// Position of a token; `axis` elements on for an axis other than the first.
 template <typename T, int D>
-__device__ __forceinline__ int64_t token_pos(const HeadArgs& a, int64_t b, int64_t s) {
+__device__ __forceinline__ int64_t token_pos(const HeadArgs& a, int64_t b, int64_t s,
+                                             int64_t axis = 0) {
   if (a.pos == nullptr) return s;
-  const int64_t o = b * a.pos_sb + s * a.pos_ss;
+  const int64_t o = b * a.pos_sb + s * a.pos_ss + axis;
   if (a.pos_dt == BLOTH_I64) return __ldg(reinterpret_cast<const long long*>(a.pos) + o);
   return __ldg(reinterpret_cast<const int*>(a.pos) + o);
 }
 
-// cos/sin of the lane's VEC pair indices i = pg*VEC + e for one token.
-template <typename T, int D>
-__device__ __forceinline__ void token_cos_sin(const HeadArgs& a, int64_t b, int64_t p, int lane,
-                                              int pg, const float (&invf)[HG<T, D>::APL],
+// cos/sin of the lane's VEC pair indices i = pg*VEC + e for one token, at
+// position pa[0], or (AX) at the position pa[q] of the axis of the lane's
+// angle q.
+template <typename T, int D, bool AX>
+__device__ __forceinline__ void token_cos_sin(const HeadArgs& a, int64_t b,
+                                              const int64_t (&pa)[AX ? HG<T, D>::APL : 1],
+                                              int lane, int pg, const float (&invf)[HG<T, D>::APL],
                                               float (&cs)[HG<T, D>::VEC],
                                               float (&sn)[HG<T, D>::VEC]) {
   using G = HG<T, D>;
-  if (a.cos != nullptr) {
+  const int64_t p = pa[0];
+  if (!AX && a.cos != nullptr) {
     const int64_t pr = p < 0 ? 0 : (p >= a.cs_rows ? a.cs_rows - 1 : p);
     const int64_t off = b * a.cs_sb + pr * a.cs_sp + (int64_t)pg * G::VEC;
     ld_any_vec<G::VEC>(a.cos, off, a.cs_dt, a.cs_vec != 0, cs);
@@ -123,7 +139,8 @@ __device__ __forceinline__ void token_cos_sin(const HeadArgs& a, int64_t b, int6
     const float pf = (float)p;
     float cv[G::APL], sv[G::APL];
 #pragma unroll
-    for (int q = 0; q < G::APL; ++q) sincosf(__fmul_rn(pf, invf[q]), &sv[q], &cv[q]);
+    for (int q = 0; q < G::APL; ++q)
+      sincosf(__fmul_rn(AX ? (float)pa[AX ? q : 0] : pf, invf[q]), &sv[q], &cv[q]);
 #pragma unroll
     for (int e = 0; e < G::VEC; ++e) {
       const int src = (pg * G::VEC + e) / G::APL;
@@ -144,13 +161,14 @@ __device__ __forceinline__ void acc_add(double& acc, float a, float b) {
   acc = fma((double)a, (double)b, acc);
 }
 
-// Host launchers, instantiated per element type in heads_<type>.cu.
-template <typename T>
+// Host launchers, instantiated per element type in heads_<type>.cu (one
+// position per token) and heads_axes_<type>.cu (AX: positions of several axes).
+template <typename T, bool AX = false>
 int heads_fwd(const HeadArgs& a, int D, bool norm, cudaStream_t st);
-template <typename T>
+template <typename T, bool AX = false>
 int heads_bwd(const HeadArgs& a, int D, void* ws, size_t ws_bytes, void* dw0, void* dw1,
               cudaStream_t st);
-template <typename T>
+template <typename T, bool AX = false>
 size_t heads_bwd_workspace(int64_t ntok, int D);
 
 }  // namespace bloth

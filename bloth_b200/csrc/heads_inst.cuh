@@ -91,10 +91,10 @@ int launch_qk_tok(const HeadArgs& a, const TokPlan& pl, int64_t grid, cudaStream
 }
 
 // CTAs of a launch over `ntok` tokens: one wave of resident CTAs, or fewer.
-template <typename T, int D, int MODE>
+template <typename T, int D, int MODE, bool AX>
 int64_t head_pipe_grid(int64_t ntok) {
   using P = HP<T, D, MODE>;
-  auto kern = head_pipe_kernel<T, D, MODE>;
+  auto kern = head_pipe_kernel<T, D, MODE, AX>;
   if (prepare_smem((const void*)kern, P::SMEM) != BLOTH_OK) return -1;
   const int occ = occupancy((const void*)kern, P::WPB * 32, P::SMEM);
   const int64_t wave = (int64_t)device_sm_count() * (occ > 0 ? occ : 1);
@@ -102,7 +102,7 @@ int64_t head_pipe_grid(int64_t ntok) {
   return need < wave ? (need > 0 ? need : 0) : wave;
 }
 
-template <typename T, int D, int MODE>
+template <typename T, int D, int MODE, bool AX>
 int launch_head_fwd(const HeadArgs& a, cudaStream_t st) {
   using P = HP<T, D, MODE>;
   TokPlan pl;
@@ -111,14 +111,14 @@ int launch_head_fwd(const HeadArgs& a, cudaStream_t st) {
     if (grid < 0) return BLOTH_ERR_CUDA;
     return grid == 0 ? BLOTH_OK : launch_qk_tok<T, D, false>(a, pl, grid, st);
   }
-  const int64_t grid = head_pipe_grid<T, D, MODE>(a.B * a.S);
+  const int64_t grid = head_pipe_grid<T, D, MODE, AX>(a.B * a.S);
   if (grid < 0) return BLOTH_ERR_CUDA;
   if (grid == 0) return BLOTH_OK;
-  return launched(launch_ex(head_pipe_kernel<T, D, MODE>, (unsigned)grid, P::WPB * 32, P::SMEM,
+  return launched(launch_ex(head_pipe_kernel<T, D, MODE, AX>, (unsigned)grid, P::WPB * 32, P::SMEM,
                             st, a));
 }
 
-template <typename T, int D>
+template <typename T, int D, bool AX>
 int launch_head_bwd(const HeadArgs& a0, void* ws, size_t ws_bytes, void* dw0, void* dw1,
                     cudaStream_t st) {
   using P = HP<T, D, kHeadNormBwd>;
@@ -126,7 +126,7 @@ int launch_head_bwd(const HeadArgs& a0, void* ws, size_t ws_bytes, void* dw0, vo
   TokPlan pl;
   const bool tok = qk_tok_plan<T, D, true>(a0, pl);
   const int64_t grid = tok ? qk_tok_grid<T, D, true>(a0, pl)
-                           : head_pipe_grid<T, D, kHeadNormBwd>(a0.B * a0.S);
+                           : head_pipe_grid<T, D, kHeadNormBwd, AX>(a0.B * a0.S);
   if (grid < 0) return BLOTH_ERR_CUDA;
   const int wrc = check_workspace<AccT>(ws, (size_t)grid * 2 * D * sizeof(AccT), ws_bytes);
   if (wrc != BLOTH_OK) return wrc;
@@ -137,7 +137,7 @@ int launch_head_bwd(const HeadArgs& a0, void* ws, size_t ws_bytes, void* dw0, vo
     if (tok) {
       rc = launch_qk_tok<T, D, true>(a, pl, grid, st);
     } else {
-      rc = launched(launch_ex(head_pipe_kernel<T, D, kHeadNormBwd>, (unsigned)grid, P::WPB * 32,
+      rc = launched(launch_ex(head_pipe_kernel<T, D, kHeadNormBwd, AX>, (unsigned)grid, P::WPB * 32,
                               P::SMEM, st, a));
     }
     if (rc != BLOTH_OK) return rc;
@@ -156,29 +156,29 @@ bool dispatch_head_dim(int D, F&& f) {
   }
 }
 
-template <typename T>
+template <typename T, bool AX>
 int heads_fwd(const HeadArgs& a, int D, bool norm, cudaStream_t st) {
   int rc = BLOTH_ERR_SHAPE;
   dispatch_head_dim(D, [&](auto dd) {
     constexpr int DD = decltype(dd)::value;
-    rc = norm ? launch_head_fwd<T, DD, kHeadNormFwd>(a, st)
-              : launch_head_fwd<T, DD, kHeadRopeFwd>(a, st);
+    rc = norm ? launch_head_fwd<T, DD, kHeadNormFwd, AX>(a, st)
+              : launch_head_fwd<T, DD, kHeadRopeFwd, AX>(a, st);
   });
   return rc;
 }
 
-template <typename T>
+template <typename T, bool AX>
 int heads_bwd(const HeadArgs& a, int D, void* ws, size_t ws_bytes, void* dw0, void* dw1,
               cudaStream_t st) {
   int rc = BLOTH_ERR_SHAPE;
   dispatch_head_dim(D, [&](auto dd) {
     constexpr int DD = decltype(dd)::value;
-    rc = launch_head_bwd<T, DD>(a, ws, ws_bytes, dw0, dw1, st);
+    rc = launch_head_bwd<T, DD, AX>(a, ws, ws_bytes, dw0, dw1, st);
   });
   return rc;
 }
 
-template <typename T>
+template <typename T, bool AX>
 size_t heads_bwd_workspace(int64_t ntok, int D) {
   using AccT = typename AccOf<T>::type;
   size_t bytes = 0;
@@ -187,7 +187,7 @@ size_t heads_bwd_workspace(int64_t ntok, int D) {
     // the head kernel's grid, or the most CTAs the token-block kernel (which
     // takes contiguous tensors; its grid depends on the head counts, which the
     // query does not know) can launch
-    int64_t g = head_pipe_grid<T, DD, kHeadNormBwd>(ntok);
+    int64_t g = head_pipe_grid<T, DD, kHeadNormBwd, AX>(ntok);
     if (ntok > 0) {
       const int64_t gt = qk_tok_bwd_max_grid<T, DD>();
       if (gt > g) g = gt;
@@ -199,10 +199,11 @@ size_t heads_bwd_workspace(int64_t ntok, int D) {
 
 }  // namespace bloth
 
-#define BLOTH_INSTANTIATE_HEADS(T)                                              \
-  namespace bloth {                                                             \
-  template int heads_fwd<T>(const HeadArgs&, int, bool, cudaStream_t);          \
-  template int heads_bwd<T>(const HeadArgs&, int, void*, size_t, void*, void*,  \
-                            cudaStream_t);                                      \
-  template size_t heads_bwd_workspace<T>(int64_t, int);                         \
+#define BLOTH_INSTANTIATE_HEADS_AX(T, AX)                                           \
+  namespace bloth {                                                                 \
+  template int heads_fwd<T, AX>(const HeadArgs&, int, bool, cudaStream_t);          \
+  template int heads_bwd<T, AX>(const HeadArgs&, int, void*, size_t, void*, void*,  \
+                                cudaStream_t);                                      \
+  template size_t heads_bwd_workspace<T, AX>(int64_t, int);                         \
   }
+#define BLOTH_INSTANTIATE_HEADS(T) BLOTH_INSTANTIATE_HEADS_AX(T, false)

@@ -286,7 +286,7 @@ __device__ __forceinline__ void fold_warp_acc(
     }
 }
 
-template <typename T, int D, int MODE>
+template <typename T, int D, int MODE, bool AX = false>
 __global__ void __launch_bounds__(HP<T, D, MODE>::WPB * 32, 1)
     head_pipe_kernel(const HeadArgs a) {
   using G = HG<T, D>;
@@ -314,7 +314,16 @@ __global__ void __launch_bounds__(HP<T, D, MODE>::WPB * 32, 1)
 #pragma unroll
   for (int q = 0; q < G::APL; ++q)
     invf[q] = a.inv_freq ? __ldg(a.inv_freq + lane * G::APL + q) : 0.f;
-
+  // positions a token needs in this lane: one, or one per angle (AX), each
+  // `axis` elements after the token's first
+  constexpr int NPOS = AX ? G::APL : 1;
+  int64_t axis[NPOS];
+#pragma unroll
+  for (int q = 0; q < NPOS; ++q) axis[q] = AX ? axis_of(a, lane * G::APL + q) * a.pos_sa : 0;
+  auto load_pos = [&](int64_t (&p)[NPOS], int b, int s) {
+#pragma unroll
+    for (int q = 0; q < NPOS; ++q) p[q] = token_pos<T, D>(a, b, s, axis[q]);
+  };
 
   const int C[2] = {(a.H[0] + P::R - 1) / P::R, (a.H[1] + P::R - 1) / P::R};
   // token counts fit in 32 bits (the host rejects B*S >= 2^31)
@@ -428,7 +437,7 @@ __global__ void __launch_bounds__(HP<T, D, MODE>::WPB * 32, 1)
     for (int e = 0; e < G::VEC; ++e) acc[j][e] = AccT(0);
   AccT* redq = reinterpret_cast<AccT*>(smem + P::REDQ) + warp * D;  // backward only
   int cur_ten = -1;
-  int64_t pos_next = 0;
+  int64_t pos_next[NPOS] = {};
   const float sgn = a.transpose ? -1.f : 1.f;
   int csl = 0;
   uint32_t cph = 0;
@@ -451,14 +460,16 @@ __global__ void __launch_bounds__(HP<T, D, MODE>::WPB * 32, 1)
       }
       cur_ten = ten;
       lane_weights<T, D, NORM>(wsm, ten, li, wc);
-      pos_next = token_pos<T, D>(a, cc.b, cc.s);
+      load_pos(pos_next, cc.b, cc.s);
     }
     if (!BWD && cur_ten < 0) {
       cur_ten = 0;
-      pos_next = token_pos<T, D>(a, cc.b, cc.s);
+      load_pos(pos_next, cc.b, cc.s);
     }
     if (cc.j == 0) {  // token start: cos/sin, and the next token's position
-      const int64_t p = pos_next;
+      int64_t p[NPOS];
+#pragma unroll
+      for (int q = 0; q < NPOS; ++q) p[q] = pos_next[q];
       if (cc.ti + 1 < my_tok) {
         int s2 = cc.s + W, b2 = cc.b;
         if (s2 >= S) {
@@ -466,9 +477,9 @@ __global__ void __launch_bounds__(HP<T, D, MODE>::WPB * 32, 1)
           b2 += q;
           s2 -= q * S;
         }
-        pos_next = token_pos<T, D>(a, b2, s2);
+        load_pos(pos_next, b2, s2);
       }
-      token_cos_sin<T, D>(a, cc.b, p, lane, pg, invf, cs, sn);
+      token_cos_sin<T, D, AX>(a, cc.b, p, lane, pg, invf, cs, sn);
       if constexpr (MODE == kHeadRopeFwd) {
 #pragma unroll
         for (int e = 0; e < G::VEC; ++e) sn[e] *= sgn;

@@ -194,11 +194,12 @@ __global__ void __launch_bounds__(128, BWD ? 3 : 4)
   // the thread's angles: pair ai of block tokens aj + m * (128 / HALF)
   const int ai = tid % HALF, aj = tid / HALF;
   const float inv_f = __ldg(a.inv_freq + ai);
+  const int64_t axis = axis_of(a, ai) * a.pos_sa;  // 0 with one position per token
   auto pos_of = [&](int t) -> int64_t {
     const int bb = (int)pl.s_div.div((uint32_t)t);
     const int ss = t - bb * S;
     if (a.pos == nullptr) return ss;
-    const int64_t o = (int64_t)bb * a.pos_sb + (int64_t)ss * a.pos_ss;
+    const int64_t o = (int64_t)bb * a.pos_sb + (int64_t)ss * a.pos_ss + axis;
     if (a.pos_dt == BLOTH_I64) return __ldg(reinterpret_cast<const long long*>(a.pos) + o);
     return __ldg(reinterpret_cast<const int*>(a.pos) + o);
   };

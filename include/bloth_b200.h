@@ -265,6 +265,42 @@ int bloth_rope(const void* q, const int64_t* q_strides, void* q_out, const int64
                int cs_dtype, float rope_scale, int64_t B, int64_t S, int64_t Hq, int64_t Hk,
                int64_t D, int transpose, int dtype, void* stream);
 /* ------------------------------------------------------------------------
+ * Positions of several axes (time, height, width of images and video): as
+ * bloth_qk_norm_rope_fwd / _bwd and bloth_rope with inv_freq, but each token
+ * has n_axes (1 to 4) positions, axis x of token (b, s) at pos +
+ * x*pos_strides[0] + b*pos_strides[1] + s*pos_strides[2], and pair i of a head
+ * (elements i and i + D/2) is rotated by float(position of axis axis_of[i]) *
+ * inv_freq[i]. axis_of: [D/2] axis numbers in HOST memory, read during the
+ * call; pos is required. Everything else is as above. The reference rotates
+ * by one position per token.
+ * ---------------------------------------------------------------------- */
+int bloth_qk_norm_mrope_fwd(const void* q, const int64_t* q_strides, const void* k,
+                            const int64_t* k_strides, const void* wq, const void* wk,
+                            float w_offset, void* q_out, const int64_t* qo_strides, void* k_out,
+                            const int64_t* ko_strides, float* rstd_q, float* rstd_k,
+                            const void* pos, const int64_t* pos_strides, int pos_dtype, int n_axes,
+                            const unsigned char* axis_of, const float* inv_freq, float rope_scale,
+                            int64_t B, int64_t S, int64_t Hq, int64_t Hk, int64_t D, float eps,
+                            int dtype, int w_dtype, void* stream);
+size_t bloth_qk_norm_mrope_bwd_workspace_bytes(int64_t B, int64_t S, int64_t D, int dtype);
+int bloth_qk_norm_mrope_bwd(const void* dq_out, const int64_t* dqo_strides, const void* dk_out,
+                            const int64_t* dko_strides, const void* q, const int64_t* q_strides,
+                            const void* k, const int64_t* k_strides, const void* wq,
+                            const void* wk, float w_offset, const float* rstd_q,
+                            const float* rstd_k, void* dq, const int64_t* dq_strides, void* dk,
+                            const int64_t* dk_strides, void* dwq, void* dwk, const void* pos,
+                            const int64_t* pos_strides, int pos_dtype, int n_axes,
+                            const unsigned char* axis_of, const float* inv_freq, float rope_scale,
+                            int64_t B, int64_t S, int64_t Hq, int64_t Hk, int64_t D, int dtype,
+                            int w_dtype, void* workspace, size_t workspace_bytes, void* stream);
+int bloth_mrope(const void* q, const int64_t* q_strides, void* q_out, const int64_t* qo_strides,
+                const void* k, const int64_t* k_strides, void* k_out, const int64_t* ko_strides,
+                const void* pos, const int64_t* pos_strides, int pos_dtype, int n_axes,
+                const unsigned char* axis_of, const float* inv_freq, float rope_scale, int64_t B,
+                int64_t S, int64_t Hq, int64_t Hk, int64_t D, int transpose, int dtype,
+                void* stream);
+
+/* ------------------------------------------------------------------------
  * Attention over head tensors: out = softmax(scale * q k^T) v per query row
  * over the keys it sees, and its backward, which recomputes the probabilities
  * from lse. q, out, dout, dq: [B, Sq, Hq, D]; k, v, dk, dv: [B, Sk, Hk, D]
