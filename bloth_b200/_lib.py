@@ -13,6 +13,7 @@ import os
 import threading
 from collections import OrderedDict
 from contextlib import contextmanager
+from functools import lru_cache
 
 import torch
 
@@ -152,16 +153,30 @@ def require_cuda(*tensors: torch.Tensor) -> None:
             assert t.is_cuda, "[Bloth] CUDA GPU required"
 
 
-def ptr(t: torch.Tensor | None):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+def ptr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+@lru_cache(maxsize=4096)
+def _stride_array(vals: tuple) -> ctypes.Array:
+    return (ctypes.c_int64 * len(vals))(*vals)
 
 
 def strides(vals) -> ctypes.Array:
-    return (ctypes.c_int64 * len(vals))(*[int(v) for v in vals])
+    """The C ABI's stride array of these values (read-only there, and shared
+    between calls with the same values)."""
+    return _stride_array(tuple(vals))
 
 
-def stream_of(t: torch.Tensor) -> ctypes.c_void_p:
-    return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+# The raw handle of a device's current stream; torch.cuda.current_stream()
+# builds a Stream object around the same handle for 2 us a call.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def stream_of(t: torch.Tensor) -> int:
+    if _raw_stream is not None:
+        return _raw_stream(t.device.index)
+    return torch.cuda.current_stream(t.device).cuda_stream
 
 
 _WS_CACHE_MAX = 4096
@@ -298,10 +313,11 @@ def _after_call(name: str, rc: int) -> int:
 def call(name: str, t: torch.Tensor, *args) -> int:
     """Calls entry point `name` with `t`'s device current (the C ABI launches
     on the calling thread's current device)."""
-    fn = getattr(load(), name)
+    fn = getattr(_lib or load(), name)
     if t.device.index != torch.cuda.current_device():
         with torch.cuda.device(t.device):
             return call(name, t, *args)
     if _timer is None:
-        return _after_call(name, fn(*args))
+        rc = fn(*args)
+        return _after_call(name, rc) if _CHECK_FAULTS else rc
     return _after_call(name, _timer.wrap(name, t, lambda: fn(*args)))

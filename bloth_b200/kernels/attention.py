@@ -17,10 +17,14 @@ from .. import _lib
 from .fused_norm_qkv_rope import _head_strides, _heads
 
 
+_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
 def _addressable(t):
     """_heads, with tensors that repeat a row of memory written out (a tensor
     map cannot describe a stride of 0)."""
-    if t is not None and any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+    st = t.stride()
+    if 0 in st and any(n > 1 and s == 0 for n, s in zip(t.shape, st)):
         t = t.contiguous()
     return _heads(t)
 
@@ -39,30 +43,34 @@ def _sequence_arg(x, n: int, device, name: str):
     return x.contiguous()
 
 
-def _sequences(q4, k4, q_lens, k_lens, cu_q, cu_k):
+def _sequences(q, k, q_lens, k_lens, cu_q, cu_k):
     """(q_seq, k_seq, packed) of the C ABI."""
+    device = q.device
+    batch = q.shape[0] if q.dim() == 4 else 1
     if cu_q is not None or cu_k is not None:
         if q_lens is not None or k_lens is not None:
             raise ValueError("[Bloth] give lengths (q_lens, k_lens) or offsets (cu_seqlens), "
                              "not both")
         if cu_q is None:
             raise ValueError("[Bloth] cu_seqlens_k needs cu_seqlens")
-        if q4.shape[0] != 1:
+        if batch != 1:
             raise ValueError("[Bloth] packed sequences take [T, H, D] or [1, T, H, D] tensors")
-        cu_q = _sequence_arg(cu_q, None, q4.device, "cu_seqlens")
+        cu_q = _sequence_arg(cu_q, None, device, "cu_seqlens")
         if cu_q.numel() < 2:
             raise ValueError("[Bloth] cu_seqlens needs at least two offsets")
         if cu_k is None:
-            if k4.shape[1] != q4.shape[1]:
+            if k.shape[-3] != q.shape[-3]:
                 raise ValueError("[Bloth] q and k differ in length: give cu_seqlens_k too")
             cu_k = cu_q
         else:
-            cu_k = _sequence_arg(cu_k, cu_q.numel(), q4.device, "cu_seqlens_k")
+            cu_k = _sequence_arg(cu_k, cu_q.numel(), device, "cu_seqlens_k")
         if cu_k.dtype != cu_q.dtype:
             cu_k = cu_k.to(cu_q.dtype)
         return cu_q, cu_k, cu_q.numel() - 1
-    q_lens = _sequence_arg(q_lens, q4.shape[0], q4.device, "q_lens")
-    k_lens = _sequence_arg(k_lens, q4.shape[0], q4.device, "k_lens")
+    if q_lens is None and k_lens is None:
+        return None, None, 0
+    q_lens = _sequence_arg(q_lens, batch, device, "q_lens")
+    k_lens = _sequence_arg(k_lens, batch, device, "k_lens")
     if q_lens is not None and k_lens is not None and q_lens.dtype != k_lens.dtype:
         q_lens, k_lens = q_lens.long(), k_lens.long()
     return q_lens, k_lens, 0
@@ -121,31 +129,28 @@ def attention_backward(do4, q4, k4, v4, out, lse, q_seq, k_seq, packed, scale, c
 class _AttentionFunction(torch.autograd.Function):
 
     @staticmethod
-    def forward(ctx, q, k, v, q_seq, k_seq, packed, scale, causal, window, want_lse):
-        q4, k4, v4 = (_addressable(t) for t in (q, k, v))
-        need = any(ctx.needs_input_grad[:3])
-        out, lse = attention_forward(q4, k4, v4, q_seq, k_seq, packed, scale, causal, window,
-                                     need or want_lse)
-        if need:
-            ctx.save_for_backward(q4, k4, v4, out, lse, q_seq, k_seq)
-            ctx.meta = (packed, scale, causal, window, q.shape, k.shape, v.shape)
-        y = out.view(q.shape)
-        if not want_lse:
-            return y
-        rows = lse[0] if q.dim() == 3 else lse
-        ctx.mark_non_differentiable(rows)
-        return y, rows
+    def forward(ctx, q, k, v, q_seq, k_seq, packed, scale, causal, window):
+        q4, k4, v4 = _addressable(q), _addressable(k), _addressable(v)
+        out, lse = attention_forward(q4, k4, v4, q_seq, k_seq, packed, scale, causal, window)
+        ctx.save_for_backward(q4, k4, v4, out, lse, q_seq, k_seq)
+        ctx.meta = (packed, scale, causal, window, q.dim() == 3)
+        ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
+        return (out[0] if q.dim() == 3 else out), lse
 
     @staticmethod
-    def backward(ctx, dout, *_):
+    def backward(ctx, dout, _):
+        if dout is None:
+            return (None,) * 9
         q4, k4, v4, out, lse, q_seq, k_seq = ctx.saved_tensors
-        packed, scale, causal, window, shape_q, shape_k, shape_v = ctx.meta
+        packed, scale, causal, window, flat = ctx.meta
         want_q, want_k, want_v = ctx.needs_input_grad[:3]
-        dq, dk, dv = attention_backward(_addressable(dout.view(q4.shape)), q4, k4, v4, out, lse,
-                                        q_seq, k_seq, packed, scale, causal, window, want_q,
-                                        want_k or want_v)
-        return (dq.view(shape_q) if want_q else None, dk.view(shape_k) if want_k else None,
-                dv.view(shape_v) if want_v else None, None, None, None, None, None, None, None)
+        grads = attention_backward(_addressable(dout), q4, k4, v4, out, lse, q_seq, k_seq, packed,
+                                   scale, causal, window, want_q, want_k or want_v)
+        if flat:
+            grads = [None if g is None else g[0] for g in grads]
+        dq, dk, dv = grads
+        return dq, dk if want_k else None, dv if want_v else None, None, None, None, None, None, None
 
 
 def fused_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = True,
@@ -176,30 +181,40 @@ def fused_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: b
     for rows that see nothing, without a gradient.
     """
     _lib.require_cuda(q, k, v, q_lens, k_lens, cu_seqlens, cu_seqlens_k)
-    if not (q.dim() == k.dim() == v.dim()) or q.dim() not in (3, 4):
+    shape, shape_k, dtype = q.shape, k.shape, q.dtype
+    dim = len(shape)
+    if dim not in (3, 4) or len(shape_k) != dim or v.dim() != dim:
         raise ValueError("[Bloth] q, k and v must be [B, S, H, D] or [S, H, D]")
-    if not (q.dtype == k.dtype == v.dtype):
-        raise TypeError(f"[Bloth] q, k and v differ in dtype: {q.dtype}, {k.dtype}, {v.dtype}")
-    if q.dtype not in (torch.float32, torch.bfloat16, torch.float16):
-        raise TypeError(f"[Bloth] unsupported dtype {q.dtype}")
-    if not (q.device == k.device == v.device):
+    if k.dtype != dtype or v.dtype != dtype:
+        raise TypeError(f"[Bloth] q, k and v differ in dtype: {dtype}, {k.dtype}, {v.dtype}")
+    if dtype not in _DTYPES:
+        raise TypeError(f"[Bloth] unsupported dtype {dtype}")
+    if k.device != q.device or v.device != q.device:
         raise ValueError("[Bloth] q, k and v must be on one device")
-    if k.shape != v.shape or q.shape[-1] != k.shape[-1] or \
-            (q.dim() == 4 and q.shape[0] != k.shape[0]):
-        raise ValueError(f"[Bloth] shapes do not match: q {tuple(q.shape)}, k {tuple(k.shape)}, "
+    Hq, D = shape[-2:]
+    Hk = shape_k[-2]
+    if v.shape != shape_k or shape_k[-1] != D or (dim == 4 and shape_k[0] != shape[0]):
+        raise ValueError(f"[Bloth] shapes do not match: q {tuple(shape)}, k {tuple(shape_k)}, "
                          f"v {tuple(v.shape)}")
-    if q.shape[-1] not in (64, 128, 256):
-        raise ValueError(f"[Bloth] head_dim {q.shape[-1]} is not one of 64, 128, 256")
-    if k.shape[-2] == 0 or q.shape[-2] % k.shape[-2] or q.shape[-2] == 0:
-        raise ValueError(f"[Bloth] {q.shape[-2]} query heads over {k.shape[-2]} key heads")
+    if D not in (64, 128, 256):
+        raise ValueError(f"[Bloth] head_dim {D} is not one of 64, 128, 256")
+    if Hk == 0 or Hq == 0 or Hq % Hk:
+        raise ValueError(f"[Bloth] {Hq} query heads over {Hk} key heads")
     if scale is None:
-        scale = 1.0 / math.sqrt(q.shape[-1])
-    if not 0.0 < scale < math.inf:
+        scale = 1.0 / math.sqrt(D)
+    elif not 0.0 < scale < math.inf:
         raise ValueError(f"[Bloth] scale must be positive and finite, got {scale}")
     if window is not None and (not causal or window < 1):
         raise ValueError("[Bloth] window must be at least 1, and needs causal=True")
-    q4 = q if q.dim() == 4 else q.unsqueeze(0)
-    k4 = k if k.dim() == 4 else k.unsqueeze(0)
-    q_seq, k_seq, packed = _sequences(q4, k4, q_lens, k_lens, cu_seqlens, cu_seqlens_k)
-    return _AttentionFunction.apply(q, k, v, q_seq, k_seq, packed, float(scale), bool(causal),
-                                    int(window or 0), bool(return_lse))
+    q_seq, k_seq, packed = _sequences(q, k, q_lens, k_lens, cu_seqlens, cu_seqlens_k)
+    how = (q_seq, k_seq, packed, float(scale), bool(causal), int(window or 0))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        out, lse = _AttentionFunction.apply(q, k, v, *how)
+    else:
+        out, lse = attention_forward(_addressable(q), _addressable(k), _addressable(v), *how,
+                                     want_lse=return_lse)
+        if dim == 3:
+            out = out[0]
+    if not return_lse:
+        return out
+    return out, lse[0] if dim == 3 else lse

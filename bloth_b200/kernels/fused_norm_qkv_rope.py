@@ -94,10 +94,6 @@ def fused_norm_rope(x: torch.Tensor, weight: torch.Tensor, cos: torch.Tensor,
 
 
 # ------------------------------------------------ per-head q/k (positions)
-def _vec(dtype: torch.dtype) -> int:
-    return 16 // torch.tensor([], dtype=dtype).element_size()
-
-
 def _heads(t: torch.Tensor | None):
     """[B, S, H, D] view (3-D [S, H, D] gets B = 1) whose last dim is
     contiguous, 16-byte aligned and with strides the kernel can address."""
@@ -107,8 +103,9 @@ def _heads(t: torch.Tensor | None):
         t = t.unsqueeze(0)
     if t.dim() != 4:
         raise ValueError("[Bloth] head tensors must be [B, S, H, D] or [S, H, D]")
-    v = _vec(t.dtype)
-    if (t.stride(3) != 1 or t.data_ptr() % 16 or any(s % v for s in t.stride()[:3])):
+    v = 16 // t.element_size()
+    sb, ss, sh, sd = t.stride()
+    if sd != 1 or t.data_ptr() % 16 or sb % v or ss % v or sh % v:
         t = _lib.aligned16(t.contiguous())
     return t
 

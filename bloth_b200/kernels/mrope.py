@@ -74,7 +74,8 @@ def _source(x4, position_ids, inv_freq, axes):
     if position_ids is None or inv_freq is None:
         raise ValueError("[Bloth] position_ids and inv_freq are required")
     pos, pos_st = _axis_positions(position_ids, B, S)
-    inv_freq = inv_freq.to(torch.float32).contiguous()
+    if inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous():
+        inv_freq = inv_freq.to(torch.float32).contiguous()
     if inv_freq.numel() != D // 2:
         raise ValueError(f"[Bloth] inv_freq must have head_dim/2 = {D // 2} elements")
     return pos, pos_st, _axes_array(tuple(axes), D // 2, pos.shape[0]), inv_freq
@@ -87,43 +88,58 @@ def _check_pair(q4, k4):
         raise TypeError(f"[Bloth] q and k differ in dtype: {q4.dtype}, {k4.dtype}")
 
 
+def _needs_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _weight(w, D: int, dtype):
+    if w.numel() != D or w.dtype != dtype:
+        raise ValueError(f"[Bloth] wq and wk must have head_dim = {D} elements of one dtype")
+    return _lib.aligned16(w.contiguous())
+
+
+def _norm_mrope_call(q, k, wq, wk, position_ids, inv_freq, axes, eps, weight_offset, rope_scale):
+    """Forward: (q_out, k_out, what the backward needs)."""
+    q4, k4 = _heads(q), _heads(k)
+    _check_pair(q4, k4)
+    B, S, Hq, D = q4.shape
+    Hk = 0 if k4 is None else k4.shape[2]
+    pos, pos_st, ax, inv_freq = _source(q4, position_ids, inv_freq, axes)
+    if k4 is not None and wk is None:
+        raise ValueError("[Bloth] wk is required with k")
+    wk = None if wk is None else _weight(wk, D, wq.dtype)
+    wq = _weight(wq, D, wq.dtype)
+    qo = torch.empty((B, S, Hq, D), dtype=q4.dtype, device=q4.device)
+    ko = None if k4 is None else torch.empty((B, S, Hk, D), dtype=k4.dtype, device=k4.device)
+    rq = torch.empty((B, S, Hq), dtype=torch.float32, device=q4.device)
+    rk = None if k4 is None else torch.empty((B, S, Hk), dtype=torch.float32, device=q4.device)
+    rc = _lib.call(
+        "bloth_qk_norm_mrope_fwd", q4, _lib.ptr(q4), _head_strides(q4), _lib.ptr(k4),
+        _head_strides(k4), _lib.ptr(wq), _lib.ptr(wk), weight_offset, _lib.ptr(qo),
+        _head_strides(qo), _lib.ptr(ko), _head_strides(ko), _lib.ptr(rq), _lib.ptr(rk),
+        _lib.ptr(pos), pos_st, _lib.dtype_code(pos.dtype), pos.shape[0], ax, _lib.ptr(inv_freq),
+        rope_scale, B, S, Hq, Hk, D, eps, _lib.dtype_code(q4.dtype), _lib.dtype_code(wq.dtype),
+        _lib.stream_of(q4))
+    _lib.check(rc, "qk norm+mrope forward")
+    saved = (q4, k4, wq, wk, rq, rk, pos, inv_freq), (pos_st, ax, q.dim() == 3, weight_offset,
+                                                      rope_scale)
+    if q.dim() == 3:
+        qo, ko = qo[0], None if ko is None else ko[0]
+    return qo, ko, saved
+
+
 class _QKNormMRoPEFunction(torch.autograd.Function):
 
     @staticmethod
-    def forward(ctx, q, k, wq, wk, position_ids, inv_freq, axes, eps, weight_offset, rope_scale):
-        q4, k4 = _heads(q), _heads(k)
-        _check_pair(q4, k4)
-        B, S, Hq, D = q4.shape
-        Hk = 0 if k4 is None else k4.shape[2]
-        pos, pos_st, ax, inv_freq = _source(q4, position_ids, inv_freq, axes)
-        wq = _lib.aligned16(wq.contiguous())
-        wk = None if wk is None else _lib.aligned16(wk.contiguous())
-        if k4 is not None and wk is None:
-            raise ValueError("[Bloth] wk is required with k")
-        for w in (wq, wk):
-            if w is not None and (w.numel() != D or w.dtype != wq.dtype):
-                raise ValueError(f"[Bloth] wq and wk must have head_dim = {D} elements of one "
-                                 "dtype")
-        qo = torch.empty((B, S, Hq, D), dtype=q4.dtype, device=q4.device)
-        ko = None if k4 is None else torch.empty((B, S, Hk, D), dtype=k4.dtype, device=k4.device)
-        rq = torch.empty((B, S, Hq), dtype=torch.float32, device=q4.device)
-        rk = None if k4 is None else torch.empty((B, S, Hk), dtype=torch.float32, device=q4.device)
-        rc = _lib.call(
-            "bloth_qk_norm_mrope_fwd", q4, _lib.ptr(q4), _head_strides(q4), _lib.ptr(k4),
-            _head_strides(k4), _lib.ptr(wq), _lib.ptr(wk), weight_offset, _lib.ptr(qo),
-            _head_strides(qo), _lib.ptr(ko), _head_strides(ko), _lib.ptr(rq), _lib.ptr(rk),
-            _lib.ptr(pos), pos_st, _lib.dtype_code(pos.dtype), pos.shape[0], ax,
-            _lib.ptr(inv_freq), rope_scale, B, S, Hq, Hk, D, eps, _lib.dtype_code(q4.dtype),
-            _lib.dtype_code(wq.dtype), _lib.stream_of(q4))
-        _lib.check(rc, "qk norm+mrope forward")
-        ctx.save_for_backward(q4, k4, wq, wk, rq, rk, pos, inv_freq)
-        ctx.meta = (pos_st, ax, q.shape, None if k is None else k.shape, weight_offset, rope_scale)
-        return qo.view(q.shape) if k4 is None else (qo.view(q.shape), ko.view(k.shape))
+    def forward(ctx, *args):
+        qo, ko, (tensors, ctx.meta) = _norm_mrope_call(*args)
+        ctx.save_for_backward(*tensors)
+        return qo if ko is None else (qo, ko)
 
     @staticmethod
     def backward(ctx, *grads):
         q4, k4, wq, wk, rq, rk, pos, inv_freq = ctx.saved_tensors
-        pos_st, ax, shape_q, shape_k, weight_offset, rope_scale = ctx.meta
+        pos_st, ax, flat, weight_offset, rope_scale = ctx.meta
         B, S, Hq, D = q4.shape
         Hk = 0 if k4 is None else k4.shape[2]
         gq = _heads(grads[0])
@@ -145,8 +161,9 @@ class _QKNormMRoPEFunction(torch.autograd.Function):
             _lib.ptr(inv_freq), rope_scale, B, S, Hq, Hk, D, code, _lib.dtype_code(wq.dtype),
             _lib.ptr(ws), n, _lib.stream_of(q4))
         _lib.check(rc, "qk norm+mrope backward")
-        return (dq.view(shape_q), None if dk is None else dk.view(shape_k), dwq, dwk, None, None,
-                None, None, None, None)
+        if flat:
+            dq, dk = dq[0], None if dk is None else dk[0]
+        return dq, dk, dwq, dwk, None, None, None, None, None, None
 
 
 def _mrope_launch(q4, qo, k4, ko, pos, pos_st, ax, inv_freq, scale, transpose):
@@ -160,29 +177,39 @@ def _mrope_launch(q4, qo, k4, ko, pos, pos_st, ax, inv_freq, scale, transpose):
     _lib.check(rc, "mrope")
 
 
+def _mrope_call(q, k, position_ids, inv_freq, axes, scale):
+    """Forward: (q_out, k_out, what the backward needs)."""
+    q4, k4 = _heads(q), _heads(k)
+    _check_pair(q4, k4)
+    pos, pos_st, ax, inv_freq = _source(q4, position_ids, inv_freq, axes)
+    qo = _out_like(q4)
+    ko = None if k4 is None else _out_like(k4)
+    _mrope_launch(q4, qo, k4, ko, pos, pos_st, ax, inv_freq, scale, False)
+    saved = (pos, inv_freq), (pos_st, ax, scale, q.dim() == 3, k4 is not None)
+    if q.dim() == 3:
+        qo, ko = qo[0], None if ko is None else ko[0]
+    return qo, ko, saved
+
+
 class _MRoPEFunction(torch.autograd.Function):
 
     @staticmethod
-    def forward(ctx, q, k, position_ids, inv_freq, axes, scale):
-        q4, k4 = _heads(q), _heads(k)
-        _check_pair(q4, k4)
-        pos, pos_st, ax, inv_freq = _source(q4, position_ids, inv_freq, axes)
-        qo = _out_like(q4)
-        ko = None if k4 is None else _out_like(k4)
-        _mrope_launch(q4, qo, k4, ko, pos, pos_st, ax, inv_freq, scale, False)
-        ctx.save_for_backward(pos, inv_freq)
-        ctx.meta = (pos_st, ax, scale, q.shape, None if k is None else k.shape)
-        return qo.view(q.shape) if k4 is None else (qo.view(q.shape), ko.view(k.shape))
+    def forward(ctx, *args):
+        qo, ko, (tensors, ctx.meta) = _mrope_call(*args)
+        ctx.save_for_backward(*tensors)
+        return qo if ko is None else (qo, ko)
 
     @staticmethod
     def backward(ctx, *grads):
         pos, inv_freq = ctx.saved_tensors
-        pos_st, ax, scale, shape_q, shape_k = ctx.meta
+        pos_st, ax, scale, flat, has_k = ctx.meta
         gq = _heads(grads[0])
-        gk = None if shape_k is None else _heads(grads[1])
+        gk = _heads(grads[1]) if has_k else None
         dq, dk = _out_like(gq), None if gk is None else _out_like(gk)
         _mrope_launch(gq, dq, gk, dk, pos, pos_st, ax, inv_freq, scale, True)
-        return dq.view(shape_q), None if dk is None else dk.view(shape_k), None, None, None, None
+        if flat:
+            dq, dk = dq[0], None if dk is None else dk[0]
+        return dq, dk, None, None, None, None
 
 
 def fused_qk_norm_mrope(q: torch.Tensor, k: torch.Tensor | None, wq: torch.Tensor,
@@ -199,8 +226,12 @@ def fused_qk_norm_mrope(q: torch.Tensor, k: torch.Tensor | None, wq: torch.Tenso
     ``weight_offset``, ``rope_scale``, k may be None. Returns (q_out, k_out),
     or q_out alone."""
     _lib.require_cuda(q, k, wq, wk, position_ids, inv_freq)
-    return _QKNormMRoPEFunction.apply(q, k, wq, wk, position_ids, inv_freq, tuple(axes),
-                                      float(eps), float(weight_offset), float(rope_scale))
+    args = (q, k, wq, wk, position_ids, inv_freq, axes, float(eps), float(weight_offset),
+            float(rope_scale))
+    if _needs_grad(q, k, wq, wk):
+        return _QKNormMRoPEFunction.apply(*args)
+    qo, ko, _ = _norm_mrope_call(*args)
+    return qo if ko is None else (qo, ko)
 
 
 def apply_mrope_qk(q: torch.Tensor, k: torch.Tensor | None, position_ids: torch.Tensor,
@@ -209,4 +240,8 @@ def apply_mrope_qk(q: torch.Tensor, k: torch.Tensor | None, position_ids: torch.
     None) by positions of several axes, in one launch; see
     :func:`fused_qk_norm_mrope`."""
     _lib.require_cuda(q, k, position_ids, inv_freq)
-    return _MRoPEFunction.apply(q, k, position_ids, inv_freq, tuple(axes), float(rope_scale))
+    args = (q, k, position_ids, inv_freq, axes, float(rope_scale))
+    if _needs_grad(q, k):
+        return _MRoPEFunction.apply(*args)
+    qo, ko, _ = _mrope_call(*args)
+    return qo if ko is None else (qo, ko)
