@@ -83,6 +83,8 @@ extern "C" {
 size_t bloth_attention_fwd_workspace_bytes(int64_t B, int64_t Sq, int64_t Sk, int64_t Hq,
                                            int64_t Hk, int64_t D, int64_t packed, int dtype) {
   if (check_sizes(B, Sq, Sk, Hq, Hk, D, packed, dtype)) return 0;
+  if (dtype != BLOTH_F32 && attn_rows_take(Sq, Hq / Hk, D, packed))
+    return attn_rows_workspace(B, Sq, Sk, Hk, Hq / Hk, D);
   return 0;
 }
 
@@ -108,11 +110,14 @@ int bloth_attention_fwd(const void* q, const int64_t* q_strides, const void* k,
   }
   if ((rc = fill(a.o, out, out_strides, dtype))) return rc;
   a.lse = lse;
-  (void)workspace;
-  (void)workspace_bytes;
+  const size_t need = bloth_attention_fwd_workspace_bytes(B, Sq, Sk, Hq, Hk, D, packed, dtype);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return BLOTH_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return BLOTH_ERR_ALIGN;
   return by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     if constexpr (sizeof(T) == 2) {
+      if (Sk > 0 && attn_rows_take(Sq, Hq / Hk, D, packed))
+        return attn_rows_fwd<T>(a, (int)D, workspace, as_stream(stream));
       if (D <= 128 && Sk > 0) return attn_tc_fwd<T>(a, (int)D, as_stream(stream));
     }
     return attn_simt_fwd<T>(a, (int)D, as_stream(stream));

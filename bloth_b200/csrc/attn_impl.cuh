@@ -171,6 +171,11 @@ template <typename T>
 int attn_tc_fwd(const AttnArgs& a, int D, cudaStream_t st);
 template <typename T>
 int attn_tc_bwd(const AttnArgs& a, int D, cudaStream_t st);
+// attn_rows_*: 16-bit dense tensors with few query rows.
+bool attn_rows_take(int64_t Sq, int64_t G, int64_t D, int64_t packed);
+size_t attn_rows_workspace(int64_t B, int64_t Sq, int64_t Sk, int64_t Hk, int64_t G, int64_t D);
+template <typename T>
+int attn_rows_fwd(const AttnArgs& a, int D, void* ws, cudaStream_t st);
 template <typename T>
 int attn_simt_fwd(const AttnArgs& a, int D, cudaStream_t st);
 template <typename T>
