@@ -34,15 +34,20 @@ struct BwdCfg {
   static constexpr int TILE = 128;
   static constexpr int THREADS = 320;
   static constexpr int OPB = TILE * D * 2;     // bytes of one operand tile
-  static constexpr int NST = D == 64 ? 4 : 2;  // stages of each streamed tensor
-  static constexpr int OWN_OFF = 0;            // the two kept tiles
-  static constexpr int A_OFF = 2 * OPB;        // stages of Q (or K)
-  static constexpr int B_OFF = A_OFF + NST * OPB;  // stages of dO (or V)
-  static constexpr int STAT_OFF = B_OFF + NST * OPB;  // lse2 and delta per stage
-  static constexpr int BAR_OFF = STAT_OFF + NST * 1024;
-  static constexpr int BARS = 1 + 4 * NST + 8;
-  static constexpr int SMEM = BAR_OFF + BARS * 8 + 16 + 1024;
+  // Stages of Q (or K) and of dO (or V). Q and K are read by a block's first
+  // and its last product, so two stages leave a copy less than a block's time;
+  // dO and V are free after half of it. D = 128, 8192 full rows of 32/8 heads:
+  // @@STAGES@@
+  static constexpr int NA = D == 64 ? 4 : 3, NB = D == 64 ? 4 : 2;
+  static constexpr int OWN_OFF = 0;                // the two kept tiles
+  static constexpr int A_OFF = 2 * OPB;            // stages of Q (or K)
+  static constexpr int B_OFF = A_OFF + NA * OPB;   // stages of dO (or V)
+  static constexpr int STAT_OFF = B_OFF + NB * OPB;  // lse2 and delta, with dO's stages
+  static constexpr int BAR_OFF = STAT_OFF + NB * 1024;
+  static constexpr int BARS = 1 + 2 * NA + 2 * NB + 8;
+  static constexpr int SMEM = BAR_OFF + BARS * 8 + 16;
   static constexpr uint32_t COLS = 512;
+  static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
 struct BwdMaps {
@@ -66,29 +71,6 @@ __device__ __forceinline__ void zero_rows(unsigned char* tile, int r0) {
         make_uint4(0, 0, 0, 0);
   }
   fence_proxy_async_smem();
-}
-
-// d (+)= A B^T: A and B operand tiles, contracted over their D columns.
-template <typename T, int D>
-__device__ __forceinline__ void product_rows(uint32_t d, uint32_t a, uint32_t b) {
-  constexpr uint32_t id = mma_desc<T>(128, 128, false);
-#pragma unroll
-  for (int kk = 0; kk < D / 16; ++kk) {
-    const uint32_t o = (kk / 4) * (128 * 128) + (kk % 4) * 32;
-    mma_ss(d, desc_k(a + o), desc_k(b + o), id, kk > 0);
-  }
-}
-// d (+)= W B: W 128 x 128 in tensor memory (16 columns of the block per 8
-// columns; columns 64.. of the block start 64 columns further), B an operand
-// tile, contracted over its 128 rows.
-template <typename T, int D>
-__device__ __forceinline__ void product_cols(uint32_t d, uint32_t w, uint32_t half, uint32_t b,
-                                             bool add) {
-  constexpr uint32_t id = mma_desc<T>(128, D, true);
-#pragma unroll
-  for (int kk = 0; kk < 8; ++kk)
-    mma_ts(d, w + (kk / 4) * half + (kk % 4) * 8, desc_mn(b + kk * 2048, 128 * 128), id,
-           add || kk > 0);
 }
 
 // 64 columns of the thread's row.
@@ -143,18 +125,16 @@ template <typename T, int D>
 __global__ void __launch_bounds__(320, 1)
     attn_dkv_kernel(const AttnArgs a, const __grid_constant__ BwdMaps maps) {
   using C = BwdCfg<D>;
-  constexpr int N = C::TILE, NST = C::NST;
+  constexpr int N = C::TILE, NA = C::NA, NB = C::NB;
   // tensor-memory columns: S^T (then P^T), dP^T (then dS^T), dV, dK
   constexpr uint32_t S_COL = 0, DP_COL = 128, DV_COL = 256, DK_COL = 256 + D;
-  extern __shared__ unsigned char smem_raw[];
-  unsigned char* smem = reinterpret_cast<unsigned char*>(
-      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  extern __shared__ __align__(1024) unsigned char smem[];
   uint64_t* own_full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
   uint64_t* q_full = own_full + 1;
-  uint64_t* q_free = q_full + NST;
-  uint64_t* o_full = q_free + NST;  // dO
-  uint64_t* o_free = o_full + NST;
-  uint64_t* s_full = o_free + NST;
+  uint64_t* q_free = q_full + NA;
+  uint64_t* o_full = q_free + NA;  // dO and the statistics
+  uint64_t* o_free = o_full + NB;
+  uint64_t* s_full = o_free + NB;
   uint64_t* p_full = s_full + 1;
   uint64_t* dp_full = p_full + 1;
   uint64_t* ds_full = dp_full + 1;
@@ -181,9 +161,11 @@ __global__ void __launch_bounds__(320, 1)
     tmem_alloc(tmem_ptr, C::COLS);
   } else if (threadIdx.x == 0) {
     mbar_init(own_full, 1);
-    for (int i = 0; i < NST; ++i) {
+    for (int i = 0; i < NA; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&q_free[i], 1);
+    }
+    for (int i = 0; i < NB; ++i) {
       mbar_init(&o_full[i], 1);
       mbar_init(&o_free[i], 1);
     }
@@ -208,29 +190,29 @@ __global__ void __launch_bounds__(320, 1)
       load_tile<D>(smem + C::OWN_OFF + C::OPB, &maps.v, s.k0 + n0, h, s.b, own_full);
       int it = 0;
       for (; it < total; ++it) {
-        const int st = it % NST;
-        const uint32_t ph = (uint32_t)(it / NST) & 1u;
+        const int sa = it % NA, sb = it % NB;
+        const uint32_t pa = (uint32_t)(it / NA) & 1u, pb = (uint32_t)(it / NB) & 1u;
         const int hq = h * a.G + it / nm, m0 = (mb + it % nm) * N;
         const int64_t stat = (int64_t)hq * a.R + s.stat0 + m0;
-        unsigned char* sp = smem + C::STAT_OFF + st * 1024;
-        if (!tc_wait(&q_free[st], ph ^ 1u, stop, a.fault)) break;
-        mbar_arrive_expect_tx(&q_full[st], C::OPB + 1024);
-        load_tile<D>(smem + C::A_OFF + st * C::OPB, &maps.q, s.q0 + m0, hq, s.b, &q_full[st]);
-        bulk_load(sp, a.lse2 + stat, 512, &q_full[st]);
-        bulk_load(sp + 512, a.delta + stat, 512, &q_full[st]);
-        if (!tc_wait(&o_free[st], ph ^ 1u, stop, a.fault)) {
-          mbar_wait(&q_full[st], ph, nullptr);
+        unsigned char* sp = smem + C::STAT_OFF + sb * 1024;
+        if (!tc_wait(&q_free[sa], pa ^ 1u, stop, a.fault)) break;
+        mbar_arrive_expect_tx(&q_full[sa], C::OPB);
+        load_tile<D>(smem + C::A_OFF + sa * C::OPB, &maps.q, s.q0 + m0, hq, s.b, &q_full[sa]);
+        if (!tc_wait(&o_free[sb], pb ^ 1u, stop, a.fault)) {
+          mbar_wait(&q_full[sa], pa, nullptr);
           break;
         }
-        mbar_arrive_expect_tx(&o_full[st], C::OPB);
-        load_tile<D>(smem + C::B_OFF + st * C::OPB, &maps.dout, s.q0 + m0, hq, s.b, &o_full[st]);
+        mbar_arrive_expect_tx(&o_full[sb], C::OPB + 1024);
+        bulk_load(sp, a.lse2 + stat, 512, &o_full[sb]);
+        bulk_load(sp + 512, a.delta + stat, 512, &o_full[sb]);
+        load_tile<D>(smem + C::B_OFF + sb * C::OPB, &maps.dout, s.q0 + m0, hq, s.b, &o_full[sb]);
       }
       if (*stop) {  // given up: not before the copies in flight have landed
         mbar_wait(own_full, 0, nullptr);
-        for (int i = max(0, it - NST); i < it; ++i) {
-          mbar_wait(&q_full[i % NST], (uint32_t)(i / NST) & 1u, nullptr);
-          mbar_wait(&o_full[i % NST], (uint32_t)(i / NST) & 1u, nullptr);
-        }
+        for (int i = max(0, it - NA); i < it; ++i)
+          mbar_wait(&q_full[i % NA], (uint32_t)(i / NA) & 1u, nullptr);
+        for (int i = max(0, it - NB); i < it; ++i)
+          mbar_wait(&o_full[i % NB], (uint32_t)(i / NB) & 1u, nullptr);
       }
     }
   } else if (warp == 8) {
@@ -248,24 +230,23 @@ __global__ void __launch_bounds__(320, 1)
         mma_commit(dp_full);
       }
       for (int it = 0; ok && it < total; ++it) {
-        const int st = it % NST, sn = (it + 1) % NST;
-        const uint32_t pn = (uint32_t)((it + 1) / NST) & 1u;
+        const int sa = it % NA, sb = it % NB, na = (it + 1) % NA, nb = (it + 1) % NB;
         if (!(ok = tc_wait(p_full, it & 1, stop, a.fault))) break;
         tc_fence_after();
-        product_cols<T, D>(tmem + DV_COL, tmem + S_COL, 64, oa + st * C::OPB, it > 0);
-        mma_commit(&o_free[st]);
+        product_cols<T, D>(tmem + DV_COL, tmem + S_COL, 64, oa + sb * C::OPB, it > 0);
         if (it + 1 < total) {
-          if (!(ok = tc_wait(&q_full[sn], pn, stop, a.fault))) break;
-          product_rows<T, D>(tmem + S_COL, ka, qa + sn * C::OPB);
+          if (!(ok = tc_wait(&q_full[na], (uint32_t)((it + 1) / NA) & 1u, stop, a.fault))) break;
+          product_rows<T, D>(tmem + S_COL, ka, qa + na * C::OPB);
           mma_commit(s_full);
         }
         if (!(ok = tc_wait(ds_full, it & 1, stop, a.fault))) break;
         tc_fence_after();
-        product_cols<T, D>(tmem + DK_COL, tmem + DP_COL, 64, qa + st * C::OPB, it > 0);
-        mma_commit(&q_free[st]);
+        product_cols<T, D>(tmem + DK_COL, tmem + DP_COL, 64, qa + sa * C::OPB, it > 0);
+        mma_commit(&q_free[sa]);
+        mma_commit(&o_free[sb]);  // not before dS: the statistics lie with dO
         if (it + 1 < total) {
-          if (!(ok = tc_wait(&o_full[sn], pn, stop, a.fault))) break;
-          product_rows<T, D>(tmem + DP_COL, va, oa + sn * C::OPB);
+          if (!(ok = tc_wait(&o_full[nb], (uint32_t)((it + 1) / NB) & 1u, stop, a.fault))) break;
+          product_rows<T, D>(tmem + DP_COL, va, oa + nb * C::OPB);
           mma_commit(dp_full);
         }
       }
@@ -280,13 +261,11 @@ __global__ void __launch_bounds__(320, 1)
     const uint32_t dp_at = tmem + lanes + DP_COL + half * 64;
     bool ok = true;
     for (int it = 0; it < total; ++it) {
-      const int st = it % NST;
-      const uint32_t sph = (uint32_t)(it / NST) & 1u;
+      const int sa = it % NA, sb = it % NB;
       const int m0 = (mb + it % nm) * N;
-      const float* stat = reinterpret_cast<const float*>(smem + C::STAT_OFF + st * 1024);
-      // the statistics come with Q, whose copy S^T has waited for; this wait
-      // makes them visible to this thread
-      ok = tc_wait(&q_full[st], sph, stop, a.fault) && tc_wait(s_full, it & 1, stop, a.fault);
+      const float* stat = reinterpret_cast<const float*>(smem + C::STAT_OFF + sb * 1024);
+      ok = tc_wait(&o_full[sb], (uint32_t)(it / NB) & 1u, stop, a.fault) &&
+           tc_wait(s_full, it & 1, stop, a.fault);
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       tc_fence_after();
       float x[64];
@@ -312,11 +291,8 @@ __global__ void __launch_bounds__(320, 1)
 #pragma unroll
         for (int i = 0; i < 64; ++i)
           if (i < from || i >= to) x[i] = 0.f;
-        if (tail) {  // rows of dO past the sequence's end that memory does hold
-          ok = __all_sync(0xffffffffu, tc_wait(&o_full[st], sph, stop, a.fault));
-          if (!ok) break;
-          zero_rows<D>(smem + C::B_OFF + st * C::OPB, s.qlen - m0);
-        }
+        // rows of dO past the sequence's end that memory does hold
+        if (tail) zero_rows<D>(smem + C::B_OFF + sb * C::OPB, s.qlen - m0);
       }
       store64<T>(s_at, x);
       tc_fence_before();
@@ -342,7 +318,7 @@ __global__ void __launch_bounds__(320, 1)
 #pragma unroll
         for (int i = 0; i < 64; ++i)
           if (i < from || i >= to) y[i] = 0.f;
-        if (tail) zero_rows<D>(smem + C::A_OFF + st * C::OPB, s.qlen - m0);
+        if (tail) zero_rows<D>(smem + C::A_OFF + sa * C::OPB, s.qlen - m0);
       }
       store64<T>(dp_at, y);
       tc_fence_before();
@@ -373,18 +349,16 @@ template <typename T, int D>
 __global__ void __launch_bounds__(320, 1)
     attn_dq_kernel(const AttnArgs a, const __grid_constant__ BwdMaps maps) {
   using C = BwdCfg<D>;
-  constexpr int N = C::TILE, NST = C::NST;
+  constexpr int N = C::TILE, NA = C::NA, NB = C::NB;
   // tensor-memory columns: S, dP, dQ, and two buffers of dS
   constexpr uint32_t S_COL = 0, DP_COL = 128, DQ_COL = 256, DS_COL = 384;
-  extern __shared__ unsigned char smem_raw[];
-  unsigned char* smem = reinterpret_cast<unsigned char*>(
-      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  extern __shared__ __align__(1024) unsigned char smem[];
   uint64_t* own_full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
   uint64_t* k_full = own_full + 1;
-  uint64_t* k_free = k_full + NST;
-  uint64_t* v_full = k_free + NST;
-  uint64_t* v_free = v_full + NST;
-  uint64_t* sdp_full = v_free + NST;
+  uint64_t* k_free = k_full + NA;
+  uint64_t* v_full = k_free + NA;
+  uint64_t* v_free = v_full + NB;
+  uint64_t* sdp_full = v_free + NB;
   uint64_t* read = sdp_full + 1;  // S and dP are in registers
   uint64_t* ds_full = read + 1;
   uint64_t* acc_full = ds_full + 1;
@@ -409,9 +383,11 @@ __global__ void __launch_bounds__(320, 1)
     tmem_alloc(tmem_ptr, C::COLS);
   } else if (threadIdx.x == 0) {
     mbar_init(own_full, 1);
-    for (int i = 0; i < NST; ++i) {
+    for (int i = 0; i < NA; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_free[i], 1);
+    }
+    for (int i = 0; i < NB; ++i) {
       mbar_init(&v_full[i], 1);
       mbar_init(&v_free[i], 1);
     }
@@ -435,25 +411,25 @@ __global__ void __launch_bounds__(320, 1)
       load_tile<D>(smem + C::OWN_OFF + C::OPB, &maps.dout, s.q0 + m0, h, s.b, own_full);
       int it = 0;
       for (; it < total; ++it) {
-        const int st = it % NST;
-        const uint32_t ph = (uint32_t)(it / NST) & 1u;
+        const int sa = it % NA, sb = it % NB;
+        const uint32_t pa = (uint32_t)(it / NA) & 1u, pb = (uint32_t)(it / NB) & 1u;
         const int r0 = s.k0 + (b0 + it) * N;
-        if (!tc_wait(&k_free[st], ph ^ 1u, stop, a.fault)) break;
-        mbar_arrive_expect_tx(&k_full[st], C::OPB);
-        load_tile<D>(smem + C::A_OFF + st * C::OPB, &maps.k, r0, h / a.G, s.b, &k_full[st]);
-        if (!tc_wait(&v_free[st], ph ^ 1u, stop, a.fault)) {
-          mbar_wait(&k_full[st], ph, nullptr);
+        if (!tc_wait(&k_free[sa], pa ^ 1u, stop, a.fault)) break;
+        mbar_arrive_expect_tx(&k_full[sa], C::OPB);
+        load_tile<D>(smem + C::A_OFF + sa * C::OPB, &maps.k, r0, h / a.G, s.b, &k_full[sa]);
+        if (!tc_wait(&v_free[sb], pb ^ 1u, stop, a.fault)) {
+          mbar_wait(&k_full[sa], pa, nullptr);
           break;
         }
-        mbar_arrive_expect_tx(&v_full[st], C::OPB);
-        load_tile<D>(smem + C::B_OFF + st * C::OPB, &maps.v, r0, h / a.G, s.b, &v_full[st]);
+        mbar_arrive_expect_tx(&v_full[sb], C::OPB);
+        load_tile<D>(smem + C::B_OFF + sb * C::OPB, &maps.v, r0, h / a.G, s.b, &v_full[sb]);
       }
       if (*stop) {
         mbar_wait(own_full, 0, nullptr);
-        for (int i = max(0, it - NST); i < it; ++i) {
-          mbar_wait(&k_full[i % NST], (uint32_t)(i / NST) & 1u, nullptr);
-          mbar_wait(&v_full[i % NST], (uint32_t)(i / NST) & 1u, nullptr);
-        }
+        for (int i = max(0, it - NA); i < it; ++i)
+          mbar_wait(&k_full[i % NA], (uint32_t)(i / NA) & 1u, nullptr);
+        for (int i = max(0, it - NB); i < it; ++i)
+          mbar_wait(&v_full[i % NB], (uint32_t)(i / NB) & 1u, nullptr);
       }
     }
   } else if (warp == 8) {
@@ -464,17 +440,16 @@ __global__ void __launch_bounds__(320, 1)
       // S and dP of block it are issued once those of it - 1 are in registers,
       // dQ's product of it - 1 after them
       for (int it = 0; ok && it <= total; ++it) {
-        const int st = it % NST, sp = (it + NST - 1) % NST;
-        const uint32_t ph = (uint32_t)(it / NST) & 1u;
+        const int sa = it % NA, sb = it % NB, sp = (it + NA - 1) % NA;
         if (it < total) {
-          if (!(ok = tc_wait(&k_full[st], ph, stop, a.fault))) break;
+          if (!(ok = tc_wait(&k_full[sa], (uint32_t)(it / NA) & 1u, stop, a.fault))) break;
           if (it > 0 && !(ok = tc_wait(read, (it - 1) & 1, stop, a.fault))) break;
           tc_fence_after();
-          product_rows<T, D>(tmem + S_COL, qa, ka + st * C::OPB);
-          if (!(ok = tc_wait(&v_full[st], ph, stop, a.fault))) break;
-          product_rows<T, D>(tmem + DP_COL, oa, va + st * C::OPB);
+          product_rows<T, D>(tmem + S_COL, qa, ka + sa * C::OPB);
+          if (!(ok = tc_wait(&v_full[sb], (uint32_t)(it / NB) & 1u, stop, a.fault))) break;
+          product_rows<T, D>(tmem + DP_COL, oa, va + sb * C::OPB);
           mma_commit(sdp_full);
-          mma_commit(&v_free[st]);
+          mma_commit(&v_free[sb]);
         }
         if (it > 0) {
           if (!(ok = tc_wait(ds_full, (it - 1) & 1, stop, a.fault))) break;
@@ -495,7 +470,7 @@ __global__ void __launch_bounds__(320, 1)
     const float2 lse2 = f2s(-__ldg(a.lse2 + stat)), delta = f2s(-__ldg(a.delta + stat));
     bool ok = true;
     for (int it = 0; it < total; ++it) {
-      const int st = it % NST, n0 = (b0 + it) * N;
+      const int n0 = (b0 + it) * N;
       ok = __all_sync(0xffffffffu, tc_wait(sdp_full, it & 1, stop, a.fault));
       if (!ok) break;
       tc_fence_after();
@@ -521,7 +496,7 @@ __global__ void __launch_bounds__(320, 1)
           if (i < from || i >= to) y[i] = 0.f;
         // rows of K past the sequence's end that memory does hold
         if (n0 + N > s.klen && s.k0 + s.klen < a.Sk)
-          zero_rows<D>(smem + C::A_OFF + st * C::OPB, s.klen - n0);
+          zero_rows<D>(smem + C::A_OFF + (it % NA) * C::OPB, s.klen - n0);
       }
       store64<T>(tmem + lanes + DS_COL + (it & 1) * 64 + half * 32, y);
       tc_fence_before();

@@ -2,7 +2,8 @@
 //
 // A CTA takes 256 query rows of one head as two tiles of 128 and streams the
 // keys they see in blocks of 128. Warps 0-3 and 4-7 are one softmax group per
-// tile (thread = row), warp 8 issues the matrix products, warp 9 the copies.
+// tile (thread = row), warp 8 issues the matrix products, warp 9 the copies
+// (warps 10 and 11 only complete its warpgroup).
 // Per tile t and block j:
 //   S_t = Q_t K_j^T into tensor memory (128 columns of fp32),
 //   the group reads its row of S_t, masks, takes the running maximum m (base
@@ -36,17 +37,20 @@ namespace bloth {
 template <int D>
 struct FwdCfg {
   static constexpr int TILE = 128;
-  static constexpr int THREADS = 320;
+  static constexpr int THREADS = 384;
+  // registers of a softmax thread, whose row of 128 scores stays in them, and
+  // of the third warpgroup's (12 warps are launched with 168 each)
+  static constexpr int SOFT_REGS = 224, ISSUE_REGS = 40;
   static constexpr int OPB = TILE * D * 2;           // bytes of one operand tile
-  static constexpr int NST = D == 64 ? 4 : 2;        // K and V stages each
+  static constexpr int NK = D == 64 ? 4 : 3, NV = D == 64 ? 4 : 2;  // stages of K and V
   static constexpr int Q_OFF = 0;
   static constexpr int K_OFF = 2 * OPB;
-  static constexpr int V_OFF = K_OFF + NST * OPB;
-  static constexpr int BAR_OFF = V_OFF + NST * OPB;
-  static constexpr int BARS = 1 + 4 * NST + 6 + 1;
-  // barriers, the tensor-memory address and the stop flag, and room to align
-  // the tiles to 1024 bytes
-  static constexpr int SMEM = BAR_OFF + BARS * 8 + 16 + 1024;
+  static constexpr int V_OFF = K_OFF + NK * OPB;
+  static constexpr int BAR_OFF = V_OFF + NV * OPB;
+  static constexpr int BARS = 1 + 2 * NK + 2 * NV + 8 + 1;
+  // barriers, the tensor-memory address and the stop flag
+  static constexpr int SMEM = BAR_OFF + BARS * 8 + 16;
+  static_assert(SMEM <= 227 * 1024, "shared memory");
   // tensor-memory columns: S_0, S_1, O_0, O_1
   static constexpr uint32_t COLS = 512;
   static constexpr uint32_t S_COL = 0, O_COL = 256;
@@ -65,23 +69,37 @@ __device__ __forceinline__ bool block_masked(const AttnArgs& a, const AttnSeq& s
   return a.window && n0 <= min(m0 + 127, s.qlen - 1) + off - a.window;
 }
 
+// p of quarter PART (32 columns) of a row of 128, packed into r, their sum
+// added to `sum`. A row that has seen nothing (m = -inf) is masked
+// everywhere: 2^(-inf - 0) = 0.
+template <typename T, int PART>
+__device__ __forceinline__ void softmax_part(const float (&x)[128], float2 sc, float m,
+                                             uint32_t (&r)[16], float2& sum) {
+  const float2 base = f2s(m == -INFINITY ? 0.f : -m);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float2 y = f2_fma(f2(x[PART * 32 + 2 * i], x[PART * 32 + 2 * i + 1]), sc, base);
+    const float2 p = f2(ex2(y.x), ex2(y.y));
+    sum = f2_add(sum, p);
+    r[i] = pack2<T>(p.x, p.y);
+  }
+}
+
 template <typename T, int D>
-__global__ void __launch_bounds__(320, 1)
+__global__ void __launch_bounds__(384, 1)
     attn_fwd_kernel(const AttnArgs a, const __grid_constant__ FwdMaps maps) {
   using C = FwdCfg<D>;
-  constexpr int N = C::TILE, NST = C::NST;
-  extern __shared__ unsigned char smem_raw[];
-  unsigned char* smem = reinterpret_cast<unsigned char*>(
-      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  constexpr int N = C::TILE, NK = C::NK, NV = C::NV;
+  extern __shared__ __align__(1024) unsigned char smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
   uint64_t* q_full = bars;
   uint64_t* k_full = bars + 1;
-  uint64_t* k_free = k_full + NST;
-  uint64_t* v_full = k_free + NST;
-  uint64_t* v_free = v_full + NST;
-  uint64_t* s_full = v_free + NST;
+  uint64_t* k_free = k_full + NK;
+  uint64_t* v_full = k_free + NK;
+  uint64_t* v_free = v_full + NV;
+  uint64_t* s_full = v_free + NV;
   uint64_t* p_full = s_full + 2;
-  uint64_t* o_full = p_full + 2;
+  uint64_t* o_full = p_full + 4;  // p_full: each tile's first half, then each one's second
   uint64_t* drained = o_full + 2;
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(drained + 1);
   volatile int* stop = reinterpret_cast<volatile int*>(tmem_ptr + 1);
@@ -119,15 +137,18 @@ __global__ void __launch_bounds__(320, 1)
     tmem_alloc(tmem_ptr, C::COLS);
   } else if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
-    for (int i = 0; i < NST; ++i) {
+    for (int i = 0; i < NK; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_free[i], 1);
+    }
+    for (int i = 0; i < NV; ++i) {
       mbar_init(&v_full[i], 1);
       mbar_init(&v_free[i], 1);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&s_full[t], 1);
       mbar_init(&p_full[t], 4);
+      mbar_init(&p_full[2 + t], 4);
       mbar_init(&o_full[t], 1);
     }
     mbar_init(drained, 1);
@@ -139,88 +160,91 @@ __global__ void __launch_bounds__(320, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_ptr;
 
-  if (warp == 9) {
-    // ------------------------------------------------------------- copies
-    if (lane == 0 && nb > 0) {
-      mbar_arrive_expect_tx(q_full, 2 * C::OPB);
-      for (int t = 0; t < 2; ++t)
-        for (int c = 0; c < D / 64; ++c)
-          tma_load(smem + C::Q_OFF + t * C::OPB + c * N * 128, &maps.q, c * 64,
-                   s.q0 + m0 + t * N, h, s.b, q_full);
-      int it = 0;
-      for (; it < nb; ++it) {
-        const int st = it % NST;
-        const uint32_t ph = (uint32_t)(it / NST) & 1u;
-        if (!tc_wait(&k_free[st], ph ^ 1u, stop, a.fault)) break;
-        mbar_arrive_expect_tx(&k_full[st], C::OPB);
-        for (int c = 0; c < D / 64; ++c)
-          tma_load(smem + C::K_OFF + st * C::OPB + c * N * 128, &maps.k, c * 64,
-                   s.k0 + (b0 + it) * N, h / a.G, s.b, &k_full[st]);
-        if (!tc_wait(&v_free[st], ph ^ 1u, stop, a.fault)) {
-          mbar_wait(&k_full[st], ph, nullptr);
-          break;
-        }
-        mbar_arrive_expect_tx(&v_full[st], C::OPB);
-        for (int c = 0; c < D / 64; ++c)
-          tma_load(smem + C::V_OFF + st * C::OPB + c * N * 128, &maps.v, c * 64,
-                   s.k0 + (b0 + it) * N, h / a.G, s.b, &v_full[st]);
-      }
-      if (*stop) {  // given up: not before the copies in flight have landed
-        mbar_wait(q_full, 0, nullptr);
-        for (int i = max(0, it - NST); i < it; ++i) {
-          mbar_wait(&k_full[i % NST], (uint32_t)(i / NST) & 1u, nullptr);
-          mbar_wait(&v_full[i % NST], (uint32_t)(i / NST) & 1u, nullptr);
-        }
-      }
-    }
-  } else if (warp == 8) {
-    // ----------------------------------------------------------- products
-    if (lane == 0 && nb > 0) {
-      constexpr uint32_t dqk = mma_desc<T>(N, N, false), dpv = mma_desc<T>(N, D, true);
-      const uint32_t qa = smem_addr(smem + C::Q_OFF), ka = smem_addr(smem + C::K_OFF),
-                     va = smem_addr(smem + C::V_OFF);
-      uint32_t p_ph[2] = {0, 0};
-      bool ok = tc_wait(q_full, 0, stop, a.fault);
-      for (int it = 0; ok && it <= nb; ++it) {
-        const int st = it % NST, sp = (it + NST - 1) % NST;
-        const uint32_t ph = (uint32_t)(it / NST) & 1u;
-        if (it > 0) ok = tc_wait(&v_full[sp], (uint32_t)((it - 1) / NST) & 1u, stop, a.fault);
-        if (ok && it < nb) ok = tc_wait(&k_full[st], ph, stop, a.fault);
-        if (!ok) break;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int jp = b0 + it - 1, j = b0 + it;
-          if (it > 0 && jp >= first[t] && jp < last[t]) {
-            ok = tc_wait(&p_full[t], p_ph[t], stop, a.fault);
-            if (!ok) break;
-            p_ph[t] ^= 1u;
-            tc_fence_after();
-#pragma unroll
-            for (int kk = 0; kk < N / 16; ++kk)
-              mma_ts(tmem + C::O_COL + t * D, tmem + C::S_COL + t * N + kk * 8,
-                     desc_mn(va + sp * C::OPB + kk * 2048, N * 128), dpv, jp > first[t] || kk > 0);
-            if (jp == last[t] - 1) mma_commit(&o_full[t]);
+  if (warp >= 8) {
+    lower_registers<C::ISSUE_REGS>();
+    if (warp == 9) {
+      // ------------------------------------------------------------- copies
+      if (lane == 0 && nb > 0) {
+        mbar_arrive_expect_tx(q_full, 2 * C::OPB);
+        for (int t = 0; t < 2; ++t)
+          for (int c = 0; c < D / 64; ++c)
+            tma_load(smem + C::Q_OFF + t * C::OPB + c * N * 128, &maps.q, c * 64,
+                     s.q0 + m0 + t * N, h, s.b, q_full);
+        int it = 0;
+        for (; it < nb; ++it) {
+          const int sk = it % NK, sv = it % NV;
+          const uint32_t pk = (uint32_t)(it / NK) & 1u, pv = (uint32_t)(it / NV) & 1u;
+          if (!tc_wait(&k_free[sk], pk ^ 1u, stop, a.fault)) break;
+          mbar_arrive_expect_tx(&k_full[sk], C::OPB);
+          for (int c = 0; c < D / 64; ++c)
+            tma_load(smem + C::K_OFF + sk * C::OPB + c * N * 128, &maps.k, c * 64,
+                     s.k0 + (b0 + it) * N, h / a.G, s.b, &k_full[sk]);
+          if (!tc_wait(&v_free[sv], pv ^ 1u, stop, a.fault)) {
+            mbar_wait(&k_full[sk], pk, nullptr);
+            break;
           }
-          if (it < nb && j >= first[t] && j < last[t]) {
+          mbar_arrive_expect_tx(&v_full[sv], C::OPB);
+          for (int c = 0; c < D / 64; ++c)
+            tma_load(smem + C::V_OFF + sv * C::OPB + c * N * 128, &maps.v, c * 64,
+                     s.k0 + (b0 + it) * N, h / a.G, s.b, &v_full[sv]);
+        }
+        if (*stop) {  // given up: not before the copies in flight have landed
+          mbar_wait(q_full, 0, nullptr);
+          for (int i = max(0, it - NK); i < it; ++i)
+            mbar_wait(&k_full[i % NK], (uint32_t)(i / NK) & 1u, nullptr);
+          for (int i = max(0, it - NV); i < it; ++i)
+            mbar_wait(&v_full[i % NV], (uint32_t)(i / NV) & 1u, nullptr);
+        }
+      }
+    } else if (warp == 8) {
+      // ----------------------------------------------------------- products
+      if (lane == 0 && nb > 0) {
+        const uint32_t qa = smem_addr(smem + C::Q_OFF), ka = smem_addr(smem + C::K_OFF),
+                       va = smem_addr(smem + C::V_OFF);
+        uint32_t p_ph[2] = {0, 0};
+        bool ok = tc_wait(q_full, 0, stop, a.fault);
+        for (int it = 0; ok && it <= nb; ++it) {
+          const int sk = it % NK, sv = (it + NV - 1) % NV;  // K of block it, V of the one before
+          if (it > 0) ok = tc_wait(&v_full[sv], (uint32_t)((it - 1) / NV) & 1u, stop, a.fault);
+          if (ok && it < nb) ok = tc_wait(&k_full[sk], (uint32_t)(it / NK) & 1u, stop, a.fault);
+          if (!ok) break;
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-              const uint32_t o = (kk / 4) * (N * 128) + (kk % 4) * 32;
-              mma_ss(tmem + C::S_COL + t * N, desc_k(qa + t * C::OPB + o),
-                     desc_k(ka + st * C::OPB + o), dqk, kk > 0);
+          for (int t = 0; t < 2; ++t) {
+            const int jp = b0 + it - 1, j = b0 + it;
+            if (it > 0 && jp >= first[t] && jp < last[t]) {
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                ok = tc_wait(&p_full[2 * half + t], p_ph[t], stop, a.fault);
+                if (!ok) break;
+                tc_fence_after();
+                if (half == 0)
+                  product_cols<T, D, 0, 4>(tmem + C::O_COL + t * D, tmem + C::S_COL + t * N, 32,
+                                           va + sv * C::OPB, jp > first[t]);
+                else
+                  product_cols<T, D, 4, 8>(tmem + C::O_COL + t * D, tmem + C::S_COL + t * N, 32,
+                                           va + sv * C::OPB, true);
+              }
+              if (!ok) break;
+              p_ph[t] ^= 1u;
+              if (jp == last[t] - 1) mma_commit(&o_full[t]);
             }
-            mma_commit(&s_full[t]);
+            if (it < nb && j >= first[t] && j < last[t]) {
+              product_rows<T, D>(tmem + C::S_COL + t * N, qa + t * C::OPB, ka + sk * C::OPB);
+              mma_commit(&s_full[t]);
+            }
           }
+          if (!ok) break;
+          if (it > 0) mma_commit(&v_free[sv]);
+          if (it < nb) mma_commit(&k_free[sk]);
         }
-        if (!ok) break;
-        if (it > 0) mma_commit(&v_free[sp]);
-        if (it < nb) mma_commit(&k_free[st]);
-      }
-      if (!ok) {  // given up: not before the products in flight have completed
-        mma_commit(drained);
-        mbar_wait(drained, 0, nullptr);
+        if (!ok) {  // given up: not before the products in flight have completed
+          mma_commit(drained);
+          mbar_wait(drained, 0, nullptr);
+        }
       }
     }
   } else {
+    raise_registers<C::SOFT_REGS>();
     // ------------------------------------------------------------ softmax
     const int t = warp >> 2;
     const int row = m0 + t * N + (threadIdx.x & 127);  // of the sequence
@@ -255,60 +279,69 @@ __global__ void __launch_bounds__(320, 1)
           if (i >= hi || i < lo) x[i] = -INFINITY;
         // rows of V past the sequence's end that memory does hold
         if (n0 + N > s.klen && s.k0 + s.klen < a.Sk) {
-          const int it = j - b0, st = it % NST;
-          ok = __all_sync(0xffffffffu, tc_wait(&v_full[st], (uint32_t)(it / NST) & 1u, stop, a.fault));
+          const int it = j - b0, sv = it % NV;
+          ok = __all_sync(0xffffffffu, tc_wait(&v_full[sv], (uint32_t)(it / NV) & 1u, stop, a.fault));
           if (!ok) break;
           const int r0 = s.klen - n0;
           for (int c = threadIdx.x & 127; c < (N - r0) * (D / 8); c += 128) {
             const int r = r0 + c / (D / 8), b = c % (D / 8);
-            *reinterpret_cast<uint4*>(smem + C::V_OFF + st * C::OPB + (b / 8) * (N * 128) +
+            *reinterpret_cast<uint4*>(smem + C::V_OFF + sv * C::OPB + (b / 8) * (N * 128) +
                                       r * 128 + (b % 8) * 16) = make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async_smem();
         }
       }
+      // p of the first 32 columns with the maximum so far, while the block's
+      // maximum is found: it seldom moves, and the exponentials' unit would
+      // idle for 450 cycles otherwise
+      const float2 sc = f2s(a.scale_log2);
+      uint32_t r[16];
+      float2 sum = f2(0.f, 0.f);
+      if (j > f) softmax_part<T, 0>(x, sc, m, r, sum);
       float top[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-      for (int i = 4; i < N; i += 4)
+      for (int i = 4; i + 8 <= N; i += 8)
 #pragma unroll
-        for (int u = 0; u < 4; ++u) top[u] = fmaxf(top[u], x[i + u]);
-      const float mb = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
+        for (int u = 0; u < 4; ++u) top[u] = max3(top[u], x[i + u], x[i + 4 + u]);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) top[u] = fmaxf(top[u], x[N - 4 + u]);
+      const float mb = max3(fmaxf(top[0], top[1]), top[2], top[3]) * a.scale_log2;
       if (j == f) {
         m = mb;
+        softmax_part<T, 0>(x, sc, m, r, sum);
       } else if (__any_sync(0xffffffffu, mb > m + 8.f)) {
         const float mn = mb > m + 8.f ? mb : m;
         const float w = mn == m ? 1.f : ex2(m - mn);
         m = mn;
         l *= w;
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t r[32];
-          tmem_ld32(o_at + c * 32, r);
+        for (int c = 0; c < D / 16; ++c) {
+          uint32_t o[16];
+          tmem_ld16(o_at + c * 16, o);
           tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * w);
-          tmem_st32(o_at + c * 32, r);
+          for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * w);
+          tmem_st16(o_at + c * 16, o);
         }
+        sum = f2(0.f, 0.f);
+        softmax_part<T, 0>(x, sc, m, r, sum);
       }
-      const float2 base = f2s(m == -INFINITY ? 0.f : -m), sc = f2s(a.scale_log2);
-      float2 sum[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
-#pragma unroll
-      for (int c = 0; c < N / 64; ++c) {
-        uint32_t r[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float2 y = f2_fma(f2(x[c * 64 + 2 * i], x[c * 64 + 2 * i + 1]), sc, base);
-          const float2 p = f2(ex2(y.x), ex2(y.y));
-          sum[i & 1] = f2_add(sum[i & 1], p);
-          r[i] = pack2<T>(p.x, p.y);
-        }
-        tmem_st32(s_at + c * 32, r);
-      }
-      l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+      tmem_st16(s_at, r);
+      softmax_part<T, 1>(x, sc, m, r, sum);
+      tmem_st16(s_at + 16, r);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[t]);
+      softmax_part<T, 2>(x, sc, m, r, sum);
+      tmem_st16(s_at + 32, r);
+      softmax_part<T, 3>(x, sc, m, r, sum);
+      tmem_st16(s_at + 48, r);
+      l += sum.x + sum.y;
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[2 + t]);
     }
     if (ok && e > f) {
       ok = __all_sync(0xffffffffu, tc_wait(&o_full[t], 0, stop, a.fault));
@@ -366,6 +399,9 @@ int launch_attn_fwd(const AttnArgs& a0, cudaStream_t st) {
   if (rc != BLOTH_OK) return rc;
   auto kern = attn_fwd_kernel<T, D>;
   if ((rc = prepare_smem((const void*)kern, C::SMEM)) != BLOTH_OK) return rc;
+  static const bool enough =
+      registers_cover((const void*)kern, 3, 2 * C::SOFT_REGS + C::ISSUE_REGS);
+  if (!enough) return cuda_status(cudaErrorLaunchOutOfResources);
   const int64_t grid = attn_tiles(a.Sq, a.packed, 2 * C::TILE) * a.Hq * a.B;
   if (grid > 0x7fffffff) return BLOTH_ERR_SHAPE;
   kern<<<(unsigned)grid, C::THREADS, C::SMEM, st>>>(a, m);

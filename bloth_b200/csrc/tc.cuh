@@ -6,8 +6,8 @@
 // Tiles. A 16-bit operand tile of R rows and D columns lies in shared memory
 // as D / 64 blocks of [R][64] elements (128 bytes a row), each written by one
 // tiled copy with the 128-byte swizzle, 1024-byte aligned. The same tile
-// serves as an operand whose contracted index runs along its columns
-// (desc_k: "K-major") or along its rows (desc_mn: "MN-major").
+// serves as an operand whose contracted index runs along its columns or along
+// its rows.
 #pragma once
 
 #include <cuda.h>
@@ -17,14 +17,28 @@
 namespace bloth {
 
 // ------------------------------------------------------------------ waits
+// One test of phase `parity`, suspended for the default time at most: the
+// hand-over of tiles between warps takes a fraction of a microsecond.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_addr(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+
 // Waits for phase `parity` of `bar`. False once the CTA has given up: when
 // this wait takes longer than kWaitLimitNs (recorded in the fault word), or
 // another thread's did (*stop, in shared memory).
 __device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, volatile int* stop,
                                         unsigned int* fault) {
-  if (mbar_try_wait(bar, parity)) return true;
+  if (mbar_test(bar, parity)) return true;
   const unsigned long long t0 = global_ns();
-  while (!mbar_try_wait(bar, parity)) {
+  while (!mbar_test(bar, parity)) {
     if (*stop) return false;
     if (global_ns() - t0 > kWaitLimitNs) {
       *stop = 1;
@@ -51,19 +65,23 @@ __device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int 
 }
 
 // ------------------------------------------------------------ descriptors
-// Shared-memory operand descriptor: address and offsets in 16-byte units,
-// version 1 (bit 46), 128-byte swizzle (2 in bits 61-63).
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead, uint32_t stride) {
-  return (uint64_t)((addr & 0x3ffff) >> 4) | ((uint64_t)(lead >> 4) << 16) |
-         ((uint64_t)(stride >> 4) << 32) | (1ull << 46) | (2ull << 61);
+// Shared-memory operand descriptor, addresses and offsets in 16-byte units.
+// Upper word, the same for every tile here: groups of 8 rows are 1024 bytes
+// apart (bits 32-45), version 1 (bit 46), 128-byte swizzle (2 in bits 61-63).
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+// Lower word: the address, and the offset between blocks of 64 columns (bits
+// 16-29), which counts where the contracted index runs along the rows.
+//   along the columns ("K-major"): a step of 16 columns is 32 bytes inside a
+//   64-column block;
+//   along the rows ("MN-major"): a step of 16 rows is 2048 bytes.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t block) {
+  return ((addr & 0x3ffff) >> 4) | ((block >> 4) << 16);
 }
-// Contracted index along the columns: groups of 8 rows are 1024 bytes apart;
-// a step of 16 columns is 32 bytes inside a 64-column block.
-__device__ __forceinline__ uint64_t desc_k(uint32_t addr) { return smem_desc(addr, 0, 1024); }
-// Contracted index along the rows: groups of 8 rows are 1024 bytes apart, the
-// next 64 columns one block of `block` bytes further.
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t block) {
-  return smem_desc(addr, block, 1024);
+// Keeps the compiler from holding what it derives from x across iterations
+// (dozens of descriptors, in the registers that the softmax needs).
+__device__ __forceinline__ uint32_t opaque(uint32_t x) {
+  asm volatile("" : "+r"(x));
+  return x;
 }
 
 // Instruction descriptor: fp32 accumulator, A and B of type T, M x N, B's
@@ -78,21 +96,48 @@ __host__ __device__ constexpr uint32_t mma_desc(int m, int n, bool b_mn) {
 // --------------------------------------------------------- matrix products
 // Tensor memory [d] (+)= A x B for 16 contracted elements; issued by one
 // thread. A in shared memory (mma_ss) or in tensor memory (mma_ts).
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc,
                                        bool add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((int)add)
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"((int)add), "r"(kDescHi)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc,
                                        bool add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"((int)add)
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"((int)add), "r"(kDescHi)
       : "memory");
+}
+
+// Operand tiles of 128 rows and D columns, at shared-memory addresses.
+// d = A B^T, contracted over the columns.
+template <typename T, int D>
+__device__ __forceinline__ void product_rows(uint32_t d, uint32_t a, uint32_t b) {
+  constexpr uint32_t id = mma_desc<T>(128, 128, false);
+  const uint32_t la = opaque(desc_lo(a, 0)), lb = opaque(desc_lo(b, 0));
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk) {
+    const uint32_t o = ((kk / 4) * (128 * 128) + (kk % 4) * 32) >> 4;
+    mma_ss(d, la + o, lb + o, id, kk > 0);
+  }
+}
+// d (+)= W B over the rows [16 FROM, 16 TO) of B: W 128 x 128 in tensor memory,
+// 16 of its columns per 8 there, those from 64 on `half` columns after the
+// first.
+template <typename T, int D, int FROM = 0, int TO = 8>
+__device__ __forceinline__ void product_cols(uint32_t d, uint32_t w, uint32_t half, uint32_t b,
+                                             bool add) {
+  constexpr uint32_t id = mma_desc<T>(128, D, true);
+  const uint32_t lb = opaque(desc_lo(b, 128 * 128));
+#pragma unroll
+  for (int kk = FROM; kk < TO; ++kk)
+    mma_ts(d, w + (kk / 4) * half + (kk % 4) * 8, lb + kk * (2048 >> 4), id, add || kk > FROM);
 }
 // `bar` completes a phase when every product issued so far has completed.
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
@@ -142,6 +187,16 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
       : "r"(addr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(addr)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
@@ -164,12 +219,30 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]
       : "memory");
 }
 
+// Registers a thread of this warpgroup may hold from here on; the whole
+// warpgroup executes it. RAISE waits until the block's launch has that many
+// left, so the shares of all warpgroups must not exceed what it was launched
+// with (registers_cover, host).
+template <int REGS>
+__device__ __forceinline__ void raise_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+template <int REGS>
+__device__ __forceinline__ void lower_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+
 // ------------------------------------------------------------- arithmetic
 // 2^x; 2 ulp, results below the normal range are 0.
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 // Two floats rounded to T in one register, the first in the lower half.
 template <typename T>
@@ -186,5 +259,9 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 // `rows` rows x 64 columns of one head, 128-byte swizzle, zeros outside.
 int head_map(CUtensorMap* map, const void* p, int64_t sb, int64_t ss, int64_t sh, int B, int64_t S,
              int H, int D, int rows, int dtype);
+
+// Host: whether func's launches of `groups` warpgroups hold `shares` registers
+// (the sum of a thread's share over the warpgroups).
+bool registers_cover(const void* func, int groups, int shares);
 
 }  // namespace bloth
