@@ -4,8 +4,8 @@
 // kernels that hand tiles between warps.
 //
 // Tiles. A 16-bit operand tile of R rows and D columns lies in shared memory
-// as D / 64 blocks of [R][64] elements (128 bytes a row), each written by one
-// tiled copy with the 128-byte swizzle, 1024-byte aligned. The same tile
+// as D / 64 blocks of [R][64] elements (128 bytes a row), each written by
+// tiled copies with the 128-byte swizzle, 1024-byte aligned. The same tile
 // serves as an operand whose contracted index runs along its columns or along
 // its rows.
 #pragma once
@@ -16,10 +16,44 @@
 
 namespace bloth {
 
+// ------------------------------------------------------------- arithmetic
+// 2^x; 2 ulp, results below the normal range are 0.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// Two floats rounded to T in one register, the first in the lower half.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
 // ------------------------------------------------------------------ waits
-// One test of phase `parity`, suspended for the default time at most: the
-// hand-over of tiles between warps takes a fraction of a microsecond.
+// One test of phase `parity`: at once (mbar_test), or suspended for the default
+// time at most (mbar_try).
 __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_addr(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+__device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
@@ -36,9 +70,9 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
 // another thread's did (*stop, in shared memory).
 __device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, volatile int* stop,
                                         unsigned int* fault) {
-  if (mbar_test(bar, parity)) return true;
+  if (mbar_try(bar, parity)) return true;
   const unsigned long long t0 = global_ns();
-  while (!mbar_test(bar, parity)) {
+  while (!mbar_try(bar, parity)) {
     if (*stop) return false;
     if (global_ns() - t0 > kWaitLimitNs) {
       *stop = 1;
@@ -47,6 +81,13 @@ __device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, volatile
     }
   }
   return true;
+}
+
+// The same when a test of the phase made earlier (mbar_test), whose result
+// was not waited for, may have found it complete.
+__device__ __forceinline__ bool tc_wait(bool done, uint64_t* bar, uint32_t parity,
+                                        volatile int* stop, unsigned int* fault) {
+  return done || tc_wait(bar, parity, stop, fault);
 }
 
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
@@ -115,29 +156,25 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint3
       : "memory");
 }
 
-// Operand tiles of 128 rows and D columns, at shared-memory addresses.
-// d = A B^T, contracted over the columns.
+// d = A B^T, contracted over the D columns: A an operand tile of 128 rows, B of
+// 64, at shared-memory addresses.
 template <typename T, int D>
 __device__ __forceinline__ void product_rows(uint32_t d, uint32_t a, uint32_t b) {
-  constexpr uint32_t id = mma_desc<T>(128, 128, false);
+  constexpr uint32_t id = mma_desc<T>(128, 64, false);
   const uint32_t la = opaque(desc_lo(a, 0)), lb = opaque(desc_lo(b, 0));
 #pragma unroll
-  for (int kk = 0; kk < D / 16; ++kk) {
-    const uint32_t o = ((kk / 4) * (128 * 128) + (kk % 4) * 32) >> 4;
-    mma_ss(d, la + o, lb + o, id, kk > 0);
-  }
+  for (int kk = 0; kk < D / 16; ++kk)
+    mma_ss(d, la + (((kk / 4) * (128 * 128) + (kk % 4) * 32) >> 4),
+           lb + (((kk / 4) * (64 * 128) + (kk % 4) * 32) >> 4), id, kk > 0);
 }
-// d (+)= W B over the rows [16 FROM, 16 TO) of B: W 128 x 128 in tensor memory,
-// 16 of its columns per 8 there, those from 64 on `half` columns after the
-// first.
-template <typename T, int D, int FROM = 0, int TO = 8>
-__device__ __forceinline__ void product_cols(uint32_t d, uint32_t w, uint32_t half, uint32_t b,
-                                             bool add) {
+// d (+)= W B, contracted over the 64 rows of operand tile B: W 128 x 64 of
+// 16-bit elements in 32 columns of tensor memory.
+template <typename T, int D>
+__device__ __forceinline__ void product_cols(uint32_t d, uint32_t w, uint32_t b, bool add) {
   constexpr uint32_t id = mma_desc<T>(128, D, true);
-  const uint32_t lb = opaque(desc_lo(b, 128 * 128));
+  const uint32_t lb = opaque(desc_lo(b, 64 * 128));
 #pragma unroll
-  for (int kk = FROM; kk < TO; ++kk)
-    mma_ts(d, w + (kk / 4) * half + (kk % 4) * 8, lb + kk * (2048 >> 4), id, add || kk > FROM);
+  for (int kk = 0; kk < 4; ++kk) mma_ts(d, w + kk * 8, lb + kk * (2048 >> 4), id, add || kk > 0);
 }
 // `bar` completes a phase when every product issued so far has completed.
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
@@ -219,49 +256,52 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]
       : "memory");
 }
 
-// Registers a thread of this warpgroup may hold from here on; the whole
-// warpgroup executes it. RAISE waits until the block's launch has that many
-// left, so the shares of all warpgroups must not exceed what it was launched
-// with (registers_cover, host).
-template <int REGS>
-__device__ __forceinline__ void raise_registers() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
+// 64 columns of the thread's row, and 64 values rounded to T in 32 columns
+// (not waited for).
+__device__ __forceinline__ void load64(uint32_t at, float (&x)[64]) {
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    uint32_t r[32];
+    tmem_ld32(at + c * 32, r);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) x[c * 32 + i] = __uint_as_float(r[i]);
+  }
+  tmem_wait_ld();
 }
-template <int REGS>
-__device__ __forceinline__ void lower_registers() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
+template <typename T>
+__device__ __forceinline__ void store64(uint32_t at, const float (&x)[64]) {
+  uint32_t r[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) r[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
+  tmem_st32(at, r);
 }
 
-// ------------------------------------------------------------- arithmetic
-// 2^x; 2 ulp, results below the normal range are 0.
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
+// An operand tile of ROWS rows r0.. of a head: boxes of 64 rows x 64 columns.
+template <int D, int ROWS>
+__device__ __forceinline__ void load_tile(unsigned char* dst, const CUtensorMap* map, int r0, int h,
+                                          int b, uint64_t* bar) {
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+    for (int r = 0; r < ROWS; r += 64)
+      tma_load(dst + c * ROWS * 128 + r * 128, map, c * 64, r0 + r, h, b, bar);
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-// Two floats rounded to T in one register, the first in the lower half.
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  uint32_t r;
-  if constexpr (std::is_same<T, __nv_bfloat16>::value)
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  else
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
+
+// Rows [r0, 64) of an operand tile of 64 in shared memory become zeros, before
+// later products read them (128 threads).
+template <int D>
+__device__ __forceinline__ void zero_rows(unsigned char* tile, int r0) {
+  for (int c = threadIdx.x & 127; c < (64 - r0) * (D / 8); c += 128) {
+    const int r = r0 + c / (D / 8), b = c % (D / 8);
+    *reinterpret_cast<uint4*>(tile + (b / 8) * (64 * 128) + r * 128 + (b % 8) * 16) =
+        make_uint4(0, 0, 0, 0);
+  }
+  fence_proxy_async_smem();
 }
 
 // Host: tensor map of a head tensor [B, S, H, D] of 16-bit elements, boxes of
 // `rows` rows x 64 columns of one head, 128-byte swizzle, zeros outside.
 int head_map(CUtensorMap* map, const void* p, int64_t sb, int64_t ss, int64_t sh, int B, int64_t S,
              int H, int D, int rows, int dtype);
-
-// Host: whether func's launches of `groups` warpgroups hold `shares` registers
-// (the sum of a thread's share over the warpgroups).
-bool registers_cover(const void* func, int groups, int shares);
 
 }  // namespace bloth

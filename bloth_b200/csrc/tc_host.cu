@@ -47,13 +47,4 @@ int head_map(CUtensorMap* map, const void* p, int64_t sb, int64_t ss, int64_t sh
   return r == CUDA_SUCCESS ? BLOTH_OK : BLOTH_ERR_ALIGN;
 }
 
-bool registers_cover(const void* func, int groups, int shares) {
-  cudaFuncAttributes at;
-  if (cudaFuncGetAttributes(&at, func) != cudaSuccess) {
-    cudaGetLastError();
-    return false;
-  }
-  return at.numRegs * groups >= shares;
-}
-
 }  // namespace bloth
