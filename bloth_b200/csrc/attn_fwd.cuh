@@ -75,20 +75,19 @@ __global__ void __launch_bounds__(352, 1)
   using C = FwdCfg<D>;
   constexpr int N = C::TILE, BLK = C::BLK, NST = C::NST;
   extern __shared__ __align__(1024) unsigned char smem[];
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
-  uint64_t* q_full = bars;
-  uint64_t* k_full = bars + 1;
-  uint64_t* k_free = k_full + NST;
-  uint64_t* v_full = k_free + NST;
-  uint64_t* v_free = v_full + NST;
-  uint64_t* s_full = v_free + NST;  // [tile][buffer]
-  uint64_t* p_full = s_full + 4;   // [tile][buffer]
-  uint64_t* o_done = p_full + 4;   // [tile]: a block's product with V has completed
-  uint64_t* drained = o_done + 2;
-  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(drained + 2);
-  volatile int* stop = reinterpret_cast<volatile int*>(tmem_ptr + 1);
+  const uint32_t base = smem_addr(smem);
+  // barriers (8 bytes each)
+  const uint32_t q_full = base + C::BAR_OFF;
+  const uint32_t k_full = q_full + 8, k_free = k_full + 8 * NST;
+  const uint32_t v_full = k_free + 8 * NST, v_free = v_full + 8 * NST;
+  const uint32_t s_full = v_free + 8 * NST;  // [tile][buffer]
+  const uint32_t p_full = s_full + 8 * 4;    // [tile][buffer]
+  const uint32_t o_done = p_full + 8 * 4;    // [tile]: a block's product with V has completed
+  const uint32_t drained = o_done + 8 * 2;
+  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(smem + C::BAR_OFF + 8 * C::BARS);
+  const Waits waits{reinterpret_cast<volatile int*>(tmem_ptr + 1), a.fault};
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int heads = a.Hq * a.B;
   const int tiles = (int)(gridDim.x / heads);
   const int hb = blockIdx.x % heads, h = hb % a.Hq;
@@ -120,22 +119,22 @@ __global__ void __launch_bounds__(352, 1)
   if (warp == 8) {
     tmem_alloc(tmem_ptr, C::COLS);
   } else if (threadIdx.x == 0) {
-    mbar_init(q_full, 1);
+    bar_init(q_full, 1);
     for (int i = 0; i < NST; ++i) {
-      mbar_init(&k_full[i], 1);
-      mbar_init(&k_free[i], 2);
-      mbar_init(&v_full[i], 1);
-      mbar_init(&v_free[i], 2);
+      bar_init(k_full + 8 * i, 1);
+      bar_init(k_free + 8 * i, 2);
+      bar_init(v_full + 8 * i, 1);
+      bar_init(v_free + 8 * i, 2);
     }
     for (int i = 0; i < 4; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
+      bar_init(s_full + 8 * i, 1);
+      bar_init(p_full + 8 * i, 4);
     }
     for (int t = 0; t < 2; ++t) {
-      mbar_init(&o_done[t], 1);
-      mbar_init(&drained[t], 1);
+      bar_init(o_done + 8 * t, 1);
+      bar_init(drained + 8 * t, 1);
     }
-    *stop = 0;
+    *waits.stop = 0;
     mbar_init_fence();
   }
   tc_fence_before();
@@ -146,75 +145,84 @@ __global__ void __launch_bounds__(352, 1)
   if (warp == 10) {
     // ------------------------------------------------------------- copies
     if (lane == 0 && nb > 0) {
-      mbar_arrive_expect_tx(q_full, 2 * C::QB);
-      load_tile<D, N>(smem + C::Q_OFF, &maps.q, s.q0 + m0, h, s.b, q_full);
-      load_tile<D, N>(smem + C::Q_OFF + C::QB, &maps.q, s.q0 + m0 + N, h, s.b, q_full);
-      int it = 0;
-      for (; it < nb; ++it) {
-        const int st = it % NST;
-        const uint32_t ph = (uint32_t)(it / NST) & 1u;
-        const int r0 = s.k0 + (b0 + it) * BLK;
-        if (!tc_wait(&k_free[st], ph ^ 1u, stop, a.fault)) break;
-        mbar_arrive_expect_tx(&k_full[st], C::KB);
-        load_tile<D, BLK>(smem + C::K_OFF + st * C::KB, &maps.k, r0, h / a.G, s.b, &k_full[st]);
-        if (!tc_wait(&v_free[st], ph ^ 1u, stop, a.fault)) {
-          mbar_wait(&k_full[st], ph, nullptr);
+      bar_expect(q_full, 2 * C::QB);
+      load_tile<D, N>(base + C::Q_OFF, &maps.q, s.q0 + m0, h, s.b, q_full);
+      load_tile<D, N>(base + C::Q_OFF + C::QB, &maps.q, s.q0 + m0 + N, h, s.b, q_full);
+      const int hk = h / a.G;
+      int r0 = s.k0 + b0 * BLK, it = 0;
+      Ring<NST> st;
+      for (; it < nb; ++it, r0 += BLK, st.next()) {
+        const uint32_t kf = k_full + 8 * st.at, vf = v_full + 8 * st.at;
+        if (!bar_wait(k_free + 8 * st.at, st.phase ^ 1u, waits)) break;
+        bar_expect(kf, C::KB);
+        load_tile<D, BLK>(base + C::K_OFF + st.at * C::KB, &maps.k, r0, hk, s.b, kf);
+        if (!bar_wait(v_free + 8 * st.at, st.phase ^ 1u, waits)) {
+          bar_drain(kf, st.phase, waits);
           break;
         }
-        mbar_arrive_expect_tx(&v_full[st], C::KB);
-        load_tile<D, BLK>(smem + C::V_OFF + st * C::KB, &maps.v, r0, h / a.G, s.b, &v_full[st]);
+        bar_expect(vf, C::KB);
+        load_tile<D, BLK>(base + C::V_OFF + st.at * C::KB, &maps.v, r0, hk, s.b, vf);
       }
-      if (*stop) {  // given up: not before the copies in flight have landed
-        mbar_wait(q_full, 0, nullptr);
+      if (*waits.stop) {  // given up: not before the copies in flight have landed
+        bar_drain(q_full, 0, waits);
         for (int i = max(0, it - NST); i < it; ++i) {
-          mbar_wait(&k_full[i % NST], (uint32_t)(i / NST) & 1u, nullptr);
-          mbar_wait(&v_full[i % NST], (uint32_t)(i / NST) & 1u, nullptr);
+          bar_drain(k_full + 8 * (i % NST), (uint32_t)(i / NST) & 1u, waits);
+          bar_drain(v_full + 8 * (i % NST), (uint32_t)(i / NST) & 1u, waits);
         }
       }
     }
   } else if (warp >= 8) {
     // ----------------------------------------------------------- products
-    if (lane == 0 && nb > 0) {
+    if (nb > 0) {
       const int t = warp - 8;
       const int f = (t ? first[1] : first[0]) - b0, e = (t ? last[1] : last[0]) - b0;
-      const uint32_t qa = smem_addr(smem + C::Q_OFF) + t * C::QB,
-                     ka = smem_addr(smem + C::K_OFF), va = smem_addr(smem + C::V_OFF);
+      const uint32_t qa = base + C::Q_OFF + t * C::QB;
       const uint32_t s_at = tmem + C::S_COL + t * N, o_at = tmem + C::O_COL + t * D;
-      bool ok = tc_wait(q_full, 0, stop, a.fault);
+      const bool lead = elect();
+      Ring<NST> kst, vst;
+      Ring<2> kb, vb;  // score buffers of the S and of the O to come
+      bool ok = bar_wait(q_full, 0, waits);
       // step j: O of block j - 2, then S of block j where that one's P was;
       // of the CTA's blocks [f, e) are this tile's
       for (int j = 0; ok && j < nb + 2; ++j) {
-        const int jp = j - 2, buf = 2 * t + ((j - f) & 1);
-        const uint32_t s_buf = s_at + ((j - f) & 1) * BLK;
-        if (jp >= 0) {
-          const int st = jp % NST;
-          ok = tc_wait(&v_full[st], (uint32_t)(jp / NST) & 1u, stop, a.fault);
+        if (j >= 2) {
+          const bool mine = j - 2 >= f && j - 2 < e;
+          ok = bar_wait(v_full + 8 * vst.at, vst.phase, waits);
+          if (ok && mine) ok = bar_wait(p_full + 16 * t + 8 * vb.at, vb.phase, waits);
           if (!ok) break;
-          if (jp >= f && jp < e) {
-            ok = tc_wait(&p_full[buf], (uint32_t)((jp - f) >> 1) & 1u, stop, a.fault);
-            if (!ok) break;
-            tc_fence_after();
-            product_cols<T, D>(o_at, s_buf, va + st * C::KB, jp > f);
-            mma_commit(&o_done[t]);
+          tc_fence_after();
+          if (lead) {
+            if (mine) {
+              product_cols<T, D>(o_at, s_at + vb.at * BLK, base + C::V_OFF + vst.at * C::KB,
+                                 j - 2 > f);
+              mma_commit(o_done + 8 * t);
+            }
+            // (a commit completes with the products before it, if there are any)
+            mma_commit(v_free + 8 * vst.at);
           }
-          // (a commit completes with the products before it, if there are any)
-          mma_commit(&v_free[st]);
+          vst.next();
+          if (mine) vb.next();
         }
         if (j < nb) {
-          const int st = j % NST;
-          ok = tc_wait(&k_full[st], (uint32_t)(j / NST) & 1u, stop, a.fault);
+          const bool mine = j >= f && j < e;
+          ok = bar_wait(k_full + 8 * kst.at, kst.phase, waits);
           if (!ok) break;
-          if (j >= f && j < e) {
-            product_rows<T, D>(s_buf, qa, ka + st * C::KB);
-            mma_commit(&s_full[buf]);
+          if (lead) {
+            if (mine) {
+              product_rows<T, D>(s_at + kb.at * BLK, qa, base + C::K_OFF + kst.at * C::KB);
+              mma_commit(s_full + 16 * t + 8 * kb.at);
+            }
+            mma_commit(k_free + 8 * kst.at);
           }
-          mma_commit(&k_free[st]);
+          kst.next();
+          if (mine) kb.next();
         }
       }
-      if (!ok) {  // given up: not before the products in flight have completed
-        mma_commit(&drained[t]);
-        mbar_wait(&drained[t], 0, nullptr);
+      if (!ok && lead) {  // given up: not before the products in flight have completed
+        mma_commit(drained + 8 * t);
+        bar_drain(drained + 8 * t, 0, waits);
       }
+      __syncwarp();
     }
   } else {
     // ------------------------------------------------------------ softmax
@@ -232,19 +240,20 @@ __global__ void __launch_bounds__(352, 1)
     // told to the issuing warp on the way, so that the wait for its stores
     // costs nothing.
     float x[BLK];
-    for (int j = f; j < e; ++j) {
-      const int i0 = j - f, b = i0 & 1;
-      const uint32_t s_buf = tmem + lanes + C::S_COL + t * N + b * BLK;
-      ok = __all_sync(0xffffffffu, tc_wait(there, &s_full[2 * t + b], (uint32_t)(i0 >> 1) & 1u,
-                                           stop, a.fault));
+    Ring<2> buf;
+    for (int j = f; j < e; ++j, buf.next()) {
+      const uint32_t s_buf = tmem + lanes + C::S_COL + t * N + buf.at * BLK;
+      const uint32_t other = 16 * t + 8 * (buf.at ^ 1u);
+      if (!there) there = bar_wait(s_full + 16 * t + 8 * buf.at, buf.phase, waits);
+      ok = __all_sync(0xffffffffu, there);
       if (!ok) break;
       tc_fence_after();
       load64(s_buf, x);
-      if (i0 > 0) {
+      if (j > f) {
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[2 * t + (b ^ 1)]);
+        if (lane == 0) bar_arrive(p_full + other);
       }
       const int n0 = j * BLK;
       if (block_masked(a, s, m0 + t * N, n0)) {
@@ -256,8 +265,7 @@ __global__ void __launch_bounds__(352, 1)
         // rows of V past the sequence's end that memory does hold
         if (n0 + BLK > s.klen && s.k0 + s.klen < a.Sk) {
           const int it = j - b0, st = it % NST;
-          ok = __all_sync(0xffffffffu,
-                          tc_wait(&v_full[st], (uint32_t)(it / NST) & 1u, stop, a.fault));
+          ok = __all_sync(0xffffffffu, bar_wait(v_full + 8 * st, (uint32_t)(it / NST) & 1u, waits));
           if (!ok) break;
           zero_rows<D>(smem + C::V_OFF + st * C::KB, s.klen - n0);
         }
@@ -270,7 +278,7 @@ __global__ void __launch_bounds__(352, 1)
 #pragma unroll
       for (int u = 0; u < 4; ++u) top[u] = fmaxf(top[u], x[BLK - 4 + u]);
       const float mb = max3(fmaxf(top[0], top[1]), top[2], top[3]) * a.scale_log2;
-      if (i0 == 0) {
+      if (j == f) {
         m = mb;
       } else if (__any_sync(0xffffffffu, mb > m + 8.f)) {
         const float mn = mb > m + 8.f ? mb : m;
@@ -279,7 +287,7 @@ __global__ void __launch_bounds__(352, 1)
         l *= w;
         // O_t, after the product of the block before; the one before that has
         // completed, since S of this block was issued after it
-        ok = __all_sync(0xffffffffu, tc_wait(&o_done[t], (uint32_t)(i0 - 1) & 1u, stop, a.fault));
+        ok = __all_sync(0xffffffffu, bar_wait(o_done + 8 * t, (uint32_t)(j - f - 1) & 1u, waits));
         if (!ok) break;
         tc_fence_after();
 #pragma unroll 1
@@ -294,13 +302,13 @@ __global__ void __launch_bounds__(352, 1)
       }
       // whether the next block's S is there: asked before the exponentials, so
       // that the answer (200 cycles) comes during them
-      there = j + 1 < e && mbar_test(&s_full[2 * t + (b ^ 1)], (uint32_t)((i0 + 1) >> 1) & 1u);
+      there = j + 1 < e && bar_test(s_full + other, buf.phase ^ buf.at);
       // a row that has seen nothing (m = -inf) is masked everywhere: 2^(-inf - 0) = 0
-      const float2 base = f2s(m == -INFINITY ? 0.f : -m);
+      const float2 from = f2s(m == -INFINITY ? 0.f : -m);
       float2 sum[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
 #pragma unroll
       for (int i = 0; i < BLK; i += 2) {
-        const float2 y = f2_fma(f2(x[i], x[i + 1]), sc, base);
+        const float2 y = f2_fma(f2(x[i], x[i + 1]), sc, from);
         x[i] = ex2(y.x);
         x[i + 1] = ex2(y.y);
         sum[(i / 2) & 1] = f2_add(sum[(i / 2) & 1], f2(x[i], x[i + 1]));
@@ -313,10 +321,10 @@ __global__ void __launch_bounds__(352, 1)
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[2 * t + ((n - 1) & 1)]);
+      if (lane == 0) bar_arrive(p_full + 16 * t + 8 * ((n - 1) & 1));
       // the last two products: a parity tells one phase from the next only
-      ok = (n < 2 || tc_wait(&o_done[t], (uint32_t)(n - 2) & 1u, stop, a.fault)) &&
-           tc_wait(&o_done[t], (uint32_t)(n - 1) & 1u, stop, a.fault);
+      ok = (n < 2 || bar_wait(o_done + 8 * t, (uint32_t)(n - 2) & 1u, waits)) &&
+           bar_wait(o_done + 8 * t, (uint32_t)(n - 1) & 1u, waits);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
     }

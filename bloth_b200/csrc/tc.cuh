@@ -39,70 +39,136 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return r;
 }
 
-// ------------------------------------------------------------------ waits
-// One test of phase `parity`: at once (mbar_test), or suspended for the default
-// time at most (mbar_try).
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+// --------------------------------------------------------------- barriers
+// Barriers are named by their 32-bit shared-memory address: the warps that
+// issue copies and products run little else than waits and address
+// arithmetic, one after the other, and every instruction there costs the
+// tensor core its latency.
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+               : "memory");
+}
+// One test of phase `parity`: at once (bar_test), or suspended for the default
+// time at most (bar_try).
+__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(done)
-      : "r"(smem_addr(bar)), "r"(parity)
+      : "r"(bar), "r"(parity)
       : "memory");
   return done != 0;
 }
-__device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t parity) {
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(done)
-      : "r"(smem_addr(bar)), "r"(parity)
+      : "r"(bar), "r"(parity)
       : "memory");
   return done != 0;
 }
 
-// Waits for phase `parity` of `bar`. False once the CTA has given up: when
-// this wait takes longer than kWaitLimitNs (recorded in the fault word), or
-// another thread's did (*stop, in shared memory).
-__device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, volatile int* stop,
-                                        unsigned int* fault) {
-  if (mbar_try(bar, parity)) return true;
-  const unsigned long long t0 = global_ns();
-  while (!mbar_try(bar, parity)) {
-    if (*stop) return false;
-    if (global_ns() - t0 > kWaitLimitNs) {
-      *stop = 1;
-      if (fault != nullptr) atomicOr(fault, kFaultCopyTimeout);
+// What a CTA's waits share: the flag (in shared memory) by which a thread
+// whose wait took longer than kWaitLimitNs makes all others give up, and the
+// device's fault word, where that is recorded.
+struct Waits {
+  volatile int* stop;
+  unsigned int* fault;
+};
+static __device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, Waits w) {
+  unsigned long long t0 = 0;
+  for (int i = 1;; ++i) {
+    if (bar_try(bar, parity)) return true;
+    // the time is read now and then only: reading it takes longer than most waits
+    if ((i & 63) != 0) continue;
+    if (*w.stop) return false;
+    const unsigned long long t = global_ns();
+    if (t0 == 0) t0 = t;
+    if (t - t0 > kWaitLimitNs) {
+      *w.stop = 1;
+      if (w.fault != nullptr) atomicOr(w.fault, kFaultCopyTimeout);
       return false;
     }
   }
-  return true;
+}
+// Waits for phase `parity` of `bar`; false once the CTA has given up.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, const Waits& w) {
+  if (bar_try(bar, parity)) return true;
+  return bar_wait_slow(bar, parity, w);
+}
+// After giving up: waits, as long again, for a copy or product in flight.
+__device__ __forceinline__ void bar_drain(uint32_t bar, uint32_t parity, const Waits& w) {
+  const unsigned long long t0 = global_ns();
+  while (!bar_try(bar, parity)) {
+    if (global_ns() - t0 > kWaitLimitNs) {
+      if (w.fault != nullptr) atomicOr(w.fault, kFaultDrainTimeout);
+      return;
+    }
+  }
 }
 
-// The same when a test of the phase made earlier (mbar_test), whose result
-// was not waited for, may have found it complete.
-__device__ __forceinline__ bool tc_wait(bool done, uint64_t* bar, uint32_t parity,
-                                        volatile int* stop, unsigned int* fault) {
-  return done || tc_wait(bar, parity, stop, fault);
-}
+// Stage and phase of a ring of barriers, advanced without a division.
+template <int STAGES>
+struct Ring {
+  uint32_t at = 0, phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++at == STAGES) {
+      at = 0;
+      phase ^= 1u;
+    }
+  }
+};
 
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+// True in one lane of a converged warp. The issuing warps run their loops as
+// a whole and let this lane issue, so that addresses and descriptors are
+// computed in uniform registers, where the instructions take them from.
+__device__ __forceinline__ bool elect() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
 }
 
 // ----------------------------------------------------------- tiled copies
 // One box of a 4-D tensor map (column, row, head, batch) into shared memory.
-__device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int col, int row,
-                                         int head, int batch, uint64_t* bar) {
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int col, int row,
+                                         int head, int batch, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-      "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_addr(dst)),
-      "l"(map), "r"(col), "r"(row), "r"(head), "r"(batch), "r"(smem_addr(bar))
+      "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(map), "r"(col), "r"(row), "r"(head), "r"(batch), "r"(bar)
       : "memory");
+}
+// `bytes` consecutive bytes, both addresses and the size multiples of 16.
+__device__ __forceinline__ void run_load(uint32_t dst, const void* src, uint32_t bytes,
+                                         uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          dst),
+      "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
+}
+// An operand tile of ROWS rows r0.. of a head: boxes of 64 rows x 64 columns.
+template <int D, int ROWS>
+__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, int r0, int h,
+                                          int b, uint32_t bar) {
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+    for (int r = 0; r < ROWS; r += 64)
+      tma_load(dst + c * ROWS * 128 + r * 128, map, c * 64, r0 + r, h, b, bar);
 }
 
 // ------------------------------------------------------------ descriptors
@@ -118,13 +184,6 @@ constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
 __device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t block) {
   return ((addr & 0x3ffff) >> 4) | ((block >> 4) << 16);
 }
-// Keeps the compiler from holding what it derives from x across iterations
-// (dozens of descriptors, in the registers that the softmax needs).
-__device__ __forceinline__ uint32_t opaque(uint32_t x) {
-  asm volatile("" : "+r"(x));
-  return x;
-}
-
 // Instruction descriptor: fp32 accumulator, A and B of type T, M x N, B's
 // contracted index along its rows (b_mn) or columns.
 template <typename T>
@@ -161,7 +220,7 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint3
 template <typename T, int D>
 __device__ __forceinline__ void product_rows(uint32_t d, uint32_t a, uint32_t b) {
   constexpr uint32_t id = mma_desc<T>(128, 64, false);
-  const uint32_t la = opaque(desc_lo(a, 0)), lb = opaque(desc_lo(b, 0));
+  const uint32_t la = desc_lo(a, 0), lb = desc_lo(b, 0);
 #pragma unroll
   for (int kk = 0; kk < D / 16; ++kk)
     mma_ss(d, la + (((kk / 4) * (128 * 128) + (kk % 4) * 32) >> 4),
@@ -172,14 +231,14 @@ __device__ __forceinline__ void product_rows(uint32_t d, uint32_t a, uint32_t b)
 template <typename T, int D>
 __device__ __forceinline__ void product_cols(uint32_t d, uint32_t w, uint32_t b, bool add) {
   constexpr uint32_t id = mma_desc<T>(128, D, true);
-  const uint32_t lb = opaque(desc_lo(b, 64 * 128));
+  const uint32_t lb = desc_lo(b, 64 * 128);
 #pragma unroll
   for (int kk = 0; kk < 4; ++kk) mma_ts(d, w + kk * 8, lb + kk * (2048 >> 4), id, add || kk > 0);
 }
 // `bar` completes a phase when every product issued so far has completed.
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   smem_addr(bar))
+                   bar)
                : "memory");
 }
 
@@ -274,17 +333,6 @@ __device__ __forceinline__ void store64(uint32_t at, const float (&x)[64]) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) r[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
   tmem_st32(at, r);
-}
-
-// An operand tile of ROWS rows r0.. of a head: boxes of 64 rows x 64 columns.
-template <int D, int ROWS>
-__device__ __forceinline__ void load_tile(unsigned char* dst, const CUtensorMap* map, int r0, int h,
-                                          int b, uint64_t* bar) {
-#pragma unroll
-  for (int c = 0; c < D / 64; ++c)
-#pragma unroll
-    for (int r = 0; r < ROWS; r += 64)
-      tma_load(dst + c * ROWS * 128 + r * 128, map, c * 64, r0 + r, h, b, bar);
 }
 
 // Rows [r0, 64) of an operand tile of 64 in shared memory become zeros, before
