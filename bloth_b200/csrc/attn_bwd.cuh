@@ -1,27 +1,31 @@
 // Attention backward on the tensor cores: 16-bit tensors, head_dim 64 or 128.
 //
 // Two kernels, each of which recomputes the probabilities p = 2^(s scale
-// log2 e - lse2) of a block of 128 queries x 128 keys from the rows'
-// statistics and writes each gradient element once:
+// log2 e - lse2) of a block of queries and keys from the rows' statistics and
+// writes each gradient element once:
 //   dK, dV: a CTA keeps 128 keys and streams the queries that see them, of
-//           every head of the group: S^T = K Q^T, dP^T = V dO^T,
-//           dV += P^T dO, dK += dS^T Q;
-//   dQ:     a CTA keeps 128 queries and streams keys: S = Q K^T,
-//           dP = dO V^T, dQ += dS K.
+//           every head of the group, in blocks of 64: S^T = K Q^T,
+//           dP^T = V dO^T, dV += P^T dO, dK += dS^T Q;
+//   dQ:     a CTA keeps 128 queries and streams keys in blocks of 64:
+//           S = Q K^T, dP = dO V^T, dQ += dS K.
 // Seven products instead of the five of a single kernel, whose dQ would be a
 // sum over CTAs: fp32 atomics, whose order changes the result, and a pass to
 // clear and one to round them (12 bytes an element of dQ and 4 more an
 // addition). The gradients here do not depend on scheduling.
 //
-// P^T, dS^T and dS are rounded to the tensors' type and stay in tensor memory
-// as the products' first operand; the streamed tiles are read by the products
-// both by rows and by columns, so nothing is transposed or stored again.
-// Thread = row of the kept tile, 64 of the block's columns: warps 0-3 columns
-// 0-63, warps 4-7 columns 64-127. Warp 8 issues the products, warp 9 the
-// copies.
+// P^T, dS^T and dS are rounded to the tensors' type and stay in tensor memory,
+// where S^T and dP lay, as the products' first operand; the streamed tiles are
+// read by the products both by rows and by columns, so nothing is transposed
+// or stored again. Blocks alternate between two buffers of S and of dP in
+// tensor memory and two groups of four warps (thread = row of the kept tile,
+// 64 columns): a group has two blocks' time for its own, so neither the
+// hand-over between warps nor its own latencies stop the tensor core. Warps 8
+// and 9 issue the products, warp 10 the copies.
 //
-// Bound: the products (128 x 128 x 128 in 512 cycles), 2048 cycles a block
-// for dK, dV and 1536 for dQ, beside 1024 for its exponentials.
+// Bound: the products. 64 streamed rows against 128 kept ones read 6 KB of
+// shared memory for 32 cycles of arithmetic: 384 cycles each for S and dP at
+// head_dim 128, 256 for dV, dK or dQ: 1280 cycles a block for dK and dV, 1024
+// for dQ, beside 512 for its exponentials.
 #pragma once
 
 #include "attn_impl.cuh"
@@ -31,67 +35,73 @@ namespace bloth {
 
 template <int D>
 struct BwdCfg {
-  static constexpr int TILE = 128;
-  static constexpr int THREADS = 320;
-  static constexpr int OPB = TILE * D * 2;     // bytes of one operand tile
-  // Stages of Q (or K) and of dO (or V). Q and K are read by a block's first
-  // and its last product, so two stages leave a copy less than a block's time;
-  // dO and V are free after half of it. D = 128, 8192 full rows of 32/8 heads:
-  // @@STAGES@@
-  static constexpr int NA = D == 64 ? 4 : 3, NB = D == 64 ? 4 : 2;
-  static constexpr int OWN_OFF = 0;                // the two kept tiles
-  static constexpr int A_OFF = 2 * OPB;            // stages of Q (or K)
-  static constexpr int B_OFF = A_OFF + NA * OPB;   // stages of dO (or V)
-  static constexpr int STAT_OFF = B_OFF + NB * OPB;  // lse2 and delta, with dO's stages
-  static constexpr int BAR_OFF = STAT_OFF + NB * 1024;
-  static constexpr int BARS = 1 + 2 * NA + 2 * NB + 8;
+  static constexpr int TILE = 128;             // rows of the kept tiles
+  static constexpr int BLK = 64;               // rows of a streamed block
+  static constexpr int THREADS = 352;
+  static constexpr int OWNB = TILE * D * 2, STRB = BLK * D * 2;  // bytes of a tile
+  static constexpr int NST = D == 64 ? 8 : 5;  // stages of each streamed tensor
+  static constexpr int OWN_OFF = 0;                  // the two kept tiles
+  static constexpr int A_OFF = 2 * OWNB;             // stages of Q (or K)
+  static constexpr int B_OFF = A_OFF + NST * STRB;   // stages of dO (or V)
+  static constexpr int STAT_OFF = B_OFF + NST * STRB;  // lse2 and delta, with dO's stages
+  static constexpr int BAR_OFF = STAT_OFF + NST * 512;
+  static constexpr int BARS = 1 + 4 * NST + 8 + 3;
   static constexpr int SMEM = BAR_OFF + BARS * 8 + 16;
-  static constexpr uint32_t COLS = 512;
   static_assert(SMEM <= 227 * 1024, "shared memory");
+  // tensor-memory columns: S (two buffers), dP (two buffers), the sums
+  static constexpr uint32_t COLS = 512;
+  static constexpr uint32_t S_COL = 0, DP_COL = 128, ACC_COL = 256;
 };
 
 struct BwdMaps {
   CUtensorMap q, k, v, dout;
 };
 
-// One operand tile: rows r0.. of a head, D / 64 boxes.
-template <int D>
-__device__ __forceinline__ void load_tile(unsigned char* dst, const CUtensorMap* map, int r0, int h,
-                                          int b, uint64_t* bar) {
-#pragma unroll
-  for (int c = 0; c < D / 64; ++c) tma_load(dst + c * 128 * 128, map, c * 64, r0, h, b, bar);
-}
-
-// Rows [r0, 128) of an operand tile in shared memory become zeros (256 threads).
-template <int D>
-__device__ __forceinline__ void zero_rows(unsigned char* tile, int r0) {
-  for (int c = threadIdx.x; c < (128 - r0) * (D / 8); c += 256) {
-    const int r = r0 + c / (D / 8), b = c % (D / 8);
-    *reinterpret_cast<uint4*>(tile + (b / 8) * (128 * 128) + r * 128 + (b % 8) * 16) =
-        make_uint4(0, 0, 0, 0);
+// Barriers of both kernels; A and B are the streamed tensors (Q and dO, or K
+// and V), [2] one for each buffer.
+template <int NST>
+struct BwdBars {
+  uint32_t own, a_full, a_free, b_full, b_free, s_full, p_full, dp_full, ds_full, acc, drained;
+  __device__ __forceinline__ explicit BwdBars(uint32_t at) {
+    own = at;
+    a_full = own + 8;
+    a_free = a_full + 8 * NST;
+    b_full = a_free + 8 * NST;
+    b_free = b_full + 8 * NST;
+    s_full = b_free + 8 * NST;
+    p_full = s_full + 16;
+    dp_full = p_full + 16;
+    ds_full = dp_full + 16;
+    acc = ds_full + 16;
+    drained = acc + 8;
   }
-  fence_proxy_async_smem();
-}
-
-// 64 columns of the thread's row.
-__device__ __forceinline__ void load64(uint32_t at, float (&x)[64]) {
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    uint32_t r[32];
-    tmem_ld32(at + c * 32, r);
-#pragma unroll
-    for (int i = 0; i < 32; ++i) x[c * 32 + i] = __uint_as_float(r[i]);
+  // b_free completes with `b_uses` arrivals, acc with `sums`
+  __device__ __forceinline__ void init(int b_uses, int sums) const {
+    bar_init(own, 1);
+    for (int i = 0; i < NST; ++i) {
+      bar_init(a_full + 8 * i, 1);
+      bar_init(a_free + 8 * i, 1);
+      bar_init(b_full + 8 * i, 1);
+      bar_init(b_free + 8 * i, b_uses);
+    }
+    for (int i = 0; i < 2; ++i) {
+      bar_init(s_full + 8 * i, 1);
+      bar_init(p_full + 8 * i, 4);
+      bar_init(dp_full + 8 * i, 1);
+      bar_init(ds_full + 8 * i, 4);
+      bar_init(drained + 8 * i, 1);
+    }
+    bar_init(acc, sums);
   }
-  tmem_wait_ld();
-}
-template <typename T>
-__device__ __forceinline__ void store64(uint32_t at, const float (&x)[64]) {
-  uint32_t r[32];
-#pragma unroll
-  for (int i = 0; i < 32; ++i) r[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
-  tmem_st32(at, r);
-  tmem_wait_st();
-}
+  // given up: not before the copies in flight have landed (blocks [0, it))
+  __device__ __forceinline__ void drain_copies(int it, const Waits& w) const {
+    bar_drain(own, 0, w);
+    for (int i = max(0, it - NST); i < it; ++i) {
+      bar_drain(a_full + 8 * (i % NST), (uint32_t)(i / NST) & 1u, w);
+      bar_drain(b_full + 8 * (i % NST), (uint32_t)(i / NST) & 1u, w);
+    }
+  }
+};
 
 // `cols` accumulator columns of the thread's row, times f, to 16-bit memory
 // (in), or zeros (!keep). `any`, alike in the whole warp: there are sums.
@@ -122,28 +132,18 @@ __device__ __forceinline__ void store_row(uint32_t at, int cols, float f, T* dst
 
 // ------------------------------------------------------------------ dK, dV
 template <typename T, int D>
-__global__ void __launch_bounds__(320, 1)
+__global__ void __launch_bounds__(352, 1)
     attn_dkv_kernel(const AttnArgs a, const __grid_constant__ BwdMaps maps) {
   using C = BwdCfg<D>;
-  constexpr int N = C::TILE, NA = C::NA, NB = C::NB;
-  // tensor-memory columns: S^T (then P^T), dP^T (then dS^T), dV, dK
-  constexpr uint32_t S_COL = 0, DP_COL = 128, DV_COL = 256, DK_COL = 256 + D;
+  constexpr int N = C::TILE, BLK = C::BLK, NST = C::NST;
+  constexpr uint32_t DV_COL = C::ACC_COL, DK_COL = C::ACC_COL + D;
   extern __shared__ __align__(1024) unsigned char smem[];
-  uint64_t* own_full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
-  uint64_t* q_full = own_full + 1;
-  uint64_t* q_free = q_full + NA;
-  uint64_t* o_full = q_free + NA;  // dO and the statistics
-  uint64_t* o_free = o_full + NB;
-  uint64_t* s_full = o_free + NB;
-  uint64_t* p_full = s_full + 1;
-  uint64_t* dp_full = p_full + 1;
-  uint64_t* ds_full = dp_full + 1;
-  uint64_t* acc_full = ds_full + 1;
-  uint64_t* drained = acc_full + 1;
-  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(own_full + C::BARS);
-  volatile int* stop = reinterpret_cast<volatile int*>(tmem_ptr + 1);
+  const uint32_t base = smem_addr(smem);
+  const BwdBars<NST> bar(base + C::BAR_OFF);
+  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(smem + C::BAR_OFF + 8 * C::BARS);
+  const Waits waits{reinterpret_cast<volatile int*>(tmem_ptr + 1), a.fault};
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int heads = a.Hk * a.B;
   const int hb = blockIdx.x % heads, h = hb % a.Hk;
   // the first keys are seen by most queries (causal): they start first
@@ -154,28 +154,14 @@ __global__ void __launch_bounds__(320, 1)
   if (n0 >= limit) return;
   int lo, hi;
   query_range(a, s, n0, min(n0 + N, s.klen), lo, hi);
-  const int mb = lo / N, nm = hi > lo ? (hi + N - 1) / N - mb : 0;  // query blocks per head
+  const int mb = lo / BLK, nm = hi > lo ? (hi + BLK - 1) / BLK - mb : 0;  // blocks per head
   const int total = nm * a.G;
 
   if (warp == 8) {
     tmem_alloc(tmem_ptr, C::COLS);
   } else if (threadIdx.x == 0) {
-    mbar_init(own_full, 1);
-    for (int i = 0; i < NA; ++i) {
-      mbar_init(&q_full[i], 1);
-      mbar_init(&q_free[i], 1);
-    }
-    for (int i = 0; i < NB; ++i) {
-      mbar_init(&o_full[i], 1);
-      mbar_init(&o_free[i], 1);
-    }
-    mbar_init(s_full, 1);
-    mbar_init(p_full, 8);
-    mbar_init(dp_full, 1);
-    mbar_init(ds_full, 8);
-    mbar_init(acc_full, 1);
-    mbar_init(drained, 1);
-    *stop = 0;
+    bar.init(2, 2);
+    *waits.stop = 0;
     mbar_init_fence();
   }
   tc_fence_before();
@@ -183,129 +169,184 @@ __global__ void __launch_bounds__(320, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_ptr;
 
-  if (warp == 9) {
+  if (warp == 10) {
+    // ------------------------------------------------------------- copies
     if (lane == 0 && total > 0) {
-      mbar_arrive_expect_tx(own_full, 2 * C::OPB);
-      load_tile<D>(smem + C::OWN_OFF, &maps.k, s.k0 + n0, h, s.b, own_full);
-      load_tile<D>(smem + C::OWN_OFF + C::OPB, &maps.v, s.k0 + n0, h, s.b, own_full);
-      int it = 0;
-      for (; it < total; ++it) {
-        const int sa = it % NA, sb = it % NB;
-        const uint32_t pa = (uint32_t)(it / NA) & 1u, pb = (uint32_t)(it / NB) & 1u;
-        const int hq = h * a.G + it / nm, m0 = (mb + it % nm) * N;
+      bar_expect(bar.own, 2 * C::OWNB);
+      load_tile<D, N>(base + C::OWN_OFF, &maps.k, s.k0 + n0, h, s.b, bar.own);
+      load_tile<D, N>(base + C::OWN_OFF + C::OWNB, &maps.v, s.k0 + n0, h, s.b, bar.own);
+      Ring<NST> st;
+      int it = 0, mi = 0, hq = h * a.G;
+      for (; it < total; ++it, st.next()) {
+        const int m0 = (mb + mi) * BLK;
         const int64_t stat = (int64_t)hq * a.R + s.stat0 + m0;
-        unsigned char* sp = smem + C::STAT_OFF + sb * 1024;
-        if (!tc_wait(&q_free[sa], pa ^ 1u, stop, a.fault)) break;
-        mbar_arrive_expect_tx(&q_full[sa], C::OPB);
-        load_tile<D>(smem + C::A_OFF + sa * C::OPB, &maps.q, s.q0 + m0, hq, s.b, &q_full[sa]);
-        if (!tc_wait(&o_free[sb], pb ^ 1u, stop, a.fault)) {
-          mbar_wait(&q_full[sa], pa, nullptr);
+        const uint32_t qf = bar.a_full + 8 * st.at, of = bar.b_full + 8 * st.at;
+        const uint32_t sp = base + C::STAT_OFF + st.at * 512;
+        if (!bar_wait(bar.a_free + 8 * st.at, st.phase ^ 1u, waits)) break;
+        bar_expect(qf, C::STRB);
+        load_tile<D, BLK>(base + C::A_OFF + st.at * C::STRB, &maps.q, s.q0 + m0, hq, s.b, qf);
+        if (!bar_wait(bar.b_free + 8 * st.at, st.phase ^ 1u, waits)) {
+          bar_drain(qf, st.phase, waits);
           break;
         }
-        mbar_arrive_expect_tx(&o_full[sb], C::OPB + 1024);
-        bulk_load(sp, a.lse2 + stat, 512, &o_full[sb]);
-        bulk_load(sp + 512, a.delta + stat, 512, &o_full[sb]);
-        load_tile<D>(smem + C::B_OFF + sb * C::OPB, &maps.dout, s.q0 + m0, hq, s.b, &o_full[sb]);
+        bar_expect(of, C::STRB + 512);
+        run_load(sp, a.lse2 + stat, 256, of);
+        run_load(sp + 256, a.delta + stat, 256, of);
+        load_tile<D, BLK>(base + C::B_OFF + st.at * C::STRB, &maps.dout, s.q0 + m0, hq, s.b, of);
+        if (++mi == nm) {
+          mi = 0;
+          ++hq;
+        }
       }
-      if (*stop) {  // given up: not before the copies in flight have landed
-        mbar_wait(own_full, 0, nullptr);
-        for (int i = max(0, it - NA); i < it; ++i)
-          mbar_wait(&q_full[i % NA], (uint32_t)(i / NA) & 1u, nullptr);
-        for (int i = max(0, it - NB); i < it; ++i)
-          mbar_wait(&o_full[i % NB], (uint32_t)(i / NB) & 1u, nullptr);
-      }
+      if (*waits.stop) bar.drain_copies(it, waits);
     }
   } else if (warp == 8) {
-    if (lane == 0 && total > 0) {
-      const uint32_t ka = smem_addr(smem + C::OWN_OFF), va = ka + C::OPB;
-      const uint32_t qa = smem_addr(smem + C::A_OFF), oa = smem_addr(smem + C::B_OFF);
-      bool ok = tc_wait(own_full, 0, stop, a.fault) && tc_wait(&q_full[0], 0, stop, a.fault);
-      if (ok) {
-        product_rows<T, D>(tmem + S_COL, ka, qa);
-        mma_commit(s_full);
-        ok = tc_wait(&o_full[0], 0, stop, a.fault);
-      }
-      if (ok) {
-        product_rows<T, D>(tmem + DP_COL, va, oa);
-        mma_commit(dp_full);
-      }
-      for (int it = 0; ok && it < total; ++it) {
-        const int sa = it % NA, sb = it % NB, na = (it + 1) % NA, nb = (it + 1) % NB;
-        if (!(ok = tc_wait(p_full, it & 1, stop, a.fault))) break;
-        tc_fence_after();
-        product_cols<T, D>(tmem + DV_COL, tmem + S_COL, 64, oa + sb * C::OPB, it > 0);
-        if (it + 1 < total) {
-          if (!(ok = tc_wait(&q_full[na], (uint32_t)((it + 1) / NA) & 1u, stop, a.fault))) break;
-          product_rows<T, D>(tmem + S_COL, ka, qa + na * C::OPB);
-          mma_commit(s_full);
+    // S^T and dV: P^T lies where S^T was, so S^T of block j follows dV of j - 2
+    if (total > 0) {
+      const uint32_t ka = base + C::OWN_OFF;
+      const bool lead = elect();
+      Ring<NST> qst, ost;
+      Ring<2> buf, pbuf;
+      bool ok = bar_wait(bar.own, 0, waits);
+      for (int j = 0; ok && j < total + 2; ++j) {
+        if (j >= 2) {
+          ok = bar_wait(bar.b_full + 8 * ost.at, ost.phase, waits) &&
+               bar_wait(bar.p_full + 8 * pbuf.at, pbuf.phase, waits);
+          if (!ok) break;
+          tc_fence_after();
+          if (lead) {
+            product_cols<T, D>(tmem + DV_COL, tmem + C::S_COL + pbuf.at * BLK,
+                               base + C::B_OFF + ost.at * C::STRB, j > 2);
+            mma_commit(bar.b_free + 8 * ost.at);
+          }
+          ost.next();
+          pbuf.next();
         }
-        if (!(ok = tc_wait(ds_full, it & 1, stop, a.fault))) break;
-        tc_fence_after();
-        product_cols<T, D>(tmem + DK_COL, tmem + DP_COL, 64, qa + sa * C::OPB, it > 0);
-        mma_commit(&q_free[sa]);
-        mma_commit(&o_free[sb]);  // not before dS: the statistics lie with dO
-        if (it + 1 < total) {
-          if (!(ok = tc_wait(&o_full[nb], (uint32_t)((it + 1) / NB) & 1u, stop, a.fault))) break;
-          product_rows<T, D>(tmem + DP_COL, va, oa + nb * C::OPB);
-          mma_commit(dp_full);
+        if (j < total) {
+          ok = bar_wait(bar.a_full + 8 * qst.at, qst.phase, waits);
+          if (!ok) break;
+          if (lead) {
+            product_rows<T, D>(tmem + C::S_COL + buf.at * BLK, ka,
+                               base + C::A_OFF + qst.at * C::STRB);
+            mma_commit(bar.s_full + 8 * buf.at);
+          }
+          qst.next();
+          buf.next();
         }
       }
-      mma_commit(ok ? acc_full : drained);
-      if (!ok) mbar_wait(drained, 0, nullptr);
+      if (lead) {
+        mma_commit(ok ? bar.acc : bar.drained);
+        if (!ok) bar_drain(bar.drained, 0, waits);
+      }
+      __syncwarp();
+    }
+  } else if (warp == 9) {
+    // dP^T and dK, dS^T where dP^T was
+    if (total > 0) {
+      const uint32_t va = base + C::OWN_OFF + C::OWNB;
+      const bool lead = elect();
+      Ring<NST> qst, ost;
+      Ring<2> buf, dbuf;
+      uint32_t done = 0;  // stage whose statistics the group has read
+      bool ok = bar_wait(bar.own, 0, waits);
+      for (int j = 0; ok && j < total + 2; ++j) {
+        if (j >= 2) {
+          ok = bar_wait(bar.a_full + 8 * qst.at, qst.phase, waits) &&
+               bar_wait(bar.ds_full + 8 * dbuf.at, dbuf.phase, waits);
+          if (!ok) break;
+          tc_fence_after();
+          if (lead) {
+            product_cols<T, D>(tmem + DK_COL, tmem + C::DP_COL + dbuf.at * BLK,
+                               base + C::A_OFF + qst.at * C::STRB, j > 2);
+            mma_commit(bar.a_free + 8 * qst.at);
+            // dP^T of that block has completed with dS^T, which the statistics
+            // beside dO went into
+            bar_arrive(bar.b_free + 8 * done);
+          }
+          if (++done == NST) done = 0;
+          qst.next();
+          dbuf.next();
+        }
+        if (j < total) {
+          ok = bar_wait(bar.b_full + 8 * ost.at, ost.phase, waits);
+          if (!ok) break;
+          if (lead) {
+            product_rows<T, D>(tmem + C::DP_COL + buf.at * BLK, va,
+                               base + C::B_OFF + ost.at * C::STRB);
+            mma_commit(bar.dp_full + 8 * buf.at);
+          }
+          ost.next();
+          buf.next();
+        }
+      }
+      if (lead) {
+        mma_commit(ok ? bar.acc : bar.drained + 8);
+        if (!ok) bar_drain(bar.drained + 8, 0, waits);
+      }
+      __syncwarp();
     }
   } else {
-    const int half = warp >> 2, r = threadIdx.x & 127;
+    // ------------------------------------------- blocks `group`, group + 2, ...
+    const int group = warp >> 2, r = threadIdx.x & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const int key = n0 + r, off = s.klen - s.qlen;
-    const uint32_t s_at = tmem + lanes + S_COL + half * 64;
-    const uint32_t dp_at = tmem + lanes + DP_COL + half * 64;
+    const uint32_t s_at = tmem + lanes + C::S_COL + group * BLK;
+    const uint32_t dp_at = tmem + lanes + C::DP_COL + group * BLK;
+    const float2 sc = f2s(a.scale_log2);
+    Ring<NST> st;
+    int mi = 0;
+    if (group) {
+      st.next();
+      mi = nm > 1 ? 1 : 0;
+    }
+    uint32_t ph = 0;
     bool ok = true;
-    for (int it = 0; it < total; ++it) {
-      const int sa = it % NA, sb = it % NB;
-      const int m0 = (mb + it % nm) * N;
-      const float* stat = reinterpret_cast<const float*>(smem + C::STAT_OFF + sb * 1024);
-      ok = tc_wait(&o_full[sb], (uint32_t)(it / NB) & 1u, stop, a.fault) &&
-           tc_wait(s_full, it & 1, stop, a.fault);
+    for (int it = group; it < total; it += 2, ph ^= 1u) {
+      const int m0 = (mb + mi) * BLK;
+      const float* stat = reinterpret_cast<const float*>(smem + C::STAT_OFF + st.at * 512);
+      ok = bar_wait(bar.b_full + 8 * st.at, st.phase, waits) &&
+           bar_wait(bar.s_full + 8 * group, ph, waits);
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       tc_fence_after();
-      float x[64];
+      float x[BLK];
       load64(s_at, x);
 #pragma unroll
-      for (int i = 0; i < 64; i += 4) {
-        const float4 l = *reinterpret_cast<const float4*>(stat + half * 64 + i);
-        const float2 u = f2_fma(f2(x[i], x[i + 1]), f2s(a.scale_log2), f2(-l.x, -l.y));
-        const float2 w = f2_fma(f2(x[i + 2], x[i + 3]), f2s(a.scale_log2), f2(-l.z, -l.w));
+      for (int i = 0; i < BLK; i += 4) {
+        const float4 l = *reinterpret_cast<const float4*>(stat + i);
+        const float2 u = f2_fma(f2(x[i], x[i + 1]), sc, f2(-l.x, -l.y));
+        const float2 w = f2_fma(f2(x[i + 2], x[i + 3]), sc, f2(-l.z, -l.w));
         x[i] = ex2(u.x);
         x[i + 1] = ex2(u.y);
         x[i + 2] = ex2(w.x);
         x[i + 3] = ex2(w.y);
       }
-      // columns of this thread's 64 that see its key: [from, to)
-      const int c0 = m0 + half * 64;
-      const int from = a.causal ? key - off - c0 : 0;
-      const int to = min(s.qlen, a.window ? key - off + a.window : s.qlen) - c0;
-      const bool masked = m0 + N > s.qlen || (a.causal && n0 + N - 1 - off > m0) ||
-                          (a.window && n0 - off + a.window < m0 + N);
-      const bool tail = m0 + N > s.qlen && s.q0 + s.qlen < a.Sq;
+      // the block's columns that see this thread's key: [from, to)
+      const int from = a.causal ? key - off - m0 : 0;
+      const int to = min(s.qlen, a.window ? key - off + a.window : s.qlen) - m0;
+      const bool masked = m0 + BLK > s.qlen || (a.causal && n0 + N - 1 - off > m0) ||
+                          (a.window && n0 - off + a.window < m0 + BLK);
+      const bool tail = m0 + BLK > s.qlen && s.q0 + s.qlen < a.Sq;
       if (masked) {
 #pragma unroll
-        for (int i = 0; i < 64; ++i)
+        for (int i = 0; i < BLK; ++i)
           if (i < from || i >= to) x[i] = 0.f;
         // rows of dO past the sequence's end that memory does hold
-        if (tail) zero_rows<D>(smem + C::B_OFF + sb * C::OPB, s.qlen - m0);
+        if (tail) zero_rows<D>(smem + C::B_OFF + st.at * C::STRB, s.qlen - m0);
       }
       store64<T>(s_at, x);
+      const bool there = bar_test(bar.dp_full + 8 * group, ph);
+      tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_full);
-      ok = __all_sync(0xffffffffu, tc_wait(dp_full, it & 1, stop, a.fault));
+      if (lane == 0) bar_arrive(bar.p_full + 8 * group);
+      ok = __all_sync(0xffffffffu, there || bar_wait(bar.dp_full + 8 * group, ph, waits));
       if (!ok) break;
       tc_fence_after();
-      float y[64];
+      float y[BLK];
       load64(dp_at, y);
 #pragma unroll
-      for (int i = 0; i < 64; i += 4) {
-        const float4 d = *reinterpret_cast<const float4*>(stat + 128 + half * 64 + i);
+      for (int i = 0; i < BLK; i += 4) {
+        const float4 d = *reinterpret_cast<const float4*>(stat + 64 + i);
         const float2 u = f2_mul(f2(x[i], x[i + 1]), f2_add(f2(y[i], y[i + 1]), f2(-d.x, -d.y)));
         const float2 w =
             f2_mul(f2(x[i + 2], x[i + 3]), f2_add(f2(y[i + 2], y[i + 3]), f2(-d.z, -d.w)));
@@ -316,25 +357,32 @@ __global__ void __launch_bounds__(320, 1)
       }
       if (masked) {
 #pragma unroll
-        for (int i = 0; i < 64; ++i)
+        for (int i = 0; i < BLK; ++i)
           if (i < from || i >= to) y[i] = 0.f;
-        if (tail) zero_rows<D>(smem + C::A_OFF + sa * C::OPB, s.qlen - m0);
+        if (tail) zero_rows<D>(smem + C::A_OFF + st.at * C::STRB, s.qlen - m0);
       }
       store64<T>(dp_at, y);
+      tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(ds_full);
+      if (lane == 0) bar_arrive(bar.ds_full + 8 * group);
+      st.next();
+      st.next();
+      mi += 2;
+      if (mi >= nm) mi -= nm;
+      if (mi >= nm) mi -= nm;  // nm == 1
     }
     if (ok && total > 0) {
-      ok = __all_sync(0xffffffffu, tc_wait(acc_full, 0, stop, a.fault));
+      ok = __all_sync(0xffffffffu, bar_wait(bar.acc, 0, waits));
       tc_fence_after();
     }
     if (ok) {
-      const HT& t = half ? a.dk : a.dv;
+      // group 0 writes dV, group 1 dK; keys past the sequence's end (dense
+      // tensors) get zeros
+      const HT& t = group ? a.dk : a.dv;
       T* dst = reinterpret_cast<T*>(const_cast<void*>(t.p)) + (int64_t)s.b * t.sb +
                (int64_t)h * t.sh + (int64_t)(s.k0 + key) * t.ss;
-      // keys past the sequence's end (dense tensors) get zeros
-      store_row<T>(tmem + lanes + (half ? DK_COL : DV_COL), D, half ? a.scale : 1.f, dst,
+      store_row<T>(tmem + lanes + (group ? DK_COL : DV_COL), D, group ? a.scale : 1.f, dst,
                    key < limit, key < s.klen, total > 0);
     }
   }
@@ -346,30 +394,21 @@ __global__ void __launch_bounds__(320, 1)
 
 // ---------------------------------------------------------------------- dQ
 template <typename T, int D>
-__global__ void __launch_bounds__(320, 1)
+__global__ void __launch_bounds__(352, 1)
     attn_dq_kernel(const AttnArgs a, const __grid_constant__ BwdMaps maps) {
   using C = BwdCfg<D>;
-  constexpr int N = C::TILE, NA = C::NA, NB = C::NB;
-  // tensor-memory columns: S, dP, dQ, and two buffers of dS
-  constexpr uint32_t S_COL = 0, DP_COL = 128, DQ_COL = 256, DS_COL = 384;
+  constexpr int N = C::TILE, BLK = C::BLK, NST = C::NST;
   extern __shared__ __align__(1024) unsigned char smem[];
-  uint64_t* own_full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
-  uint64_t* k_full = own_full + 1;
-  uint64_t* k_free = k_full + NA;
-  uint64_t* v_full = k_free + NA;
-  uint64_t* v_free = v_full + NB;
-  uint64_t* sdp_full = v_free + NB;
-  uint64_t* read = sdp_full + 1;  // S and dP are in registers
-  uint64_t* ds_full = read + 1;
-  uint64_t* acc_full = ds_full + 1;
-  uint64_t* drained = acc_full + 1;
-  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(own_full + C::BARS);
-  volatile int* stop = reinterpret_cast<volatile int*>(tmem_ptr + 1);
+  const uint32_t base = smem_addr(smem);
+  const BwdBars<NST> bar(base + C::BAR_OFF);
+  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(smem + C::BAR_OFF + 8 * C::BARS);
+  const Waits waits{reinterpret_cast<volatile int*>(tmem_ptr + 1), a.fault};
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int heads = a.Hq * a.B;
   const int tiles = (int)(gridDim.x / heads);
   const int hb = blockIdx.x % heads, h = hb % a.Hq;
+  // the last queries see most keys (causal): they start first
   const AttnSeq s = find_seq<true>(a, hb / a.Hq, tiles - 1 - (int)(blockIdx.x / heads), N);
   if (s.tile < 0) return;
   const int m0 = s.tile * N;
@@ -377,26 +416,13 @@ __global__ void __launch_bounds__(320, 1)
   if (m0 >= limit) return;
   int lo, hi;
   key_range(a, s, m0, min(m0 + N, s.qlen), lo, hi);
-  const int b0 = lo / N, total = hi > lo ? (hi + N - 1) / N - b0 : 0;
+  const int b0 = lo / BLK, total = hi > lo ? (hi + BLK - 1) / BLK - b0 : 0;
 
   if (warp == 8) {
     tmem_alloc(tmem_ptr, C::COLS);
   } else if (threadIdx.x == 0) {
-    mbar_init(own_full, 1);
-    for (int i = 0; i < NA; ++i) {
-      mbar_init(&k_full[i], 1);
-      mbar_init(&k_free[i], 1);
-    }
-    for (int i = 0; i < NB; ++i) {
-      mbar_init(&v_full[i], 1);
-      mbar_init(&v_free[i], 1);
-    }
-    mbar_init(sdp_full, 1);
-    mbar_init(read, 8);
-    mbar_init(ds_full, 8);
-    mbar_init(acc_full, 1);
-    mbar_init(drained, 1);
-    *stop = 0;
+    bar.init(1, 1);
+    *waits.stop = 0;
     mbar_init_fence();
   }
   tc_fence_before();
@@ -404,114 +430,159 @@ __global__ void __launch_bounds__(320, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_ptr;
 
-  if (warp == 9) {
+  if (warp == 10) {
+    // ------------------------------------------------------------- copies
     if (lane == 0 && total > 0) {
-      mbar_arrive_expect_tx(own_full, 2 * C::OPB);
-      load_tile<D>(smem + C::OWN_OFF, &maps.q, s.q0 + m0, h, s.b, own_full);
-      load_tile<D>(smem + C::OWN_OFF + C::OPB, &maps.dout, s.q0 + m0, h, s.b, own_full);
-      int it = 0;
-      for (; it < total; ++it) {
-        const int sa = it % NA, sb = it % NB;
-        const uint32_t pa = (uint32_t)(it / NA) & 1u, pb = (uint32_t)(it / NB) & 1u;
-        const int r0 = s.k0 + (b0 + it) * N;
-        if (!tc_wait(&k_free[sa], pa ^ 1u, stop, a.fault)) break;
-        mbar_arrive_expect_tx(&k_full[sa], C::OPB);
-        load_tile<D>(smem + C::A_OFF + sa * C::OPB, &maps.k, r0, h / a.G, s.b, &k_full[sa]);
-        if (!tc_wait(&v_free[sb], pb ^ 1u, stop, a.fault)) {
-          mbar_wait(&k_full[sa], pa, nullptr);
+      bar_expect(bar.own, 2 * C::OWNB);
+      load_tile<D, N>(base + C::OWN_OFF, &maps.q, s.q0 + m0, h, s.b, bar.own);
+      load_tile<D, N>(base + C::OWN_OFF + C::OWNB, &maps.dout, s.q0 + m0, h, s.b, bar.own);
+      const int hk = h / a.G;
+      Ring<NST> st;
+      int it = 0, r0 = s.k0 + b0 * BLK;
+      for (; it < total; ++it, r0 += BLK, st.next()) {
+        const uint32_t kf = bar.a_full + 8 * st.at, vf = bar.b_full + 8 * st.at;
+        if (!bar_wait(bar.a_free + 8 * st.at, st.phase ^ 1u, waits)) break;
+        bar_expect(kf, C::STRB);
+        load_tile<D, BLK>(base + C::A_OFF + st.at * C::STRB, &maps.k, r0, hk, s.b, kf);
+        if (!bar_wait(bar.b_free + 8 * st.at, st.phase ^ 1u, waits)) {
+          bar_drain(kf, st.phase, waits);
           break;
         }
-        mbar_arrive_expect_tx(&v_full[sb], C::OPB);
-        load_tile<D>(smem + C::B_OFF + sb * C::OPB, &maps.v, r0, h / a.G, s.b, &v_full[sb]);
+        bar_expect(vf, C::STRB);
+        load_tile<D, BLK>(base + C::B_OFF + st.at * C::STRB, &maps.v, r0, hk, s.b, vf);
       }
-      if (*stop) {
-        mbar_wait(own_full, 0, nullptr);
-        for (int i = max(0, it - NA); i < it; ++i)
-          mbar_wait(&k_full[i % NA], (uint32_t)(i / NA) & 1u, nullptr);
-        for (int i = max(0, it - NB); i < it; ++i)
-          mbar_wait(&v_full[i % NB], (uint32_t)(i / NB) & 1u, nullptr);
-      }
+      if (*waits.stop) bar.drain_copies(it, waits);
     }
   } else if (warp == 8) {
-    if (lane == 0 && total > 0) {
-      const uint32_t qa = smem_addr(smem + C::OWN_OFF), oa = qa + C::OPB;
-      const uint32_t ka = smem_addr(smem + C::A_OFF), va = smem_addr(smem + C::B_OFF);
-      bool ok = tc_wait(own_full, 0, stop, a.fault);
-      // S and dP of block it are issued once those of it - 1 are in registers,
-      // dQ's product of it - 1 after them
-      for (int it = 0; ok && it <= total; ++it) {
-        const int sa = it % NA, sb = it % NB, sp = (it + NA - 1) % NA;
-        if (it < total) {
-          if (!(ok = tc_wait(&k_full[sa], (uint32_t)(it / NA) & 1u, stop, a.fault))) break;
-          if (it > 0 && !(ok = tc_wait(read, (it - 1) & 1, stop, a.fault))) break;
-          tc_fence_after();
-          product_rows<T, D>(tmem + S_COL, qa, ka + sa * C::OPB);
-          if (!(ok = tc_wait(&v_full[sb], (uint32_t)(it / NB) & 1u, stop, a.fault))) break;
-          product_rows<T, D>(tmem + DP_COL, oa, va + sb * C::OPB);
-          mma_commit(sdp_full);
-          mma_commit(&v_free[sb]);
+    // S, into the buffer that the group has read when its dS is there
+    if (total > 0) {
+      const uint32_t qa = base + C::OWN_OFF;
+      const bool lead = elect();
+      Ring<NST> st;
+      Ring<2> buf;
+      bool ok = bar_wait(bar.own, 0, waits);
+      for (int j = 0; ok && j < total; ++j) {
+        ok = bar_wait(bar.a_full + 8 * st.at, st.phase, waits);
+        if (ok && j >= 2) ok = bar_wait(bar.ds_full + 8 * buf.at, buf.phase ^ 1u, waits);
+        if (!ok) break;
+        tc_fence_after();
+        if (lead) {
+          product_rows<T, D>(tmem + C::S_COL + buf.at * BLK, qa,
+                             base + C::A_OFF + st.at * C::STRB);
+          mma_commit(bar.s_full + 8 * buf.at);
         }
-        if (it > 0) {
-          if (!(ok = tc_wait(ds_full, (it - 1) & 1, stop, a.fault))) break;
+        st.next();
+        buf.next();
+      }
+      if (!ok && lead) {
+        mma_commit(bar.drained);
+        bar_drain(bar.drained, 0, waits);
+      }
+      __syncwarp();
+    }
+  } else if (warp == 9) {
+    // dP and dQ: dS lies where dP was, so dP of block j follows dQ of j - 2
+    if (total > 0) {
+      const uint32_t oa = base + C::OWN_OFF + C::OWNB;
+      const bool lead = elect();
+      Ring<NST> kst, vst;
+      Ring<2> buf, dbuf;
+      bool ok = bar_wait(bar.own, 0, waits);
+      for (int j = 0; ok && j < total + 2; ++j) {
+        if (j >= 2) {
+          ok = bar_wait(bar.a_full + 8 * kst.at, kst.phase, waits) &&
+               bar_wait(bar.ds_full + 8 * dbuf.at, dbuf.phase, waits);
+          if (!ok) break;
           tc_fence_after();
-          product_cols<T, D>(tmem + DQ_COL, tmem + DS_COL + ((it - 1) & 1) * 64, 32,
-                             ka + sp * C::OPB, it > 1);
-          mma_commit(&k_free[sp]);
+          if (lead) {
+            product_cols<T, D>(tmem + C::ACC_COL, tmem + C::DP_COL + dbuf.at * BLK,
+                               base + C::A_OFF + kst.at * C::STRB, j > 2);
+            mma_commit(bar.a_free + 8 * kst.at);
+          }
+          kst.next();
+          dbuf.next();
+        }
+        if (j < total) {
+          ok = bar_wait(bar.b_full + 8 * vst.at, vst.phase, waits);
+          if (!ok) break;
+          if (lead) {
+            product_rows<T, D>(tmem + C::DP_COL + buf.at * BLK, oa,
+                               base + C::B_OFF + vst.at * C::STRB);
+            mma_commit(bar.dp_full + 8 * buf.at);
+            mma_commit(bar.b_free + 8 * vst.at);
+          }
+          vst.next();
+          buf.next();
         }
       }
-      mma_commit(ok ? acc_full : drained);
-      if (!ok) mbar_wait(drained, 0, nullptr);
+      if (lead) {
+        mma_commit(ok ? bar.acc : bar.drained + 8);
+        if (!ok) bar_drain(bar.drained + 8, 0, waits);
+      }
+      __syncwarp();
     }
   } else {
-    const int half = warp >> 2, r = threadIdx.x & 127;
+    // ------------------------------------------- blocks `group`, group + 2, ...
+    const int group = warp >> 2, r = threadIdx.x & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const int row = m0 + r, off = s.klen - s.qlen;
     const int64_t stat = (int64_t)h * a.R + s.stat0 + row;
     const float2 lse2 = f2s(-__ldg(a.lse2 + stat)), delta = f2s(-__ldg(a.delta + stat));
+    const float2 sc = f2s(a.scale_log2);
+    const uint32_t s_at = tmem + lanes + C::S_COL + group * BLK;
+    const uint32_t dp_at = tmem + lanes + C::DP_COL + group * BLK;
+    uint32_t ph = 0;
     bool ok = true;
-    for (int it = 0; it < total; ++it) {
-      const int n0 = (b0 + it) * N;
-      ok = __all_sync(0xffffffffu, tc_wait(sdp_full, it & 1, stop, a.fault));
+    for (int it = group; it < total; it += 2, ph ^= 1u) {
+      const int n0 = (b0 + it) * BLK;
+      ok = __all_sync(0xffffffffu, bar_wait(bar.s_full + 8 * group, ph, waits));
       if (!ok) break;
       tc_fence_after();
-      float x[64], y[64];
-      load64(tmem + lanes + S_COL + half * 64, x);
-      load64(tmem + lanes + DP_COL + half * 64, y);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(read);
+      float x[BLK], y[BLK];
+      load64(s_at, x);
+      const bool there = bar_test(bar.dp_full + 8 * group, ph);
 #pragma unroll
-      for (int i = 0; i < 64; i += 2) {
-        const float2 u = f2_fma(f2(x[i], x[i + 1]), f2s(a.scale_log2), lse2);
-        const float2 d = f2_mul(f2(ex2(u.x), ex2(u.y)), f2_add(f2(y[i], y[i + 1]), delta));
+      for (int i = 0; i < BLK; i += 2) {
+        const float2 u = f2_fma(f2(x[i], x[i + 1]), sc, lse2);
+        x[i] = ex2(u.x);
+        x[i + 1] = ex2(u.y);
+      }
+      ok = __all_sync(0xffffffffu, there || bar_wait(bar.dp_full + 8 * group, ph, waits));
+      if (!ok) break;
+      tc_fence_after();
+      load64(dp_at, y);
+#pragma unroll
+      for (int i = 0; i < BLK; i += 2) {
+        const float2 d = f2_mul(f2(x[i], x[i + 1]), f2_add(f2(y[i], y[i + 1]), delta));
         y[i] = d.x;
         y[i + 1] = d.y;
       }
-      if (n0 + N > s.klen || (a.causal && n0 + N - 1 > m0 + off) ||
+      if (n0 + BLK > s.klen || (a.causal && n0 + BLK - 1 > m0 + off) ||
           (a.window && n0 <= m0 + N - 1 + off - a.window)) {
-        const int to = (a.causal ? min(s.klen, row + off + 1) : s.klen) - n0 - half * 64;
-        const int from = a.window ? row + off - a.window + 1 - n0 - half * 64 : 0;
+        const int to = (a.causal ? min(s.klen, row + off + 1) : s.klen) - n0;
+        const int from = a.window ? row + off - a.window + 1 - n0 : 0;
 #pragma unroll
-        for (int i = 0; i < 64; ++i)
+        for (int i = 0; i < BLK; ++i)
           if (i < from || i >= to) y[i] = 0.f;
         // rows of K past the sequence's end that memory does hold
-        if (n0 + N > s.klen && s.k0 + s.klen < a.Sk)
-          zero_rows<D>(smem + C::A_OFF + (it % NA) * C::OPB, s.klen - n0);
+        if (n0 + BLK > s.klen && s.k0 + s.klen < a.Sk)
+          zero_rows<D>(smem + C::A_OFF + (it % NST) * C::STRB, s.klen - n0);
       }
-      store64<T>(tmem + lanes + DS_COL + (it & 1) * 64 + half * 32, y);
+      store64<T>(dp_at, y);
+      tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(ds_full);
+      if (lane == 0) bar_arrive(bar.ds_full + 8 * group);
     }
     if (ok && total > 0) {
-      ok = __all_sync(0xffffffffu, tc_wait(acc_full, 0, stop, a.fault));
+      ok = __all_sync(0xffffffffu, bar_wait(bar.acc, 0, waits));
       tc_fence_after();
     }
     if (ok) {
       T* dst = reinterpret_cast<T*>(const_cast<void*>(a.dq.p)) + (int64_t)s.b * a.dq.sb +
-               (int64_t)h * a.dq.sh + (int64_t)(s.q0 + row) * a.dq.ss + half * (D / 2);
+               (int64_t)h * a.dq.sh + (int64_t)(s.q0 + row) * a.dq.ss + group * (D / 2);
       // queries past the sequence's end (dense tensors) get zeros
-      store_row<T>(tmem + lanes + DQ_COL + half * (D / 2), D / 2, a.scale, dst, row < limit,
+      store_row<T>(tmem + lanes + C::ACC_COL + group * (D / 2), D / 2, a.scale, dst, row < limit,
                    row < s.qlen, total > 0);
     }
   }
@@ -529,13 +600,13 @@ int launch_attn_bwd(const AttnArgs& a0, cudaStream_t st) {
   if (a.fault == nullptr) return cuda_status(cudaErrorInvalidDevice);
   BwdMaps m;
   const int dt = DTypeOf<T>::value;
-  int rc = head_map(&m.q, a.q.p, a.q.sb, a.q.ss, a.q.sh, a.B, a.Sq, a.Hq, D, C::TILE, dt);
+  int rc = head_map(&m.q, a.q.p, a.q.sb, a.q.ss, a.q.sh, a.B, a.Sq, a.Hq, D, C::BLK, dt);
   if (rc == BLOTH_OK)
-    rc = head_map(&m.k, a.k.p, a.k.sb, a.k.ss, a.k.sh, a.B, a.Sk, a.Hk, D, C::TILE, dt);
+    rc = head_map(&m.k, a.k.p, a.k.sb, a.k.ss, a.k.sh, a.B, a.Sk, a.Hk, D, C::BLK, dt);
   if (rc == BLOTH_OK)
-    rc = head_map(&m.v, a.v.p, a.v.sb, a.v.ss, a.v.sh, a.B, a.Sk, a.Hk, D, C::TILE, dt);
+    rc = head_map(&m.v, a.v.p, a.v.sb, a.v.ss, a.v.sh, a.B, a.Sk, a.Hk, D, C::BLK, dt);
   if (rc == BLOTH_OK)
-    rc = head_map(&m.dout, a.dout.p, a.dout.sb, a.dout.ss, a.dout.sh, a.B, a.Sq, a.Hq, D, C::TILE,
+    rc = head_map(&m.dout, a.dout.p, a.dout.sb, a.dout.ss, a.dout.sh, a.B, a.Sq, a.Hq, D, C::BLK,
                   dt);
   if (rc != BLOTH_OK) return rc;
   auto run = [&](auto kern, int64_t grid) {
