@@ -88,11 +88,11 @@ _SIGNATURES = {
                            _vp, _vp, _f32, _i64, _i64, _i64, _i64, _i64, _int, _int, _vp]),
     "bloth_attention_fwd_workspace_bytes": (_sz, [_i64] * 7 + [_int]),
     "bloth_attention_fwd": (_int, [_vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _vp, _vp,
-                                   _int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _int,
+                                   _vp, _int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _int,
                                    _i64, _int, _vp, _sz, _vp]),
     "bloth_attention_bwd_workspace_bytes": (_sz, [_i64] * 7 + [_int]),
     "bloth_attention_bwd": (_int, [_vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p,
-                                   _vp, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _vp, _int, _i64,
+                                   _vp, _vp, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _vp, _int, _i64,
                                    _i64, _i64, _i64, _i64, _i64, _i64, _f32, _int, _i64, _int,
                                    _vp, _sz, _vp]),
 }

@@ -90,7 +90,7 @@ size_t bloth_attention_fwd_workspace_bytes(int64_t B, int64_t Sq, int64_t Sk, in
 
 int bloth_attention_fwd(const void* q, const int64_t* q_strides, const void* k,
                         const int64_t* k_strides, const void* v, const int64_t* v_strides,
-                        void* out, const int64_t* out_strides, float* lse, const void* q_seq,
+                        void* out, const int64_t* out_strides, void* out_rest, float* lse, const void* q_seq,
                         const void* k_seq, int seq_dtype, int64_t packed, int64_t B, int64_t Sq,
                         int64_t Sk, int64_t Hq, int64_t Hk, int64_t D, float scale, int causal,
                         int64_t window, int dtype, void* workspace, size_t workspace_bytes,
@@ -109,6 +109,8 @@ int bloth_attention_fwd(const void* q, const int64_t* q_strides, const void* k,
     if ((rc = fill(a.v, v, v_strides, dtype))) return rc;
   }
   if ((rc = fill(a.o, out, out_strides, dtype))) return rc;
+  if (reinterpret_cast<uintptr_t>(out_rest) % 16 != 0) return BLOTH_ERR_ALIGN;
+  a.rest = dtype == BLOTH_F32 ? nullptr : out_rest;
   a.lse = lse;
   const size_t need = bloth_attention_fwd_workspace_bytes(B, Sq, Sk, Hq, Hk, D, packed, dtype);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return BLOTH_ERR_WORKSPACE;
@@ -133,7 +135,7 @@ size_t bloth_attention_bwd_workspace_bytes(int64_t B, int64_t Sq, int64_t Sk, in
 int bloth_attention_bwd(const void* dout, const int64_t* dout_strides, const void* q,
                         const int64_t* q_strides, const void* k, const int64_t* k_strides,
                         const void* v, const int64_t* v_strides, const void* out,
-                        const int64_t* out_strides, const float* lse, void* dq,
+                        const int64_t* out_strides, const void* out_rest, const float* lse, void* dq,
                         const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
                         const int64_t* dv_strides, const void* q_seq, const void* k_seq,
                         int seq_dtype, int64_t packed, int64_t B, int64_t Sq, int64_t Sk,
@@ -165,6 +167,8 @@ int bloth_attention_bwd(const void* dout, const int64_t* dout_strides, const voi
   const size_t need = bloth_attention_bwd_workspace_bytes(B, Sq, Sk, Hq, Hk, D, packed, dtype);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return BLOTH_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return BLOTH_ERR_ALIGN;
+  if (reinterpret_cast<uintptr_t>(out_rest) % 16 != 0) return BLOTH_ERR_ALIGN;
+  a.rest = dtype == BLOTH_F32 ? nullptr : const_cast<void*>(out_rest);
   a.lse = const_cast<float*>(lse);
   a.R = attn_stat_rows(B, Sq, packed);
   a.lse2 = reinterpret_cast<float*>(workspace);

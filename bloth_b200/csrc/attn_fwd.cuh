@@ -331,8 +331,10 @@ __global__ void __launch_bounds__(352, 1)
     if (ok) {
       const bool in = row < s.qlen, any = e > f && in;
       const float inv = any && l != 0.f ? 1.f / l : 0.f;
-      T* out = reinterpret_cast<T*>(const_cast<void*>(a.o.p)) + (int64_t)s.b * a.o.sb +
-               (int64_t)h * a.o.sh + (int64_t)(s.q0 + row) * a.o.ss;
+      const int64_t at = (int64_t)s.b * a.o.sb + (int64_t)h * a.o.sh +
+                         (int64_t)(s.q0 + row) * a.o.ss;
+      T* out = reinterpret_cast<T*>(const_cast<void*>(a.o.p)) + at;
+      T* rest = a.rest != nullptr ? reinterpret_cast<T*>(a.rest) + at : nullptr;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         uint32_t r[32];
@@ -343,13 +345,16 @@ __global__ void __launch_bounds__(352, 1)
         if (row < limit) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            uint32_t w[4];
+            uint32_t w[4] = {0, 0, 0, 0}, v[4] = {0, 0, 0, 0};
+            if (inv != 0.f) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-              w[u] = inv != 0.f ? pack2<T>(__uint_as_float(r[8 * i + 2 * u]) * inv,
-                                           __uint_as_float(r[8 * i + 2 * u + 1]) * inv)
-                                : 0u;
+              for (int u = 0; u < 4; ++u)
+                split2<T>(__uint_as_float(r[8 * i + 2 * u]) * inv,
+                          __uint_as_float(r[8 * i + 2 * u + 1]) * inv, w[u], v[u]);
+            }
             *reinterpret_cast<uint4*>(out + c * 32 + i * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+            if (rest != nullptr)
+              *reinterpret_cast<uint4*>(rest + c * 32 + i * 8) = make_uint4(v[0], v[1], v[2], v[3]);
           }
         }
       }

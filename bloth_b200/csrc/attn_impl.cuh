@@ -9,6 +9,9 @@
 //   delta_i = do_i . o_i,  dp_ij = do_i . v_j,  ds_ij = p_ij (dp_ij - delta_i),
 //   dv_j = sum_i p_ij do_i,  dq_i = scale sum_j ds_ij k_j,
 //   dk_j = scale sum_i ds_ij q_i.
+// delta takes o to twice the precision of 16-bit tensors (o and `rest`): with
+// o as rounded, rows of few keys, whose dp nearly equal delta, would get twice
+// the error.
 // A row that sees no key has o = 0, lse = -inf and no gradient. Query heads
 // h of a group of G = Hq / Hk share key head h / G, whose gradients sum over
 // the group inside one CTA, in a fixed order: no atomics anywhere.
@@ -19,8 +22,26 @@
 
 namespace bloth {
 
+// Two floats y rounded to T, and what that took off them rounded to T.
+template <typename T>
+__device__ __forceinline__ void split2(float y0, float y1, uint32_t& hi, uint32_t& lo) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(y0, y1);
+    const __nv_bfloat162 r =
+        __floats2bfloat162_rn(y0 - __bfloat162float(h.x), y1 - __bfloat162float(h.y));
+    memcpy(&hi, &h, 4);
+    memcpy(&lo, &r, 4);
+  } else {
+    const __half2 h = __floats2half2_rn(y0, y1);
+    const __half2 r = __floats2half2_rn(y0 - __half2float(h.x), y1 - __half2float(h.y));
+    memcpy(&hi, &h, 4);
+    memcpy(&lo, &r, 4);
+  }
+}
+
 struct AttnArgs {
   HT q, k, v, o, dout, dq, dk, dv;
+  void* rest;         // what rounding took off o, laid out as o (16-bit tensors), or NULL
   float* lse;         // [B, Hq, Sq] natural logarithm (forward writes, backward reads)
   float* lse2;        // backward workspace: [Hq, R] lse * log2(e), +inf where nothing is seen
   float* delta;       // backward workspace: [Hq, R]

@@ -83,11 +83,16 @@ struct RowsPlan {
   float* stat;
 };
 
-// One row of the result: x / l to the output, and its lse.
-template <typename T, int D>
-__device__ __forceinline__ T* rows_out(const AttnArgs& a, int b, int h, int r) {
-  return reinterpret_cast<T*>(const_cast<void*>(a.o.p)) + (int64_t)b * a.o.sb +
-         (int64_t)(h * a.G + r % a.G) * a.o.sh + (int64_t)(r / a.G) * a.o.ss;
+// Two neighbouring elements of one row of the result, and the row's lse.
+template <typename T>
+__device__ __forceinline__ void rows_out(const AttnArgs& a, int b, int h, int r, int c, float y0,
+                                         float y1) {
+  const int64_t at = (int64_t)b * a.o.sb + (int64_t)(h * a.G + r % a.G) * a.o.sh +
+                     (int64_t)(r / a.G) * a.o.ss + c;
+  uint32_t hi, lo;
+  split2<T>(y0, y1, hi, lo);
+  *reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(const_cast<void*>(a.o.p)) + at) = hi;
+  if (a.rest != nullptr) *reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(a.rest) + at) = lo;
 }
 __device__ __forceinline__ void rows_lse(const AttnArgs& a, int b, int h, int r, float m, float l) {
   if (a.lse != nullptr)
@@ -313,8 +318,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32)
         y = f2_fma(v, f2s(w[i]), y);
       }
       if (pl.splits == 1)
-        *reinterpret_cast<uint32_t*>(rows_out<T, D>(a, b, h, r) + c) =
-            pack2<T>(y.x * inv, y.y * inv);
+        rows_out<T>(a, b, h, r, c, y.x * inv, y.y * inv);
       else
         *reinterpret_cast<float2*>(pl.sums + (part + r) * D + c) = y;
     }
@@ -362,10 +366,9 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a, const 
     }
   }
   const float inv = ll == 0.f ? 0.f : 1.f / ll;
-  T* out = rows_out<T, D>(a, bh / a.Hk, bh % a.Hk, r) + lane * V;
 #pragma unroll
   for (int e = 0; e < V; e += 2)
-    *reinterpret_cast<uint32_t*>(out + e) = pack2<T>(y[e] * inv, y[e + 1] * inv);
+    rows_out<T>(a, bh / a.Hk, bh % a.Hk, r, lane * V + e, y[e] * inv, y[e + 1] * inv);
   if (lane == 0) rows_lse(a, bh / a.Hk, bh % a.Hk, r, mm, ll);
 }
 

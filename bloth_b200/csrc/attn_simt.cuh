@@ -199,6 +199,22 @@ __global__ void __launch_bounds__(kSimtThreads) attn_simt_fwd_kernel(const AttnA
   for (int i = 0; i < 4; ++i) f[i] = l[i] > 0.f || l[i] != l[i] ? 1.f / l[i] : 0.f;
   const int out_rows = min(N, limit - m0);
   simt_store<T, D>(a.o, s.b, h, s.q0 + m0, out_rows, ty, tx, acc, f);
+  if constexpr (sizeof(T) == 2) {
+    if (a.rest != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) {
+          const float y = acc[i][c] * f[i];
+          acc[i][c] = y - to_f(from_f<T>(y));
+        }
+        f[i] = 1.f;
+      }
+      HT rest = a.o;
+      rest.p = a.rest;
+      simt_store<T, D>(rest, s.b, h, s.q0 + m0, out_rows, ty, tx, acc, f);
+    }
+  }
   if (tx == 0 && a.lse != nullptr) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -301,7 +317,7 @@ __global__ void __launch_bounds__(kSimtThreads) attn_simt_bwd_kernel(const AttnA
 // delta = rowsum(dO * O) and lse in base 2 for the backward kernels, for every
 // row of every 128-row tile of a sequence: a row past the sequence's end, or
 // one that sees nothing, gets lse2 = +inf and delta = 0, so its recomputed
-// probabilities are exp2(x - inf) = 0. HBM-bound: reads O and dO once. A row
+// probabilities are exp2(x - inf) = 0. HBM-bound: reads O, its rest and dO once. A row
 // takes D / 8 lanes of 16-bit (D / 4 of fp32) elements, one 16-byte load of
 // each tensor per lane and pass.
 template <typename T, int D>
@@ -316,6 +332,8 @@ __global__ void __launch_bounds__(256) attn_stats_kernel(const AttnArgs a) {
   const int m0 = s.tile * 128;
   const int64_t stat = (int64_t)h * a.R + s.stat0 + m0;
   const T* op = reinterpret_cast<const T*>(a.o.p) + (int64_t)s.b * a.o.sb + (int64_t)h * a.o.sh;
+  const T* rp =
+      reinterpret_cast<const T*>(a.rest) + (int64_t)s.b * a.o.sb + (int64_t)h * a.o.sh;
   const T* dp =
       reinterpret_cast<const T*>(a.dout.p) + (int64_t)s.b * a.dout.sb + (int64_t)h * a.dout.sh;
 #pragma unroll
@@ -330,6 +348,12 @@ __global__ void __launch_bounds__(256) attn_stats_kernel(const AttnArgs a) {
         float f[VEC], g[VEC];
         unpack(ldg_pack<T, VEC>(op + row * a.o.ss + x), f);
         unpack(ldg_pack<T, VEC>(dp + row * a.dout.ss + x), g);
+        if (sizeof(T) == 2 && a.rest != nullptr) {
+          float e[VEC];
+          unpack(ldg_pack<T, VEC>(rp + row * a.o.ss + x), e);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) f[i] += e[i];
+        }
 #pragma unroll
         for (int e = 0; e < VEC; ++e) sum = fmaf(f[e], g[e], sum);
       }

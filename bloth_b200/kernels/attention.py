@@ -15,6 +15,7 @@ import torch
 
 from .. import _lib
 from .fused_norm_qkv_rope import _head_strides, _heads
+from .rope import _out_like
 
 
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
@@ -86,39 +87,41 @@ def _workspace(entry: str, device, *args):
     return (torch.empty(n, dtype=torch.uint8, device=device) if n else None), n
 
 
-def attention_forward(q4, k4, v4, q_seq, k_seq, packed, scale, causal, window, want_lse=True):
-    """(out, lse) of addressable head tensors; lse is None unless wanted."""
+def attention_forward(q4, k4, v4, q_seq, k_seq, packed, scale, causal, window, want_lse=True,
+                      want_rest=False):
+    """(out, lse, rest) of addressable head tensors: lse if wanted, and for
+    16-bit tensors what rounding took off out, for the backward."""
     B, Sq, Hq, D = q4.shape
     Sk, Hk = k4.shape[1], k4.shape[2]
     out = torch.empty((B, Sq, Hq, D), dtype=q4.dtype, device=q4.device)
+    rest = torch.empty_like(out) if want_rest and q4.dtype != torch.float32 else None
     lse = torch.empty((B, Hq, Sq), dtype=torch.float32, device=q4.device) if want_lse else None
     code = _lib.dtype_code(q4.dtype)
     ws, n = _workspace("bloth_attention_fwd_workspace_bytes", q4.device, B, Sq, Sk, Hq, Hk, D,
                        packed, code)
     rc = _lib.call("bloth_attention_fwd", q4, _lib.ptr(q4), _head_strides(q4), _lib.ptr(k4),
                    _head_strides(k4), _lib.ptr(v4), _head_strides(v4), _lib.ptr(out),
-                   _head_strides(out), _lib.ptr(lse), _lib.ptr(q_seq), _lib.ptr(k_seq),
-                   _seq_dtype(q_seq, k_seq), packed, B, Sq, Sk, Hq, Hk, D, scale, int(causal),
-                   window, code, _lib.ptr(ws), n, _lib.stream_of(q4))
+                   _head_strides(out), _lib.ptr(rest), _lib.ptr(lse), _lib.ptr(q_seq),
+                   _lib.ptr(k_seq), _seq_dtype(q_seq, k_seq), packed, B, Sq, Sk, Hq, Hk, D, scale,
+                   int(causal), window, code, _lib.ptr(ws), n, _lib.stream_of(q4))
     _lib.check(rc, "attention forward")
-    return out, lse
+    return out, lse, rest
 
 
-def attention_backward(do4, q4, k4, v4, out, lse, q_seq, k_seq, packed, scale, causal, window,
+def attention_backward(do4, q4, k4, v4, out, rest, lse, q_seq, k_seq, packed, scale, causal, window,
                        want_q=True, want_kv=True):
     """(dq, dk, dv); None for those not wanted."""
     B, Sq, Hq, D = q4.shape
     Sk, Hk = k4.shape[1], k4.shape[2]
-    dq = torch.empty((B, Sq, Hq, D), dtype=q4.dtype, device=q4.device) if want_q else None
-    dk = torch.empty((B, Sk, Hk, D), dtype=q4.dtype, device=q4.device) if want_kv else None
-    dv = torch.empty((B, Sk, Hk, D), dtype=q4.dtype, device=q4.device) if want_kv else None
+    dq = _out_like(q4) if want_q else None
+    dk, dv = (_out_like(k4), _out_like(v4)) if want_kv else (None, None)
     code = _lib.dtype_code(q4.dtype)
     ws, n = _workspace("bloth_attention_bwd_workspace_bytes", q4.device, B, Sq, Sk, Hq, Hk, D,
                        packed, code)
     rc = _lib.call("bloth_attention_bwd", q4, _lib.ptr(do4), _head_strides(do4), _lib.ptr(q4),
                    _head_strides(q4), _lib.ptr(k4), _head_strides(k4), _lib.ptr(v4),
-                   _head_strides(v4), _lib.ptr(out), _head_strides(out), _lib.ptr(lse),
-                   _lib.ptr(dq), _head_strides(dq), _lib.ptr(dk), _head_strides(dk),
+                   _head_strides(v4), _lib.ptr(out), _head_strides(out), _lib.ptr(rest),
+                   _lib.ptr(lse), _lib.ptr(dq), _head_strides(dq), _lib.ptr(dk), _head_strides(dk),
                    _lib.ptr(dv), _head_strides(dv), _lib.ptr(q_seq), _lib.ptr(k_seq),
                    _seq_dtype(q_seq, k_seq), packed, B, Sq, Sk, Hq, Hk, D, scale, int(causal),
                    window, code, _lib.ptr(ws), n, _lib.stream_of(q4))
@@ -131,8 +134,9 @@ class _AttentionFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, q_seq, k_seq, packed, scale, causal, window):
         q4, k4, v4 = _addressable(q), _addressable(k), _addressable(v)
-        out, lse = attention_forward(q4, k4, v4, q_seq, k_seq, packed, scale, causal, window)
-        ctx.save_for_backward(q4, k4, v4, out, lse, q_seq, k_seq)
+        out, lse, rest = attention_forward(q4, k4, v4, q_seq, k_seq, packed, scale, causal, window,
+                                           want_rest=True)
+        ctx.save_for_backward(q4, k4, v4, out, rest, lse, q_seq, k_seq)
         ctx.meta = (packed, scale, causal, window, q.dim() == 3)
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
@@ -142,11 +146,11 @@ class _AttentionFunction(torch.autograd.Function):
     def backward(ctx, dout, _):
         if dout is None:
             return (None,) * 9
-        q4, k4, v4, out, lse, q_seq, k_seq = ctx.saved_tensors
+        q4, k4, v4, out, rest, lse, q_seq, k_seq = ctx.saved_tensors
         packed, scale, causal, window, flat = ctx.meta
         want_q, want_k, want_v = ctx.needs_input_grad[:3]
-        grads = attention_backward(_addressable(dout), q4, k4, v4, out, lse, q_seq, k_seq, packed,
-                                   scale, causal, window, want_q, want_k or want_v)
+        grads = attention_backward(_addressable(dout), q4, k4, v4, out, rest, lse, q_seq, k_seq,
+                                   packed, scale, causal, window, want_q, want_k or want_v)
         if flat:
             grads = [None if g is None else g[0] for g in grads]
         dq, dk, dv = grads
@@ -211,8 +215,8 @@ def fused_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: b
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = _AttentionFunction.apply(q, k, v, *how)
     else:
-        out, lse = attention_forward(_addressable(q), _addressable(k), _addressable(v), *how,
-                                     want_lse=return_lse)
+        out, lse, _ = attention_forward(_addressable(q), _addressable(k), _addressable(v), *how,
+                                        want_lse=return_lse)
         if dim == 3:
             out = out[0]
     if not return_lse:

@@ -111,7 +111,7 @@ def _heads(t: torch.Tensor | None):
 
 
 def _head_strides(t):
-    return _lib.strides(t.stride()[:3]) if t is not None else None
+    return None if t is None else _lib._stride_array(t.stride()[:3])
 
 
 def _positions(position_ids, B: int, S: int):

@@ -35,7 +35,7 @@ def _rope_launch(q4, qo, k4, ko, pos, pos_st, inv_freq, cos, sin, cs_st, cs_rows
 def _out_like(x4):
     """Output buffer with x4's strides when they are dense, else contiguous."""
     y = torch.empty_like(x4)
-    if y.stride() != x4.stride():
+    if y.stride() != x4.stride() and not y.is_contiguous():
         y = torch.empty(x4.shape, dtype=x4.dtype, device=x4.device)
     return y
 

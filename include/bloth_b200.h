@@ -328,23 +328,26 @@ int bloth_mrope(const void* q, const int64_t* q_strides, void* q_out, const int6
  * ---------------------------------------------------------------------- */
 size_t bloth_attention_fwd_workspace_bytes(int64_t B, int64_t Sq, int64_t Sk, int64_t Hq,
                                            int64_t Hk, int64_t D, int64_t packed, int dtype);
-/* lse may be NULL when no backward follows. The workspace may be NULL when the
+/* lse may be NULL when no backward follows. out_rest, for the backward of
+   16-bit tensors: what rounding took off out, with out's type and strides, or
+   NULL. The workspace may be NULL when the
    function above reports 0 bytes; its base is aligned to 16 bytes. */
 int bloth_attention_fwd(const void* q, const int64_t* q_strides, const void* k,
                         const int64_t* k_strides, const void* v, const int64_t* v_strides,
-                        void* out, const int64_t* out_strides, float* lse, const void* q_seq,
-                        const void* k_seq, int seq_dtype, int64_t packed, int64_t B, int64_t Sq,
+                        void* out, const int64_t* out_strides, void* out_rest, float* lse,
+                        const void* q_seq, const void* k_seq, int seq_dtype, int64_t packed, int64_t B, int64_t Sq,
                         int64_t Sk, int64_t Hq, int64_t Hk, int64_t D, float scale, int causal,
                         int64_t window, int dtype, void* workspace, size_t workspace_bytes,
                         void* stream);
 size_t bloth_attention_bwd_workspace_bytes(int64_t B, int64_t Sq, int64_t Sk, int64_t Hq,
                                            int64_t Hk, int64_t D, int64_t packed, int dtype);
-/* out and lse are the forward's. dq may be NULL, and dk and dv both (not one
+/* out, out_rest and lse are the forward's; with out_rest NULL the row sums
+   dout . out are those of the rounded out. dq may be NULL, and dk and dv both (not one
    of them), when they are not wanted. */
 int bloth_attention_bwd(const void* dout, const int64_t* dout_strides, const void* q,
                         const int64_t* q_strides, const void* k, const int64_t* k_strides,
                         const void* v, const int64_t* v_strides, const void* out,
-                        const int64_t* out_strides, const float* lse, void* dq,
+                        const int64_t* out_strides, const void* out_rest, const float* lse, void* dq,
                         const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
                         const int64_t* dv_strides, const void* q_seq, const void* k_seq,
                         int seq_dtype, int64_t packed, int64_t B, int64_t Sq, int64_t Sk,

@@ -44,7 +44,7 @@ def _fwd(**kw):
              D=64, scale=0.125, causal=1, window=0, dtype=_lib.BF16)
     a.update(kw)
     return _lib.load().bloth_attention_fwd(
-        None, None, None, None, None, None, None, None, None, a["q_seq"], a["k_seq"],
+        None, None, None, None, None, None, None, None, None, None, a["q_seq"], a["k_seq"],
         a["seq_dtype"], a["packed"], a["B"], a["Sq"], a["Sk"], a["Hq"], a["Hk"], a["D"],
         a["scale"], a["causal"], a["window"], a["dtype"], None, 0, None)
 
