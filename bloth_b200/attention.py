@@ -13,6 +13,11 @@ its q/k normalisation and rotary embedding through the sm_100a kernels:
 * ``LlamaAttention``, ``MistralAttention``, ``Qwen2Attention`` -
   ``apply_rotary_pos_emb`` of q and k becomes one ``apply_rope_qk`` launch.
 
+With ``fuse_attention=True`` the attention itself is ``fused_attention`` too,
+where HF passes no mask tensor (unpadded batches under ``sdpa`` or
+``flash_attention_2`` kwargs, whose ``cu_seq_lens_q`` / ``_k`` are passed on)
+and no dropout; other calls keep HF's attention.
+
 The rest of the forward is HuggingFace's own code path, restated for the
 transformers 5.x signature ``forward(hidden_states, position_embeddings,
 attention_mask, past_key_values=None, **kwargs)``: the projections, the KV
@@ -41,6 +46,7 @@ from dataclasses import dataclass
 import torch.nn as nn
 
 from .kernels.add_rms_norm import fused_add_rms_norm
+from .kernels.attention import fused_attention
 from .kernels.fused_norm_qkv_rope import fused_qk_norm_rope
 from .kernels.rope import apply_rope_qk
 from .modules import BlothRMSNorm
@@ -63,6 +69,7 @@ _HEAD_DIMS = (64, 128, 256)
 class _Binding:
     norms: bool
     window: str | None
+    core: bool = False
 
 
 def _norm_params(norm: nn.Module):
@@ -97,14 +104,13 @@ def _attention_forward(self, hidden_states, position_embeddings=None, attention_
     q, k = q.transpose(1, 2), k.transpose(1, 2)
     if past_key_values is not None:
         k, v = past_key_values.update(k, v, self.layer_idx)
+    if bind.core and _takes_core(self, q, v, attention_mask, kwargs):
+        o = _core(self, bind, q, k, v, kwargs)
+        return self.o_proj(o.reshape(*input_shape, -1)), None
     hf = sys.modules[type(self).__module__]
     attention_interface = hf.ALL_ATTENTION_FUNCTIONS.get_interface(
         self.config._attn_implementation, hf.eager_attention_forward)
-    extra = {}
-    if bind.window == "module":
-        extra["sliding_window"] = self.sliding_window
-    elif bind.window == "config":
-        extra["sliding_window"] = getattr(self.config, "sliding_window", None)
+    extra = {} if bind.window is None else {"sliding_window": _window(self, bind)}
     attn_output, attn_weights = attention_interface(
         self, q, k, v, attention_mask,
         dropout=0.0 if not self.training else self.attention_dropout,
@@ -112,6 +118,33 @@ def _attention_forward(self, hidden_states, position_embeddings=None, attention_
     attn_output = attn_output.reshape(*input_shape, -1).contiguous()
     attn_output = self.o_proj(attn_output)
     return attn_output, attn_weights
+
+
+def _takes_core(self, q, v, attention_mask, kwargs) -> bool:
+    """Whether a call's attention is what fused_attention computes: causal to
+    the last key, no mask tensor, no dropout, no weights asked for."""
+    if attention_mask is not None or not q.is_cuda or v.shape[-1] != q.shape[-1] or \
+            q.dtype != v.dtype:
+        return False
+    if not kwargs.get("is_causal", getattr(self, "is_causal", True)) or \
+            kwargs.get("output_attentions") or kwargs.get("softcap") is not None:
+        return False
+    return not self.training or not self.attention_dropout
+
+
+def _window(self, bind):
+    if bind.window == "module":
+        return self.sliding_window
+    return getattr(self.config, "sliding_window", None) if bind.window == "config" else None
+
+
+def _core(self, bind, q, k, v, kwargs):
+    """fused_attention of q, k, v [B, H, S, D]; returns [B, S, H, D]."""
+    cu = kwargs.get("cu_seq_lens_q") if q.shape[0] == 1 else None
+    return fused_attention(q.transpose(1, 2), k.to(q.dtype).transpose(1, 2), v.transpose(1, 2),
+                           causal=True, window=_window(self, bind) or None, scale=self.scaling,
+                           cu_seqlens=cu,
+                           cu_seqlens_k=None if cu is None else kwargs.get("cu_seq_lens_k", cu))
 
 
 def _why_not(module: nn.Module, norms: bool) -> str | None:
@@ -137,9 +170,10 @@ def _why_not(module: nn.Module, norms: bool) -> str | None:
     return None
 
 
-def patch_attention_layers(model: nn.Module, verbose: bool = True) -> int:
-    """Binds the fused forward to every supported attention module of model;
-    returns how many were bound."""
+def patch_attention_layers(model: nn.Module, verbose: bool = True, core: bool = False) -> int:
+    """Binds the fused forward to every supported attention module of model
+    (core: with fused_attention where HF passes no mask); returns how many
+    were bound."""
     bound, skipped = 0, []
     for name, module in model.named_modules():
         spec = _ATTENTION_CLASSES.get(type(module).__name__)
@@ -149,14 +183,15 @@ def patch_attention_layers(model: nn.Module, verbose: bool = True) -> int:
         if reason is not None:
             skipped.append(f"{name}: {reason}")
             continue
-        module._bloth_attention = _Binding(norms=spec[0], window=spec[1])
+        module._bloth_attention = _Binding(norms=spec[0], window=spec[1], core=core)
         module.forward = types.MethodType(_attention_forward, module)
         bound += 1
     if skipped:
         warnings.warn("[Bloth] attention left unpatched - " + "; ".join(skipped[:4]) +
                       (f" (+{len(skipped) - 4} more)" if len(skipped) > 4 else ""))
     if verbose and bound > 0:
-        print(f"[Bloth] Patched {bound} attention layer(s) -> fused q/k norm + RoPE")
+        print(f"[Bloth] Patched {bound} attention layer(s) -> fused q/k norm + RoPE"
+              + (" + attention" if core else ""))
     return bound
 
 

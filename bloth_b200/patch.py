@@ -84,7 +84,8 @@ def _replace_norm_layers(model: nn.Module, verbose: bool = True) -> int:
 
 
 def patch_model(model: nn.Module, patch_norms: bool = True, patch_attention: bool = False,
-                verbose: bool = True, patch_residual: bool = False) -> nn.Module:
+                verbose: bool = True, patch_residual: bool = False,
+                fuse_attention: bool = False) -> nn.Module:
     """Applies the Bloth kernels to a HuggingFace model in place and returns it.
 
     patch_norms: replace RMSNorm layers (reference behaviour).
@@ -94,6 +95,10 @@ def patch_model(model: nn.Module, patch_norms: bool = True, patch_attention: boo
         for q and k). The reference accepts this flag and does nothing.
     patch_residual: fuse each decoder layer's attention residual add with its
         post_attention_layernorm (fused_add_rms_norm). Not in the reference.
+    fuse_attention: as patch_attention, with the attention itself on
+        fused_attention wherever HuggingFace passes it no mask tensor
+        (unpadded batches with attn_implementation="sdpa"). Not in the
+        reference.
     """
     if verbose:
         print(f"\n[Bloth] Patching: {type(model).__name__}")
@@ -103,9 +108,9 @@ def patch_model(model: nn.Module, patch_norms: bool = True, patch_attention: boo
     total = 0
     if patch_norms:
         total += _replace_norm_layers(model, verbose)
-    if patch_attention:
+    if patch_attention or fuse_attention:
         from .attention import patch_attention_layers
-        total += patch_attention_layers(model, verbose)
+        total += patch_attention_layers(model, verbose, core=fuse_attention)
     if patch_residual:
         from .attention import patch_decoder_layers
         total += patch_decoder_layers(model, verbose)
