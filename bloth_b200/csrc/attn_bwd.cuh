@@ -22,10 +22,12 @@
 // hand-over between warps nor its own latencies stop the tensor core. Warps 8
 // and 9 issue the products, warp 10 the copies.
 //
-// Bound: the products. 64 streamed rows against 128 kept ones read 6 KB of
-// shared memory for 32 cycles of arithmetic: 384 cycles each for S and dP at
-// head_dim 128, 256 for dV, dK or dQ: 1280 cycles a block for dK and dV, 1024
-// for dQ, beside 512 for its exponentials.
+// Bound: the products. 64 streamed rows against 128 kept ones in shared memory
+// take the time of 128 (a step reads 4 KB of the kept tile whatever the
+// streamed one has): 512 cycles each for S and dP at head_dim 128, 256 for dV
+// or dK. With the kept tiles in tensor memory, where the sums leave room for
+// them (dQ; dK and dV at head_dim 64), S and dP take 256 as well. Beside them
+// 512 cycles a block for its exponentials.
 #pragma once
 
 #include "attn_impl.cuh"
@@ -45,10 +47,11 @@ struct BwdCfg {
   static constexpr int B_OFF = A_OFF + NST * STRB;   // stages of dO (or V)
   static constexpr int STAT_OFF = B_OFF + NST * STRB;  // lse2 and delta, with dO's stages
   static constexpr int BAR_OFF = STAT_OFF + NST * 512;
-  static constexpr int BARS = 1 + 4 * NST + 8 + 3;
+  static constexpr int BARS = 1 + 4 * NST + 8 + 3 + 1;
   static constexpr int SMEM = BAR_OFF + BARS * 8 + 16;
   static_assert(SMEM <= 227 * 1024, "shared memory");
-  // tensor-memory columns: S (two buffers), dP (two buffers), the sums
+  // tensor-memory columns: S (two buffers), dP (two buffers), the sums, and
+  // behind them, where there is room, the kept tiles
   static constexpr uint32_t COLS = 512;
   static constexpr uint32_t S_COL = 0, DP_COL = 128, ACC_COL = 256;
 };
@@ -61,7 +64,8 @@ struct BwdMaps {
 // and V), [2] one for each buffer.
 template <int NST>
 struct BwdBars {
-  uint32_t own, a_full, a_free, b_full, b_free, s_full, p_full, dp_full, ds_full, acc, drained;
+  uint32_t own, a_full, a_free, b_full, b_free, s_full, p_full, dp_full, ds_full, acc, drained,
+      there;
   __device__ __forceinline__ explicit BwdBars(uint32_t at) {
     own = at;
     a_full = own + 8;
@@ -74,10 +78,12 @@ struct BwdBars {
     ds_full = dp_full + 16;
     acc = ds_full + 16;
     drained = acc + 8;
+    there = drained + 16;  // the kept tiles are in tensor memory
   }
   // b_free completes with `b_uses` arrivals, acc with `sums`
   __device__ __forceinline__ void init(int b_uses, int sums) const {
     bar_init(own, 1);
+    bar_init(there, 8);
     for (int i = 0; i < NST; ++i) {
       bar_init(a_full + 8 * i, 1);
       bar_init(a_free + 8 * i, 1);
@@ -137,6 +143,9 @@ __global__ void __launch_bounds__(352, 1)
   using C = BwdCfg<D>;
   constexpr int N = C::TILE, BLK = C::BLK, NST = C::NST;
   constexpr uint32_t DV_COL = C::ACC_COL, DK_COL = C::ACC_COL + D;
+  // K and V in tensor memory, beside dV and dK of 64 columns
+  constexpr bool OWN_TMEM = D == 64;
+  constexpr uint32_t K_COL = C::ACC_COL + 2 * D, V_COL = K_COL + D / 2;
   extern __shared__ __align__(1024) unsigned char smem[];
   const uint32_t base = smem_addr(smem);
   const BwdBars<NST> bar(base + C::BAR_OFF);
@@ -207,7 +216,8 @@ __global__ void __launch_bounds__(352, 1)
       const bool lead = elect();
       Ring<NST> qst, ost;
       Ring<2> buf, pbuf;
-      bool ok = bar_wait(bar.own, 0, waits);
+      bool ok = bar_wait(OWN_TMEM ? bar.there : bar.own, 0, waits);
+      tc_fence_after();
       for (int j = 0; ok && j < total + 2; ++j) {
         if (j >= 2) {
           ok = bar_wait(bar.b_full + 8 * ost.at, ost.phase, waits) &&
@@ -226,8 +236,11 @@ __global__ void __launch_bounds__(352, 1)
           ok = bar_wait(bar.a_full + 8 * qst.at, qst.phase, waits);
           if (!ok) break;
           if (lead) {
-            product_rows<T, D>(tmem + C::S_COL + buf.at * BLK, ka,
-                               base + C::A_OFF + qst.at * C::STRB);
+            const uint32_t qt = base + C::A_OFF + qst.at * C::STRB;
+            if constexpr (OWN_TMEM)
+              product_rows_ts<T, D>(tmem + C::S_COL + buf.at * BLK, tmem + K_COL, qt);
+            else
+              product_rows<T, D>(tmem + C::S_COL + buf.at * BLK, ka, qt);
             mma_commit(bar.s_full + 8 * buf.at);
           }
           qst.next();
@@ -248,7 +261,8 @@ __global__ void __launch_bounds__(352, 1)
       Ring<NST> qst, ost;
       Ring<2> buf, dbuf;
       uint32_t done = 0;  // stage whose statistics the group has read
-      bool ok = bar_wait(bar.own, 0, waits);
+      bool ok = bar_wait(OWN_TMEM ? bar.there : bar.own, 0, waits);
+      tc_fence_after();
       for (int j = 0; ok && j < total + 2; ++j) {
         if (j >= 2) {
           ok = bar_wait(bar.a_full + 8 * qst.at, qst.phase, waits) &&
@@ -271,8 +285,11 @@ __global__ void __launch_bounds__(352, 1)
           ok = bar_wait(bar.b_full + 8 * ost.at, ost.phase, waits);
           if (!ok) break;
           if (lead) {
-            product_rows<T, D>(tmem + C::DP_COL + buf.at * BLK, va,
-                               base + C::B_OFF + ost.at * C::STRB);
+            const uint32_t ot = base + C::B_OFF + ost.at * C::STRB;
+            if constexpr (OWN_TMEM)
+              product_rows_ts<T, D>(tmem + C::DP_COL + buf.at * BLK, tmem + V_COL, ot);
+            else
+              product_rows<T, D>(tmem + C::DP_COL + buf.at * BLK, va, ot);
             mma_commit(bar.dp_full + 8 * buf.at);
           }
           ost.next();
@@ -301,7 +318,17 @@ __global__ void __launch_bounds__(352, 1)
     }
     uint32_t ph = 0;
     bool ok = true;
-    for (int it = group; it < total; it += 2, ph ^= 1u) {
+    if (OWN_TMEM && total > 0) {
+      ok = __all_sync(0xffffffffu, bar_wait(bar.own, 0, waits));
+      if (ok) {
+        copy_operand<D>(smem + C::OWN_OFF + group * C::OWNB, r,
+                        tmem + lanes + K_COL + group * (D / 2));
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(bar.there);
+      }
+    }
+    for (int it = group; ok && it < total; it += 2, ph ^= 1u) {
       const int m0 = (mb + mi) * BLK;
       const float* stat = reinterpret_cast<const float*>(smem + C::STAT_OFF + st.at * 512);
       ok = bar_wait(bar.b_full + 8 * st.at, st.phase, waits) &&
@@ -398,6 +425,8 @@ __global__ void __launch_bounds__(352, 1)
     attn_dq_kernel(const AttnArgs a, const __grid_constant__ BwdMaps maps) {
   using C = BwdCfg<D>;
   constexpr int N = C::TILE, BLK = C::BLK, NST = C::NST;
+  // Q and dO in tensor memory
+  constexpr uint32_t Q_COL = C::ACC_COL + D, O_COL = Q_COL + D / 2;
   extern __shared__ __align__(1024) unsigned char smem[];
   const uint32_t base = smem_addr(smem);
   const BwdBars<NST> bar(base + C::BAR_OFF);
@@ -456,19 +485,19 @@ __global__ void __launch_bounds__(352, 1)
   } else if (warp == 8) {
     // S, into the buffer that the group has read when its dS is there
     if (total > 0) {
-      const uint32_t qa = base + C::OWN_OFF;
       const bool lead = elect();
       Ring<NST> st;
       Ring<2> buf;
-      bool ok = bar_wait(bar.own, 0, waits);
+      bool ok = bar_wait(bar.there, 0, waits);
+      tc_fence_after();
       for (int j = 0; ok && j < total; ++j) {
         ok = bar_wait(bar.a_full + 8 * st.at, st.phase, waits);
         if (ok && j >= 2) ok = bar_wait(bar.ds_full + 8 * buf.at, buf.phase ^ 1u, waits);
         if (!ok) break;
         tc_fence_after();
         if (lead) {
-          product_rows<T, D>(tmem + C::S_COL + buf.at * BLK, qa,
-                             base + C::A_OFF + st.at * C::STRB);
+          product_rows_ts<T, D>(tmem + C::S_COL + buf.at * BLK, tmem + Q_COL,
+                                base + C::A_OFF + st.at * C::STRB);
           mma_commit(bar.s_full + 8 * buf.at);
         }
         st.next();
@@ -483,11 +512,11 @@ __global__ void __launch_bounds__(352, 1)
   } else if (warp == 9) {
     // dP and dQ: dS lies where dP was, so dP of block j follows dQ of j - 2
     if (total > 0) {
-      const uint32_t oa = base + C::OWN_OFF + C::OWNB;
       const bool lead = elect();
       Ring<NST> kst, vst;
       Ring<2> buf, dbuf;
-      bool ok = bar_wait(bar.own, 0, waits);
+      bool ok = bar_wait(bar.there, 0, waits);
+      tc_fence_after();
       for (int j = 0; ok && j < total + 2; ++j) {
         if (j >= 2) {
           ok = bar_wait(bar.a_full + 8 * kst.at, kst.phase, waits) &&
@@ -506,8 +535,8 @@ __global__ void __launch_bounds__(352, 1)
           ok = bar_wait(bar.b_full + 8 * vst.at, vst.phase, waits);
           if (!ok) break;
           if (lead) {
-            product_rows<T, D>(tmem + C::DP_COL + buf.at * BLK, oa,
-                               base + C::B_OFF + vst.at * C::STRB);
+            product_rows_ts<T, D>(tmem + C::DP_COL + buf.at * BLK, tmem + O_COL,
+                                  base + C::B_OFF + vst.at * C::STRB);
             mma_commit(bar.dp_full + 8 * buf.at);
             mma_commit(bar.b_free + 8 * vst.at);
           }
@@ -533,7 +562,17 @@ __global__ void __launch_bounds__(352, 1)
     const uint32_t dp_at = tmem + lanes + C::DP_COL + group * BLK;
     uint32_t ph = 0;
     bool ok = true;
-    for (int it = group; it < total; it += 2, ph ^= 1u) {
+    if (total > 0) {
+      ok = __all_sync(0xffffffffu, bar_wait(bar.own, 0, waits));
+      if (ok) {
+        copy_operand<D>(smem + C::OWN_OFF + group * C::OWNB, r,
+                        tmem + lanes + Q_COL + group * (D / 2));
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(bar.there);
+      }
+    }
+    for (int it = group; ok && it < total; it += 2, ph ^= 1u) {
       const int n0 = (b0 + it) * BLK;
       ok = __all_sync(0xffffffffu, bar_wait(bar.s_full + 8 * group, ph, waits));
       if (!ok) break;

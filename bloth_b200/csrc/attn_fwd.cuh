@@ -47,13 +47,15 @@ struct FwdCfg {
   static constexpr int K_OFF = 2 * QB;
   static constexpr int V_OFF = K_OFF + NST * KB;
   static constexpr int BAR_OFF = V_OFF + NST * KB;
-  static constexpr int BARS = 1 + 4 * NST + 4 + 4 + 2 + 2;
+  static constexpr int BARS = 1 + 4 * NST + 4 + 4 + 2 + 2 + 1;
   // barriers, the tensor-memory address and the stop flag
   static constexpr int SMEM = BAR_OFF + BARS * 8 + 16;
   static_assert(SMEM <= 227 * 1024, "shared memory");
-  // tensor-memory columns: the tiles' S (two buffers of 64 each), O_0, O_1
+  // tensor-memory columns: the tiles' S (two buffers of 64 each), O_0, O_1,
+  // and where there is room Q_0, Q_1
+  static constexpr bool Q_TMEM = D == 64;
   static constexpr uint32_t COLS = 512;
-  static constexpr uint32_t S_COL = 0, O_COL = 256;
+  static constexpr uint32_t S_COL = 0, O_COL = 256, Q_COL = 384;
 };
 
 struct FwdMaps {
@@ -84,6 +86,7 @@ __global__ void __launch_bounds__(352, 1)
   const uint32_t p_full = s_full + 8 * 4;    // [tile][buffer]
   const uint32_t o_done = p_full + 8 * 4;    // [tile]: a block's product with V has completed
   const uint32_t drained = o_done + 8 * 2;
+  const uint32_t q_there = drained + 8 * 2;  // Q_TMEM: both tiles are in tensor memory
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(smem + C::BAR_OFF + 8 * C::BARS);
   const Waits waits{reinterpret_cast<volatile int*>(tmem_ptr + 1), a.fault};
 
@@ -120,6 +123,7 @@ __global__ void __launch_bounds__(352, 1)
     tmem_alloc(tmem_ptr, C::COLS);
   } else if (threadIdx.x == 0) {
     bar_init(q_full, 1);
+    bar_init(q_there, 8);
     for (int i = 0; i < NST; ++i) {
       bar_init(k_full + 8 * i, 1);
       bar_init(k_free + 8 * i, 2);
@@ -181,7 +185,8 @@ __global__ void __launch_bounds__(352, 1)
       const bool lead = elect();
       Ring<NST> kst, vst;
       Ring<2> kb, vb;  // score buffers of the S and of the O to come
-      bool ok = bar_wait(q_full, 0, waits);
+      bool ok = bar_wait(C::Q_TMEM ? q_there : q_full, 0, waits);
+      tc_fence_after();
       // step j: O of block j - 2, then S of block j where that one's P was;
       // of the CTA's blocks [f, e) are this tile's
       for (int j = 0; ok && j < nb + 2; ++j) {
@@ -209,7 +214,11 @@ __global__ void __launch_bounds__(352, 1)
           if (!ok) break;
           if (lead) {
             if (mine) {
-              product_rows<T, D>(s_at + kb.at * BLK, qa, base + C::K_OFF + kst.at * C::KB);
+              const uint32_t kt = base + C::K_OFF + kst.at * C::KB;
+              if constexpr (C::Q_TMEM)
+                product_rows_ts<T, D>(s_at + kb.at * BLK, tmem + C::Q_COL + t * (D / 2), kt);
+              else
+                product_rows<T, D>(s_at + kb.at * BLK, qa, kt);
               mma_commit(s_full + 16 * t + 8 * kb.at);
             }
             mma_commit(k_free + 8 * kst.at);
@@ -235,13 +244,23 @@ __global__ void __launch_bounds__(352, 1)
     const float2 sc = f2s(a.scale_log2);
     float m = -INFINITY, l = 0.f;
     bool ok = true, there = false;
+    if (C::Q_TMEM && nb > 0) {
+      ok = __all_sync(0xffffffffu, bar_wait(q_full, 0, waits));
+      if (ok) {
+        copy_operand<D>(smem + C::Q_OFF + t * C::QB, threadIdx.x & 127,
+                        tmem + lanes + C::Q_COL + t * (D / 2));
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(q_there);
+      }
+    }
     // Block j's row of S and what its p are taken relative to, before the
     // exponentials of the loop below; that P of block j - 1 is written is
     // told to the issuing warp on the way, so that the wait for its stores
     // costs nothing.
     float x[BLK];
     Ring<2> buf;
-    for (int j = f; j < e; ++j, buf.next()) {
+    for (int j = f; ok && j < e; ++j, buf.next()) {
       const uint32_t s_buf = tmem + lanes + C::S_COL + t * N + buf.at * BLK;
       const uint32_t other = 16 * t + 8 * (buf.at ^ 1u);
       if (!there) there = bar_wait(s_full + 16 * t + 8 * buf.at, buf.phase, waits);
@@ -318,14 +337,18 @@ __global__ void __launch_bounds__(352, 1)
     }
     if (ok && e > f) {
       const int n = e - f;
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) bar_arrive(p_full + 16 * t + 8 * ((n - 1) & 1));
-      // the last two products: a parity tells one phase from the next only
-      ok = (n < 2 || bar_wait(o_done + 8 * t, (uint32_t)(n - 2) & 1u, waits)) &&
-           bar_wait(o_done + 8 * t, (uint32_t)(n - 1) & 1u, waits);
-      ok = __all_sync(0xffffffffu, ok);
+      // A parity tells a phase from the next one only: the product before the
+      // last is waited for before the last one can complete, which needs P of
+      // every warp.
+      ok = __all_sync(0xffffffffu,
+                      n < 2 || bar_wait(o_done + 8 * t, (uint32_t)(n - 2) & 1u, waits));
+      if (ok) {
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(p_full + 16 * t + 8 * ((n - 1) & 1));
+        ok = __all_sync(0xffffffffu, bar_wait(o_done + 8 * t, (uint32_t)(n - 1) & 1u, waits));
+      }
       tc_fence_after();
     }
     if (ok) {

@@ -226,6 +226,15 @@ __device__ __forceinline__ void product_rows(uint32_t d, uint32_t a, uint32_t b)
     mma_ss(d, la + (((kk / 4) * (128 * 128) + (kk % 4) * 32) >> 4),
            lb + (((kk / 4) * (64 * 128) + (kk % 4) * 32) >> 4), id, kk > 0);
 }
+// The same with A in tensor memory (copy_operand).
+template <typename T, int D>
+__device__ __forceinline__ void product_rows_ts(uint32_t d, uint32_t a, uint32_t b) {
+  constexpr uint32_t id = mma_desc<T>(128, 64, false);
+  const uint32_t lb = desc_lo(b, 0);
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk)
+    mma_ts(d, a + kk * 8, lb + (((kk / 4) * (64 * 128) + (kk % 4) * 32) >> 4), id, kk > 0);
+}
 // d (+)= W B, contracted over the 64 rows of operand tile B: W 128 x 64 of
 // 16-bit elements in 32 columns of tensor memory.
 template <typename T, int D>
@@ -333,6 +342,28 @@ __device__ __forceinline__ void store64(uint32_t at, const float (&x)[64]) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) r[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
   tmem_st32(at, r);
+}
+
+// Row `r` of an operand tile of 128 rows, from shared memory to the thread's row
+// of D / 2 tensor-memory columns, two elements each: a first operand there
+// leaves the products half of their shared-memory reads.
+template <int D>
+__device__ __forceinline__ void copy_operand(const unsigned char* tile, int r, uint32_t at) {
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c) {
+    uint32_t w[32];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint4 v = *reinterpret_cast<const uint4*>(tile + c * (128 * 128) + r * 128 +
+                                                      ((i ^ (r & 7)) * 16));
+      w[4 * i] = v.x;
+      w[4 * i + 1] = v.y;
+      w[4 * i + 2] = v.z;
+      w[4 * i + 3] = v.w;
+    }
+    tmem_st32(at + c * 32, w);
+  }
+  tmem_wait_st();
 }
 
 // Rows [r0, 64) of an operand tile of 64 in shared memory become zeros, before
