@@ -47,7 +47,7 @@ struct FwdCfg {
   static constexpr int K_OFF = 2 * QB;
   static constexpr int V_OFF = K_OFF + NST * KB;
   static constexpr int BAR_OFF = V_OFF + NST * KB;
-  static constexpr int BARS = 1 + 4 * NST + 4 + 4 + 2 + 2 + 1;
+  static constexpr int BARS = 1 + 4 * NST + 4 + 4 + 2 + 2 + 2 + 1;
   // barriers, the tensor-memory address and the stop flag
   static constexpr int SMEM = BAR_OFF + BARS * 8 + 16;
   static_assert(SMEM <= 227 * 1024, "shared memory");
@@ -86,7 +86,8 @@ __global__ void __launch_bounds__(352, 1)
   const uint32_t p_full = s_full + 8 * 4;    // [tile][buffer]
   const uint32_t o_done = p_full + 8 * 4;    // [tile]: a block's product with V has completed
   const uint32_t drained = o_done + 8 * 2;
-  const uint32_t q_there = drained + 8 * 2;  // Q_TMEM: both tiles are in tensor memory
+  const uint32_t o_last = drained + 8 * 2;   // [tile]: all have
+  const uint32_t q_there = o_last + 8 * 2;  // Q_TMEM: both tiles are in tensor memory
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(smem + C::BAR_OFF + 8 * C::BARS);
   const Waits waits{reinterpret_cast<volatile int*>(tmem_ptr + 1), a.fault};
 
@@ -137,6 +138,7 @@ __global__ void __launch_bounds__(352, 1)
     for (int t = 0; t < 2; ++t) {
       bar_init(o_done + 8 * t, 1);
       bar_init(drained + 8 * t, 1);
+      bar_init(o_last + 8 * t, 1);
     }
     *waits.stop = 0;
     mbar_init_fence();
@@ -200,7 +202,7 @@ __global__ void __launch_bounds__(352, 1)
             if (mine) {
               product_cols<T, D>(o_at, s_at + vb.at * BLK, base + C::V_OFF + vst.at * C::KB,
                                  j - 2 > f);
-              mma_commit(o_done + 8 * t);
+              mma_commit((j - 2 < e - 1 ? o_done : o_last) + 8 * t);
             }
             // (a commit completes with the products before it, if there are any)
             mma_commit(v_free + 8 * vst.at);
@@ -260,10 +262,10 @@ __global__ void __launch_bounds__(352, 1)
     // costs nothing.
     float x[BLK];
     Ring<2> buf;
-    for (int j = f; ok && j < e; ++j, buf.next()) {
+    for (int j = f; j < e; ++j, buf.next()) {
       const uint32_t s_buf = tmem + lanes + C::S_COL + t * N + buf.at * BLK;
       const uint32_t other = 16 * t + 8 * (buf.at ^ 1u);
-      if (!there) there = bar_wait(s_full + 16 * t + 8 * buf.at, buf.phase, waits);
+      if (!there) there = ok && bar_wait(s_full + 16 * t + 8 * buf.at, buf.phase, waits);
       ok = __all_sync(0xffffffffu, there);
       if (!ok) break;
       tc_fence_after();
@@ -336,19 +338,11 @@ __global__ void __launch_bounds__(352, 1)
       l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
     }
     if (ok && e > f) {
-      const int n = e - f;
-      // A parity tells a phase from the next one only: the product before the
-      // last is waited for before the last one can complete, which needs P of
-      // every warp.
-      ok = __all_sync(0xffffffffu,
-                      n < 2 || bar_wait(o_done + 8 * t, (uint32_t)(n - 2) & 1u, waits));
-      if (ok) {
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) bar_arrive(p_full + 16 * t + 8 * ((n - 1) & 1));
-        ok = __all_sync(0xffffffffu, bar_wait(o_done + 8 * t, (uint32_t)(n - 1) & 1u, waits));
-      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) bar_arrive(p_full + 16 * t + 8 * ((e - f - 1) & 1));
+      ok = __all_sync(0xffffffffu, bar_wait(o_last + 8 * t, 0, waits));
       tc_fence_after();
     }
     if (ok) {
