@@ -1,4 +1,4 @@
-// Attention backward on the tensor cores: 16-bit tensors, head_dim 64 or 128.
+// Attention backward on the tensor cores: 16-bit tensors.
 //
 // Two kernels, each of which recomputes the probabilities p = 2^(s scale
 // log2 e - lse2) of a block of queries and keys from the rows' statistics and
@@ -22,6 +22,10 @@
 // hand-over between warps nor its own latencies stop the tensor core. Warps 8
 // and 9 issue the products, warp 10 the copies.
 //
+// At head_dim 256 the sums of dV and dK would fill tensor memory, so they are
+// two launches of the first kernel: one with S^T and dV, one with S^T, dP^T
+// and dK.
+//
 // Bound: the products. 64 streamed rows against 128 kept ones in shared memory
 // take the time of 128 (a step reads 4 KB of the kept tile whatever the
 // streamed one has): 512 cycles each for S and dP at head_dim 128, 256 for dV
@@ -35,25 +39,34 @@
 
 namespace bloth {
 
-template <int D>
+// What a launch sums up.
+enum BwdSums : int { kSumDQ = 0, kSumDV = 1, kSumDK = 2, kSumDKV = 3 };
+
+template <int D, int SUMS>
 struct BwdCfg {
   static constexpr int TILE = 128;             // rows of the kept tiles
   static constexpr int BLK = 64;               // rows of a streamed block
   static constexpr int THREADS = 352;
   static constexpr int OWNB = TILE * D * 2, STRB = BLK * D * 2;  // bytes of a tile
-  static constexpr int NST = D == 64 ? 8 : 5;  // stages of each streamed tensor
-  static constexpr int OWN_OFF = 0;                  // the two kept tiles
-  static constexpr int A_OFF = 2 * OWNB;             // stages of Q (or K)
-  static constexpr int B_OFF = A_OFF + NST * STRB;   // stages of dO (or V)
-  static constexpr int STAT_OFF = B_OFF + NST * STRB;  // lse2 and delta, with dO's stages
-  static constexpr int BAR_OFF = STAT_OFF + NST * 512;
-  static constexpr int BARS = 1 + 4 * NST + 8 + 3 + 1;
+  static constexpr int OWN = SUMS == kSumDV ? 1 : 2;  // kept tiles: K and V, or Q and dO
+  // Stages of A (Q, or K) and of B (dO, or V): as many as fit. Two of A at
+  // least, which a block's last product reads; one of B where only dP reads it.
+  static constexpr int NA = D == 64 ? 8 : D == 128 ? 5 : SUMS == kSumDV ? 3 : 2;
+  static constexpr int NB = D == 64 ? 8 : D == 128 ? 5 : SUMS == kSumDV ? 2 : 1;
+  static constexpr int OWN_OFF = 0;                    // the kept tiles
+  static constexpr int A_OFF = OWN * OWNB;
+  static constexpr int B_OFF = A_OFF + NA * STRB;
+  static constexpr int STAT_OFF = B_OFF + NB * STRB;   // lse2 and delta, with A's stages
+  static constexpr int BAR_OFF = STAT_OFF + NA * 512;
+  static constexpr int BARS = 1 + 2 * NA + 2 * NB + 8 + 3 + 1;
   static constexpr int SMEM = BAR_OFF + BARS * 8 + 16;
   static_assert(SMEM <= 227 * 1024, "shared memory");
-  // tensor-memory columns: S (two buffers), dP (two buffers), the sums, and
-  // behind them, where there is room, the kept tiles
+  // tensor-memory columns: S (two buffers), dP (two buffers, not for dV alone),
+  // the sums, and behind them, where there is room, the kept tiles
   static constexpr uint32_t COLS = 512;
-  static constexpr uint32_t S_COL = 0, DP_COL = 128, ACC_COL = 256;
+  static constexpr uint32_t S_COL = 0, DP_COL = 128, ACC_COL = SUMS == kSumDV ? 128 : 256;
+  static constexpr uint32_t OWN_COL = ACC_COL + (SUMS == kSumDKV ? 2 * D : D);
+  static constexpr bool OWN_TMEM = OWN_COL + OWN * D / 2 <= COLS;
 };
 
 struct BwdMaps {
@@ -62,17 +75,17 @@ struct BwdMaps {
 
 // Barriers of both kernels; A and B are the streamed tensors (Q and dO, or K
 // and V), [2] one for each buffer.
-template <int NST>
+template <int NA, int NB>
 struct BwdBars {
   uint32_t own, a_full, a_free, b_full, b_free, s_full, p_full, dp_full, ds_full, acc, drained,
       there;
   __device__ __forceinline__ explicit BwdBars(uint32_t at) {
     own = at;
     a_full = own + 8;
-    a_free = a_full + 8 * NST;
-    b_full = a_free + 8 * NST;
-    b_free = b_full + 8 * NST;
-    s_full = b_free + 8 * NST;
+    a_free = a_full + 8 * NA;
+    b_full = a_free + 8 * NA;
+    b_free = b_full + 8 * NB;
+    s_full = b_free + 8 * NB;
     p_full = s_full + 16;
     dp_full = p_full + 16;
     ds_full = dp_full + 16;
@@ -80,13 +93,15 @@ struct BwdBars {
     drained = acc + 8;
     there = drained + 16;  // the kept tiles are in tensor memory
   }
-  // b_free completes with `b_uses` arrivals, acc with `sums`
+  // b_free completes when `b_uses` products have, acc with `sums` of them
   __device__ __forceinline__ void init(int b_uses, int sums) const {
     bar_init(own, 1);
     bar_init(there, 8);
-    for (int i = 0; i < NST; ++i) {
+    for (int i = 0; i < NA; ++i) {
       bar_init(a_full + 8 * i, 1);
       bar_init(a_free + 8 * i, 1);
+    }
+    for (int i = 0; i < NB; ++i) {
       bar_init(b_full + 8 * i, 1);
       bar_init(b_free + 8 * i, b_uses);
     }
@@ -102,10 +117,10 @@ struct BwdBars {
   // given up: not before the copies in flight have landed (blocks [0, it))
   __device__ __forceinline__ void drain_copies(int it, const Waits& w) const {
     bar_drain(own, 0, w);
-    for (int i = max(0, it - NST); i < it; ++i) {
-      bar_drain(a_full + 8 * (i % NST), (uint32_t)(i / NST) & 1u, w);
-      bar_drain(b_full + 8 * (i % NST), (uint32_t)(i / NST) & 1u, w);
-    }
+    for (int i = max(0, it - NA); i < it; ++i)
+      bar_drain(a_full + 8 * (i % NA), (uint32_t)(i / NA) & 1u, w);
+    for (int i = max(0, it - NB); i < it; ++i)
+      bar_drain(b_full + 8 * (i % NB), (uint32_t)(i / NB) & 1u, w);
   }
 };
 
@@ -137,18 +152,18 @@ __device__ __forceinline__ void store_row(uint32_t at, int cols, float f, T* dst
 }
 
 // ------------------------------------------------------------------ dK, dV
-template <typename T, int D>
+template <typename T, int D, int SUMS>
 __global__ void __launch_bounds__(352, 1)
     attn_dkv_kernel(const AttnArgs a, const __grid_constant__ BwdMaps maps) {
-  using C = BwdCfg<D>;
-  constexpr int N = C::TILE, BLK = C::BLK, NST = C::NST;
-  constexpr uint32_t DV_COL = C::ACC_COL, DK_COL = C::ACC_COL + D;
-  // K and V in tensor memory, beside dV and dK of 64 columns
-  constexpr bool OWN_TMEM = D == 64;
-  constexpr uint32_t K_COL = C::ACC_COL + 2 * D, V_COL = K_COL + D / 2;
+  using C = BwdCfg<D, SUMS>;
+  constexpr bool DV = (SUMS & kSumDV) != 0, DK = (SUMS & kSumDK) != 0;
+  constexpr int N = C::TILE, BLK = C::BLK, NA = C::NA, NB = C::NB;
+  constexpr uint32_t DV_COL = C::ACC_COL, DK_COL = C::ACC_COL + (DV ? D : 0);
+  constexpr bool OWN_TMEM = C::OWN_TMEM;
+  constexpr uint32_t K_COL = C::OWN_COL, V_COL = K_COL + D / 2;
   extern __shared__ __align__(1024) unsigned char smem[];
   const uint32_t base = smem_addr(smem);
-  const BwdBars<NST> bar(base + C::BAR_OFF);
+  const BwdBars<NA, NB> bar(base + C::BAR_OFF);
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(smem + C::BAR_OFF + 8 * C::BARS);
   const Waits waits{reinterpret_cast<volatile int*>(tmem_ptr + 1), a.fault};
 
@@ -169,7 +184,7 @@ __global__ void __launch_bounds__(352, 1)
   if (warp == 8) {
     tmem_alloc(tmem_ptr, C::COLS);
   } else if (threadIdx.x == 0) {
-    bar.init(2, 2);
+    bar.init(DV && DK ? 2 : 1, DV && DK ? 2 : 1);
     *waits.stop = 0;
     mbar_init_fence();
   }
@@ -181,27 +196,28 @@ __global__ void __launch_bounds__(352, 1)
   if (warp == 10) {
     // ------------------------------------------------------------- copies
     if (lane == 0 && total > 0) {
-      bar_expect(bar.own, 2 * C::OWNB);
+      bar_expect(bar.own, C::OWN * C::OWNB);
       load_tile<D, N>(base + C::OWN_OFF, &maps.k, s.k0 + n0, h, s.b, bar.own);
-      load_tile<D, N>(base + C::OWN_OFF + C::OWNB, &maps.v, s.k0 + n0, h, s.b, bar.own);
-      Ring<NST> st;
+      if (DK) load_tile<D, N>(base + C::OWN_OFF + C::OWNB, &maps.v, s.k0 + n0, h, s.b, bar.own);
+      Ring<NA> qst;
+      Ring<NB> ost;
       int it = 0, mi = 0, hq = h * a.G;
-      for (; it < total; ++it, st.next()) {
+      for (; it < total; ++it, qst.next(), ost.next()) {
         const int m0 = (mb + mi) * BLK;
         const int64_t stat = (int64_t)hq * a.R + s.stat0 + m0;
-        const uint32_t qf = bar.a_full + 8 * st.at, of = bar.b_full + 8 * st.at;
-        const uint32_t sp = base + C::STAT_OFF + st.at * 512;
-        if (!bar_wait(bar.a_free + 8 * st.at, st.phase ^ 1u, waits)) break;
-        bar_expect(qf, C::STRB);
-        load_tile<D, BLK>(base + C::A_OFF + st.at * C::STRB, &maps.q, s.q0 + m0, hq, s.b, qf);
-        if (!bar_wait(bar.b_free + 8 * st.at, st.phase ^ 1u, waits)) {
-          bar_drain(qf, st.phase, waits);
+        const uint32_t qf = bar.a_full + 8 * qst.at, of = bar.b_full + 8 * ost.at;
+        const uint32_t sp = base + C::STAT_OFF + qst.at * 512;
+        if (!bar_wait(bar.a_free + 8 * qst.at, qst.phase ^ 1u, waits)) break;
+        bar_expect(qf, C::STRB + 512);
+        run_load(sp, a.lse2 + stat, 256, qf);
+        run_load(sp + 256, a.delta + stat, 256, qf);
+        load_tile<D, BLK>(base + C::A_OFF + qst.at * C::STRB, &maps.q, s.q0 + m0, hq, s.b, qf);
+        if (!bar_wait(bar.b_free + 8 * ost.at, ost.phase ^ 1u, waits)) {
+          bar_drain(qf, qst.phase, waits);
           break;
         }
-        bar_expect(of, C::STRB + 512);
-        run_load(sp, a.lse2 + stat, 256, of);
-        run_load(sp + 256, a.delta + stat, 256, of);
-        load_tile<D, BLK>(base + C::B_OFF + st.at * C::STRB, &maps.dout, s.q0 + m0, hq, s.b, of);
+        bar_expect(of, C::STRB);
+        load_tile<D, BLK>(base + C::B_OFF + ost.at * C::STRB, &maps.dout, s.q0 + m0, hq, s.b, of);
         if (++mi == nm) {
           mi = 0;
           ++hq;
@@ -214,22 +230,26 @@ __global__ void __launch_bounds__(352, 1)
     if (total > 0) {
       const uint32_t ka = base + C::OWN_OFF;
       const bool lead = elect();
-      Ring<NST> qst, ost;
+      Ring<NA> qst, qold;
+      Ring<NB> ost;
       Ring<2> buf, pbuf;
       bool ok = bar_wait(OWN_TMEM ? bar.there : bar.own, 0, waits);
       tc_fence_after();
       for (int j = 0; ok && j < total + 2; ++j) {
         if (j >= 2) {
-          ok = bar_wait(bar.b_full + 8 * ost.at, ost.phase, waits) &&
+          ok = (!DV || bar_wait(bar.b_full + 8 * ost.at, ost.phase, waits)) &&
                bar_wait(bar.p_full + 8 * pbuf.at, pbuf.phase, waits);
           if (!ok) break;
           tc_fence_after();
-          if (lead) {
+          if (DV && lead) {
             product_cols<T, D>(tmem + DV_COL, tmem + C::S_COL + pbuf.at * BLK,
                                base + C::B_OFF + ost.at * C::STRB, j > 2);
             mma_commit(bar.b_free + 8 * ost.at);
+            // Q and the statistics went into P^T, which this product has read
+            if (!DK) mma_commit(bar.a_free + 8 * qold.at);
           }
           ost.next();
+          qold.next();
           pbuf.next();
         }
         if (j < total) {
@@ -247,7 +267,7 @@ __global__ void __launch_bounds__(352, 1)
           buf.next();
         }
       }
-      if (lead) {
+      if (lead && (DV || !ok)) {
         mma_commit(ok ? bar.acc : bar.drained);
         if (!ok) bar_drain(bar.drained, 0, waits);
       }
@@ -255,12 +275,12 @@ __global__ void __launch_bounds__(352, 1)
     }
   } else if (warp == 9) {
     // dP^T and dK, dS^T where dP^T was
-    if (total > 0) {
+    if (DK && total > 0) {
       const uint32_t va = base + C::OWN_OFF + C::OWNB;
       const bool lead = elect();
-      Ring<NST> qst, ost;
+      Ring<NA> qst;
+      Ring<NB> ost;
       Ring<2> buf, dbuf;
-      uint32_t done = 0;  // stage whose statistics the group has read
       bool ok = bar_wait(OWN_TMEM ? bar.there : bar.own, 0, waits);
       tc_fence_after();
       for (int j = 0; ok && j < total + 2; ++j) {
@@ -273,11 +293,7 @@ __global__ void __launch_bounds__(352, 1)
             product_cols<T, D>(tmem + DK_COL, tmem + C::DP_COL + dbuf.at * BLK,
                                base + C::A_OFF + qst.at * C::STRB, j > 2);
             mma_commit(bar.a_free + 8 * qst.at);
-            // dP^T of that block has completed with dS^T, which the statistics
-            // beside dO went into
-            bar_arrive(bar.b_free + 8 * done);
           }
-          if (++done == NST) done = 0;
           qst.next();
           dbuf.next();
         }
@@ -291,6 +307,7 @@ __global__ void __launch_bounds__(352, 1)
             else
               product_rows<T, D>(tmem + C::DP_COL + buf.at * BLK, va, ot);
             mma_commit(bar.dp_full + 8 * buf.at);
+            mma_commit(bar.b_free + 8 * ost.at);
           }
           ost.next();
           buf.next();
@@ -310,10 +327,12 @@ __global__ void __launch_bounds__(352, 1)
     const uint32_t s_at = tmem + lanes + C::S_COL + group * BLK;
     const uint32_t dp_at = tmem + lanes + C::DP_COL + group * BLK;
     const float2 sc = f2s(a.scale_log2);
-    Ring<NST> st;
+    Ring<NA> st;
+    Ring<NB> ost;
     int mi = 0;
     if (group) {
       st.next();
+      ost.next();
       mi = nm > 1 ? 1 : 0;
     }
     uint32_t ph = 0;
@@ -321,8 +340,9 @@ __global__ void __launch_bounds__(352, 1)
     if (OWN_TMEM && total > 0) {
       ok = __all_sync(0xffffffffu, bar_wait(bar.own, 0, waits));
       if (ok) {
-        copy_operand<D>(smem + C::OWN_OFF + group * C::OWNB, r,
-                        tmem + lanes + K_COL + group * (D / 2));
+        if (group < C::OWN)
+          copy_operand<D>(smem + C::OWN_OFF + group * C::OWNB, r,
+                          tmem + lanes + K_COL + group * (D / 2));
         tc_fence_before();
         __syncwarp();
         if (lane == 0) bar_arrive(bar.there);
@@ -331,7 +351,7 @@ __global__ void __launch_bounds__(352, 1)
     for (int it = group; ok && it < total; it += 2, ph ^= 1u) {
       const int m0 = (mb + mi) * BLK;
       const float* stat = reinterpret_cast<const float*>(smem + C::STAT_OFF + st.at * 512);
-      ok = bar_wait(bar.b_full + 8 * st.at, st.phase, waits) &&
+      ok = bar_wait(bar.a_full + 8 * st.at, st.phase, waits) &&
            bar_wait(bar.s_full + 8 * group, ph, waits);
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       tc_fence_after();
@@ -357,11 +377,14 @@ __global__ void __launch_bounds__(352, 1)
 #pragma unroll
         for (int i = 0; i < BLK; ++i)
           if (i < from || i >= to) x[i] = 0.f;
-        // rows of dO past the sequence's end that memory does hold
-        if (tail) zero_rows<D>(smem + C::B_OFF + st.at * C::STRB, s.qlen - m0);
+        if (DV && tail) {  // rows of dO past the sequence's end that memory does hold
+          ok = __all_sync(0xffffffffu, bar_wait(bar.b_full + 8 * ost.at, ost.phase, waits));
+          if (!ok) break;
+          zero_rows<D>(smem + C::B_OFF + ost.at * C::STRB, s.qlen - m0);
+        }
       }
-      store64<T>(s_at, x);
-      const bool there = bar_test(bar.dp_full + 8 * group, ph);
+      if (DV) store64<T>(s_at, x);
+      const bool there = !DK || bar_test(bar.dp_full + 8 * group, ph);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -369,32 +392,36 @@ __global__ void __launch_bounds__(352, 1)
       ok = __all_sync(0xffffffffu, there || bar_wait(bar.dp_full + 8 * group, ph, waits));
       if (!ok) break;
       tc_fence_after();
-      float y[BLK];
-      load64(dp_at, y);
+      if constexpr (DK) {
+        float y[BLK];
+        load64(dp_at, y);
 #pragma unroll
-      for (int i = 0; i < BLK; i += 4) {
-        const float4 d = *reinterpret_cast<const float4*>(stat + 64 + i);
-        const float2 u = f2_mul(f2(x[i], x[i + 1]), f2_add(f2(y[i], y[i + 1]), f2(-d.x, -d.y)));
-        const float2 w =
-            f2_mul(f2(x[i + 2], x[i + 3]), f2_add(f2(y[i + 2], y[i + 3]), f2(-d.z, -d.w)));
-        y[i] = u.x;
-        y[i + 1] = u.y;
-        y[i + 2] = w.x;
-        y[i + 3] = w.y;
-      }
-      if (masked) {
+        for (int i = 0; i < BLK; i += 4) {
+          const float4 d = *reinterpret_cast<const float4*>(stat + 64 + i);
+          const float2 u = f2_mul(f2(x[i], x[i + 1]), f2_add(f2(y[i], y[i + 1]), f2(-d.x, -d.y)));
+          const float2 w =
+              f2_mul(f2(x[i + 2], x[i + 3]), f2_add(f2(y[i + 2], y[i + 3]), f2(-d.z, -d.w)));
+          y[i] = u.x;
+          y[i + 1] = u.y;
+          y[i + 2] = w.x;
+          y[i + 3] = w.y;
+        }
+        if (masked) {
 #pragma unroll
-        for (int i = 0; i < BLK; ++i)
-          if (i < from || i >= to) y[i] = 0.f;
-        if (tail) zero_rows<D>(smem + C::A_OFF + st.at * C::STRB, s.qlen - m0);
+          for (int i = 0; i < BLK; ++i)
+            if (i < from || i >= to) y[i] = 0.f;
+          if (tail) zero_rows<D>(smem + C::A_OFF + st.at * C::STRB, s.qlen - m0);
+        }
+        store64<T>(dp_at, y);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(bar.ds_full + 8 * group);
       }
-      store64<T>(dp_at, y);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) bar_arrive(bar.ds_full + 8 * group);
       st.next();
       st.next();
+      ost.next();
+      ost.next();
       mi += 2;
       if (mi >= nm) mi -= nm;
       if (mi >= nm) mi -= nm;  // nm == 1
@@ -404,12 +431,14 @@ __global__ void __launch_bounds__(352, 1)
       tc_fence_after();
     }
     if (ok) {
-      // group 0 writes dV, group 1 dK; keys past the sequence's end (dense
-      // tensors) get zeros
-      const HT& t = group ? a.dk : a.dv;
+      // group 0 writes dV, group 1 dK, or each half of the one there is; keys
+      // past the sequence's end (dense tensors) get zeros
+      const bool is_k = DV && DK ? group != 0 : DK;
+      const int cols = DV && DK ? D : D / 2, c0 = DV && DK ? 0 : group * cols;
+      const HT& t = is_k ? a.dk : a.dv;
       T* dst = reinterpret_cast<T*>(const_cast<void*>(t.p)) + (int64_t)s.b * t.sb +
-               (int64_t)h * t.sh + (int64_t)(s.k0 + key) * t.ss;
-      store_row<T>(tmem + lanes + (group ? DK_COL : DV_COL), D, group ? a.scale : 1.f, dst,
+               (int64_t)h * t.sh + (int64_t)(s.k0 + key) * t.ss + c0;
+      store_row<T>(tmem + lanes + (is_k ? DK_COL : DV_COL) + c0, cols, is_k ? a.scale : 1.f, dst,
                    key < limit, key < s.klen, total > 0);
     }
   }
@@ -423,13 +452,13 @@ __global__ void __launch_bounds__(352, 1)
 template <typename T, int D>
 __global__ void __launch_bounds__(352, 1)
     attn_dq_kernel(const AttnArgs a, const __grid_constant__ BwdMaps maps) {
-  using C = BwdCfg<D>;
-  constexpr int N = C::TILE, BLK = C::BLK, NST = C::NST;
-  // Q and dO in tensor memory
-  constexpr uint32_t Q_COL = C::ACC_COL + D, O_COL = Q_COL + D / 2;
+  using C = BwdCfg<D, kSumDQ>;
+  constexpr int N = C::TILE, BLK = C::BLK, NA = C::NA, NB = C::NB;
+  constexpr bool OWN_TMEM = C::OWN_TMEM;
+  constexpr uint32_t Q_COL = C::OWN_COL, O_COL = Q_COL + D / 2;
   extern __shared__ __align__(1024) unsigned char smem[];
   const uint32_t base = smem_addr(smem);
-  const BwdBars<NST> bar(base + C::BAR_OFF);
+  const BwdBars<NA, NB> bar(base + C::BAR_OFF);
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(smem + C::BAR_OFF + 8 * C::BARS);
   const Waits waits{reinterpret_cast<volatile int*>(tmem_ptr + 1), a.fault};
 
@@ -466,19 +495,20 @@ __global__ void __launch_bounds__(352, 1)
       load_tile<D, N>(base + C::OWN_OFF, &maps.q, s.q0 + m0, h, s.b, bar.own);
       load_tile<D, N>(base + C::OWN_OFF + C::OWNB, &maps.dout, s.q0 + m0, h, s.b, bar.own);
       const int hk = h / a.G;
-      Ring<NST> st;
+      Ring<NA> kst;
+      Ring<NB> vst;
       int it = 0, r0 = s.k0 + b0 * BLK;
-      for (; it < total; ++it, r0 += BLK, st.next()) {
-        const uint32_t kf = bar.a_full + 8 * st.at, vf = bar.b_full + 8 * st.at;
-        if (!bar_wait(bar.a_free + 8 * st.at, st.phase ^ 1u, waits)) break;
+      for (; it < total; ++it, r0 += BLK, kst.next(), vst.next()) {
+        const uint32_t kf = bar.a_full + 8 * kst.at, vf = bar.b_full + 8 * vst.at;
+        if (!bar_wait(bar.a_free + 8 * kst.at, kst.phase ^ 1u, waits)) break;
         bar_expect(kf, C::STRB);
-        load_tile<D, BLK>(base + C::A_OFF + st.at * C::STRB, &maps.k, r0, hk, s.b, kf);
-        if (!bar_wait(bar.b_free + 8 * st.at, st.phase ^ 1u, waits)) {
-          bar_drain(kf, st.phase, waits);
+        load_tile<D, BLK>(base + C::A_OFF + kst.at * C::STRB, &maps.k, r0, hk, s.b, kf);
+        if (!bar_wait(bar.b_free + 8 * vst.at, vst.phase ^ 1u, waits)) {
+          bar_drain(kf, kst.phase, waits);
           break;
         }
         bar_expect(vf, C::STRB);
-        load_tile<D, BLK>(base + C::B_OFF + st.at * C::STRB, &maps.v, r0, hk, s.b, vf);
+        load_tile<D, BLK>(base + C::B_OFF + vst.at * C::STRB, &maps.v, r0, hk, s.b, vf);
       }
       if (*waits.stop) bar.drain_copies(it, waits);
     }
@@ -486,9 +516,9 @@ __global__ void __launch_bounds__(352, 1)
     // S, into the buffer that the group has read when its dS is there
     if (total > 0) {
       const bool lead = elect();
-      Ring<NST> st;
+      Ring<NA> st;
       Ring<2> buf;
-      bool ok = bar_wait(bar.there, 0, waits);
+      bool ok = bar_wait(OWN_TMEM ? bar.there : bar.own, 0, waits);
       tc_fence_after();
       for (int j = 0; ok && j < total; ++j) {
         ok = bar_wait(bar.a_full + 8 * st.at, st.phase, waits);
@@ -496,8 +526,11 @@ __global__ void __launch_bounds__(352, 1)
         if (!ok) break;
         tc_fence_after();
         if (lead) {
-          product_rows_ts<T, D>(tmem + C::S_COL + buf.at * BLK, tmem + Q_COL,
-                                base + C::A_OFF + st.at * C::STRB);
+          const uint32_t kt = base + C::A_OFF + st.at * C::STRB;
+          if constexpr (OWN_TMEM)
+            product_rows_ts<T, D>(tmem + C::S_COL + buf.at * BLK, tmem + Q_COL, kt);
+          else
+            product_rows<T, D>(tmem + C::S_COL + buf.at * BLK, base + C::OWN_OFF, kt);
           mma_commit(bar.s_full + 8 * buf.at);
         }
         st.next();
@@ -513,9 +546,10 @@ __global__ void __launch_bounds__(352, 1)
     // dP and dQ: dS lies where dP was, so dP of block j follows dQ of j - 2
     if (total > 0) {
       const bool lead = elect();
-      Ring<NST> kst, vst;
+      Ring<NA> kst;
+      Ring<NB> vst;
       Ring<2> buf, dbuf;
-      bool ok = bar_wait(bar.there, 0, waits);
+      bool ok = bar_wait(OWN_TMEM ? bar.there : bar.own, 0, waits);
       tc_fence_after();
       for (int j = 0; ok && j < total + 2; ++j) {
         if (j >= 2) {
@@ -535,8 +569,11 @@ __global__ void __launch_bounds__(352, 1)
           ok = bar_wait(bar.b_full + 8 * vst.at, vst.phase, waits);
           if (!ok) break;
           if (lead) {
-            product_rows_ts<T, D>(tmem + C::DP_COL + buf.at * BLK, tmem + O_COL,
-                                  base + C::B_OFF + vst.at * C::STRB);
+            const uint32_t vt = base + C::B_OFF + vst.at * C::STRB;
+            if constexpr (OWN_TMEM)
+              product_rows_ts<T, D>(tmem + C::DP_COL + buf.at * BLK, tmem + O_COL, vt);
+            else
+              product_rows<T, D>(tmem + C::DP_COL + buf.at * BLK, base + C::OWN_OFF + C::OWNB, vt);
             mma_commit(bar.dp_full + 8 * buf.at);
             mma_commit(bar.b_free + 8 * vst.at);
           }
@@ -562,7 +599,7 @@ __global__ void __launch_bounds__(352, 1)
     const uint32_t dp_at = tmem + lanes + C::DP_COL + group * BLK;
     uint32_t ph = 0;
     bool ok = true;
-    if (total > 0) {
+    if (OWN_TMEM && total > 0) {
       ok = __all_sync(0xffffffffu, bar_wait(bar.own, 0, waits));
       if (ok) {
         copy_operand<D>(smem + C::OWN_OFF + group * C::OWNB, r,
@@ -605,7 +642,7 @@ __global__ void __launch_bounds__(352, 1)
           if (i < from || i >= to) y[i] = 0.f;
         // rows of K past the sequence's end that memory does hold
         if (n0 + BLK > s.klen && s.k0 + s.klen < a.Sk)
-          zero_rows<D>(smem + C::A_OFF + (it % NST) * C::STRB, s.klen - n0);
+          zero_rows<D>(smem + C::A_OFF + (it % NA) * C::STRB, s.klen - n0);
       }
       store64<T>(dp_at, y);
       tmem_wait_st();
@@ -633,32 +670,45 @@ __global__ void __launch_bounds__(352, 1)
 
 template <typename T, int D>
 int launch_attn_bwd(const AttnArgs& a0, cudaStream_t st) {
-  using C = BwdCfg<D>;
   AttnArgs a = a0;
   a.fault = fault_word();
   if (a.fault == nullptr) return cuda_status(cudaErrorInvalidDevice);
   BwdMaps m;
   const int dt = DTypeOf<T>::value;
-  int rc = head_map(&m.q, a.q.p, a.q.sb, a.q.ss, a.q.sh, a.B, a.Sq, a.Hq, D, C::BLK, dt);
+  int rc = head_map(&m.q, a.q.p, a.q.sb, a.q.ss, a.q.sh, a.B, a.Sq, a.Hq, D, 64, dt);
   if (rc == BLOTH_OK)
-    rc = head_map(&m.k, a.k.p, a.k.sb, a.k.ss, a.k.sh, a.B, a.Sk, a.Hk, D, C::BLK, dt);
+    rc = head_map(&m.k, a.k.p, a.k.sb, a.k.ss, a.k.sh, a.B, a.Sk, a.Hk, D, 64, dt);
   if (rc == BLOTH_OK)
-    rc = head_map(&m.v, a.v.p, a.v.sb, a.v.ss, a.v.sh, a.B, a.Sk, a.Hk, D, C::BLK, dt);
+    rc = head_map(&m.v, a.v.p, a.v.sb, a.v.ss, a.v.sh, a.B, a.Sk, a.Hk, D, 64, dt);
   if (rc == BLOTH_OK)
-    rc = head_map(&m.dout, a.dout.p, a.dout.sb, a.dout.ss, a.dout.sh, a.B, a.Sq, a.Hq, D, C::BLK,
-                  dt);
+    rc = head_map(&m.dout, a.dout.p, a.dout.sb, a.dout.ss, a.dout.sh, a.B, a.Sq, a.Hq, D, 64, dt);
   if (rc != BLOTH_OK) return rc;
-  auto run = [&](auto kern, int64_t grid) {
-    const int r = prepare_smem((const void*)kern, C::SMEM);
+  auto run = [&](auto kern, int smem, int threads, int64_t grid) {
+    const int r = prepare_smem((const void*)kern, smem);
     if (r != BLOTH_OK) return r;
     if (grid > 0x7fffffff) return BLOTH_ERR_SHAPE;
-    kern<<<(unsigned)grid, C::THREADS, C::SMEM, st>>>(a, m);
+    kern<<<(unsigned)grid, threads, smem, st>>>(a, m);
     return launched(cudaGetLastError());
   };
-  if (a.dk.p != nullptr)
-    rc = run(attn_dkv_kernel<T, D>, attn_tiles(a.Sk, a.packed, C::TILE) * a.Hk * a.B);
-  if (rc == BLOTH_OK && a.dq.p != nullptr)
-    rc = run(attn_dq_kernel<T, D>, attn_tiles(a.Sq, a.packed, C::TILE) * a.Hq * a.B);
+  auto keys = [&](auto sums) {
+    constexpr int S = decltype(sums)::value;
+    using C = BwdCfg<D, S>;
+    return run(attn_dkv_kernel<T, D, S>, C::SMEM, C::THREADS,
+               attn_tiles(a.Sk, a.packed, C::TILE) * a.Hk * a.B);
+  };
+  if (a.dk.p != nullptr) {
+    if constexpr (D == 256) {
+      rc = keys(std::integral_constant<int, kSumDV>{});
+      if (rc == BLOTH_OK) rc = keys(std::integral_constant<int, kSumDK>{});
+    } else {
+      rc = keys(std::integral_constant<int, kSumDKV>{});
+    }
+  }
+  if (rc == BLOTH_OK && a.dq.p != nullptr) {
+    using C = BwdCfg<D, kSumDQ>;
+    rc = run(attn_dq_kernel<T, D>, C::SMEM, C::THREADS,
+             attn_tiles(a.Sq, a.packed, C::TILE) * a.Hq * a.B);
+  }
   return rc;
 }
 

@@ -120,7 +120,7 @@ int bloth_attention_fwd(const void* q, const int64_t* q_strides, const void* k,
     if constexpr (sizeof(T) == 2) {
       if (Sk > 0 && attn_rows_take(Sq, Hq / Hk, D, packed))
         return attn_rows_fwd<T>(a, (int)D, workspace, as_stream(stream));
-      if (D <= 128 && Sk > 0) return attn_tc_fwd<T>(a, (int)D, as_stream(stream));
+      if (Sk > 0) return attn_tc_fwd<T>(a, (int)D, as_stream(stream));
     }
     return attn_simt_fwd<T>(a, (int)D, as_stream(stream));
   });
@@ -180,7 +180,7 @@ int bloth_attention_bwd(const void* dout, const int64_t* dout_strides, const voi
       if (r != BLOTH_OK) return r;
     }
     if constexpr (sizeof(T) == 2) {
-      if (D <= 128 && Sq > 0 && Sk > 0) return attn_tc_bwd<T>(a, (int)D, as_stream(stream));
+      if (Sq > 0 && Sk > 0) return attn_tc_bwd<T>(a, (int)D, as_stream(stream));
     }
     return attn_simt_bwd<T>(a, (int)D, as_stream(stream));
   });

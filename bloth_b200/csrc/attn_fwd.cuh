@@ -1,7 +1,7 @@
-// Attention forward on the tensor cores: 16-bit tensors, head_dim 64 or 128.
+// Attention forward on the tensor cores: 16-bit tensors.
 //
-// A CTA takes 256 query rows of one head as two tiles of 128 and streams the
-// keys they see in blocks of 64. Warps 0-3 and 4-7 are
+// A CTA takes 256 query rows of one head as two tiles of 128 (128 rows, one
+// tile, at head_dim 256) and streams the keys they see in blocks of 64. Warps 0-3 and 4-7 are
 // one softmax group per tile (thread = row), warps 8 and 9 issue one tile's
 // matrix products each, warp 10 the copies.
 // Per tile t and block j, in the buffer j % 2 of the tile's two:
@@ -41,21 +41,22 @@ struct FwdCfg {
   static constexpr int TILE = 128;                   // query rows of a tile
   static constexpr int BLK = 64;                     // keys of a block
   static constexpr int THREADS = 352;
+  static constexpr int TILES = D == 256 ? 1 : 2;     // tiles of a CTA
   static constexpr int QB = TILE * D * 2, KB = BLK * D * 2;  // bytes of an operand tile
-  static constexpr int NST = D == 64 ? 8 : 5;        // stages of K and of V
+  static constexpr int NST = D == 64 ? 8 : D == 128 ? 5 : 2;  // stages of K and of V
   static constexpr int Q_OFF = 0;
-  static constexpr int K_OFF = 2 * QB;
+  static constexpr int K_OFF = TILES * QB;
   static constexpr int V_OFF = K_OFF + NST * KB;
   static constexpr int BAR_OFF = V_OFF + NST * KB;
   static constexpr int BARS = 1 + 4 * NST + 4 + 4 + 2 + 2 + 2 + 1;
   // barriers, the tensor-memory address and the stop flag
   static constexpr int SMEM = BAR_OFF + BARS * 8 + 16;
   static_assert(SMEM <= 227 * 1024, "shared memory");
-  // tensor-memory columns: the tiles' S (two buffers of 64 each), O_0, O_1,
-  // and where there is room Q_0, Q_1
-  static constexpr bool Q_TMEM = D == 64;
+  // tensor-memory columns: the tiles' S (two buffers of 64 each), their O, and
+  // where there is room their Q
+  static constexpr bool Q_TMEM = D != 128;
   static constexpr uint32_t COLS = 512;
-  static constexpr uint32_t S_COL = 0, O_COL = 256, Q_COL = 384;
+  static constexpr uint32_t S_COL = 0, O_COL = TILES * 128, Q_COL = 384;
 };
 
 struct FwdMaps {
@@ -96,9 +97,10 @@ __global__ void __launch_bounds__(352, 1)
   const int tiles = (int)(gridDim.x / heads);
   const int hb = blockIdx.x % heads, h = hb % a.Hq;
   // the tiles that see most keys (causal) start first
-  const AttnSeq s = find_seq<true>(a, hb / a.Hq, tiles - 1 - (int)(blockIdx.x / heads), 2 * N);
+  const AttnSeq s = find_seq<true>(a, hb / a.Hq, tiles - 1 - (int)(blockIdx.x / heads),
+                                  C::TILES * N);
   if (s.tile < 0) return;
-  const int m0 = s.tile * 2 * N;
+  const int m0 = s.tile * C::TILES * N;
   const int limit = a.packed ? s.qlen : a.Sq;
   if (m0 >= limit) return;
 
@@ -111,7 +113,7 @@ __global__ void __launch_bounds__(352, 1)
     key_range(a, s, r, min(r + N, s.qlen), lo, hi);
     first[t] = lo / BLK;
     last[t] = (hi + BLK - 1) / BLK;
-    if (hi <= lo) first[t] = last[t] = 0;
+    if (hi <= lo || t >= C::TILES) first[t] = last[t] = 0;
   }
   int b0 = first[0], b1 = last[0];
   if (last[1] > first[1]) {
@@ -124,12 +126,12 @@ __global__ void __launch_bounds__(352, 1)
     tmem_alloc(tmem_ptr, C::COLS);
   } else if (threadIdx.x == 0) {
     bar_init(q_full, 1);
-    bar_init(q_there, 8);
+    bar_init(q_there, 4 * C::TILES);
     for (int i = 0; i < NST; ++i) {
       bar_init(k_full + 8 * i, 1);
-      bar_init(k_free + 8 * i, 2);
+      bar_init(k_free + 8 * i, C::TILES);
       bar_init(v_full + 8 * i, 1);
-      bar_init(v_free + 8 * i, 2);
+      bar_init(v_free + 8 * i, C::TILES);
     }
     for (int i = 0; i < 4; ++i) {
       bar_init(s_full + 8 * i, 1);
@@ -151,9 +153,10 @@ __global__ void __launch_bounds__(352, 1)
   if (warp == 10) {
     // ------------------------------------------------------------- copies
     if (lane == 0 && nb > 0) {
-      bar_expect(q_full, 2 * C::QB);
+      bar_expect(q_full, C::TILES * C::QB);
       load_tile<D, N>(base + C::Q_OFF, &maps.q, s.q0 + m0, h, s.b, q_full);
-      load_tile<D, N>(base + C::Q_OFF + C::QB, &maps.q, s.q0 + m0 + N, h, s.b, q_full);
+      if (C::TILES == 2)
+        load_tile<D, N>(base + C::Q_OFF + C::QB, &maps.q, s.q0 + m0 + N, h, s.b, q_full);
       const int hk = h / a.G;
       int r0 = s.k0 + b0 * BLK, it = 0;
       Ring<NST> st;
@@ -179,7 +182,7 @@ __global__ void __launch_bounds__(352, 1)
     }
   } else if (warp >= 8) {
     // ----------------------------------------------------------- products
-    if (nb > 0) {
+    if (nb > 0 && warp - 8 < C::TILES) {
       const int t = warp - 8;
       const int f = (t ? first[1] : first[0]) - b0, e = (t ? last[1] : last[0]) - b0;
       const uint32_t qa = base + C::Q_OFF + t * C::QB;
@@ -235,7 +238,7 @@ __global__ void __launch_bounds__(352, 1)
       }
       __syncwarp();
     }
-  } else {
+  } else if (warp < 4 * C::TILES) {
     // ------------------------------------------------------------ softmax
     const int t = warp >> 2;
     const int row = m0 + t * N + (threadIdx.x & 127);  // of the sequence
@@ -402,7 +405,7 @@ int launch_attn_fwd(const AttnArgs& a0, cudaStream_t st) {
   if (rc != BLOTH_OK) return rc;
   auto kern = attn_fwd_kernel<T, D>;
   if ((rc = prepare_smem((const void*)kern, C::SMEM)) != BLOTH_OK) return rc;
-  const int64_t grid = attn_tiles(a.Sq, a.packed, 2 * C::TILE) * a.Hq * a.B;
+  const int64_t grid = attn_tiles(a.Sq, a.packed, C::TILES * C::TILE) * a.Hq * a.B;
   if (grid > 0x7fffffff) return BLOTH_ERR_SHAPE;
   kern<<<(unsigned)grid, C::THREADS, C::SMEM, st>>>(a, m);
   return launched(cudaGetLastError());
