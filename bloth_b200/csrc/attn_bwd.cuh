@@ -675,17 +675,22 @@ int launch_attn_bwd(const AttnArgs& a0, cudaStream_t st) {
   if (a.fault == nullptr) return cuda_status(cudaErrorInvalidDevice);
   BwdMaps m;
   const int dt = DTypeOf<T>::value;
-  int rc = head_map(&m.q, a.q.p, a.q.sb, a.q.ss, a.q.sh, a.B, a.Sq, a.Hq, D, 64, dt);
+  // no keys or no queries, hence no copies: maps of any memory
+  if (a.Sk == 0) a.k = a.v = a.q;
+  if (a.Sq == 0) a.q = a.dout = a.k;
+  const int Sq = a.Sq > 0 ? a.Sq : 1, Sk = a.Sk > 0 ? a.Sk : 1;
+  int rc = head_map(&m.q, a.q.p, a.q.sb, a.q.ss, a.q.sh, a.B, Sq, a.Hq, D, 64, dt);
   if (rc == BLOTH_OK)
-    rc = head_map(&m.k, a.k.p, a.k.sb, a.k.ss, a.k.sh, a.B, a.Sk, a.Hk, D, 64, dt);
+    rc = head_map(&m.k, a.k.p, a.k.sb, a.k.ss, a.k.sh, a.B, Sk, a.Hk, D, 64, dt);
   if (rc == BLOTH_OK)
-    rc = head_map(&m.v, a.v.p, a.v.sb, a.v.ss, a.v.sh, a.B, a.Sk, a.Hk, D, 64, dt);
+    rc = head_map(&m.v, a.v.p, a.v.sb, a.v.ss, a.v.sh, a.B, Sk, a.Hk, D, 64, dt);
   if (rc == BLOTH_OK)
-    rc = head_map(&m.dout, a.dout.p, a.dout.sb, a.dout.ss, a.dout.sh, a.B, a.Sq, a.Hq, D, 64, dt);
+    rc = head_map(&m.dout, a.dout.p, a.dout.sb, a.dout.ss, a.dout.sh, a.B, Sq, a.Hq, D, 64, dt);
   if (rc != BLOTH_OK) return rc;
   auto run = [&](auto kern, int smem, int threads, int64_t grid) {
     const int r = prepare_smem((const void*)kern, smem);
     if (r != BLOTH_OK) return r;
+    if (grid == 0) return BLOTH_OK;
     if (grid > 0x7fffffff) return BLOTH_ERR_SHAPE;
     kern<<<(unsigned)grid, threads, smem, st>>>(a, m);
     return launched(cudaGetLastError());

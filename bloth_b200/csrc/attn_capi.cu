@@ -83,8 +83,11 @@ extern "C" {
 size_t bloth_attention_fwd_workspace_bytes(int64_t B, int64_t Sq, int64_t Sk, int64_t Hq,
                                            int64_t Hk, int64_t D, int64_t packed, int dtype) {
   if (check_sizes(B, Sq, Sk, Hq, Hk, D, packed, dtype)) return 0;
-  if (dtype != BLOTH_F32 && attn_rows_take(Sq, Hq / Hk, D, packed))
-    return attn_rows_workspace(B, Sq, Sk, Hk, Hq / Hk, D);
+  const int64_t G = Hq / Hk;
+  if (dtype == BLOTH_F32)
+    return attn_simt_rows_take(Sq, G, packed) ? attn_rows_workspace(B, Sk, Hk, D, 16) : 0;
+  if (attn_rows_take(Sq, G, D, packed))
+    return attn_rows_workspace(B, Sk, Hk, D, Sq * G <= 16 ? 16 : 32);
   return 0;
 }
 
@@ -117,19 +120,22 @@ int bloth_attention_fwd(const void* q, const int64_t* q_strides, const void* k,
   if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return BLOTH_ERR_ALIGN;
   return by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    if constexpr (sizeof(T) == 2) {
+    if constexpr (sizeof(T) == 4) {
+      return attn_simt_fwd<T>(a, (int)D, workspace, as_stream(stream));
+    } else {
       if (Sk > 0 && attn_rows_take(Sq, Hq / Hk, D, packed))
         return attn_rows_fwd<T>(a, (int)D, workspace, as_stream(stream));
-      if (Sk > 0) return attn_tc_fwd<T>(a, (int)D, as_stream(stream));
+      return attn_tc_fwd<T>(a, (int)D, as_stream(stream));
     }
-    return attn_simt_fwd<T>(a, (int)D, as_stream(stream));
   });
 }
 
 size_t bloth_attention_bwd_workspace_bytes(int64_t B, int64_t Sq, int64_t Sk, int64_t Hq,
                                            int64_t Hk, int64_t D, int64_t packed, int dtype) {
   if (check_sizes(B, Sq, Sk, Hq, Hk, D, packed, dtype)) return 0;
-  return (size_t)(2 * Hq * attn_stat_rows(B, Sq, packed)) * sizeof(float);
+  int64_t n = 2 * Hq * attn_stat_rows(B, Sq, packed);
+  if (dtype == BLOTH_F32 && simt_split(B, Sk, Hk, Hq / Hk, packed)) n += 2 * B * Hq * Sk * D;
+  return (size_t)n * sizeof(float);
 }
 
 int bloth_attention_bwd(const void* dout, const int64_t* dout_strides, const void* q,
@@ -179,10 +185,10 @@ int bloth_attention_bwd(const void* dout, const int64_t* dout_strides, const voi
       const int r = attn_stats<T>(a, (int)D, as_stream(stream));
       if (r != BLOTH_OK) return r;
     }
-    if constexpr (sizeof(T) == 2) {
-      if (Sq > 0 && Sk > 0) return attn_tc_bwd<T>(a, (int)D, as_stream(stream));
-    }
-    return attn_simt_bwd<T>(a, (int)D, as_stream(stream));
+    if constexpr (sizeof(T) == 4)
+      return attn_simt_bwd<T>(a, (int)D, a.delta + Hq * a.R, as_stream(stream));
+    else
+      return attn_tc_bwd<T>(a, (int)D, as_stream(stream));
   });
 }
 

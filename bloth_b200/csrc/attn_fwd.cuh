@@ -398,10 +398,12 @@ int launch_attn_fwd(const AttnArgs& a0, cudaStream_t st) {
   FwdMaps m;
   const int dt = DTypeOf<T>::value;
   int rc = head_map(&m.q, a.q.p, a.q.sb, a.q.ss, a.q.sh, a.B, a.Sq, a.Hq, D, 64, dt);
+  if (a.Sk == 0) a.k = a.v = a.q;  // no keys, hence no copies: a map of any memory
+  const int Sk = a.Sk > 0 ? a.Sk : 1;
   if (rc == BLOTH_OK)
-    rc = head_map(&m.k, a.k.p, a.k.sb, a.k.ss, a.k.sh, a.B, a.Sk, a.Hk, D, 64, dt);
+    rc = head_map(&m.k, a.k.p, a.k.sb, a.k.ss, a.k.sh, a.B, Sk, a.Hk, D, 64, dt);
   if (rc == BLOTH_OK)
-    rc = head_map(&m.v, a.v.p, a.v.sb, a.v.ss, a.v.sh, a.B, a.Sk, a.Hk, D, 64, dt);
+    rc = head_map(&m.v, a.v.p, a.v.sb, a.v.ss, a.v.sh, a.B, Sk, a.Hk, D, 64, dt);
   if (rc != BLOTH_OK) return rc;
   auto kern = attn_fwd_kernel<T, D>;
   if ((rc = prepare_smem((const void*)kern, C::SMEM)) != BLOTH_OK) return rc;

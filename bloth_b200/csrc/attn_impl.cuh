@@ -187,21 +187,38 @@ __device__ __forceinline__ void query_range(const AttnArgs& a, const AttnSeq& s,
   if (n1 <= n0 || hi <= lo) lo = hi = 0;
 }
 
-// Host launchers. attn_tc_*: 16-bit tensors, head_dim 64 or 128.
+// Host launchers.
+// attn_tc_*: 16-bit tensors, on the tensor cores.
 template <typename T>
 int attn_tc_fwd(const AttnArgs& a, int D, cudaStream_t st);
 template <typename T>
 int attn_tc_bwd(const AttnArgs& a, int D, cudaStream_t st);
-// attn_rows_*: 16-bit dense tensors with few query rows.
+// attn_rows_*: 16-bit dense tensors with few query rows; the workspace of
+// `rows` rows (16 or 32) per key head, fp32 as well.
 bool attn_rows_take(int64_t Sq, int64_t G, int64_t D, int64_t packed);
-size_t attn_rows_workspace(int64_t B, int64_t Sq, int64_t Sk, int64_t Hk, int64_t G, int64_t D);
+size_t attn_rows_workspace(int64_t B, int64_t Sk, int64_t Hk, int64_t D, int rows);
 template <typename T>
 int attn_rows_fwd(const AttnArgs& a, int D, void* ws, cudaStream_t st);
+// attn_simt_*: fp32 tensors. attn_simt_rows_take: few query rows (16 rows in
+// the workspace). simt_split: the backward takes fp32 partial sums of dk and
+// dv, [2][B, Hq, Sk, D].
+bool attn_simt_rows_take(int64_t Sq, int64_t G, int64_t packed);
+bool simt_split(int64_t B, int64_t Sk, int64_t Hk, int64_t G, int64_t packed);
 template <typename T>
-int attn_simt_fwd(const AttnArgs& a, int D, cudaStream_t st);
+int attn_simt_fwd(const AttnArgs& a, int D, void* ws, cudaStream_t st);
 template <typename T>
-int attn_simt_bwd(const AttnArgs& a, int D, cudaStream_t st);
+int attn_simt_bwd(const AttnArgs& a, int D, void* partial, cudaStream_t st);
 template <typename T>
 int attn_stats(const AttnArgs& a, int D, cudaStream_t st);
+
+template <typename F>
+int attn_head_dim(int D, F&& f) {
+  switch (D) {
+    case 64: return f(std::integral_constant<int, 64>{});
+    case 128: return f(std::integral_constant<int, 128>{});
+    case 256: return f(std::integral_constant<int, 256>{});
+    default: return BLOTH_ERR_SHAPE;
+  }
+}
 
 }  // namespace bloth

@@ -9,12 +9,12 @@ bool attn_rows_take(int64_t Sq, int64_t G, int64_t D, int64_t packed) {
   return packed == 0 && Sq * G <= (D == 256 ? 16 : 32);
 }
 
-size_t attn_rows_workspace(int64_t B, int64_t Sq, int64_t Sk, int64_t Hk, int64_t G, int64_t D) {
+size_t attn_rows_workspace(int64_t B, int64_t Sk, int64_t Hk, int64_t D, int rows) {
   int64_t chunk, splits;
   if (B * Hk == 0) return 0;
   rows_split(B * Hk, Sk, chunk, splits);
   if (splits == 1) return 0;
-  return (size_t)(splits * B * Hk * (Sq * G <= 16 ? 16 : 32) * (D + 2)) * sizeof(float);
+  return (size_t)(splits * B * Hk * rows * (D + 2)) * sizeof(float);
 }
 
 template <typename T>

@@ -89,10 +89,15 @@ __device__ __forceinline__ void rows_out(const AttnArgs& a, int b, int h, int r,
                                          float y1) {
   const int64_t at = (int64_t)b * a.o.sb + (int64_t)(h * a.G + r % a.G) * a.o.sh +
                      (int64_t)(r / a.G) * a.o.ss + c;
-  uint32_t hi, lo;
-  split2<T>(y0, y1, hi, lo);
-  *reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(const_cast<void*>(a.o.p)) + at) = hi;
-  if (a.rest != nullptr) *reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(a.rest) + at) = lo;
+  T* out = reinterpret_cast<T*>(const_cast<void*>(a.o.p)) + at;
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float2*>(out) = f2(y0, y1);
+  } else {
+    uint32_t hi, lo;
+    split2<T>(y0, y1, hi, lo);
+    *reinterpret_cast<uint32_t*>(out) = hi;
+    if (a.rest != nullptr) *reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(a.rest) + at) = lo;
+  }
 }
 __device__ __forceinline__ void rows_lse(const AttnArgs& a, int b, int h, int r, float m, float l) {
   if (a.lse != nullptr)
@@ -382,9 +387,8 @@ inline void rows_split(int64_t pairs, int64_t Sk, int64_t& chunk, int64_t& split
   splits = Sk > 0 ? (Sk + chunk - 1) / chunk : 1;
 }
 
-template <typename T, int D, int MT>
-int launch_attn_rows(const AttnArgs& a, void* ws, cudaStream_t st) {
-  using C = RowsCfg<D, MT>;
+// The plan of a call whose key heads have `rows` rows each.
+inline RowsPlan rows_plan(const AttnArgs& a, int rows, int D, void* ws) {
   int64_t chunk, splits;
   const int64_t pairs = (int64_t)a.B * a.Hk;
   rows_split(pairs, a.Sk, chunk, splits);
@@ -392,16 +396,29 @@ int launch_attn_rows(const AttnArgs& a, void* ws, cudaStream_t st) {
   pl.chunk = (int)chunk;
   pl.splits = (int)splits;
   pl.sums = reinterpret_cast<float*>(ws);
-  pl.stat = pl.sums + splits * pairs * C::ROWS * D;
+  pl.stat = pl.sums + splits * pairs * rows * D;
+  return pl;
+}
+
+template <typename T, int D>
+int launch_attn_join(const AttnArgs& a, const RowsPlan& pl, int rows, cudaStream_t st) {
+  const int64_t n = (int64_t)a.B * a.Hk * a.Sq * a.G;
+  return launched(launch_dependent(attn_join_kernel<T, D>, (unsigned)((n + 3) / 4), 128u, 0, st, a,
+                                   pl, rows));
+}
+
+template <typename T, int D, int MT>
+int launch_attn_rows(const AttnArgs& a, void* ws, cudaStream_t st) {
+  using C = RowsCfg<D, MT>;
+  const RowsPlan pl = rows_plan(a, C::ROWS, D, ws);
   auto kern = attn_rows_kernel<T, D, MT>;
   int rc = prepare_smem((const void*)kern, C::SMEM);
   if (rc != BLOTH_OK) return rc;
-  if (splits * pairs > 0x7fffffff) return BLOTH_ERR_SHAPE;
-  rc = launched(launch_ex(kern, (unsigned)(splits * pairs), kRowsWarps * 32, C::SMEM, st, a, pl));
-  if (rc != BLOTH_OK || splits == 1) return rc;
-  const int64_t rows = pairs * a.Sq * a.G;
-  return launched(launch_dependent(attn_join_kernel<T, D>, (unsigned)((rows + 3) / 4), 128u, 0, st,
-                                   a, pl, C::ROWS));
+  const int64_t grid = (int64_t)pl.splits * a.B * a.Hk;
+  if (grid > 0x7fffffff) return BLOTH_ERR_SHAPE;
+  rc = launched(launch_ex(kern, (unsigned)grid, kRowsWarps * 32, C::SMEM, st, a, pl));
+  if (rc != BLOTH_OK || pl.splits == 1) return rc;
+  return launch_attn_join<T, D>(a, pl, C::ROWS, st);
 }
 
 }  // namespace bloth

@@ -1,34 +1,38 @@
-// Attention on the fp32 units, forward and backward: fp32 tensors (whose
-// products the tensor cores would round to 16 or 19 bits) and head_dim 256.
+// Attention of fp32 tensors, on the fp32 units (the tensor cores would round
+// the products' operands to 19 bits): forward and backward.
 //
-// A CTA of 256 threads keeps a tile of 64 rows of one head ("own" rows) in
-// shared memory as fp32 and streams the rows of the other side past it in
-// tiles. Thread (ty, tx) of 16 x 16 holds a 4 x (tile/16) block of a product
-// of two tiles: own rows 4*ty.., streamed rows tx, tx + 16, ... Rows are
-// padded by 4 floats, so the 16-byte reads of eight neighbouring rows fall in
-// different banks. Rows past the sequence's end are zero in shared memory,
-// whatever memory holds there.
+// A CTA keeps a tile of OWN rows of one head ("own" rows) in shared memory and
+// streams the rows of the other side past it in tiles. Thread (ty, tx) of
+// OWN/4 x 16 holds a 4 x (tile/16) block of a product of two tiles: own rows
+// 4*ty.., streamed rows tx, tx + 16, ... Rows are padded by 4 floats, so the
+// 16-byte reads of eight neighbouring rows fall in different banks. Rows past
+// the sequence's end are zero in shared memory, whatever memory holds there.
 //
-// Bound: fp32 FMA issue. A product of two 4-wide rows costs one 16-byte read
-// of each row per 4 values, so a 4 x 4 block does 64 FMA for 8 reads.
+// OWN is 64 where that gives a CTA for every SM, else 32: half the threads and
+// half the work of a CTA (@@OWN@@).
+// dK and dV are written by one CTA per key tile and key head, or, where those
+// are fewer than two for an SM, by one per query head into fp32 partial sums
+// that simt_sum_kernel adds over the group in order (@@SPLIT@@).
+//
+// Bound: fp32 FMA issue; a 4 x 4 block does 64 FMA for 8 shared-memory reads of
+// 16 bytes, which leaves about half of the FMA rate.
 #pragma once
 
-#include "attn_impl.cuh"
+#include "attn_rows.cuh"
 
 namespace bloth {
 
-constexpr int kSimtOwn = 64;
-constexpr int kSimtThreads = 256;
+constexpr int kSimtKeys = 64;  // streamed rows of a forward tile
 
 // `rows` rows of D of head tensor t (batch b, head h, rows r0..) as fp32 into
 // dst [tile][D + 4], rows from `rows` on as zeros.
-template <typename T, int D>
+template <typename T, int D, int THREADS>
 __device__ __forceinline__ void simt_load(float* dst, int tile, const HT& t, int b, int h, int r0,
                                           int rows) {
   constexpr int VEC = 16 / (int)sizeof(T);
   const T* base = reinterpret_cast<const T*>(t.p) + (int64_t)b * t.sb + (int64_t)h * t.sh +
                   (int64_t)r0 * t.ss;
-  for (int c = threadIdx.x; c < tile * (D / VEC); c += kSimtThreads) {
+  for (int c = threadIdx.x; c < tile * (D / VEC); c += THREADS) {
     const int r = c / (D / VEC), x = c % (D / VEC) * VEC;
     float f[VEC];
     if (r < rows) {
@@ -122,18 +126,65 @@ __device__ __forceinline__ void simt_store(const HT& t, int b, int h, int r0, in
   }
 }
 
-template <int D>
+template <int D, int OWN>
 constexpr size_t simt_fwd_smem() {
-  return (2 * kSimtOwn * (D + 4) + kSimtOwn * (kSimtOwn + 4)) * sizeof(float);
+  return ((OWN + kSimtKeys) * (D + 4) + OWN * (kSimtKeys + 4)) * sizeof(float);
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kSimtThreads) attn_simt_fwd_kernel(const AttnArgs a) {
-  constexpr int N = kSimtOwn, LD = D + 4, LP = N + 4;
+// One tile of keys for the own rows in qs: scores, running maximum m (natural
+// logarithm's units) and sum l, and acc += p V. `sees(i, j)`: whether own row i
+// sees key j of the tile.
+template <typename T, int D, int THREADS, typename Sees>
+__device__ __forceinline__ void simt_fwd_tile(const AttnArgs& a, const float* qs, float* ks,
+                                              float* ps, int b, int h, int r0, int nk, int ty,
+                                              int tx, float (&acc)[4][D / 16], float (&m)[4],
+                                              float (&l)[4], Sees sees) {
+  constexpr int N = kSimtKeys, LP = N + 4;
+  __syncthreads();
+  simt_load<T, D, THREADS>(ks, N, a.k, b, h, r0, nk);
+  __syncthreads();
+  float x[4][4];
+  simt_dot<D, 4>(qs, ks, ty, tx, x);
+  __syncthreads();
+  simt_load<T, D, THREADS>(ks, N, a.v, b, h, r0, nk);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[i][j] = sees(4 * ty + i, tx + 16 * j) ? x[i][j] * a.scale : -INFINITY;
+      top = fmaxf(top, x[i][j]);
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float mn = fmaxf(m[i], top);
+    const float from = mn == -INFINITY ? 0.f : mn;  // nothing seen yet: all terms are 0
+    const float f = expf(m[i] - from);
+    m[i] = mn;
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float p = expf(x[i][j] - from);
+      sum += p;
+      ps[(4 * ty + i) * LP + tx + 16 * j] = p;
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    l[i] = fmaf(l[i], f, sum);
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) acc[i][c] *= f;
+  }
+  __syncthreads();
+  simt_acc<D, N>(ps, LP, ks, ty, tx, acc);
+}
+
+template <typename T, int D, int OWN>
+__global__ void __launch_bounds__(4 * OWN) attn_simt_fwd_kernel(const AttnArgs a) {
+  constexpr int N = OWN, LD = D + 4, THREADS = 4 * OWN;
   extern __shared__ __align__(16) float sm[];
   float* qs = sm;
   float* ks = qs + N * LD;  // a tile of K, then the same rows of V
-  float* ps = ks + N * LD;
+  float* ps = ks + kSimtKeys * LD;
   const int heads = a.Hq * a.B;
   const int tiles = (int)(gridDim.x / heads);
   const int hb = blockIdx.x % heads, h = hb % a.Hq;
@@ -146,7 +197,7 @@ __global__ void __launch_bounds__(kSimtThreads) attn_simt_fwd_kernel(const AttnA
   const int rows = max(0, min(N, s.qlen - m0));
   int lo, hi;
   key_range(a, s, m0, m0 + rows, lo, hi);
-  simt_load<T, D>(qs, N, a.q, s.b, h, s.q0 + m0, rows);
+  simt_load<T, D, THREADS>(qs, N, a.q, s.b, h, s.q0 + m0, rows);
   float acc[4][D / 16], m[4], l[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -155,66 +206,15 @@ __global__ void __launch_bounds__(kSimtThreads) attn_simt_fwd_kernel(const AttnA
 #pragma unroll
     for (int c = 0; c < D / 16; ++c) acc[i][c] = 0.f;
   }
-  for (int n0 = lo / N * N; n0 < hi; n0 += N) {
-    const int nk = min(N, s.klen - n0);
-    __syncthreads();
-    simt_load<T, D>(ks, N, a.k, s.b, h / a.G, s.k0 + n0, nk);
-    __syncthreads();
-    float x[4][4];
-    simt_dot<D, 4>(qs, ks, ty, tx, x);
-    __syncthreads();
-    simt_load<T, D>(ks, N, a.v, s.b, h / a.G, s.k0 + n0, nk);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float top = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[i][j] = see_keys(a, s, m0 + 4 * ty + i, n0 + tx + 16 * j) ? x[i][j] * a.scale : -INFINITY;
-        top = fmaxf(top, x[i][j]);
-      }
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const float mn = fmaxf(m[i], top);
-      const float from = mn == -INFINITY ? 0.f : mn;  // nothing seen yet: all terms are 0
-      const float f = expf(m[i] - from);
-      m[i] = mn;
-      float sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float p = expf(x[i][j] - from);
-        sum += p;
-        ps[(4 * ty + i) * LP + tx + 16 * j] = p;
-      }
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      l[i] = fmaf(l[i], f, sum);
-#pragma unroll
-      for (int c = 0; c < D / 16; ++c) acc[i][c] *= f;
-    }
-    __syncthreads();
-    simt_acc<D, N>(ps, LP, ks, ty, tx, acc);
-  }
+  for (int n0 = lo / kSimtKeys * kSimtKeys; n0 < hi; n0 += kSimtKeys)
+    simt_fwd_tile<T, D, THREADS>(
+        a, qs, ks, ps, s.b, h / a.G, s.k0 + n0, min(kSimtKeys, s.klen - n0), ty, tx, acc, m, l,
+        [&](int i, int j) { return see_keys(a, s, m0 + i, n0 + j); });
   float f[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) f[i] = l[i] > 0.f || l[i] != l[i] ? 1.f / l[i] : 0.f;
   const int out_rows = min(N, limit - m0);
   simt_store<T, D>(a.o, s.b, h, s.q0 + m0, out_rows, ty, tx, acc, f);
-  if constexpr (sizeof(T) == 2) {
-    if (a.rest != nullptr) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int c = 0; c < D / 16; ++c) {
-          const float y = acc[i][c] * f[i];
-          acc[i][c] = y - to_f(from_f<T>(y));
-        }
-        f[i] = 1.f;
-      }
-      HT rest = a.o;
-      rest.p = a.rest;
-      simt_store<T, D>(rest, s.b, h, s.q0 + m0, out_rows, ty, tx, acc, f);
-    }
-  }
   if (tx == 0 && a.lse != nullptr) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -224,22 +224,89 @@ __global__ void __launch_bounds__(kSimtThreads) attn_simt_fwd_kernel(const AttnA
   }
 }
 
+// Few query rows over many keys: the group's rows (row r = query r / G of head
+// h*G + r % G, at most 16) are one own tile, so K and V are read once for the
+// group, and the keys are split over CTAs in chunks (as in attn_rows.cuh, whose
+// join adds the chunks up). Bound: HBM, K and V once, and close to it the FMA
+// of 16 rows.
+constexpr int kSimtRows = 16;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(4 * kSimtRows)
+    attn_simt_rows_kernel(const AttnArgs a, const RowsPlan pl) {
+  constexpr int N = kSimtRows, LD = D + 4, THREADS = 4 * N;
+  extern __shared__ __align__(16) float sm[];
+  allow_dependent_launch();
+  float* qs = sm;
+  float* ks = qs + N * LD;
+  float* ps = ks + kSimtKeys * LD;
+  const int bh = blockIdx.x % (a.B * a.Hk), split = blockIdx.x / (a.B * a.Hk);
+  const int b = bh / a.Hk, h = bh % a.Hk;
+  const AttnSeq s = find_seq<true>(a, b, 0, 1);
+  const int rows = a.Sq * a.G;
+  int lo, hi;
+  key_range(a, s, 0, s.qlen, lo, hi);
+  lo = max(lo, split * pl.chunk) / kSimtKeys * kSimtKeys;
+  hi = min(hi, (split + 1) * pl.chunk);
+  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+  for (int r = 0; r < N; ++r) {
+    const bool in = r < rows;
+    simt_load<T, D, THREADS>(qs + r * LD, 1, a.q, b, h * a.G + (in ? r % a.G : 0),
+                             in ? r / a.G : 0, in ? 1 : 0);
+  }
+  float acc[4][D / 16], m[4], l[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) acc[i][c] = 0.f;
+  }
+  for (int n0 = lo; n0 < hi; n0 += kSimtKeys)
+    simt_fwd_tile<T, D, THREADS>(
+        a, qs, ks, ps, b, h, n0, min(kSimtKeys, s.klen - n0), ty, tx, acc, m, l,
+        [&](int i, int j) { return i < rows && see_keys(a, s, i / a.G, n0 + j); });
+  const int64_t part = ((int64_t)split * a.B * a.Hk + bh) * N;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = 4 * ty + i;
+    if (r >= rows) continue;
+    const float m2 = m[i] * kLog2e;  // the join's units
+    const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
+#pragma unroll
+    for (int c = 0; c < D / 16; c += 2) {
+      const int col = 64 * (c / 4) + 4 * tx + c % 4;
+      if (pl.splits == 1) rows_out<T>(a, b, h, r, col, acc[i][c] * inv, acc[i][c + 1] * inv);
+      else *reinterpret_cast<float2*>(pl.sums + (part + r) * D + col) = f2(acc[i][c], acc[i][c + 1]);
+    }
+    if (tx == 0) {
+      if (pl.splits == 1) {
+        rows_lse(a, b, h, r, m2, l[i]);
+      } else {
+        pl.stat[(part + r) * 2] = m2;
+        pl.stat[(part + r) * 2 + 1] = l[i];
+      }
+    }
+  }
+}
+
 // Rows of a streamed tile of the backward: two own tiles, two streamed ones
 // and the two weight tiles have to fit in shared memory.
 template <int D> constexpr int kSimtStr = D == 256 ? 32 : 64;
 
-template <int D>
+template <int D, int OWN>
 constexpr size_t simt_bwd_smem() {
-  return (2 * (kSimtOwn + kSimtStr<D>) * (D + 4) + 2 * kSimtOwn * (kSimtStr<D> + 4)) *
-         sizeof(float);
+  return (2 * (OWN + kSimtStr<D>) * (D + 4) + 2 * OWN * (kSimtStr<D> + 4)) * sizeof(float);
 }
 
 // DKV: own rows are keys (K, V), the queries of every head of the group (Q,
-// dO) stream past, dk and dv are written. Else own rows are queries, the keys
+// dO) stream past, dk and dv are written; SPLIT: of one head, whose sums go to
+// head h of dk and dv (the partial sums). Else own rows are queries, the keys
 // stream, dq is written.
-template <typename T, int D, bool DKV>
-__global__ void __launch_bounds__(kSimtThreads) attn_simt_bwd_kernel(const AttnArgs a) {
-  constexpr int N = kSimtOwn, M = kSimtStr<D>, NJ = M / 16, LD = D + 4, LP = M + 4;
+template <typename T, int D, int OWN, bool DKV, bool SPLIT>
+__global__ void __launch_bounds__(4 * OWN) attn_simt_bwd_kernel(const AttnArgs a) {
+  constexpr int N = OWN, M = kSimtStr<D>, NJ = M / 16, LD = D + 4, LP = M + 4;
+  constexpr int THREADS = 4 * OWN;
   extern __shared__ __align__(16) float sm[];
   float* own1 = sm;  // K or Q
   float* own2 = own1 + N * LD;  // V or dO
@@ -247,7 +314,7 @@ __global__ void __launch_bounds__(kSimtThreads) attn_simt_bwd_kernel(const AttnA
   float* str2 = str1 + M * LD;  // dO or V
   float* ps = str2 + M * LD;
   float* ds = ps + N * LP;
-  const int H = DKV ? a.Hk : a.Hq;
+  const int H = DKV && !SPLIT ? a.Hk : a.Hq;
   const int heads = H * a.B;
   const int hb = blockIdx.x % heads, h = hb % H;
   const int tiles = (int)(gridDim.x / heads), bt = (int)(blockIdx.x / heads);
@@ -263,8 +330,9 @@ __global__ void __launch_bounds__(kSimtThreads) attn_simt_bwd_kernel(const AttnA
   if (DKV) query_range(a, s, r0, r0 + rows, lo, hi);
   else key_range(a, s, r0, r0 + rows, lo, hi);
   const int own0 = (DKV ? s.k0 : s.q0) + r0, strb = DKV ? s.q0 : s.k0;
-  simt_load<T, D>(own1, N, DKV ? a.k : a.q, s.b, h, own0, rows);
-  simt_load<T, D>(own2, N, DKV ? a.v : a.dout, s.b, h, own0, rows);
+  const int ho = SPLIT ? h / a.G : h;  // head of the own rows
+  simt_load<T, D, THREADS>(own1, N, DKV ? a.k : a.q, s.b, ho, own0, rows);
+  simt_load<T, D, THREADS>(own2, N, DKV ? a.v : a.dout, s.b, ho, own0, rows);
   float acc1[4][D / 16], acc2[DKV ? 4 : 1][D / 16];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -273,14 +341,14 @@ __global__ void __launch_bounds__(kSimtThreads) attn_simt_bwd_kernel(const AttnA
       acc1[i][c] = 0.f;
       if (DKV) acc2[i][c] = 0.f;
     }
-  const int h1 = DKV ? h * a.G : h / a.G;
-  for (int g = 0; g < (DKV ? a.G : 1); ++g) {
+  const int h1 = !DKV ? h / a.G : SPLIT ? h : h * a.G;
+  for (int g = 0; g < (DKV && !SPLIT ? a.G : 1); ++g) {
     const int64_t stat = (int64_t)(DKV ? h1 + g : h) * a.R + s.stat0;
     for (int t0 = lo / M * M; t0 < hi; t0 += M) {
       const int nt = min(M, (DKV ? s.qlen : s.klen) - t0);
       __syncthreads();
-      simt_load<T, D>(str1, M, DKV ? a.q : a.k, s.b, h1 + g, strb + t0, nt);
-      simt_load<T, D>(str2, M, DKV ? a.dout : a.v, s.b, h1 + g, strb + t0, nt);
+      simt_load<T, D, THREADS>(str1, M, DKV ? a.q : a.k, s.b, h1 + g, strb + t0, nt);
+      simt_load<T, D, THREADS>(str2, M, DKV ? a.dout : a.v, s.b, h1 + g, strb + t0, nt);
       __syncthreads();
       float x[4][NJ], y[4][NJ];
       simt_dot<D, NJ>(own1, str1, ty, tx, x);
@@ -314,122 +382,116 @@ __global__ void __launch_bounds__(kSimtThreads) attn_simt_bwd_kernel(const AttnA
   }
 }
 
-// delta = rowsum(dO * O) and lse in base 2 for the backward kernels, for every
-// row of every 128-row tile of a sequence: a row past the sequence's end, or
-// one that sees nothing, gets lse2 = +inf and delta = 0, so its recomputed
-// probabilities are exp2(x - inf) = 0. HBM-bound: reads O, its rest and dO once. A row
-// takes D / 8 lanes of 16-bit (D / 4 of fp32) elements, one 16-byte load of
-// each tensor per lane and pass.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) attn_stats_kernel(const AttnArgs a) {
-  constexpr int VEC = 16 / (int)sizeof(T), LPR = D / VEC < 32 ? D / VEC : 32;
-  constexpr int PASS = D / (VEC * LPR), RPW = 32 / LPR;
-  const int heads = a.Hq * a.B;
-  const int hb = blockIdx.x % heads, h = hb % a.Hq;
-  const AttnSeq s = find_seq<true>(a, hb / a.Hq, (int)(blockIdx.x / heads), 128);
-  if (s.tile < 0) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int m0 = s.tile * 128;
-  const int64_t stat = (int64_t)h * a.R + s.stat0 + m0;
-  const T* op = reinterpret_cast<const T*>(a.o.p) + (int64_t)s.b * a.o.sb + (int64_t)h * a.o.sh;
-  const T* rp =
-      reinterpret_cast<const T*>(a.rest) + (int64_t)s.b * a.o.sb + (int64_t)h * a.o.sh;
-  const T* dp =
-      reinterpret_cast<const T*>(a.dout.p) + (int64_t)s.b * a.dout.sb + (int64_t)h * a.dout.sh;
-#pragma unroll
-  for (int r = warp * 16 + lane / LPR; r < warp * 16 + 16; r += RPW) {
-    const bool in = m0 + r < s.qlen;
-    const int64_t row = s.q0 + m0 + r;
-    float sum = 0.f;
-    if (in) {
-#pragma unroll
-      for (int u = 0; u < PASS; ++u) {
-        const int x = (u * LPR + lane % LPR) * VEC;
-        float f[VEC], g[VEC];
-        unpack(ldg_pack<T, VEC>(op + row * a.o.ss + x), f);
-        unpack(ldg_pack<T, VEC>(dp + row * a.dout.ss + x), g);
-        if (sizeof(T) == 2 && a.rest != nullptr) {
-          float e[VEC];
-          unpack(ldg_pack<T, VEC>(rp + row * a.o.ss + x), e);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) f[i] += e[i];
-        }
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) sum = fmaf(f[e], g[e], sum);
-      }
-    }
-    sum = group_lane_sum<LPR>(sum);
-    if (lane % LPR == 0) {
-      const float l = in ? a.lse[((int64_t)s.b * a.Hq + h) * a.Sq + row] : -INFINITY;
-      const bool none = l == -INFINITY;
-      a.lse2[stat + r] = none ? INFINITY : l * kLog2e;
-      a.delta[stat + r] = none ? 0.f : sum;
-    }
+// The group's partial sums of dk and dv [B, Hq, Sk, D], added in head order.
+template <int D>
+__global__ void __launch_bounds__(256) simt_sum_kernel(const float* pk, const float* pv, HT dk,
+                                                       HT dv, int B, int Sk, int Hk, int G) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;  // 4 elements each
+  const int c = (int)(i % (D / 4)) * 4;
+  const int64_t row = i / (D / 4);  // (b * Hk + h) * Sk + key
+  if (row >= (int64_t)B * Hk * Sk) return;
+  const int key = (int)(row % Sk), h = (int)(row / Sk % Hk), b = (int)(row / Sk / Hk);
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+  for (int g = 0; g < G; ++g) {
+    const int64_t at = ((((int64_t)b * Hk + h) * G + g) * Sk + key) * D + c;
+    const float4 u = *reinterpret_cast<const float4*>(pk + at);
+    const float4 w = *reinterpret_cast<const float4*>(pv + at);
+    x = make_float4(x.x + u.x, x.y + u.y, x.z + u.z, x.w + u.w);
+    y = make_float4(y.x + w.x, y.y + w.y, y.z + w.z, y.w + w.w);
   }
+  auto put = [&](const HT& t, float4 v) {
+    *reinterpret_cast<float4*>(reinterpret_cast<float*>(const_cast<void*>(t.p)) +
+                               (int64_t)b * t.sb + (int64_t)key * t.ss + (int64_t)h * t.sh + c) = v;
+  };
+  put(dk, x);
+  put(dv, y);
 }
 
+// Own rows of a tile: 64 where `tiles64` CTAs of 64 give every SM one.
+inline int simt_own(int64_t tiles64) { return tiles64 >= device_sm_count() ? 64 : 32; }
+
 template <typename F>
-int attn_head_dim(int D, F&& f) {
-  switch (D) {
-    case 64: return f(std::integral_constant<int, 64>{});
-    case 128: return f(std::integral_constant<int, 128>{});
-    case 256: return f(std::integral_constant<int, 256>{});
-    default: return BLOTH_ERR_SHAPE;
-  }
+int simt_own_tile(int own, F&& f) {
+  return own == 64 ? f(std::integral_constant<int, 64>{}) : f(std::integral_constant<int, 32>{});
+}
+
+template <typename T, int D>
+int simt_rows(const AttnArgs& a, void* ws, cudaStream_t st) {
+  auto kern = attn_simt_rows_kernel<T, D>;
+  constexpr size_t smem = simt_fwd_smem<D, kSimtRows>();
+  const RowsPlan pl = rows_plan(a, kSimtRows, D, ws);
+  int rc = prepare_smem((const void*)kern, smem);
+  if (rc != BLOTH_OK) return rc;
+  const int64_t grid = (int64_t)pl.splits * a.B * a.Hk;
+  if (grid > 0x7fffffff) return BLOTH_ERR_SHAPE;
+  rc = launched(launch_ex(kern, (unsigned)grid, 4 * kSimtRows, smem, st, a, pl));
+  if (rc != BLOTH_OK || pl.splits == 1) return rc;
+  return launch_attn_join<T, D>(a, pl, kSimtRows, st);
 }
 
 template <typename T>
-int attn_simt_fwd(const AttnArgs& a, int D, cudaStream_t st) {
+int attn_simt_fwd(const AttnArgs& a, int D, void* ws, cudaStream_t st) {
   return attn_head_dim(D, [&](auto dd) {
     constexpr int DD = decltype(dd)::value;
-    auto kern = attn_simt_fwd_kernel<T, DD>;
-    const int rc = prepare_smem((const void*)kern, simt_fwd_smem<DD>());
-    if (rc != BLOTH_OK) return rc;
-    const int64_t grid = attn_tiles(a.Sq, a.packed, kSimtOwn) * a.Hq * a.B;
-    if (grid == 0) return BLOTH_OK;
-    if (grid > 0x7fffffff) return BLOTH_ERR_SHAPE;
-    return launched(launch_ex(kern, (unsigned)grid, kSimtThreads, simt_fwd_smem<DD>(), st, a));
+    if (attn_simt_rows_take(a.Sq, a.G, a.packed) && a.Sk > 0) return simt_rows<T, DD>(a, ws, st);
+    const int64_t heads = (int64_t)a.Hq * a.B;
+    return simt_own_tile(simt_own(attn_tiles(a.Sq, a.packed, 64) * heads), [&](auto oo) {
+      constexpr int OWN = decltype(oo)::value;
+      auto kern = attn_simt_fwd_kernel<T, DD, OWN>;
+      constexpr size_t smem = simt_fwd_smem<DD, OWN>();
+      const int rc = prepare_smem((const void*)kern, smem);
+      if (rc != BLOTH_OK) return rc;
+      const int64_t grid = attn_tiles(a.Sq, a.packed, OWN) * heads;
+      if (grid == 0) return BLOTH_OK;
+      if (grid > 0x7fffffff) return BLOTH_ERR_SHAPE;
+      return launched(launch_ex(kern, (unsigned)grid, 4 * OWN, smem, st, a));
+    });
   });
 }
 
 template <typename T>
-int attn_simt_bwd(const AttnArgs& a, int D, cudaStream_t st) {
+int attn_simt_bwd(const AttnArgs& a0, int D, void* partial, cudaStream_t st) {
   return attn_head_dim(D, [&](auto dd) {
     constexpr int DD = decltype(dd)::value;
-    auto run = [&](auto kern, int64_t grid) {
-      const int rc = prepare_smem((const void*)kern, simt_bwd_smem<DD>());
-      if (rc != BLOTH_OK) return rc;
-      if (grid == 0) return BLOTH_OK;
-      if (grid > 0x7fffffff) return BLOTH_ERR_SHAPE;
-      return launched(launch_ex(kern, (unsigned)grid, kSimtThreads, simt_bwd_smem<DD>(), st, a));
+    AttnArgs a = a0;
+    auto run = [&](auto dkv, auto split, int64_t heads, int64_t S) {
+      constexpr bool DKV = decltype(dkv)::value, SPLIT = decltype(split)::value;
+      return simt_own_tile(simt_own(attn_tiles(S, a.packed, 64) * heads), [&](auto oo) {
+        constexpr int OWN = decltype(oo)::value;
+        auto kern = attn_simt_bwd_kernel<T, DD, OWN, DKV, SPLIT>;
+        constexpr size_t smem = simt_bwd_smem<DD, OWN>();
+        const int rc = prepare_smem((const void*)kern, smem);
+        if (rc != BLOTH_OK) return rc;
+        const int64_t grid = attn_tiles(S, a.packed, OWN) * heads;
+        if (grid == 0) return BLOTH_OK;
+        if (grid > 0x7fffffff) return BLOTH_ERR_SHAPE;
+        return launched(launch_ex(kern, (unsigned)grid, 4 * OWN, smem, st, a));
+      });
     };
+    using Yes = std::true_type;
+    using No = std::false_type;
     int rc = BLOTH_OK;
-    if (a.dk.p != nullptr)
-      rc = run(attn_simt_bwd_kernel<T, DD, true>,
-               attn_tiles(a.Sk, a.packed, kSimtOwn) * a.Hk * a.B);
+    if (a.dk.p != nullptr) {
+      if (simt_split(a.B, a.Sk, a.Hk, a.G, a.packed)) {
+        // partial sums [B, Hq, Sk, D] of dk, then of dv
+        const int64_t n = (int64_t)a.B * a.Hq * a.Sk * DD;
+        float* pk = reinterpret_cast<float*>(partial);
+        a.dk = HT{pk, (int64_t)a.Hq * a.Sk * DD, DD, (int64_t)a.Sk * DD};
+        a.dv = a.dk;
+        a.dv.p = pk + n;
+        rc = run(Yes{}, Yes{}, (int64_t)a.Hq * a.B, a.Sk);
+        const int64_t four = (int64_t)a.B * a.Hk * a.Sk * (DD / 4);
+        if (rc == BLOTH_OK)
+          rc = launched(launch_ex(simt_sum_kernel<DD>, (unsigned)((four + 255) / 256), 256u, 0, st,
+                                  pk, pk + n, a0.dk, a0.dv, a.B, a.Sk, a.Hk, a.G));
+      } else {
+        rc = run(Yes{}, No{}, (int64_t)a.Hk * a.B, a.Sk);
+      }
+    }
     if (rc == BLOTH_OK && a.dq.p != nullptr)
-      rc = run(attn_simt_bwd_kernel<T, DD, false>,
-               attn_tiles(a.Sq, a.packed, kSimtOwn) * a.Hq * a.B);
+      rc = run(No{}, No{}, (int64_t)a.Hq * a.B, a.Sq);
     return rc;
   });
 }
 
-template <typename T>
-int attn_stats(const AttnArgs& a, int D, cudaStream_t st) {
-  return attn_head_dim(D, [&](auto dd) {
-    constexpr int DD = decltype(dd)::value;
-    const int64_t grid = attn_tiles(a.Sq, a.packed, 128) * a.Hq * a.B;
-    if (grid == 0) return BLOTH_OK;
-    if (grid > 0x7fffffff) return BLOTH_ERR_SHAPE;
-    return launched(launch_ex(attn_stats_kernel<T, DD>, (unsigned)grid, 256u, 0, st, a));
-  });
-}
-
 }  // namespace bloth
-
-#define BLOTH_INSTANTIATE_ATTN_SIMT(T)                                  \
-  namespace bloth {                                                     \
-  template int attn_simt_fwd<T>(const AttnArgs&, int, cudaStream_t);    \
-  template int attn_simt_bwd<T>(const AttnArgs&, int, cudaStream_t);    \
-  template int attn_stats<T>(const AttnArgs&, int, cudaStream_t);       \
-  }
