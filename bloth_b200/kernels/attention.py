@@ -24,6 +24,8 @@ _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 def _addressable(t):
     """_heads, with tensors that repeat a row of memory written out (a tensor
     map cannot describe a stride of 0)."""
+    if t.is_contiguous():
+        return _heads(t)
     st = t.stride()
     if 0 in st and any(n > 1 and s == 0 for n, s in zip(t.shape, st)):
         t = t.contiguous()
@@ -87,15 +89,19 @@ def _workspace(entry: str, device, *args):
     return (torch.empty(n, dtype=torch.uint8, device=device) if n else None), n
 
 
+def _contiguous_like(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def attention_forward(q4, k4, v4, q_seq, k_seq, packed, scale, causal, window, want_lse=True,
                       want_rest=False):
     """(out, lse, rest) of addressable head tensors: lse if wanted, and for
     16-bit tensors what rounding took off out, for the backward."""
     B, Sq, Hq, D = q4.shape
     Sk, Hk = k4.shape[1], k4.shape[2]
-    out = torch.empty((B, Sq, Hq, D), dtype=q4.dtype, device=q4.device)
+    out = _contiguous_like(q4)
     rest = torch.empty_like(out) if want_rest and q4.dtype != torch.float32 else None
-    lse = torch.empty((B, Hq, Sq), dtype=torch.float32, device=q4.device) if want_lse else None
+    lse = q4.new_empty((B, Hq, Sq), dtype=torch.float32) if want_lse else None
     code = _lib.dtype_code(q4.dtype)
     ws, n = _workspace("bloth_attention_fwd_workspace_bytes", q4.device, B, Sq, Sk, Hq, Hk, D,
                        packed, code)
@@ -132,29 +138,28 @@ def attention_backward(do4, q4, k4, v4, out, rest, lse, q_seq, k_seq, packed, sc
 class _AttentionFunction(torch.autograd.Function):
 
     @staticmethod
-    def forward(ctx, q, k, v, q_seq, k_seq, packed, scale, causal, window):
+    def forward(ctx, q, k, v, want_lse, *how):
         q4, k4, v4 = _addressable(q), _addressable(k), _addressable(v)
-        out, lse, rest = attention_forward(q4, k4, v4, q_seq, k_seq, packed, scale, causal, window,
-                                           want_rest=True)
-        ctx.save_for_backward(q4, k4, v4, out, rest, lse, q_seq, k_seq)
-        ctx.meta = (packed, scale, causal, window, q.dim() == 3)
+        out, lse, rest = attention_forward(q4, k4, v4, *how, want_rest=True)
+        ctx.save_for_backward(q4, k4, v4, out, rest, lse, *how[:2])
+        ctx.how = how[2:]
+        if q.dim() == 3:
+            out = out[0]
+        if not want_lse:
+            return out
         ctx.mark_non_differentiable(lse)
-        ctx.set_materialize_grads(False)
-        return (out[0] if q.dim() == 3 else out), lse
+        return out, lse
 
     @staticmethod
-    def backward(ctx, dout, _):
-        if dout is None:
-            return (None,) * 9
+    def backward(ctx, dout, *_):
         q4, k4, v4, out, rest, lse, q_seq, k_seq = ctx.saved_tensors
-        packed, scale, causal, window, flat = ctx.meta
-        want_q, want_k, want_v = ctx.needs_input_grad[:3]
-        grads = attention_backward(_addressable(dout), q4, k4, v4, out, rest, lse, q_seq, k_seq,
-                                   packed, scale, causal, window, want_q, want_k or want_v)
-        if flat:
-            grads = [None if g is None else g[0] for g in grads]
-        dq, dk, dv = grads
-        return dq, dk if want_k else None, dv if want_v else None, None, None, None, None, None, None
+        want = ctx.needs_input_grad
+        dq, dk, dv = attention_backward(_addressable(dout), q4, k4, v4, out, rest, lse, q_seq,
+                                        k_seq, *ctx.how, want[0], want[1] or want[2])
+        if dout.dim() == 3:
+            dq, dk, dv = (None if g is None else g[0] for g in (dq, dk, dv))
+        return (dq, dk if want[1] else None, dv if want[2] else None, None, None, None, None, None,
+                None, None)
 
 
 def fused_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = True,
@@ -213,7 +218,10 @@ def fused_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: b
     q_seq, k_seq, packed = _sequences(q, k, q_lens, k_lens, cu_seqlens, cu_seqlens_k)
     how = (q_seq, k_seq, packed, float(scale), bool(causal), int(window or 0))
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        out, lse = _AttentionFunction.apply(q, k, v, *how)
+        out = _AttentionFunction.apply(q, k, v, return_lse, *how)
+        if not return_lse:
+            return out
+        out, lse = out
     else:
         out, lse, _ = attention_forward(_addressable(q), _addressable(k), _addressable(v), *how,
                                         want_lse=return_lse)

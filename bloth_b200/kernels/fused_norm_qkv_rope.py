@@ -104,6 +104,8 @@ def _heads(t: torch.Tensor | None):
     if t.dim() != 4:
         raise ValueError("[Bloth] head tensors must be [B, S, H, D] or [S, H, D]")
     v = 16 // t.element_size()
+    if t.is_contiguous() and t.shape[3] % v == 0 and t.data_ptr() % 16 == 0:
+        return t
     sb, ss, sh, sd = t.stride()
     if sd != 1 or t.data_ptr() % 16 or sb % v or ss % v or sh % v:
         t = _lib.aligned16(t.contiguous())

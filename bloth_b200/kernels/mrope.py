@@ -21,6 +21,10 @@ from .rope import _out_like
 MAX_AXES = 4
 
 
+def _contiguous_like(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 @lru_cache(maxsize=64)
 def _mrope_axes(sections: tuple, interleaved: bool) -> tuple:
     if not 1 <= len(sections) <= MAX_AXES or any(n < 0 for n in sections):
@@ -109,10 +113,10 @@ def _norm_mrope_call(q, k, wq, wk, position_ids, inv_freq, axes, eps, weight_off
         raise ValueError("[Bloth] wk is required with k")
     wk = None if wk is None else _weight(wk, D, wq.dtype)
     wq = _weight(wq, D, wq.dtype)
-    qo = torch.empty((B, S, Hq, D), dtype=q4.dtype, device=q4.device)
-    ko = None if k4 is None else torch.empty((B, S, Hk, D), dtype=k4.dtype, device=k4.device)
-    rq = torch.empty((B, S, Hq), dtype=torch.float32, device=q4.device)
-    rk = None if k4 is None else torch.empty((B, S, Hk), dtype=torch.float32, device=q4.device)
+    qo = _contiguous_like(q4)
+    ko = None if k4 is None else _contiguous_like(k4)
+    rq = q4.new_empty((B, S, Hq), dtype=torch.float32)
+    rk = None if k4 is None else q4.new_empty((B, S, Hk), dtype=torch.float32)
     rc = _lib.call(
         "bloth_qk_norm_mrope_fwd", q4, _lib.ptr(q4), _head_strides(q4), _lib.ptr(k4),
         _head_strides(k4), _lib.ptr(wq), _lib.ptr(wk), weight_offset, _lib.ptr(qo),
@@ -144,10 +148,10 @@ class _QKNormMRoPEFunction(torch.autograd.Function):
         Hk = 0 if k4 is None else k4.shape[2]
         gq = _heads(grads[0])
         gk = None if k4 is None else _heads(grads[1])
-        dq = torch.empty((B, S, Hq, D), dtype=q4.dtype, device=q4.device)
-        dk = None if k4 is None else torch.empty((B, S, Hk, D), dtype=q4.dtype, device=q4.device)
-        dwq = torch.empty(D, dtype=wq.dtype, device=q4.device)
-        dwk = None if k4 is None else torch.empty(D, dtype=wk.dtype, device=q4.device)
+        dq = _contiguous_like(q4)
+        dk = None if k4 is None else _contiguous_like(k4)
+        dwq = torch.empty_like(wq)
+        dwk = None if k4 is None else torch.empty_like(wk)
         code = _lib.dtype_code(q4.dtype)
         n = _lib.workspace_bytes("bloth_qk_norm_mrope_bwd_workspace_bytes", q4.device, B, S, D,
                                  code)
