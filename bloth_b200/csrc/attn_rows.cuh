@@ -338,31 +338,31 @@ __global__ void __launch_bounds__(kRowsWarps * 32)
   }
 }
 
-// The chunks' partial rows to one row, in chunk order: a warp per row.
+// The chunks' partial rows to one row: a CTA per row, whose four warps take the
+// chunks in turn, their sums then added in warp order.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a, const RowsPlan pl,
                                                         int part_rows) {
-  wait_for_prior_grid();
-  const int rows = a.Sq * a.G, lane = threadIdx.x & 31;
-  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (i >= (int64_t)a.B * a.Hk * rows) return;
-  const int bh = (int)(i / rows), r = (int)(i % rows);
+  constexpr int V = D / 32;
+  __shared__ float sums[4][D + 1];
+  const int rows = a.Sq * a.G, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int bh = (int)(blockIdx.x / rows), r = (int)(blockIdx.x % rows);
   const int64_t step = (int64_t)a.B * a.Hk * part_rows;
   const int64_t p0 = (int64_t)bh * part_rows + r;
+  wait_for_prior_grid();
   float mm = -INFINITY;
   for (int c = lane; c < pl.splits; c += 32) mm = fmaxf(mm, pl.stat[(p0 + c * step) * 2]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
-  constexpr int V = D / 32;
   float y[V], ll = 0.f;
 #pragma unroll
   for (int e = 0; e < V; ++e) y[e] = 0.f;
 #pragma unroll 4
-  for (int c = 0; c < pl.splits; ++c) {
+  for (int c = warp; c < pl.splits; c += 4) {
     const int64_t p = p0 + c * step;
-    const float mi = pl.stat[p * 2];
-    const float w = mi == -INFINITY ? 0.f : ex2(mi - mm);
-    ll = fmaf(pl.stat[p * 2 + 1], w, ll);
+    const float2 st = *reinterpret_cast<const float2*>(pl.stat + p * 2);
+    const float w = st.x == -INFINITY ? 0.f : ex2(st.x - mm);
+    ll = fmaf(st.y, w, ll);
 #pragma unroll
     for (int e = 0; e < V; e += 2) {
       const float2 v = *reinterpret_cast<const float2*>(pl.sums + p * D + lane * V + e);
@@ -370,18 +370,27 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a, const 
       y[e + 1] = fmaf(v.y, w, y[e + 1]);
     }
   }
-  const float inv = ll == 0.f ? 0.f : 1.f / ll;
 #pragma unroll
-  for (int e = 0; e < V; e += 2)
-    rows_out<T>(a, bh / a.Hk, bh % a.Hk, r, lane * V + e, y[e] * inv, y[e + 1] * inv);
-  if (lane == 0) rows_lse(a, bh / a.Hk, bh % a.Hk, r, mm, ll);
+  for (int e = 0; e < V; ++e) sums[warp][lane * V + e] = y[e];
+  if (lane == 0) sums[warp][D] = ll;
+  __syncthreads();
+  const float l = (sums[0][D] + sums[1][D]) + (sums[2][D] + sums[3][D]);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  for (int c = 2 * threadIdx.x; c < D; c += 256) {
+    const float y0 = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
+    const float y1 = (sums[0][c + 1] + sums[1][c + 1]) + (sums[2][c + 1] + sums[3][c + 1]);
+    rows_out<T>(a, bh / a.Hk, bh % a.Hk, r, c, y0 * inv, y1 * inv);
+  }
+  if (threadIdx.x == 0) rows_lse(a, bh / a.Hk, bh % a.Hk, r, mm, l);
 }
 
-// Keys per chunk and chunks: as many CTAs as fill the device four times over
-// (two are resident per SM), but at least 256 keys each, a ring's worth of
-// strips for every warp several times over.
+// Keys per chunk and chunks: as many CTAs as fill the device twice over (two
+// are resident per SM), but at least 256 keys each, a ring's worth of strips for
+// every warp several times over. 16 tokens over caches of 2048 to 8192 rows of
+// 8 heads of 128: once over 90 us, twice 77, four times 85 (more partial rows
+// to write and join); one token over 65536 rows: 54, 60 and 70 us.
 inline void rows_split(int64_t pairs, int64_t Sk, int64_t& chunk, int64_t& splits) {
-  const int64_t want = (8 * (int64_t)device_sm_count() + pairs - 1) / pairs;
+  const int64_t want = (4 * (int64_t)device_sm_count() + pairs - 1) / pairs;
   chunk = ((Sk + want - 1) / want + 63) / 64 * 64;
   if (chunk < 256) chunk = 256;
   splits = Sk > 0 ? (Sk + chunk - 1) / chunk : 1;
@@ -403,8 +412,9 @@ inline RowsPlan rows_plan(const AttnArgs& a, int rows, int D, void* ws) {
 template <typename T, int D>
 int launch_attn_join(const AttnArgs& a, const RowsPlan& pl, int rows, cudaStream_t st) {
   const int64_t n = (int64_t)a.B * a.Hk * a.Sq * a.G;
-  return launched(launch_dependent(attn_join_kernel<T, D>, (unsigned)((n + 3) / 4), 128u, 0, st, a,
-                                   pl, rows));
+  if (n > 0x7fffffff) return BLOTH_ERR_SHAPE;
+  return launched(
+      launch_dependent(attn_join_kernel<T, D>, (unsigned)n, 128u, 0, st, a, pl, rows));
 }
 
 template <typename T, int D, int MT>
