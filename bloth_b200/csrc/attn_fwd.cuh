@@ -259,10 +259,6 @@ __global__ void __launch_bounds__(352, 1)
         if (lane == 0) bar_arrive(q_there);
       }
     }
-    // Block j's row of S and what its p are taken relative to, before the
-    // exponentials of the loop below; that P of block j - 1 is written is
-    // told to the issuing warp on the way, so that the wait for its stores
-    // costs nothing.
     float x[BLK];
     Ring<2> buf;
     for (int j = f; j < e; ++j, buf.next()) {
@@ -273,12 +269,6 @@ __global__ void __launch_bounds__(352, 1)
       if (!ok) break;
       tc_fence_after();
       load64(s_buf, x);
-      if (j > f) {
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) bar_arrive(p_full + other);
-      }
       const int n0 = j * BLK;
       if (block_masked(a, s, m0 + t * N, n0)) {
         const int hi = (a.causal ? min(s.klen, row + off + 1) : s.klen) - n0;
@@ -339,12 +329,12 @@ __global__ void __launch_bounds__(352, 1)
       }
       store64<T>(s_buf, x);
       l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-    }
-    if (ok && e > f) {
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) bar_arrive(p_full + 16 * t + 8 * ((e - f - 1) & 1));
+      if (lane == 0) bar_arrive(p_full + 16 * t + 8 * buf.at);
+    }
+    if (ok && e > f) {
       ok = __all_sync(0xffffffffu, bar_wait(o_last + 8 * t, 0, waits));
       tc_fence_after();
     }
