@@ -63,15 +63,6 @@ struct FwdMaps {
   CUtensorMap q, k, v;
 };
 
-// Whether any (row, column) of rows [m0, m0 + 128) and keys [n0, n0 + 64) is
-// not seen (rows past the sequence's end do not count: they are not written).
-__device__ __forceinline__ bool block_masked(const AttnArgs& a, const AttnSeq& s, int m0, int n0) {
-  const int off = s.klen - s.qlen;
-  if (n0 + 64 > s.klen) return true;
-  if (a.causal && n0 + 63 > m0 + off) return true;
-  return a.window && n0 <= min(m0 + 127, s.qlen - 1) + off - a.window;
-}
-
 template <typename T, int D>
 __global__ void __launch_bounds__(352, 1)
     attn_fwd_kernel(const AttnArgs a, const __grid_constant__ FwdMaps maps) {
@@ -247,6 +238,13 @@ __global__ void __launch_bounds__(352, 1)
     const int f = t ? first[1] : first[0], e = t ? last[1] : last[0];
     const int off = s.klen - s.qlen;
     const float2 sc = f2s(a.scale_log2);
+    // Every row of the tile sees every key of the blocks that start at keys
+    // [clear0, clear1] (rows past the sequence's end do not count: they are not
+    // written); in the others row sees keys [lo, hi).
+    const int clear1 = min(s.klen, a.causal ? m0 + t * N + off + 1 : s.klen) - BLK;
+    const int clear0 = a.window ? min(m0 + t * N + N, s.qlen) + off - a.window : 0;
+    const int row_hi = a.causal ? min(s.klen, row + off + 1) : s.klen;
+    const int row_lo = a.window ? row + off - a.window + 1 : 0;
     float m = -INFINITY, l = 0.f;
     bool ok = true, there = false;
     if (C::Q_TMEM && nb > 0) {
@@ -270,9 +268,8 @@ __global__ void __launch_bounds__(352, 1)
       tc_fence_after();
       load64(s_buf, x);
       const int n0 = j * BLK;
-      if (block_masked(a, s, m0 + t * N, n0)) {
-        const int hi = (a.causal ? min(s.klen, row + off + 1) : s.klen) - n0;
-        const int lo = a.window ? row + off - a.window + 1 - n0 : 0;
+      if (n0 > clear1 || n0 < clear0) {
+        const int hi = row_hi - n0, lo = row_lo - n0;
 #pragma unroll
         for (int i = 0; i < BLK; ++i)
           if (i >= hi || i < lo) x[i] = -INFINITY;
