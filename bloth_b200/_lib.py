@@ -153,7 +153,12 @@ def require_cuda(*tensors: torch.Tensor) -> None:
             assert t.is_cuda, "[Bloth] CUDA GPU required"
 
 
-def ptr(t: torch.Tensor | None) -> int | None:
+def ptr(t: torch.Tensor | None):
+    return None if t is None else ctypes.c_void_p(t.data_ptr())
+
+
+def address(t: torch.Tensor | None) -> int | None:
+    """ptr() as a plain number, which the declared argument types convert."""
     return None if t is None else t.data_ptr()
 
 

@@ -1,20 +1,22 @@
 // Attention forward on the tensor cores: 16-bit tensors.
 //
 // A CTA takes 256 query rows of one head as two tiles of 128 (128 rows, one
-// tile, at head_dim 256) and streams the keys they see in blocks of 64. Warps 0-3 and 4-7 are
-// one softmax group per tile (thread = row), warps 8 and 9 issue one tile's
-// matrix products each, warp 10 the copies.
-// Per tile t and block j, in the buffer j % 2 of the tile's two:
+// tile, at head_dim 256) and streams the keys they see in blocks of 64. Warps
+// 0-3 and 4-7 are one softmax group per tile (thread = row), warps 8 and 9
+// issue one tile's matrix products each, warp 10 the copies.
+// Per tile t and block j:
 //   S = Q_t K_j^T into tensor memory (64 columns of fp32),
-//   the group reads its rows of S, masks, takes the running maximum m (base
-//   2), p = 2^(S scale log2 e - m), adds the row's p, and writes P, rounded to
-//   the tensors' type, over the first 32 columns of S,
-//   O_t += P V_j with P read from tensor memory; then S of block j + 2.
-// With two buffers S of the next block is there when a group has written P,
-// so neither the products' latency nor the hand-over between warps (200 to
-// 300 cycles each way while the tensor core reads shared memory at its full
-// rate) stops the exponentials. Blocks of 128 in one buffer, where it does:
-// @@OLD@@.
+//   the group reads its rows of S (S of block j + 1 may then follow), masks,
+//   takes the running maximum m (base 2), p = 2^(S scale log2 e - m), adds the
+//   row's p, and writes P, rounded to the tensors' type, to one of two buffers
+//   of 32 columns,
+//   O_t += P V_j with P read from tensor memory.
+// What costs here is the hand-over between warps and the issuing warps' own
+// instructions, one after the other. At 8192 full rows of 32/8 heads of 128
+// (bf16): blocks of 128 keys in one buffer, P over S, and one issuing thread
+// 1050 us; blocks of 64 in two buffers of S, P over S, and two issuing warps
+// that run converged on uniform addresses 850 us; S freed when it has been read
+// 831 us (1323 TFLOP/s, 80% of cuBLAS's burst rate of 1660).
 //
 // The running maximum moves only when a block's maximum exceeds it by more
 // than 2^8 (then the group rescales O_t in tensor memory, after its last
@@ -26,9 +28,14 @@
 // in shared memory by the groups (rows past the tensor's end are zero-filled
 // by the copy).
 //
-// Bound at head_dim 128: a block pair's products (64 rows of K against 128 of
-// Q read 6 KB of shared memory for 32 cycles of arithmetic: 384 cycles, and
-// 256 with V) and its exponentials (512 cycles, 16 a cycle and SM).
+// Bound at head_dim 128: the products. A block's for one tile take 392 cycles
+// with K (a step reads 6 KB of shared memory for 32 cycles of arithmetic) and
+// 263 with V, 1310 for both tiles; a block takes 1760. At head_dim 64 the
+// groups: 1480 cycles a block, of them 730 for the exponentials (512 alone, at
+// 16 a cycle and SM), 320 for maximum and mask, 130 for the wait for S and 130
+// to store P. A quarter of the exponentials as polynomials on the FMA units
+// made it slower (700 to 860 us at 8192 full rows), as did leaving the maximum
+// out until a block's sum shows that it is needed.
 #pragma once
 
 #include "attn_impl.cuh"
@@ -74,8 +81,9 @@ __global__ void __launch_bounds__(352, 1)
   const uint32_t q_full = base + C::BAR_OFF;
   const uint32_t k_full = q_full + 8, k_free = k_full + 8 * NST;
   const uint32_t v_full = k_free + 8 * NST, v_free = v_full + 8 * NST;
-  const uint32_t s_full = v_free + 8 * NST;  // [tile][buffer]
-  const uint32_t p_full = s_full + 8 * 4;    // [tile][buffer]
+  const uint32_t s_full = v_free + 8 * NST;  // [tile]
+  const uint32_t s_read = s_full + 8 * 2;    // [tile]: S is in registers
+  const uint32_t p_full = s_read + 8 * 2;    // [tile][buffer]
   const uint32_t o_done = p_full + 8 * 4;    // [tile]: a block's product with V has completed
   const uint32_t drained = o_done + 8 * 2;
   const uint32_t o_last = drained + 8 * 2;   // [tile]: all have
@@ -124,11 +132,10 @@ __global__ void __launch_bounds__(352, 1)
       bar_init(v_full + 8 * i, 1);
       bar_init(v_free + 8 * i, C::TILES);
     }
-    for (int i = 0; i < 4; ++i) {
-      bar_init(s_full + 8 * i, 1);
-      bar_init(p_full + 8 * i, 4);
-    }
+    for (int i = 0; i < 4; ++i) bar_init(p_full + 8 * i, 4);
     for (int t = 0; t < 2; ++t) {
+      bar_init(s_full + 8 * t, 1);
+      bar_init(s_read + 8 * t, 4);
       bar_init(o_done + 8 * t, 1);
       bar_init(drained + 8 * t, 1);
       bar_init(o_last + 8 * t, 1);
@@ -180,47 +187,48 @@ __global__ void __launch_bounds__(352, 1)
       const uint32_t s_at = tmem + C::S_COL + t * N, o_at = tmem + C::O_COL + t * D;
       const bool lead = elect();
       Ring<NST> kst, vst;
-      Ring<2> kb, vb;  // score buffers of the S and of the O to come
+      Ring<2> pb;
       bool ok = bar_wait(C::Q_TMEM ? q_there : q_full, 0, waits);
       tc_fence_after();
-      // step j: O of block j - 2, then S of block j where that one's P was;
-      // of the CTA's blocks [f, e) are this tile's
-      for (int j = 0; ok && j < nb + 2; ++j) {
-        if (j >= 2) {
-          const bool mine = j - 2 >= f && j - 2 < e;
-          ok = bar_wait(v_full + 8 * vst.at, vst.phase, waits);
-          if (ok && mine) ok = bar_wait(p_full + 16 * t + 8 * vb.at, vb.phase, waits);
+      // step j: S of block j, then O of block j - 1; of the CTA's blocks [f, e)
+      // are this tile's
+      for (int j = 0; ok && j <= nb; ++j) {
+        if (j < nb) {
+          const bool mine = j >= f && j < e;
+          ok = bar_wait(k_full + 8 * kst.at, kst.phase, waits);
+          if (ok && mine && j > f) ok = bar_wait(s_read + 8 * t, (uint32_t)(j - f - 1) & 1u, waits);
           if (!ok) break;
           tc_fence_after();
           if (lead) {
             if (mine) {
-              product_cols<T, D>(o_at, s_at + vb.at * BLK, base + C::V_OFF + vst.at * C::KB,
-                                 j - 2 > f);
-              mma_commit((j - 2 < e - 1 ? o_done : o_last) + 8 * t);
-            }
-            // (a commit completes with the products before it, if there are any)
-            mma_commit(v_free + 8 * vst.at);
-          }
-          vst.next();
-          if (mine) vb.next();
-        }
-        if (j < nb) {
-          const bool mine = j >= f && j < e;
-          ok = bar_wait(k_full + 8 * kst.at, kst.phase, waits);
-          if (!ok) break;
-          if (lead) {
-            if (mine) {
               const uint32_t kt = base + C::K_OFF + kst.at * C::KB;
               if constexpr (C::Q_TMEM)
-                product_rows_ts<T, D>(s_at + kb.at * BLK, tmem + C::Q_COL + t * (D / 2), kt);
+                product_rows_ts<T, D>(s_at, tmem + C::Q_COL + t * (D / 2), kt);
               else
-                product_rows<T, D>(s_at + kb.at * BLK, qa, kt);
-              mma_commit(s_full + 16 * t + 8 * kb.at);
+                product_rows<T, D>(s_at, qa, kt);
+              mma_commit(s_full + 8 * t);
             }
+            // (a commit completes with the products before it, if there are any)
             mma_commit(k_free + 8 * kst.at);
           }
           kst.next();
-          if (mine) kb.next();
+        }
+        if (j > 0) {
+          const bool mine = j - 1 >= f && j - 1 < e;
+          ok = bar_wait(v_full + 8 * vst.at, vst.phase, waits);
+          if (ok && mine) ok = bar_wait(p_full + 16 * t + 8 * pb.at, pb.phase, waits);
+          if (!ok) break;
+          tc_fence_after();
+          if (lead) {
+            if (mine) {
+              product_cols<T, D>(o_at, s_at + BLK + pb.at * 32, base + C::V_OFF + vst.at * C::KB,
+                                 j - 1 > f);
+              mma_commit((j - 1 < e - 1 ? o_done : o_last) + 8 * t);
+            }
+            mma_commit(v_free + 8 * vst.at);
+          }
+          vst.next();
+          if (mine) pb.next();
         }
       }
       if (!ok && lead) {  // given up: not before the products in flight have completed
@@ -258,15 +266,16 @@ __global__ void __launch_bounds__(352, 1)
       }
     }
     float x[BLK];
-    Ring<2> buf;
-    for (int j = f; j < e; ++j, buf.next()) {
-      const uint32_t s_buf = tmem + lanes + C::S_COL + t * N + buf.at * BLK;
-      const uint32_t other = 16 * t + 8 * (buf.at ^ 1u);
-      if (!there) there = ok && bar_wait(s_full + 16 * t + 8 * buf.at, buf.phase, waits);
+    const uint32_t s_at = tmem + lanes + C::S_COL + t * N;
+    for (int j = f; j < e; ++j) {
+      if (!there) there = ok && bar_wait(s_full + 8 * t, (uint32_t)(j - f) & 1u, waits);
       ok = __all_sync(0xffffffffu, there);
       if (!ok) break;
       tc_fence_after();
-      load64(s_buf, x);
+      load64(s_at, x);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) bar_arrive(s_read + 8 * t);
       const int n0 = j * BLK;
       if (n0 > clear1 || n0 < clear0) {
         const int hi = row_hi - n0, lo = row_lo - n0;
@@ -313,7 +322,7 @@ __global__ void __launch_bounds__(352, 1)
       }
       // whether the next block's S is there: asked before the exponentials, so
       // that the answer (200 cycles) comes during them
-      there = j + 1 < e && bar_test(s_full + other, buf.phase ^ buf.at);
+      there = j + 1 < e && bar_test(s_full + 8 * t, (uint32_t)(j + 1 - f) & 1u);
       // a row that has seen nothing (m = -inf) is masked everywhere: 2^(-inf - 0) = 0
       const float2 from = f2s(m == -INFINITY ? 0.f : -m);
       float2 sum[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
@@ -324,12 +333,12 @@ __global__ void __launch_bounds__(352, 1)
         x[i + 1] = ex2(y.y);
         sum[(i / 2) & 1] = f2_add(sum[(i / 2) & 1], f2(x[i], x[i + 1]));
       }
-      store64<T>(s_buf, x);
+      store64<T>(s_at + BLK + ((j - f) & 1) * 32, x);
       l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) bar_arrive(p_full + 16 * t + 8 * buf.at);
+      if (lane == 0) bar_arrive(p_full + 16 * t + 8 * ((j - f) & 1));
     }
     if (ok && e > f) {
       ok = __all_sync(0xffffffffu, bar_wait(o_last + 8 * t, 0, waits));

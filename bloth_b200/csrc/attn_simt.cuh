@@ -9,10 +9,12 @@
 // the sequence's end are zero in shared memory, whatever memory holds there.
 //
 // OWN is 64 where that gives a CTA for every SM, else 32: half the threads and
-// half the work of a CTA (@@OWN@@).
+// half the work of a CTA (100 rows of 4 heads of 64: dK and dV 35 us with
+// 64, 17 with 32).
 // dK and dV are written by one CTA per key tile and key head, or, where those
 // are fewer than two for an SM, by one per query head into fp32 partial sums
-// that simt_sum_kernel adds over the group in order (@@SPLIT@@).
+// that simt_sum_kernel adds over the group in order (2048 rows of 16/4 heads of 128: 2139 us
+// without, 1035 us with).
 //
 // Bound: fp32 FMA issue; a 4 x 4 block does 64 FMA for 8 shared-memory reads of
 // 16 bytes, which leaves about half of the FMA rate.

@@ -105,11 +105,11 @@ def attention_forward(q4, k4, v4, q_seq, k_seq, packed, scale, causal, window, w
     code = _lib.dtype_code(q4.dtype)
     ws, n = _workspace("bloth_attention_fwd_workspace_bytes", q4.device, B, Sq, Sk, Hq, Hk, D,
                        packed, code)
-    rc = _lib.call("bloth_attention_fwd", q4, _lib.ptr(q4), _head_strides(q4), _lib.ptr(k4),
-                   _head_strides(k4), _lib.ptr(v4), _head_strides(v4), _lib.ptr(out),
-                   _head_strides(out), _lib.ptr(rest), _lib.ptr(lse), _lib.ptr(q_seq),
-                   _lib.ptr(k_seq), _seq_dtype(q_seq, k_seq), packed, B, Sq, Sk, Hq, Hk, D, scale,
-                   int(causal), window, code, _lib.ptr(ws), n, _lib.stream_of(q4))
+    rc = _lib.call("bloth_attention_fwd", q4, _lib.address(q4), _head_strides(q4), _lib.address(k4),
+                   _head_strides(k4), _lib.address(v4), _head_strides(v4), _lib.address(out),
+                   _head_strides(out), _lib.address(rest), _lib.address(lse), _lib.address(q_seq),
+                   _lib.address(k_seq), _seq_dtype(q_seq, k_seq), packed, B, Sq, Sk, Hq, Hk, D, scale,
+                   int(causal), window, code, _lib.address(ws), n, _lib.stream_of(q4))
     _lib.check(rc, "attention forward")
     return out, lse, rest
 
@@ -124,13 +124,13 @@ def attention_backward(do4, q4, k4, v4, out, rest, lse, q_seq, k_seq, packed, sc
     code = _lib.dtype_code(q4.dtype)
     ws, n = _workspace("bloth_attention_bwd_workspace_bytes", q4.device, B, Sq, Sk, Hq, Hk, D,
                        packed, code)
-    rc = _lib.call("bloth_attention_bwd", q4, _lib.ptr(do4), _head_strides(do4), _lib.ptr(q4),
-                   _head_strides(q4), _lib.ptr(k4), _head_strides(k4), _lib.ptr(v4),
-                   _head_strides(v4), _lib.ptr(out), _head_strides(out), _lib.ptr(rest),
-                   _lib.ptr(lse), _lib.ptr(dq), _head_strides(dq), _lib.ptr(dk), _head_strides(dk),
-                   _lib.ptr(dv), _head_strides(dv), _lib.ptr(q_seq), _lib.ptr(k_seq),
+    rc = _lib.call("bloth_attention_bwd", q4, _lib.address(do4), _head_strides(do4), _lib.address(q4),
+                   _head_strides(q4), _lib.address(k4), _head_strides(k4), _lib.address(v4),
+                   _head_strides(v4), _lib.address(out), _head_strides(out), _lib.address(rest),
+                   _lib.address(lse), _lib.address(dq), _head_strides(dq), _lib.address(dk), _head_strides(dk),
+                   _lib.address(dv), _head_strides(dv), _lib.address(q_seq), _lib.address(k_seq),
                    _seq_dtype(q_seq, k_seq), packed, B, Sq, Sk, Hq, Hk, D, scale, int(causal),
-                   window, code, _lib.ptr(ws), n, _lib.stream_of(q4))
+                   window, code, _lib.address(ws), n, _lib.stream_of(q4))
     _lib.check(rc, "attention backward")
     return dq, dk, dv
 
