@@ -1,4 +1,5 @@
-"""bloth_b200 - B200 (sm_100a) kernels for Bloth's fused RMSNorm + RoPE path.
+"""bloth_b200 - B200 (sm_100a) kernels for Bloth's fused RMSNorm + RoPE path and
+the attention that follows it.
 
 Drop-in for the reference's names on this path (bloth/bloth/__init__.py:18-42
 and kernels/__init__.py:7-8):
@@ -11,10 +12,14 @@ plus fused_qk_norm_rope / BlothQKNormRoPE (q and k per-head norm + RoPE in one
 launch, cos/sin from positions in-register or from HF tables), apply_rope_qk /
 apply_rotary_pos_emb (RoPE of q and k in one launch), the (1 + w) weighting of
 Gemma-family norms (weight_offset), fused_add_rms_norm (residual add + RMSNorm
-in one pass), and patch_model(..., patch_attention=True, patch_residual=True),
-which routes HF Qwen3 / Llama / Mistral / Qwen2 layers through them. The compute runs in hand-written
-CUDA behind the C ABI of include/bloth_b200.h; importing this package does not
-touch the GPU, and every op raises if the library or a CUDA device is missing.
+in one pass), fused_qk_norm_mrope / apply_mrope_qk / mrope_axes (the same q and
+k kernels with positions of several axes), fused_attention (softmax attention,
+forward and backward, for whole, padded and packed sequences and for new tokens
+over a cache), and patch_model(..., patch_attention=True, patch_residual=True,
+fuse_attention=True), which routes HF Qwen3 / Llama / Mistral / Qwen2 layers
+through them. The compute runs in hand-written CUDA behind the C ABI of
+include/bloth_b200.h; importing this package does not touch the GPU, and every
+op raises if the library or a CUDA device is missing.
 """
 from __future__ import annotations
 

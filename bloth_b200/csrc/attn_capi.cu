@@ -93,11 +93,11 @@ size_t bloth_attention_fwd_workspace_bytes(int64_t B, int64_t Sq, int64_t Sk, in
 
 int bloth_attention_fwd(const void* q, const int64_t* q_strides, const void* k,
                         const int64_t* k_strides, const void* v, const int64_t* v_strides,
-                        void* out, const int64_t* out_strides, void* out_rest, float* lse, const void* q_seq,
-                        const void* k_seq, int seq_dtype, int64_t packed, int64_t B, int64_t Sq,
-                        int64_t Sk, int64_t Hq, int64_t Hk, int64_t D, float scale, int causal,
-                        int64_t window, int dtype, void* workspace, size_t workspace_bytes,
-                        void* stream) {
+                        void* out, const int64_t* out_strides, void* out_rest, float* lse,
+                        const void* q_seq, const void* k_seq, int seq_dtype, int64_t packed,
+                        int64_t B, int64_t Sq, int64_t Sk, int64_t Hq, int64_t Hk, int64_t D,
+                        float scale, int causal, int64_t window, int dtype, void* workspace,
+                        size_t workspace_bytes, void* stream) {
   int rc = check_sizes(B, Sq, Sk, Hq, Hk, D, packed, dtype);
   if (rc) return rc;
   AttnArgs a;
@@ -141,11 +141,11 @@ size_t bloth_attention_bwd_workspace_bytes(int64_t B, int64_t Sq, int64_t Sk, in
 int bloth_attention_bwd(const void* dout, const int64_t* dout_strides, const void* q,
                         const int64_t* q_strides, const void* k, const int64_t* k_strides,
                         const void* v, const int64_t* v_strides, const void* out,
-                        const int64_t* out_strides, const void* out_rest, const float* lse, void* dq,
-                        const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
-                        const int64_t* dv_strides, const void* q_seq, const void* k_seq,
-                        int seq_dtype, int64_t packed, int64_t B, int64_t Sq, int64_t Sk,
-                        int64_t Hq, int64_t Hk, int64_t D, float scale, int causal,
+                        const int64_t* out_strides, const void* out_rest, const float* lse,
+                        void* dq, const int64_t* dq_strides, void* dk, const int64_t* dk_strides,
+                        void* dv, const int64_t* dv_strides, const void* q_seq,
+                        const void* k_seq, int seq_dtype, int64_t packed, int64_t B, int64_t Sq,
+                        int64_t Sk, int64_t Hq, int64_t Hk, int64_t D, float scale, int causal,
                         int64_t window, int dtype, void* workspace, size_t workspace_bytes,
                         void* stream) {
   int rc = check_sizes(B, Sq, Sk, Hq, Hk, D, packed, dtype);

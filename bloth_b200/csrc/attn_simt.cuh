@@ -279,7 +279,8 @@ __global__ void __launch_bounds__(4 * kSimtRows)
     for (int c = 0; c < D / 16; c += 2) {
       const int col = 64 * (c / 4) + 4 * tx + c % 4;
       if (pl.splits == 1) rows_out<T>(a, b, h, r, col, acc[i][c] * inv, acc[i][c + 1] * inv);
-      else *reinterpret_cast<float2*>(pl.sums + (part + r) * D + col) = f2(acc[i][c], acc[i][c + 1]);
+      else
+        *reinterpret_cast<float2*>(pl.sums + (part + r) * D + col) = f2(acc[i][c], acc[i][c + 1]);
     }
     if (tx == 0) {
       if (pl.splits == 1) {

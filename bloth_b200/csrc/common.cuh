@@ -2,9 +2,10 @@
 // 16-byte packed global loads and stores, warp and row-group reductions, and
 // the host-side launch bookkeeping (SM count and occupancy caches).
 //
-// Every kernel in this library is HBM-bound: each element is read once from
-// global memory as part of a 16-byte vector, converted to fp32, reduced with
-// warp shuffles, and written once. Tensor cores are not used.
+// The normalising and rotating kernels are HBM-bound: each element is read once
+// from global memory as part of a 16-byte vector, converted to fp32, reduced
+// with warp shuffles, and written once. Only the attention kernels (attn_*)
+// have products, and use the tensor cores.
 #pragma once
 
 #include <cuda_runtime.h>

@@ -14,6 +14,7 @@ import math
 import torch
 
 from .. import _lib
+from .._lib import address
 from .fused_norm_qkv_rope import _head_strides, _heads
 from .rope import _out_like
 
@@ -105,11 +106,11 @@ def attention_forward(q4, k4, v4, q_seq, k_seq, packed, scale, causal, window, w
     code = _lib.dtype_code(q4.dtype)
     ws, n = _workspace("bloth_attention_fwd_workspace_bytes", q4.device, B, Sq, Sk, Hq, Hk, D,
                        packed, code)
-    rc = _lib.call("bloth_attention_fwd", q4, _lib.address(q4), _head_strides(q4), _lib.address(k4),
-                   _head_strides(k4), _lib.address(v4), _head_strides(v4), _lib.address(out),
-                   _head_strides(out), _lib.address(rest), _lib.address(lse), _lib.address(q_seq),
-                   _lib.address(k_seq), _seq_dtype(q_seq, k_seq), packed, B, Sq, Sk, Hq, Hk, D, scale,
-                   int(causal), window, code, _lib.address(ws), n, _lib.stream_of(q4))
+    rc = _lib.call("bloth_attention_fwd", q4, address(q4), _head_strides(q4), address(k4),
+                   _head_strides(k4), address(v4), _head_strides(v4), address(out),
+                   _head_strides(out), address(rest), address(lse), address(q_seq),
+                   address(k_seq), _seq_dtype(q_seq, k_seq), packed, B, Sq, Sk, Hq, Hk, D, scale,
+                   int(causal), window, code, address(ws), n, _lib.stream_of(q4))
     _lib.check(rc, "attention forward")
     return out, lse, rest
 
@@ -124,13 +125,13 @@ def attention_backward(do4, q4, k4, v4, out, rest, lse, q_seq, k_seq, packed, sc
     code = _lib.dtype_code(q4.dtype)
     ws, n = _workspace("bloth_attention_bwd_workspace_bytes", q4.device, B, Sq, Sk, Hq, Hk, D,
                        packed, code)
-    rc = _lib.call("bloth_attention_bwd", q4, _lib.address(do4), _head_strides(do4), _lib.address(q4),
-                   _head_strides(q4), _lib.address(k4), _head_strides(k4), _lib.address(v4),
-                   _head_strides(v4), _lib.address(out), _head_strides(out), _lib.address(rest),
-                   _lib.address(lse), _lib.address(dq), _head_strides(dq), _lib.address(dk), _head_strides(dk),
-                   _lib.address(dv), _head_strides(dv), _lib.address(q_seq), _lib.address(k_seq),
+    rc = _lib.call("bloth_attention_bwd", q4, address(do4), _head_strides(do4), address(q4),
+                   _head_strides(q4), address(k4), _head_strides(k4), address(v4),
+                   _head_strides(v4), address(out), _head_strides(out), address(rest),
+                   address(lse), address(dq), _head_strides(dq), address(dk), _head_strides(dk),
+                   address(dv), _head_strides(dv), address(q_seq), address(k_seq),
                    _seq_dtype(q_seq, k_seq), packed, B, Sq, Sk, Hq, Hk, D, scale, int(causal),
-                   window, code, _lib.address(ws), n, _lib.stream_of(q4))
+                   window, code, address(ws), n, _lib.stream_of(q4))
     _lib.check(rc, "attention backward")
     return dq, dk, dv
 

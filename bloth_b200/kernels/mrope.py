@@ -15,6 +15,7 @@ from functools import lru_cache
 import torch
 
 from .. import _lib
+from .._lib import address
 from .fused_norm_qkv_rope import _head_strides, _heads
 from .rope import _out_like
 
@@ -42,7 +43,7 @@ def _mrope_axes(sections: tuple, interleaved: bool) -> tuple:
 def mrope_axes(sections, interleaved: bool = False) -> tuple:
     """The axis of each of the D/2 frequencies, from the number of frequencies
     per axis (HF's ``mrope_section``; their sum is D/2). By default the axes
-    follow one another (Qwen2-VL). ``interleaved`` (Qwen3-VL): the axes take
+    follow one another. ``interleaved`` (HF's ``mrope_interleaved``): the axes take
     turns, frequency i going to axis i mod n while that axis has some left,
     and to the first axis otherwise."""
     return _mrope_axes(tuple(int(n) for n in sections), bool(interleaved))
@@ -118,10 +119,10 @@ def _norm_mrope_call(q, k, wq, wk, position_ids, inv_freq, axes, eps, weight_off
     rq = q4.new_empty((B, S, Hq), dtype=torch.float32)
     rk = None if k4 is None else q4.new_empty((B, S, Hk), dtype=torch.float32)
     rc = _lib.call(
-        "bloth_qk_norm_mrope_fwd", q4, _lib.address(q4), _head_strides(q4), _lib.address(k4),
-        _head_strides(k4), _lib.address(wq), _lib.address(wk), weight_offset, _lib.address(qo),
-        _head_strides(qo), _lib.address(ko), _head_strides(ko), _lib.address(rq), _lib.address(rk),
-        _lib.address(pos), pos_st, _lib.dtype_code(pos.dtype), pos.shape[0], ax, _lib.address(inv_freq),
+        "bloth_qk_norm_mrope_fwd", q4, address(q4), _head_strides(q4), address(k4),
+        _head_strides(k4), address(wq), address(wk), weight_offset, address(qo),
+        _head_strides(qo), address(ko), _head_strides(ko), address(rq), address(rk),
+        address(pos), pos_st, _lib.dtype_code(pos.dtype), pos.shape[0], ax, address(inv_freq),
         rope_scale, B, S, Hq, Hk, D, eps, _lib.dtype_code(q4.dtype), _lib.dtype_code(wq.dtype),
         _lib.stream_of(q4))
     _lib.check(rc, "qk norm+mrope forward")
@@ -157,13 +158,13 @@ class _QKNormMRoPEFunction(torch.autograd.Function):
                                  code)
         ws = torch.empty(max(n, 1), dtype=torch.uint8, device=q4.device)
         rc = _lib.call(
-            "bloth_qk_norm_mrope_bwd", q4, _lib.address(gq), _head_strides(gq), _lib.address(gk),
-            _head_strides(gk), _lib.address(q4), _head_strides(q4), _lib.address(k4), _head_strides(k4),
-            _lib.address(wq), _lib.address(wk), weight_offset, _lib.address(rq), _lib.address(rk), _lib.address(dq),
-            _head_strides(dq), _lib.address(dk), _head_strides(dk), _lib.address(dwq), _lib.address(dwk),
-            _lib.address(pos), pos_st, _lib.dtype_code(pos.dtype), pos.shape[0], ax,
-            _lib.address(inv_freq), rope_scale, B, S, Hq, Hk, D, code, _lib.dtype_code(wq.dtype),
-            _lib.address(ws), n, _lib.stream_of(q4))
+            "bloth_qk_norm_mrope_bwd", q4, address(gq), _head_strides(gq), address(gk),
+            _head_strides(gk), address(q4), _head_strides(q4), address(k4), _head_strides(k4),
+            address(wq), address(wk), weight_offset, address(rq), address(rk), address(dq),
+            _head_strides(dq), address(dk), _head_strides(dk), address(dwq), address(dwk),
+            address(pos), pos_st, _lib.dtype_code(pos.dtype), pos.shape[0], ax,
+            address(inv_freq), rope_scale, B, S, Hq, Hk, D, code, _lib.dtype_code(wq.dtype),
+            address(ws), n, _lib.stream_of(q4))
         _lib.check(rc, "qk norm+mrope backward")
         if flat:
             dq, dk = dq[0], None if dk is None else dk[0]
@@ -172,10 +173,10 @@ class _QKNormMRoPEFunction(torch.autograd.Function):
 
 def _mrope_launch(q4, qo, k4, ko, pos, pos_st, ax, inv_freq, scale, transpose):
     B, S, Hq, D = q4.shape
-    rc = _lib.call("bloth_mrope", q4, _lib.address(q4), _head_strides(q4), _lib.address(qo),
-                   _head_strides(qo), _lib.address(k4), _head_strides(k4), _lib.address(ko),
-                   _head_strides(ko), _lib.address(pos), pos_st, _lib.dtype_code(pos.dtype),
-                   pos.shape[0], ax, _lib.address(inv_freq), scale, B, S, Hq,
+    rc = _lib.call("bloth_mrope", q4, address(q4), _head_strides(q4), address(qo),
+                   _head_strides(qo), address(k4), _head_strides(k4), address(ko),
+                   _head_strides(ko), address(pos), pos_st, _lib.dtype_code(pos.dtype),
+                   pos.shape[0], ax, address(inv_freq), scale, B, S, Hq,
                    0 if k4 is None else k4.shape[2], D, int(transpose),
                    _lib.dtype_code(q4.dtype), _lib.stream_of(q4))
     _lib.check(rc, "mrope")
