@@ -16,7 +16,8 @@
 // P^T, dS^T and dS are rounded to the tensors' type and stay in tensor memory,
 // where S^T and dP lay, as the products' first operand; the streamed tiles are
 // read by the products both by rows and by columns, so nothing is transposed
-// or stored again. Blocks alternate between two buffers of S and of dP in
+// or stored again. (Rows that see few keys, kFineKeys: as two terms, in the two
+// halves of where S^T and dP lay.) Blocks alternate between two buffers of S and of dP in
 // tensor memory and two groups of four warps (thread = row of the kept tile,
 // 64 columns): a group has two blocks' time for its own, so neither the
 // hand-over between warps nor its own latencies stop the tensor core. Warps 8
@@ -38,6 +39,8 @@
 // 128 queries in single buffers 1826. Sixteen softmax warps in place of eight
 // were no faster.
 #pragma once
+
+#include <climits>
 
 #include "attn_impl.cuh"
 #include "tc.cuh"
@@ -157,7 +160,7 @@ __device__ __forceinline__ void store_row(uint32_t at, int cols, float f, T* dst
 }
 
 // ------------------------------------------------------------------ dK, dV
-template <typename T, int D, int SUMS>
+template <typename T, int D, int SUMS, bool FINE>
 __global__ void __launch_bounds__(352, 1)
     attn_dkv_kernel(const AttnArgs a, const __grid_constant__ BwdMaps maps) {
   using C = BwdCfg<D, SUMS>;
@@ -247,8 +250,10 @@ __global__ void __launch_bounds__(352, 1)
           if (!ok) break;
           tc_fence_after();
           if (DV && lead) {
-            product_cols<T, D>(tmem + DV_COL, tmem + C::S_COL + pbuf.at * BLK,
-                               base + C::B_OFF + ost.at * C::STRB, j > 2);
+            const uint32_t p = tmem + C::S_COL + pbuf.at * BLK;
+            const uint32_t ot = base + C::B_OFF + ost.at * C::STRB;
+            product_cols<T, D>(tmem + DV_COL, p, ot, j > 2);
+            if (FINE) product_cols<T, D>(tmem + DV_COL, p + 32, ot, true);
             mma_commit(bar.b_free + 8 * ost.at);
             // Q and the statistics went into P^T, which this product has read
             if (!DK) mma_commit(bar.a_free + 8 * qold.at);
@@ -295,8 +300,10 @@ __global__ void __launch_bounds__(352, 1)
           if (!ok) break;
           tc_fence_after();
           if (lead) {
-            product_cols<T, D>(tmem + DK_COL, tmem + C::DP_COL + dbuf.at * BLK,
-                               base + C::A_OFF + qst.at * C::STRB, j > 2);
+            const uint32_t ds = tmem + C::DP_COL + dbuf.at * BLK;
+            const uint32_t qt = base + C::A_OFF + qst.at * C::STRB;
+            product_cols<T, D>(tmem + DK_COL, ds, qt, j > 2);
+            if (FINE) product_cols<T, D>(tmem + DK_COL, ds + 32, qt, true);
             mma_commit(bar.a_free + 8 * qst.at);
           }
           qst.next();
@@ -375,9 +382,11 @@ __global__ void __launch_bounds__(352, 1)
       // the block's columns that see this thread's key: [from, to)
       const int from = a.causal ? key - off - m0 : 0;
       const int to = min(s.qlen, a.window ? key - off + a.window : s.qlen) - m0;
-      const bool masked = m0 + BLK > s.qlen || (a.causal && n0 + N - 1 - off > m0) ||
+      const bool masked = m0 + BLK > s.qlen || s.klen == 1 || (a.causal && n0 + N - 1 - off > m0) ||
                           (a.window && n0 - off + a.window < m0 + BLK);
       const bool tail = m0 + BLK > s.qlen && s.q0 + s.qlen < a.Sq;
+      // the query that sees one key only; INT_MAX: all do, -1: none of the block
+      const int alone = s.klen == 1 || a.window == 1 ? INT_MAX : a.causal ? -off - m0 : -1;
       if (masked) {
 #pragma unroll
         for (int i = 0; i < BLK; ++i)
@@ -388,7 +397,10 @@ __global__ void __launch_bounds__(352, 1)
           zero_rows<D>(smem + C::B_OFF + ost.at * C::STRB, s.qlen - m0);
         }
       }
-      if (DV) store64<T>(s_at, x);
+      if (DV) {
+        store64<T>(s_at, x);
+        if (FINE) store64_rest<T>(s_at + 32, x);
+      }
       const bool there = !DK || bar_test(bar.dp_full + 8 * group, ph);
       tmem_wait_st();
       tc_fence_before();
@@ -414,10 +426,11 @@ __global__ void __launch_bounds__(352, 1)
         if (masked) {
 #pragma unroll
           for (int i = 0; i < BLK; ++i)
-            if (i < from || i >= to) y[i] = 0.f;
+            if (i < from || i >= to || i == alone || alone == INT_MAX) y[i] = 0.f;
           if (tail) zero_rows<D>(smem + C::A_OFF + st.at * C::STRB, s.qlen - m0);
         }
         store64<T>(dp_at, y);
+        if (FINE) store64_rest<T>(dp_at + 32, y);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -454,7 +467,7 @@ __global__ void __launch_bounds__(352, 1)
 }
 
 // ---------------------------------------------------------------------- dQ
-template <typename T, int D>
+template <typename T, int D, bool FINE>
 __global__ void __launch_bounds__(352, 1)
     attn_dq_kernel(const AttnArgs a, const __grid_constant__ BwdMaps maps) {
   using C = BwdCfg<D, kSumDQ>;
@@ -563,8 +576,10 @@ __global__ void __launch_bounds__(352, 1)
           if (!ok) break;
           tc_fence_after();
           if (lead) {
-            product_cols<T, D>(tmem + C::ACC_COL, tmem + C::DP_COL + dbuf.at * BLK,
-                               base + C::A_OFF + kst.at * C::STRB, j > 2);
+            const uint32_t ds = tmem + C::DP_COL + dbuf.at * BLK;
+            const uint32_t kt = base + C::A_OFF + kst.at * C::STRB;
+            product_cols<T, D>(tmem + C::ACC_COL, ds, kt, j > 2);
+            if (FINE) product_cols<T, D>(tmem + C::ACC_COL, ds + 32, kt, true);
             mma_commit(bar.a_free + 8 * kst.at);
           }
           kst.next();
@@ -641,7 +656,8 @@ __global__ void __launch_bounds__(352, 1)
       if (n0 + BLK > s.klen || (a.causal && n0 + BLK - 1 > m0 + off) ||
           (a.window && n0 <= m0 + N - 1 + off - a.window)) {
         const int to = (a.causal ? min(s.klen, row + off + 1) : s.klen) - n0;
-        const int from = a.window ? row + off - a.window + 1 - n0 : 0;
+        int from = a.window ? row + off - a.window + 1 - n0 : 0;
+        if (sees_one(a, s, row)) from = BLK;
 #pragma unroll
         for (int i = 0; i < BLK; ++i)
           if (i < from || i >= to) y[i] = 0.f;
@@ -650,6 +666,7 @@ __global__ void __launch_bounds__(352, 1)
           zero_rows<D>(smem + C::A_OFF + (it % NA) * C::STRB, s.klen - n0);
       }
       store64<T>(dp_at, y);
+      if (FINE) store64_rest<T>(dp_at + 32, y);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -673,7 +690,7 @@ __global__ void __launch_bounds__(352, 1)
   if (warp == 8) tmem_free(tmem, C::COLS);
 }
 
-template <typename T, int D>
+template <typename T, int D, bool FINE>
 int launch_attn_bwd(const AttnArgs& a0, cudaStream_t st) {
   AttnArgs a = a0;
   a.fault = fault_word();
@@ -703,7 +720,7 @@ int launch_attn_bwd(const AttnArgs& a0, cudaStream_t st) {
   auto keys = [&](auto sums) {
     constexpr int S = decltype(sums)::value;
     using C = BwdCfg<D, S>;
-    return run(attn_dkv_kernel<T, D, S>, C::SMEM, C::THREADS,
+    return run(attn_dkv_kernel<T, D, S, FINE>, C::SMEM, C::THREADS,
                attn_tiles(a.Sk, a.packed, C::TILE) * a.Hk * a.B);
   };
   if (a.dk.p != nullptr) {
@@ -716,7 +733,7 @@ int launch_attn_bwd(const AttnArgs& a0, cudaStream_t st) {
   }
   if (rc == BLOTH_OK && a.dq.p != nullptr) {
     using C = BwdCfg<D, kSumDQ>;
-    rc = run(attn_dq_kernel<T, D>, C::SMEM, C::THREADS,
+    rc = run(attn_dq_kernel<T, D, FINE>, C::SMEM, C::THREADS,
              attn_tiles(a.Sq, a.packed, C::TILE) * a.Hq * a.B);
   }
   return rc;

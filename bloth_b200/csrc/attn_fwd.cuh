@@ -23,6 +23,9 @@
 // product). Until then p is at most 2^8, which costs no precision: p is
 // rounded relative to its own size, and sums are fp32.
 //
+// Rows that see few keys (kFineKeys) have P as two terms, which take both
+// buffers: P of a block then waits for the product of the block before.
+//
 // Keys past the sequence's end are masked in S; their rows of V, which a
 // probability of 0 would turn into NaN if they hold an infinity, are zeroed
 // in shared memory by the groups (rows past the tensor's end are zero-filled
@@ -70,7 +73,7 @@ struct FwdMaps {
   CUtensorMap q, k, v;
 };
 
-template <typename T, int D>
+template <typename T, int D, bool FINE>
 __global__ void __launch_bounds__(352, 1)
     attn_fwd_kernel(const AttnArgs a, const __grid_constant__ FwdMaps maps) {
   using C = FwdCfg<D>;
@@ -221,8 +224,9 @@ __global__ void __launch_bounds__(352, 1)
           tc_fence_after();
           if (lead) {
             if (mine) {
-              product_cols<T, D>(o_at, s_at + BLK + pb.at * 32, base + C::V_OFF + vst.at * C::KB,
-                                 j - 1 > f);
+              const uint32_t vt = base + C::V_OFF + vst.at * C::KB;
+              product_cols<T, D>(o_at, s_at + BLK + (FINE ? 0 : pb.at * 32), vt, j - 1 > f);
+              if (FINE) product_cols<T, D>(o_at, s_at + BLK + 32, vt, true);
               mma_commit((j - 1 < e - 1 ? o_done : o_last) + 8 * t);
             }
             mma_commit(v_free + 8 * vst.at);
@@ -333,7 +337,17 @@ __global__ void __launch_bounds__(352, 1)
         x[i + 1] = ex2(y.y);
         sum[(i / 2) & 1] = f2_add(sum[(i / 2) & 1], f2(x[i], x[i + 1]));
       }
-      store64<T>(s_at + BLK + ((j - f) & 1) * 32, x);
+      if constexpr (FINE) {
+        if (j > f) {
+          ok = __all_sync(0xffffffffu, bar_wait(o_done + 8 * t, (uint32_t)(j - f - 1) & 1u, waits));
+          if (!ok) break;
+          tc_fence_after();
+        }
+        store64<T>(s_at + BLK, x);
+        store64_rest<T>(s_at + BLK + 32, x);
+      } else {
+        store64<T>(s_at + BLK + ((j - f) & 1) * 32, x);
+      }
       l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       tmem_wait_st();
       tc_fence_before();
@@ -385,7 +399,7 @@ __global__ void __launch_bounds__(352, 1)
   if (warp == 8) tmem_free(tmem, C::COLS);
 }
 
-template <typename T, int D>
+template <typename T, int D, bool FINE>
 int launch_attn_fwd(const AttnArgs& a0, cudaStream_t st) {
   using C = FwdCfg<D>;
   AttnArgs a = a0;
@@ -401,7 +415,7 @@ int launch_attn_fwd(const AttnArgs& a0, cudaStream_t st) {
   if (rc == BLOTH_OK)
     rc = head_map(&m.v, a.v.p, a.v.sb, a.v.ss, a.v.sh, a.B, Sk, a.Hk, D, 64, dt);
   if (rc != BLOTH_OK) return rc;
-  auto kern = attn_fwd_kernel<T, D>;
+  auto kern = attn_fwd_kernel<T, D, FINE>;
   if ((rc = prepare_smem((const void*)kern, C::SMEM)) != BLOTH_OK) return rc;
   const int64_t grid = attn_tiles(a.Sq, a.packed, C::TILES * C::TILE) * a.Hq * a.B;
   if (grid > 0x7fffffff) return BLOTH_ERR_SHAPE;

@@ -15,29 +15,14 @@
 // A row that sees no key has o = 0, lse = -inf and no gradient. Query heads
 // h of a group of G = Hq / Hk share key head h / G, whose gradients sum over
 // the group inside one CTA, in a fixed order: no atomics anywhere.
+// A row that sees one key has p = 1 and dp = delta whatever they are: its ds is
+// set to the 0 it is (the difference of the two sums would be their noise).
 #pragma once
 
 #include "common.cuh"
 #include "heads_impl.cuh"
 
 namespace bloth {
-
-// Two floats y rounded to T, and what that took off them rounded to T.
-template <typename T>
-__device__ __forceinline__ void split2(float y0, float y1, uint32_t& hi, uint32_t& lo) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(y0, y1);
-    const __nv_bfloat162 r =
-        __floats2bfloat162_rn(y0 - __bfloat162float(h.x), y1 - __bfloat162float(h.y));
-    memcpy(&hi, &h, 4);
-    memcpy(&lo, &r, 4);
-  } else {
-    const __half2 h = __floats2half2_rn(y0, y1);
-    const __half2 r = __floats2half2_rn(y0 - __half2float(h.x), y1 - __half2float(h.y));
-    memcpy(&hi, &h, 4);
-    memcpy(&lo, &r, 4);
-  }
-}
 
 struct AttnArgs {
   HT q, k, v, o, dout, dq, dk, dv;
@@ -54,8 +39,18 @@ struct AttnArgs {
   float scale, scale_log2;
   int causal;
   int window;         // 0: none
+  int fine;           // P and dS at twice the tensors' precision (16-bit tensors)
   unsigned int* fault;
 };
+
+// Rows that see at most this many keys have P and dS as two terms of 16 bits:
+// where few terms are summed, a gradient of two nearly equal ones lost up to
+// six times what rounding the result takes (bf16, two keys); with two terms no
+// more than that rounding. It costs a product for each of P and dS: 4 x 8192
+// rows of 32/8 heads of 128, forward and backward, 1720 us with a window of 128,
+// 1575 us with one of 129; 64 x 128 rows, 435 us, and 536 us for 64 x 129.
+// Sequences packed into more rows count as longer.
+constexpr int kFineKeys = 128;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -167,6 +162,13 @@ __device__ __forceinline__ AttnSeq find_seq(const AttnArgs& a, int b, int t, int
 __device__ __forceinline__ bool see_keys(const AttnArgs& a, const AttnSeq& s, int i, int j) {
   const int at = i + s.klen - s.qlen;
   return i < s.qlen && j < s.klen && (!a.causal || j <= at) && (!a.window || j > at - a.window);
+}
+
+// Whether query i, which sees a key, sees no other.
+__device__ __forceinline__ bool sees_one(const AttnArgs& a, const AttnSeq& s, int i) {
+  const int at = i + s.klen - s.qlen;
+  const int hi = a.causal ? min(s.klen, at + 1) : s.klen;
+  return hi - (a.window ? max(0, at - a.window + 1) : 0) == 1;
 }
 
 // Keys [lo, hi) seen by any of the query rows [m0, m1) (m1 <= qlen).

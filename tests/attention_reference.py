@@ -15,6 +15,9 @@ number of the type's subnormal range (2^-25 for fp16, else 0):
 * dq, dk: scale times the sum of the errors of ds against |k| or |q|, plus
   (n + 2) w of the sum of absolute products, plus the result's own rounding;
 * dv: (u + r + (n + 2) w) sum p|do| + t sum|do| + u|dv|.
+
+Where p and ds are two terms (and o in delta too), u is u^2 (`inner`) but for
+the results' own rounding.
 """
 import math
 
@@ -45,12 +48,13 @@ def visible(nq, nk, causal, window, device):
     return see
 
 
-def attention(q, k, v, do, seqs, causal=True, window=None, scale=None):
+def attention(q, k, v, do, seqs, causal=True, window=None, scale=None, inner=None):
     """{name: (value, bound)} of o, lse, dq, dk, dv for [B, S, H, D] tensors."""
     B, Sq, Hq, D = q.shape
     Hk = k.shape[2]
     scale = 1.0 / math.sqrt(D) if scale is None else scale
     u, t = U[q.dtype], 2.0 ** -25 if q.dtype == torch.float16 else 0.0
+    ui = u if inner is None else inner
     z = lambda x: torch.zeros(x.shape, dtype=torch.float64, device=q.device)  # noqa: E731
     val = {"o": z(q), "dq": z(q), "dk": z(k), "dv": z(v),
            "lse": torch.full((B, Hq, Sq), -math.inf, dtype=torch.float64, device=q.device)}
@@ -72,15 +76,15 @@ def attention(q, k, v, do, seqs, causal=True, window=None, scale=None):
             pe = p * r  # error of the probabilities in fp32
             seen = see.double()
             o = p @ d
-            oe = (p * (u + r + (nk + 2) * W)) @ d.abs() + t * (seen @ d.abs()) + u * o.abs()
+            oe = (p * (ui + r + (nk + 2) * W)) @ d.abs() + t * (seen @ d.abs())
             dp = da @ d.T
             delta = (da * o).sum(1, keepdim=True)
-            de = (da.abs() * ((D + 2) * W * o.abs() + oe)).sum(1, keepdim=True)
+            de = (da.abs() * ((D + 2) * W * o.abs() + oe + ui * o.abs())).sum(1, keepdim=True)
             ds = p * (dp - delta)
             dse = pe * (dp - delta).abs() + p * ((D + 2) * W * (da.abs() @ d.abs().T) + de) \
-                + u * ds.abs() + t * seen
+                + ui * ds.abs() + t * seen
             qs, ks = slice(q0, q0 + nq), slice(k0, k0 + nk)
-            val["o"][b, qs, h], err["o"][b, qs, h] = o, oe
+            val["o"][b, qs, h], err["o"][b, qs, h] = o, oe + u * o.abs()
             val["lse"][b, h, qs] = lse[:, 0]
             err["lse"][b, h, qs] = (r + 4 * W * lse.abs().clamp(max=1e300))[:, 0]
             dq = ds @ c * scale
@@ -92,7 +96,7 @@ def attention(q, k, v, do, seqs, causal=True, window=None, scale=None):
             err["dk"][b, ks, g] += scale * (dse.T @ a.abs()
                                             + (nq * (Hq // Hk) + 2) * W * (ds.abs().T @ a.abs()))
             val["dv"][b, ks, g] += p.T @ da
-            err["dv"][b, ks, g] += (p * (u + r + (nq * (Hq // Hk) + 2) * W)).T @ da.abs() \
+            err["dv"][b, ks, g] += (p * (ui + r + (nq * (Hq // Hk) + 2) * W)).T @ da.abs() \
                 + t * (seen.T @ da.abs())
     for n in ("dk", "dv"):
         err[n] += u * val[n].abs()
