@@ -69,6 +69,7 @@ struct BwdCfg {
   static constexpr int BARS = 1 + 2 * NA + 2 * NB + 8 + 3 + 1;
   static constexpr int SMEM = BAR_OFF + BARS * 8 + 16;
   static_assert(SMEM <= 227 * 1024, "shared memory");
+  static_assert(OWN * OWNB >= 8 * 4096, "4 KB of the kept tiles for each warp's results");
   // tensor-memory columns: S (two buffers), dP (two buffers, not for dV alone),
   // the sums, and behind them, where there is room, the kept tiles
   static constexpr uint32_t COLS = 512;
@@ -132,30 +133,30 @@ struct BwdBars {
   }
 };
 
-// `cols` accumulator columns of the thread's row, times f, to 16-bit memory
-// (in), or zeros (!keep). `any`, alike in the whole warp: there are sums.
-template <typename T>
-__device__ __forceinline__ void store_row(uint32_t at, int cols, float f, T* dst, bool in,
-                                          bool keep, bool any) {
-  keep = keep && any;
+// COLS accumulator columns of the thread's row, times f, to 16-bit memory, or
+// zeros (!keep): the warp's rows r < n at dst + r * ss, through 4 KB of shared
+// memory `sm`. `any`, alike in the whole warp: there are sums.
+template <int COLS, typename T>
+__device__ __forceinline__ void store_sums(uint32_t at, float f, T* dst, int64_t ss, int n,
+                                           bool keep, bool any, unsigned char* sm) {
+  constexpr int CW = COLS < 64 ? COLS : 64;
 #pragma unroll 1
-  for (int c = 0; c < cols; c += 32) {
-    uint32_t r[32];
+  for (int c = 0; c < COLS; c += CW) {
+    uint32_t w[CW / 2] = {};
     if (any) {
-      tmem_ld32(at + c, r);
-      tmem_wait_ld();
-    }
-    if (!in) continue;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t w[4];
+      for (int p = 0; p < CW; p += 32) {
+        uint32_t r[32];
+        tmem_ld32(at + c + p, r);
+        tmem_wait_ld();
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        w[u] = keep ? pack2<T>(__uint_as_float(r[8 * i + 2 * u]) * f,
-                               __uint_as_float(r[8 * i + 2 * u + 1]) * f)
-                    : 0u;
-      *reinterpret_cast<uint4*>(dst + c + i * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int i = 0; i < 16; ++i)
+          w[p / 2 + i] = keep ? pack2<T>(__uint_as_float(r[2 * i]) * f,
+                                         __uint_as_float(r[2 * i + 1]) * f)
+                              : 0u;
+      }
     }
+    store_rows<CW>(sm, w, dst + c, ss, n);
   }
 }
 
@@ -452,12 +453,15 @@ __global__ void __launch_bounds__(352, 1)
       // group 0 writes dV, group 1 dK, or each half of the one there is; keys
       // past the sequence's end (dense tensors) get zeros
       const bool is_k = DV && DK ? group != 0 : DK;
-      const int cols = DV && DK ? D : D / 2, c0 = DV && DK ? 0 : group * cols;
+      constexpr int COLS = DV && DK ? D : D / 2;
+      const int c0 = DV && DK ? 0 : group * COLS, key0 = n0 + (warp & 3) * 32;
       const HT& t = is_k ? a.dk : a.dv;
       T* dst = reinterpret_cast<T*>(const_cast<void*>(t.p)) + (int64_t)s.b * t.sb +
-               (int64_t)h * t.sh + (int64_t)(s.k0 + key) * t.ss + c0;
-      store_row<T>(tmem + lanes + (is_k ? DK_COL : DV_COL) + c0, cols, is_k ? a.scale : 1.f, dst,
-                   key < limit, key < s.klen, total > 0);
+               (int64_t)h * t.sh + (int64_t)(s.k0 + key0) * t.ss + c0;
+      // through the kept tiles, which every product has read
+      store_sums<COLS>(tmem + lanes + (is_k ? DK_COL : DV_COL) + c0, is_k ? a.scale : 1.f, dst,
+                       t.ss, limit - key0, key < s.klen, total > 0,
+                       smem + C::OWN_OFF + warp * 4096);
     }
   }
   tc_fence_before();
@@ -677,11 +681,13 @@ __global__ void __launch_bounds__(352, 1)
       tc_fence_after();
     }
     if (ok) {
+      const int row0 = m0 + (warp & 3) * 32;
       T* dst = reinterpret_cast<T*>(const_cast<void*>(a.dq.p)) + (int64_t)s.b * a.dq.sb +
-               (int64_t)h * a.dq.sh + (int64_t)(s.q0 + row) * a.dq.ss + group * (D / 2);
-      // queries past the sequence's end (dense tensors) get zeros
-      store_row<T>(tmem + lanes + C::ACC_COL + group * (D / 2), D / 2, a.scale, dst, row < limit,
-                   row < s.qlen, total > 0);
+               (int64_t)h * a.dq.sh + (int64_t)(s.q0 + row0) * a.dq.ss + group * (D / 2);
+      // queries past the sequence's end (dense tensors) get zeros; through the
+      // kept tiles, which every product has read
+      store_sums<D / 2>(tmem + lanes + C::ACC_COL + group * (D / 2), a.scale, dst, a.dq.ss,
+                        limit - row0, row < s.qlen, total > 0, smem + C::OWN_OFF + warp * 4096);
     }
   }
   tc_fence_before();

@@ -357,36 +357,32 @@ __global__ void __launch_bounds__(352, 1)
     if (ok && e > f) {
       ok = __all_sync(0xffffffffu, bar_wait(o_last + 8 * t, 0, waits));
       tc_fence_after();
+    } else if (ok && nb > 0) {  // no keys, but a copy of Q that its memory waits for
+      ok = __all_sync(0xffffffffu, bar_wait(q_full, 0, waits));
     }
     if (ok) {
       const bool in = row < s.qlen, any = e > f && in;
       const float inv = any && l != 0.f ? 1.f / l : 0.f;
+      // through the tile's Q, which every product with K has read
+      const int row0 = m0 + t * N + (warp & 3) * 32;
+      unsigned char* sm = smem + C::Q_OFF + t * C::QB + (warp & 3) * 4096;
       const int64_t at = (int64_t)s.b * a.o.sb + (int64_t)h * a.o.sh +
-                         (int64_t)(s.q0 + row) * a.o.ss;
+                         (int64_t)(s.q0 + row0) * a.o.ss;
       T* out = reinterpret_cast<T*>(const_cast<void*>(a.o.p)) + at;
-      T* rest = a.rest != nullptr ? reinterpret_cast<T*>(a.rest) + at : nullptr;
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t r[32];
+#pragma unroll 1
+      for (int c = 0; c < D; c += 64) {
+        uint32_t w[32] = {}, v[32] = {};
         if (e > f) {  // the whole group alike
-          tmem_ld32(o_at + c * 32, r);
-          tmem_wait_ld();
-        }
-        if (row < limit) {
+          load64(o_at + c, x);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t w[4] = {0, 0, 0, 0}, v[4] = {0, 0, 0, 0};
-            if (inv != 0.f) {
-#pragma unroll
-              for (int u = 0; u < 4; ++u)
-                split2<T>(__uint_as_float(r[8 * i + 2 * u]) * inv,
-                          __uint_as_float(r[8 * i + 2 * u + 1]) * inv, w[u], v[u]);
-            }
-            *reinterpret_cast<uint4*>(out + c * 32 + i * 8) = make_uint4(w[0], w[1], w[2], w[3]);
-            if (rest != nullptr)
-              *reinterpret_cast<uint4*>(rest + c * 32 + i * 8) = make_uint4(v[0], v[1], v[2], v[3]);
+          for (int i = 0; i < 32; ++i) {
+            split2<T>(x[2 * i] * inv, x[2 * i + 1] * inv, w[i], v[i]);
+            if (inv == 0.f) w[i] = v[i] = 0u;
           }
         }
+        store_rows<64>(sm, w, out + c, a.o.ss, limit - row0);
+        if (a.rest != nullptr)
+          store_rows<64>(sm, v, reinterpret_cast<T*>(a.rest) + at + c, a.o.ss, limit - row0);
       }
       if (row < limit && a.lse != nullptr)
         a.lse[((int64_t)s.b * a.Hq + h) * a.Sq + s.q0 + row] =

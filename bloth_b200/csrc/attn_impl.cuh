@@ -189,6 +189,35 @@ __device__ __forceinline__ void query_range(const AttnArgs& a, const AttnSeq& s,
   if (n1 <= n0 || hi <= lo) lo = hi = 0;
 }
 
+// CW columns of a warp's 32 rows, thread = row, as 16-bit pairs w, to global
+// memory: row r (< n) at dst + r * ss. Through 64 CW bytes of shared memory `sm`
+// of the warp's own, so that a store instruction writes 32 / (CW / 8) rows'
+// pieces of 2 CW bytes, not 16 bytes of each of 32 rows, which take it a cycle
+// apiece.
+template <int CW, typename T>
+__device__ __forceinline__ void store_rows(unsigned char* sm, const uint32_t (&w)[CW / 2], T* dst,
+                                           int64_t ss, int n) {
+  static_assert(CW == 64 || CW == 32, "a row is one line of shared memory, or half of one");
+  constexpr int CH = CW / 8;  // 16-byte chunks of a row
+  // where chunk c of row r lies: eight rows' fall in different banks
+  auto at = [&](int r, int c) {
+    return sm + r * (CW * 2) + ((c ^ (CH == 8 ? r & 7 : (r >> 1) & 3)) * 16);
+  };
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+    *reinterpret_cast<uint4*>(at(lane, c)) =
+        make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const int r = i * (32 / CH) + lane / CH, c = lane % CH;
+    if (r < n)
+      *reinterpret_cast<uint4*>(dst + r * ss + c * 8) = *reinterpret_cast<const uint4*>(at(r, c));
+  }
+  __syncwarp();
+}
+
 // Host launchers.
 // attn_tc_*: 16-bit tensors, on the tensor cores.
 template <typename T>
