@@ -33,10 +33,10 @@
 // or dK. With the kept tiles in tensor memory, where the sums leave room for
 // them (dQ up to head_dim 128; dK and dV at head_dim 64), S and dP take 256 as
 // well. Beside them 512 cycles a block for its exponentials.
-// Measured at 8192 rows of 32/8 heads of 128 (bf16): causal, dK and dV 820 us
-// (four products, 1340 TFLOP/s), dQ 610 us (three, 1350); full rows, dQ 1155 us,
-// with the kept tiles in shared memory 1370, and dK and dV 1700 us, in blocks of
-// 128 queries in single buffers 1826. Sixteen softmax warps in place of eight
+// Measured at 8192 rows of 32/8 heads of 128 (bf16): causal, dK and dV 835 us
+// (four products, 1320 TFLOP/s), dQ 585 us (three, 1410); full rows, dQ 1125 us,
+// with the kept tiles in shared memory 1370, and dK and dV 1700 to 1840 us, in
+// blocks of 128 queries in single buffers 1826. Sixteen softmax warps in place of eight
 // were no faster.
 #pragma once
 
