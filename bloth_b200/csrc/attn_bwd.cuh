@@ -36,8 +36,8 @@
 // Measured at 8192 rows of 32/8 heads of 128 (bf16): causal, dK and dV 835 us
 // (four products, 1320 TFLOP/s), dQ 585 us (three, 1410); full rows, dQ 1125 us,
 // with the kept tiles in shared memory 1370, and dK and dV 1700 to 1840 us, in
-// blocks of 128 queries in single buffers 1826. Sixteen softmax warps in place of eight
-// were no faster.
+// blocks of 128 queries in single buffers 1826. Sixteen softmax warps in place of
+// eight were no faster.
 #pragma once
 
 #include <climits>
