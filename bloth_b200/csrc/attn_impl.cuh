@@ -87,6 +87,9 @@ inline int64_t attn_tiles(int64_t S, int64_t packed, int tile) {
 
 // The sequence and tile of flat tile index `t` (BY_Q: tiles of query rows,
 // else of key rows). Called by whole warps; every warp finds the same.
+// A step of 32 sequences costs about 150 cycles: sums of their tiles, with scans
+// only where the tile is found or the offsets decrease (8192 rows as 2048
+// sequences, 32/8 heads of 128, forward: 7.7 ms with scans in each, 5.6 without).
 // Packed offsets are clamped to the tensors and to be non-decreasing, so no
 // content of the offsets leads outside of them.
 template <bool BY_Q>
@@ -107,37 +110,45 @@ __device__ __forceinline__ AttnSeq find_seq(const AttnArgs& a, int b, int t, int
   const int n = a.packed;
   int before = 0;
   int last_q = 0, last_k = 0;  // ends of the pieces before this step of 32
+  // piece i = base + lane ends at offset i: the rows before the first sequence,
+  // the n sequences, the rows past the last one
+  auto end_q = [&](int i) { return i <= n ? seq_at(a.qseq, a.seq_dt, i, a.Sq) : a.Sq; };
+  auto end_k = [&](int i) { return i <= n ? seq_at(a.kseq, a.seq_dt, i, a.Sk) : a.Sk; };
+  int next_q = end_q(lane), next_k = end_k(lane);
   for (int base = 0; base <= n + 1; base += 32) {
-    // piece i = base + lane ends at offset i: the rows before the first
-    // sequence, the n sequences, the rows past the last one
     const int i = base + lane;
-    int q1 = i <= n ? seq_at(a.qseq, a.seq_dt, i, a.Sq) : a.Sq;
-    int k1 = i <= n ? seq_at(a.kseq, a.seq_dt, i, a.Sk) : a.Sk;
-    q1 = max(q1, last_q);
-    k1 = max(k1, last_k);
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {  // running maxima: non-decreasing ends
-      const int uq = __shfl_up_sync(0xffffffffu, q1, o), uk = __shfl_up_sync(0xffffffffu, k1, o);
-      if (lane >= o) {
-        q1 = max(q1, uq);
-        k1 = max(k1, uk);
-      }
-    }
+    int q1 = max(next_q, last_q), k1 = max(next_k, last_k);
+    next_q = end_q(i + 32);
+    next_k = end_k(i + 32);
     int q0 = __shfl_up_sync(0xffffffffu, q1, 1), k0 = __shfl_up_sync(0xffffffffu, k1, 1);
     if (lane == 0) {
       q0 = last_q;
       k0 = last_k;
     }
-    const int rows = BY_Q ? q1 - q0 : k1 - k0;
-    int tiles = i <= n + 1 ? (rows + tile - 1) / tile : 0;
-    int upto = tiles;
+    if (!__all_sync(0xffffffffu, q1 >= q0 && k1 >= k0)) {
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += u;
+      for (int o = 1; o < 32; o <<= 1) {  // running maxima: non-decreasing ends
+        const int uq = __shfl_up_sync(0xffffffffu, q1, o), uk = __shfl_up_sync(0xffffffffu, k1, o);
+        if (lane >= o) {
+          q1 = max(q1, uq);
+          k1 = max(k1, uk);
+        }
+      }
+      const int uq = __shfl_up_sync(0xffffffffu, q1, 1), uk = __shfl_up_sync(0xffffffffu, k1, 1);
+      q0 = lane == 0 ? last_q : uq;
+      k0 = lane == 0 ? last_k : uk;
     }
-    const unsigned hit = __ballot_sync(0xffffffffu, t < before + upto);
-    if (hit) {
+    const int rows = BY_Q ? q1 - q0 : k1 - k0;
+    const int tiles = i <= n + 1 ? (rows + tile - 1) / tile : 0;
+    const int all = (int)__reduce_add_sync(0xffffffffu, (unsigned)tiles);
+    if (t < before + all) {
+      int upto = tiles;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += u;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, t < before + upto);
       const int src = __ffs(hit) - 1;
       s.q0 = __shfl_sync(0xffffffffu, q0, src);
       s.qlen = __shfl_sync(0xffffffffu, q1, src) - s.q0;
@@ -149,7 +160,7 @@ __device__ __forceinline__ AttnSeq find_seq(const AttnArgs& a, int b, int t, int
       if (base + src == 0 || base + src == n + 1) (BY_Q ? s.klen : s.qlen) = 0;
       return s;
     }
-    before += __shfl_sync(0xffffffffu, upto, 31);
+    before += all;
     last_q = __shfl_sync(0xffffffffu, q1, 31);
     last_k = __shfl_sync(0xffffffffu, k1, 31);
   }

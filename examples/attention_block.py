@@ -84,7 +84,7 @@ class Block(nn.Module):
 
 
 def relative(a, b):
-    return float((a.float() - b.float()).norm() / b.float().norm())
+    return float(((a.float() - b.float()).norm() / b.float().norm()).detach())
 
 
 def run(tokens=512, dtype=torch.bfloat16, device="cuda"):
