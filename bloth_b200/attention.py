@@ -16,7 +16,8 @@ its q/k normalisation and rotary embedding through the sm_100a kernels:
 With ``fuse_attention=True`` the attention itself is ``fused_attention`` too,
 where HF passes no mask tensor (unpadded batches under ``sdpa`` or
 ``flash_attention_2`` kwargs, whose ``cu_seq_lens_q`` / ``_k`` are passed on)
-and no dropout; other calls keep HF's attention.
+and no dropout; other calls keep HF's attention, and so do flattened batches
+whose documents HF's flash attention finds from ``position_ids`` alone.
 
 The rest of the forward is HuggingFace's own code path, restated for the
 transformers 5.x signature ``forward(hidden_states, position_embeddings,
@@ -104,7 +105,8 @@ def _attention_forward(self, hidden_states, position_embeddings=None, attention_
     q, k = q.transpose(1, 2), k.transpose(1, 2)
     if past_key_values is not None:
         k, v = past_key_values.update(k, v, self.layer_idx)
-    if bind.core and _takes_core(self, q, v, attention_mask, kwargs):
+    if bind.core and _takes_core(self, q, v, attention_mask, kwargs) and \
+            not _documents(self, q, kwargs):
         o = _core(self, bind, q, k, v, kwargs)
         return self.o_proj(o.reshape(*input_shape, -1)), None
     hf = sys.modules[type(self).__module__]
@@ -130,6 +132,19 @@ def _takes_core(self, q, v, attention_mask, kwargs) -> bool:
             kwargs.get("output_attentions") or kwargs.get("softcap") is not None:
         return False
     return not self.training or not self.attention_dropout
+
+
+def _documents(self, q, kwargs) -> bool:
+    """Whether HF's flash attention would split this call into documents by its
+    positions: one row whose position_ids do not go on by one, and no offsets.
+    (Elsewhere HF passes documents as a mask.) Reads the positions on the host,
+    as HF does."""
+    pos = kwargs.get("position_ids")
+    if pos is None or q.shape[0] != 1 or q.shape[2] == 1 or \
+            kwargs.get("cu_seq_lens_q") is not None or \
+            not str(self.config._attn_implementation).startswith("flash_attention"):
+        return False
+    return bool((pos[..., 1:] != pos[..., :-1] + 1).any())
 
 
 def _window(self, bind):
