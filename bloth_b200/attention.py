@@ -128,6 +128,8 @@ def _takes_core(self, q, v, attention_mask, kwargs) -> bool:
     if attention_mask is not None or not q.is_cuda or v.shape[-1] != q.shape[-1] or \
             q.dtype != v.dtype:
         return False
+    if q.shape[0] != 1 and kwargs.get("cu_seq_lens_q") is not None:
+        return False  # HF flattens the rows first
     if not kwargs.get("is_causal", getattr(self, "is_causal", True)) or \
             kwargs.get("output_attentions") or kwargs.get("softcap") is not None:
         return False
@@ -155,7 +157,7 @@ def _window(self, bind):
 
 def _core(self, bind, q, k, v, kwargs):
     """fused_attention of q, k, v [B, H, S, D]; returns [B, S, H, D]."""
-    cu = kwargs.get("cu_seq_lens_q") if q.shape[0] == 1 else None
+    cu = kwargs.get("cu_seq_lens_q")
     return fused_attention(q.transpose(1, 2), k.to(q.dtype).transpose(1, 2), v.transpose(1, 2),
                            causal=True, window=_window(self, bind) or None, scale=self.scaling,
                            cu_seqlens=cu,

@@ -105,3 +105,11 @@ def test_offsets_win_over_positions(model):
     assert _run(m, position_ids=RESTART, cu_seq_lens_q=cu, cu_seq_lens_k=cu, max_length_q=7,
                 max_length_k=7)
     assert m.core[0]["cu_seqlens"] is cu
+
+
+@pytest.mark.parametrize("name", ["sdpa", "flash_attention_2"])
+def test_offsets_over_several_rows_stay(model, name):
+    # HF flattens the rows before it applies the offsets
+    cu = torch.tensor([0, 5, 12, 24], dtype=torch.int32)
+    assert not _run(model(name), 2, cu_seq_lens_q=cu, cu_seq_lens_k=cu, max_length_q=12,
+                    max_length_k=12)
