@@ -131,7 +131,8 @@ def _takes_core(self, q, v, attention_mask, kwargs) -> bool:
     if q.shape[0] != 1 and kwargs.get("cu_seq_lens_q") is not None:
         return False  # HF flattens the rows first
     if not kwargs.get("is_causal", getattr(self, "is_causal", True)) or \
-            kwargs.get("output_attentions") or kwargs.get("softcap") is not None:
+            kwargs.get("output_attentions") or kwargs.get("softcap") is not None or \
+            kwargs.get("cache") is not None:  # a paged cache: k and v are the new tokens' only
         return False
     return not self.training or not self.attention_dropout
 

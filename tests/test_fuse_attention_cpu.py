@@ -113,3 +113,12 @@ def test_offsets_over_several_rows_stay(model, name):
     cu = torch.tensor([0, 5, 12, 24], dtype=torch.int32)
     assert not _run(model(name), 2, cu_seq_lens_q=cu, cu_seq_lens_k=cu, max_length_q=12,
                     max_length_k=12)
+
+
+@pytest.mark.parametrize("name", ["sdpa", "flash_attention_2"])
+def test_paged_caches_stay(model, name):
+    m = model(name)
+    attn = m.model.layers[0].self_attn
+    cos = torch.ones(1, 12, 64)
+    attn(torch.zeros(1, 12, 128), (cos, cos), None, cache=object())
+    assert len(m.hf) == 1 and not m.core
