@@ -124,7 +124,11 @@ def _attention_forward(self, hidden_states, position_embeddings=None, attention_
 
 def _takes_core(self, q, v, attention_mask, kwargs) -> bool:
     """Whether a call's attention is what fused_attention computes: causal to
-    the last key, no mask tensor, no dropout, no weights asked for."""
+    the last key, no mask tensor, no dropout, no weights asked for. Without a
+    mask sdpa and flash attention are causal; others need not be."""
+    how = str(self.config._attn_implementation)
+    if how != "sdpa" and not how.startswith("flash_attention"):
+        return False
     if attention_mask is not None or not q.is_cuda or v.shape[-1] != q.shape[-1] or \
             q.dtype != v.dtype:
         return False

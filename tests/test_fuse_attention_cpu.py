@@ -122,3 +122,13 @@ def test_paged_caches_stay(model, name):
     cos = torch.ones(1, 12, 64)
     attn(torch.zeros(1, 12, 128), (cos, cos), None, cache=object())
     assert len(m.hf) == 1 and not m.core
+
+
+@pytest.mark.parametrize("name", ["eager", "paged|sdpa", "paged|flash_attention_2", "my_attention"])
+def test_other_implementations_stay(model, name):
+    # without a mask these are not causal, or find their keys elsewhere
+    m = model(name)
+    attn = m.model.layers[0].self_attn
+    cos = torch.ones(1, 12, 64)
+    attn(torch.zeros(1, 12, 128), (cos, cos), None)
+    assert len(m.hf) == 1 and not m.core
