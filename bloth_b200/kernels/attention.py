@@ -12,6 +12,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from .._lib import address
@@ -152,6 +153,7 @@ class _AttentionFunction(torch.autograd.Function):
         return out, lse
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout, *_):
         q4, k4, v4, out, rest, lse, q_seq, k_seq = ctx.saved_tensors
         want = ctx.needs_input_grad

@@ -13,6 +13,7 @@ import ctypes
 from functools import lru_cache
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from .._lib import address
@@ -142,6 +143,7 @@ class _QKNormMRoPEFunction(torch.autograd.Function):
         return qo if ko is None else (qo, ko)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, *grads):
         q4, k4, wq, wk, rq, rk, pos, inv_freq = ctx.saved_tensors
         pos_st, ax, flat, weight_offset, rope_scale = ctx.meta
@@ -205,6 +207,7 @@ class _MRoPEFunction(torch.autograd.Function):
         return qo if ko is None else (qo, ko)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, *grads):
         pos, inv_freq = ctx.saved_tensors
         pos_st, ax, scale, flat, has_k = ctx.meta
