@@ -16,6 +16,7 @@ from contextlib import contextmanager
 from functools import lru_cache
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libbloth_b200.so")
 
@@ -151,6 +152,14 @@ def require_cuda(*tensors: torch.Tensor) -> None:
     for t in tensors:
         if t is not None:
             assert t.is_cuda, "[Bloth] CUDA GPU required"
+
+
+def has_tangent(*tensors: torch.Tensor | None) -> bool:
+    """Whether any of them carries a forward-mode derivative. The kernels have
+    none: such calls go to the autograd function, which refuses them."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # outside of every dual level
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def ptr(t: torch.Tensor | None):

@@ -220,7 +220,8 @@ def fused_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: b
         raise ValueError("[Bloth] window must be at least 1, and needs causal=True")
     q_seq, k_seq, packed = _sequences(q, k, q_lens, k_lens, cu_seqlens, cu_seqlens_k)
     how = (q_seq, k_seq, packed, float(scale), bool(causal), int(window or 0))
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)) or \
+            _lib.has_tangent(q, k, v):
         out = _AttentionFunction.apply(q, k, v, return_lse, *how)
         if not return_lse:
             return out

@@ -94,8 +94,9 @@ def _check_pair(q4, k4):
         raise TypeError(f"[Bloth] q and k differ in dtype: {q4.dtype}, {k4.dtype}")
 
 
-def _needs_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+def _needs_grad(inv_freq, *tensors) -> bool:
+    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or \
+        _lib.has_tangent(inv_freq, *tensors)
 
 
 def _weight(w, D: int, dtype):
@@ -236,7 +237,7 @@ def fused_qk_norm_mrope(q: torch.Tensor, k: torch.Tensor | None, wq: torch.Tenso
     _lib.require_cuda(q, k, wq, wk, position_ids, inv_freq)
     args = (q, k, wq, wk, position_ids, inv_freq, axes, float(eps), float(weight_offset),
             float(rope_scale))
-    if _needs_grad(q, k, wq, wk):
+    if _needs_grad(inv_freq, q, k, wq, wk):
         return _QKNormMRoPEFunction.apply(*args)
     qo, ko, _ = _norm_mrope_call(*args)
     return qo if ko is None else (qo, ko)
@@ -249,7 +250,7 @@ def apply_mrope_qk(q: torch.Tensor, k: torch.Tensor | None, position_ids: torch.
     :func:`fused_qk_norm_mrope`."""
     _lib.require_cuda(q, k, position_ids, inv_freq)
     args = (q, k, position_ids, inv_freq, axes, float(rope_scale))
-    if _needs_grad(q, k):
+    if _needs_grad(inv_freq, q, k):
         return _MRoPEFunction.apply(*args)
     qo, ko, _ = _mrope_call(*args)
     return qo if ko is None else (qo, ko)

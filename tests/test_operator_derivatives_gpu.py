@@ -1,7 +1,8 @@
 """Derivatives that the attention and multi-axis rotary operators do not have
-are refused, not dropped."""
+are refused, not dropped: second ones, and forward-mode ones."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwad
 
 import bloth_b200
 
@@ -34,3 +35,31 @@ def test_second_derivatives_are_refused(cuda, name):
     # another path keeps the penalty differentiable
     with pytest.raises(RuntimeError, match="once_differentiable"):
         (g.square().sum() + x[0].sum()).backward()
+
+
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_derivatives_are_refused(cuda, name, grad):
+    x, f = _calls(cuda)[name]
+    for i in range(len(x)):
+        with fwad.dual_level(), torch.set_grad_enabled(grad):
+            y = list(x)
+            y[i] = fwad.make_dual(x[i], torch.ones_like(x[i]))
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                f(*y)
+
+
+def test_forward_mode_derivatives_by_frequency_are_refused(cuda):
+    q = torch.randn(1, 6, 2, 64, device=cuda)
+    pos, inv = torch.arange(6, device=cuda).expand(3, 1, 6), torch.ones(32, device=cuda)
+    with fwad.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
+        bloth_b200.apply_mrope_qk(q, None, pos, fwad.make_dual(inv, inv.clone()),
+                                  bloth_b200.mrope_axes((12, 10, 10)))
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_plain_tensors_inside_a_dual_level(cuda, name):
+    x, f = _calls(cuda)[name]
+    want = f(*x)
+    with fwad.dual_level():
+        assert torch.equal(f(*x), want)
