@@ -74,11 +74,18 @@ def _axis_positions(position_ids, B: int, S: int):
     return p, _lib.strides((p.stride(0), 0 if p.shape[1] == 1 else p.stride(1), p.stride(2)))
 
 
+def _same_device(t, device, name: str):
+    if t.device != device:
+        raise ValueError(f"[Bloth] {name} must be on {device}, got {t.device}")
+
+
 def _source(x4, position_ids, inv_freq, axes):
     """(positions, strides, axes array, inv_freq) of a call on x4."""
     B, S, _, D = x4.shape
     if position_ids is None or inv_freq is None:
         raise ValueError("[Bloth] position_ids and inv_freq are required")
+    _same_device(position_ids, x4.device, "position_ids")
+    _same_device(inv_freq, x4.device, "inv_freq")
     pos, pos_st = _axis_positions(position_ids, B, S)
     if inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous():
         inv_freq = inv_freq.to(torch.float32).contiguous()
@@ -92,6 +99,8 @@ def _check_pair(q4, k4):
         raise ValueError("[Bloth] q and k must share batch, sequence and head_dim")
     if k4 is not None and k4.dtype != q4.dtype:
         raise TypeError(f"[Bloth] q and k differ in dtype: {q4.dtype}, {k4.dtype}")
+    if k4 is not None:
+        _same_device(k4, q4.device, "k")
 
 
 def _needs_grad(inv_freq, *tensors) -> bool:
@@ -99,7 +108,8 @@ def _needs_grad(inv_freq, *tensors) -> bool:
         _lib.has_tangent(inv_freq, *tensors)
 
 
-def _weight(w, D: int, dtype):
+def _weight(w, D: int, dtype, device):
+    _same_device(w, device, "wq and wk")
     if w.numel() != D or w.dtype != dtype:
         raise ValueError(f"[Bloth] wq and wk must have head_dim = {D} elements of one dtype")
     return _lib.aligned16(w.contiguous())
@@ -114,8 +124,8 @@ def _norm_mrope_call(q, k, wq, wk, position_ids, inv_freq, axes, eps, weight_off
     pos, pos_st, ax, inv_freq = _source(q4, position_ids, inv_freq, axes)
     if k4 is not None and wk is None:
         raise ValueError("[Bloth] wk is required with k")
-    wk = None if wk is None else _weight(wk, D, wq.dtype)
-    wq = _weight(wq, D, wq.dtype)
+    wk = None if wk is None else _weight(wk, D, wq.dtype, q4.device)
+    wq = _weight(wq, D, wq.dtype, q4.device)
     qo = _contiguous_like(q4)
     ko = None if k4 is None else _contiguous_like(k4)
     rq = q4.new_empty((B, S, Hq), dtype=torch.float32)
