@@ -42,7 +42,7 @@ import inspect
 import sys
 import types
 import warnings
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 
 import torch.nn as nn
 
@@ -199,7 +199,13 @@ def patch_attention_layers(model: nn.Module, verbose: bool = True, core: bool = 
     bound, skipped = 0, []
     for name, module in model.named_modules():
         spec = _ATTENTION_CLASSES.get(type(module).__name__)
-        if spec is None or hasattr(module, "_bloth_attention"):
+        if spec is None:
+            continue
+        have = getattr(module, "_bloth_attention", None)
+        if have is not None:
+            if core and not have.core:  # bound without it before
+                module._bloth_attention = replace(have, core=True)
+                bound += 1
             continue
         reason = _why_not(module, spec[0])
         if reason is not None:

@@ -132,3 +132,21 @@ def test_other_implementations_stay(model, name):
     cos = torch.ones(1, 12, 64)
     attn(torch.zeros(1, 12, 128), (cos, cos), None)
     assert len(m.hf) == 1 and not m.core
+
+
+@pytest.mark.parametrize("first", [dict(patch_attention=True), dict(fuse_attention=True)])
+def test_fusing_a_model_that_is_patched_already(model, first, capsys):
+    m = model("sdpa")
+    for layer in m.model.layers:  # as before any patch
+        del layer.self_attn._bloth_attention, layer.self_attn.__dict__["forward"]
+    bloth_b200.patch_model(m, patch_norms=False, verbose=False, **first)
+    fused = "fuse_attention" in first
+    assert _run(m) == fused
+    m.core.clear(), m.hf.clear()
+    bloth_b200.patch_model(m, patch_norms=False, fuse_attention=True)
+    assert (f"Patched {LAYERS} attention layer(s)" in capsys.readouterr().out) == (not fused)
+    assert _run(m)
+    # patch_attention alone takes nothing back
+    m.core.clear(), m.hf.clear()
+    bloth_b200.patch_model(m, patch_norms=False, verbose=False, patch_attention=True)
+    assert _run(m)
