@@ -35,17 +35,19 @@ int check_sizes(int64_t B, int64_t Sq, int64_t Sk, int64_t Hq, int64_t Hk, int64
   return BLOTH_OK;
 }
 
-// A head tensor the kernels can address, filled into t.
-int fill(HT& t, const void* p, const int64_t* st, int dtype) {
+// A head tensor of B x S x H rows that the kernels can address, filled into t.
+// The stride of a single element, on which no address depends, may be anything.
+int fill(HT& t, const void* p, const int64_t* st, int64_t B, int64_t S, int64_t H, int dtype) {
   if (p == nullptr || st == nullptr) return BLOTH_ERR_NULL;
   const int vec = 16 / elem_bytes(dtype);
   if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return BLOTH_ERR_ALIGN;
+  const int64_t n[3] = {B, S, H};
   for (int i = 0; i < 3; ++i)
-    if (st[i] % vec != 0) return BLOTH_ERR_ALIGN;
+    if (n[i] > 1 && st[i] % vec != 0) return BLOTH_ERR_ALIGN;
   t.p = p;
-  t.sb = st[0];
-  t.ss = st[1];
-  t.sh = st[2];
+  t.sb = B > 1 ? st[0] : 0;
+  t.ss = S > 1 ? st[1] : 0;
+  t.sh = H > 1 ? st[2] : 0;
   return BLOTH_OK;
 }
 
@@ -107,12 +109,12 @@ int bloth_attention_fwd(const void* q, const int64_t* q_strides, const void* k,
                         window)))
     return rc;
   if (B == 0 || Sq == 0) return BLOTH_OK;
-  if ((rc = fill(a.q, q, q_strides, dtype))) return rc;
+  if ((rc = fill(a.q, q, q_strides, B, Sq, Hq, dtype))) return rc;
   if (Sk > 0) {
-    if ((rc = fill(a.k, k, k_strides, dtype))) return rc;
-    if ((rc = fill(a.v, v, v_strides, dtype))) return rc;
+    if ((rc = fill(a.k, k, k_strides, B, Sk, Hk, dtype))) return rc;
+    if ((rc = fill(a.v, v, v_strides, B, Sk, Hk, dtype))) return rc;
   }
-  if ((rc = fill(a.o, out, out_strides, dtype))) return rc;
+  if ((rc = fill(a.o, out, out_strides, B, Sq, Hq, dtype))) return rc;
   if (reinterpret_cast<uintptr_t>(out_rest) % 16 != 0) return BLOTH_ERR_ALIGN;
   a.rest = dtype == BLOTH_F32 ? nullptr : out_rest;
   a.lse = lse;
@@ -159,17 +161,17 @@ int bloth_attention_bwd(const void* dout, const int64_t* dout_strides, const voi
   if ((dk == nullptr) != (dv == nullptr)) return BLOTH_ERR_NULL;
   if (B == 0 || (Sq == 0 && Sk == 0)) return BLOTH_OK;
   if (Sq > 0) {
-    if ((rc = fill(a.dout, dout, dout_strides, dtype))) return rc;
-    if ((rc = fill(a.q, q, q_strides, dtype))) return rc;
-    if ((rc = fill(a.o, out, out_strides, dtype))) return rc;
+    if ((rc = fill(a.dout, dout, dout_strides, B, Sq, Hq, dtype))) return rc;
+    if ((rc = fill(a.q, q, q_strides, B, Sq, Hq, dtype))) return rc;
+    if ((rc = fill(a.o, out, out_strides, B, Sq, Hq, dtype))) return rc;
     if (lse == nullptr) return BLOTH_ERR_NULL;
-    if (dq != nullptr && (rc = fill(a.dq, dq, dq_strides, dtype))) return rc;
+    if (dq != nullptr && (rc = fill(a.dq, dq, dq_strides, B, Sq, Hq, dtype))) return rc;
   }
   if (Sk > 0) {
-    if ((rc = fill(a.k, k, k_strides, dtype))) return rc;
-    if ((rc = fill(a.v, v, v_strides, dtype))) return rc;
-    if (dk != nullptr && (rc = fill(a.dk, dk, dk_strides, dtype))) return rc;
-    if (dv != nullptr && (rc = fill(a.dv, dv, dv_strides, dtype))) return rc;
+    if ((rc = fill(a.k, k, k_strides, B, Sk, Hk, dtype))) return rc;
+    if ((rc = fill(a.v, v, v_strides, B, Sk, Hk, dtype))) return rc;
+    if (dk != nullptr && (rc = fill(a.dk, dk, dk_strides, B, Sk, Hk, dtype))) return rc;
+    if (dv != nullptr && (rc = fill(a.dv, dv, dv_strides, B, Sk, Hk, dtype))) return rc;
   }
   const size_t need = bloth_attention_bwd_workspace_bytes(B, Sq, Sk, Hq, Hk, D, packed, dtype);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return BLOTH_ERR_WORKSPACE;

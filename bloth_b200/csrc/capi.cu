@@ -90,21 +90,23 @@ cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 bool head_dim_ok(int64_t D) { return D == 64 || D == 128 || D == 256; }
 constexpr int64_t kMaxTokens = (int64_t)1 << 31;  // B*S must stay below this
 
-int check_heads_tensor(const void* p, const int64_t* st, int dtype) {
+// n: the extents B, S and H that the strides belong to; the stride of a single
+// element, on which no address depends, may be anything.
+int check_heads_tensor(const void* p, const int64_t* st, const int64_t (&n)[3], int dtype) {
   if (p == nullptr || st == nullptr) return BLOTH_ERR_NULL;
   const int vec = 16 / elem_size(dtype);
   if (!aligned(p, 16)) return BLOTH_ERR_ALIGN;
   for (int i = 0; i < 3; ++i)
-    if (st[i] % vec != 0) return BLOTH_ERR_ALIGN;
+    if (n[i] > 1 && st[i] % vec != 0) return BLOTH_ERR_ALIGN;
   return BLOTH_OK;
 }
 
-HT make_ht(const void* p, const int64_t* st) {
+HT make_ht(const void* p, const int64_t* st, const int64_t (&n)[3], int64_t D) {
   HT t;
   t.p = p;
-  t.sb = st ? st[0] : 0;
-  t.ss = st ? st[1] : 0;
-  t.sh = st ? st[2] : 0;
+  t.sb = n[0] > 1 ? st[0] : 0;
+  t.ss = n[1] > 1 ? st[1] : 0;
+  t.sh = n[2] > 1 ? st[2] : D;
   return t;
 }
 
@@ -205,12 +207,13 @@ int qk_norm_rope_fwd(const Axes& ax, const void* q, const int64_t* q_strides, co
   const int64_t H[2] = {Hq, Hk};
   for (int t = 0; t < 2; ++t) {
     if (H[t] == 0) continue;
-    if ((rc = check_heads_tensor(src[t], sst[t], dtype))) return rc;
-    if ((rc = check_heads_tensor(dst[t], dstst[t], dtype))) return rc;
+    const int64_t n[3] = {B, S, H[t]};
+    if ((rc = check_heads_tensor(src[t], sst[t], n, dtype))) return rc;
+    if ((rc = check_heads_tensor(dst[t], dstst[t], n, dtype))) return rc;
     if (w[t] == nullptr || rs[t] == nullptr) return BLOTH_ERR_NULL;
     if (!aligned(w[t], 16)) return BLOTH_ERR_ALIGN;
-    a.src[t] = make_ht(src[t], sst[t]);
-    a.dst[t] = make_ht(dst[t], dstst[t]);
+    a.src[t] = make_ht(src[t], sst[t], n, D);
+    a.dst[t] = make_ht(dst[t], dstst[t], n, D);
     a.w[t] = w[t];
     a.rstd_out[t] = rs[t];
     a.H[t] = (int)H[t];
@@ -260,18 +263,19 @@ int qk_norm_rope_bwd(const Axes& ax, const void* dq_out, const int64_t* dqo_stri
   const int64_t H[2] = {Hq, Hk};
   for (int t = 0; t < 2; ++t) {
     if (H[t] == 0) continue;
+    const int64_t n[3] = {B, S, H[t]};
     if (w[t] == nullptr || dw[t] == nullptr) return BLOTH_ERR_NULL;
     if (!aligned(w[t], 16)) return BLOTH_ERR_ALIGN;
     a.w[t] = w[t];
     a.H[t] = (int)H[t];
     if (B * S == 0) continue;
-    if ((rc = check_heads_tensor(g[t], gst[t], dtype))) return rc;
-    if ((rc = check_heads_tensor(x[t], xst[t], dtype))) return rc;
-    if ((rc = check_heads_tensor(dst[t], dstst[t], dtype))) return rc;
+    if ((rc = check_heads_tensor(g[t], gst[t], n, dtype))) return rc;
+    if ((rc = check_heads_tensor(x[t], xst[t], n, dtype))) return rc;
+    if ((rc = check_heads_tensor(dst[t], dstst[t], n, dtype))) return rc;
     if (rs[t] == nullptr) return BLOTH_ERR_NULL;
-    a.src[t] = make_ht(g[t], gst[t]);
-    a.x[t] = make_ht(x[t], xst[t]);
-    a.dst[t] = make_ht(dst[t], dstst[t]);
+    a.src[t] = make_ht(g[t], gst[t], n, D);
+    a.x[t] = make_ht(x[t], xst[t], n, D);
+    a.dst[t] = make_ht(dst[t], dstst[t], n, D);
     a.rstd_in[t] = rs[t];
   }
   a.w_dt = w_dtype;
@@ -315,10 +319,11 @@ int rope_call(const Axes& ax, const void* q, const int64_t* q_strides, void* q_o
   const int64_t H[2] = {Hq, Hk};
   for (int t = 0; t < 2; ++t) {
     if (H[t] == 0) continue;
-    if ((rc = check_heads_tensor(src[t], sst[t], dtype))) return rc;
-    if ((rc = check_heads_tensor(dst[t], dstst[t], dtype))) return rc;
-    a.src[t] = make_ht(src[t], sst[t]);
-    a.dst[t] = make_ht(dst[t], dstst[t]);
+    const int64_t n[3] = {B, S, H[t]};
+    if ((rc = check_heads_tensor(src[t], sst[t], n, dtype))) return rc;
+    if ((rc = check_heads_tensor(dst[t], dstst[t], n, dtype))) return rc;
+    a.src[t] = make_ht(src[t], sst[t], n, D);
+    a.dst[t] = make_ht(dst[t], dstst[t], n, D);
     a.H[t] = (int)H[t];
   }
   a.B = B;
