@@ -70,7 +70,7 @@ def _sequences(q, k, q_lens, k_lens, cu_q, cu_k):
         else:
             cu_k = _sequence_arg(cu_k, cu_q.numel(), device, "cu_seqlens_k")
         if cu_k.dtype != cu_q.dtype:
-            cu_k = cu_k.to(cu_q.dtype)
+            cu_q, cu_k = cu_q.long(), cu_k.long()
         return cu_q, cu_k, cu_q.numel() - 1
     if q_lens is None and k_lens is None:
         return None, None, 0

@@ -1,4 +1,5 @@
-"""Layouts of the attention and rotary operators that no address depends on."""
+"""Layouts and arguments of the attention and multi-axis rotary operators that
+no address depends on, or that come in other types than each other."""
 import pytest
 import torch
 
@@ -36,3 +37,20 @@ def test_strides_of_single_elements(cuda, dtype, B, S, Hq, Hk):
 
     for a, b in zip(run(q, k, v, do), run(*(_odd(x) for x in (q, k, v, do)))):
         assert torch.equal(a, b)
+
+
+def test_offsets_of_two_types(cuda):
+    # 64-bit offsets beside 32-bit ones keep their value: past the keys' end here
+    gen = torch.Generator(device=cuda).manual_seed(2)
+    q, k, v = (torch.randn(100, h, 64, generator=gen, device=cuda).to(BF) for h in (2, 1, 1))
+    t = lambda x, d: torch.tensor(x, device=cuda, dtype=d)  # noqa: E731
+    far = [0, 30, 2 ** 32 + 60]
+    want = bloth_b200.fused_attention(q, k, v, cu_seqlens=t([0, 50, 100], torch.int64),
+                                      cu_seqlens_k=t([0, 30, 100], torch.int64))
+    for d in (torch.int32, torch.int64):
+        assert torch.equal(want, bloth_b200.fused_attention(
+            q, k, v, cu_seqlens=t([0, 50, 100], d), cu_seqlens_k=t(far, torch.int64)))
+    want = bloth_b200.fused_attention(q, k, v, cu_seqlens=t([0, 30, 100], torch.int64),
+                                      cu_seqlens_k=t([0, 50, 100], torch.int64))
+    assert torch.equal(want, bloth_b200.fused_attention(
+        q, k, v, cu_seqlens=t(far, torch.int64), cu_seqlens_k=t([0, 50, 100], torch.int32)))
