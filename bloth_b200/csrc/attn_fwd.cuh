@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(352, 1)
           const int it = j - b0, st = it % NST;
           ok = __all_sync(0xffffffffu, bar_wait(v_full + 8 * st, (uint32_t)(it / NST) & 1u, waits));
           if (!ok) break;
-          zero_rows<D>(smem + C::V_OFF + st * C::KB, s.klen - n0);
+          zero_rows<D>(smem + C::V_OFF + st * C::KB, s.klen - n0, BLK);
         }
       }
       float top[4] = {x[0], x[1], x[2], x[3]};

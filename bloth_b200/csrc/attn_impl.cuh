@@ -200,6 +200,13 @@ __device__ __forceinline__ void query_range(const AttnArgs& a, const AttnSeq& s,
   if (n1 <= n0 || hi <= lo) lo = hi = 0;
 }
 
+// The first query of a sequence that sees a key. The ones before it are used by
+// nobody: where a tile holds some beside others, they are cleared in shared
+// memory, since a probability of 0 times a NaN is a NaN.
+__device__ __forceinline__ int first_query(const AttnArgs& a, const AttnSeq& s) {
+  return a.causal ? max(0, s.qlen - s.klen) : 0;
+}
+
 // CW columns of a warp's 32 rows, thread = row, as 16-bit pairs w, to global
 // memory: row r (< n) at dst + r * ss. Through 64 CW bytes of shared memory `sm`
 // of the warp's own, so that a store instruction writes 32 / (CW / 8) rows'

@@ -6,7 +6,8 @@
 // OWN/4 x 16 holds a 4 x (tile/16) block of a product of two tiles: own rows
 // 4*ty.., streamed rows tx, tx + 16, ... Rows are padded by 4 floats, so the
 // 16-byte reads of eight neighbouring rows fall in different banks. Rows past
-// the sequence's end are zero in shared memory, whatever memory holds there.
+// the sequence's end are zero in shared memory, whatever memory holds there, and
+// so are queries before the first that sees a key.
 //
 // OWN is 64 where that gives a CTA for every SM, else 32: half the threads and
 // half the work of a CTA (100 rows of 4 heads of 64: dK and dV 35 us with
@@ -47,6 +48,21 @@ __device__ __forceinline__ void simt_load(float* dst, int tile, const HT& t, int
     for (int e = 0; e < VEC; e += 4)
       *reinterpret_cast<float4*>(dst + r * (D + 4) + x + e) =
           make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+  }
+}
+
+// Rows before `first` of such a tile become zeros: each thread clears what it
+// wrote itself. (2 x 1024 rows of 16/4 heads of 64, forward and backward: 738 us with
+// this bound inside simt_load, 735 with a call that is not inlined, 663 so, and 663
+// without.)
+template <typename T, int D, int THREADS>
+__device__ __forceinline__ void simt_clear(float* dst, int first) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  for (int c = threadIdx.x; c < first * (D / VEC); c += THREADS) {
+    const int r = c / (D / VEC), x = c % (D / VEC) * VEC;
+#pragma unroll
+    for (int e = 0; e < VEC; e += 4)
+      *reinterpret_cast<float4*>(dst + r * (D + 4) + x + e) = make_float4(0.f, 0.f, 0.f, 0.f);
   }
 }
 
@@ -344,6 +360,7 @@ __global__ void __launch_bounds__(4 * OWN) attn_simt_bwd_kernel(const AttnArgs a
       acc1[i][c] = 0.f;
       if (DKV) acc2[i][c] = 0.f;
     }
+  const int seen0 = DKV ? first_query(a, s) : 0;
   const int h1 = !DKV ? h / a.G : SPLIT ? h : h * a.G;
   for (int g = 0; g < (DKV && !SPLIT ? a.G : 1); ++g) {
     const int64_t stat = (int64_t)(DKV ? h1 + g : h) * a.R + s.stat0;
@@ -352,6 +369,10 @@ __global__ void __launch_bounds__(4 * OWN) attn_simt_bwd_kernel(const AttnArgs a
       __syncthreads();
       simt_load<T, D, THREADS>(str1, M, DKV ? a.q : a.k, s.b, h1 + g, strb + t0, nt);
       simt_load<T, D, THREADS>(str2, M, DKV ? a.dout : a.v, s.b, h1 + g, strb + t0, nt);
+      if (DKV && t0 < seen0) {
+        simt_clear<T, D, THREADS>(str1, seen0 - t0);
+        simt_clear<T, D, THREADS>(str2, seen0 - t0);
+      }
       __syncthreads();
       float x[4][NJ], y[4][NJ];
       simt_dot<D, NJ>(own1, str1, ty, tx, x);

@@ -390,11 +390,11 @@ __device__ __forceinline__ void copy_operand(const unsigned char* tile, int r, u
   tmem_wait_st();
 }
 
-// Rows [r0, 64) of an operand tile of 64 in shared memory become zeros, before
+// Rows [r0, r1) of an operand tile of 64 in shared memory become zeros, before
 // later products read them (128 threads).
 template <int D>
-__device__ __forceinline__ void zero_rows(unsigned char* tile, int r0) {
-  for (int c = threadIdx.x & 127; c < (64 - r0) * (D / 8); c += 128) {
+__device__ __forceinline__ void zero_rows(unsigned char* tile, int r0, int r1) {
+  for (int c = threadIdx.x & 127; c < (r1 - r0) * (D / 8); c += 128) {
     const int r = r0 + c / (D / 8), b = c % (D / 8);
     *reinterpret_cast<uint4*>(tile + (b / 8) * (64 * 128) + r * 128 + (b % 8) * 16) =
         make_uint4(0, 0, 0, 0);
