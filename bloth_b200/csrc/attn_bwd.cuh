@@ -386,21 +386,24 @@ __global__ void __launch_bounds__(352, 1)
       const int to = min(s.qlen, a.window ? key - off + a.window : s.qlen) - m0;
       const bool masked = m0 + BLK > s.qlen || s.klen == 1 || (a.causal && n0 + N - 1 - off > m0) ||
                           (a.window && n0 - off + a.window < m0 + BLK);
-      // rows of the block that nothing may be read from: before the first query that
-      // sees a key, and past the sequence's end where memory does hold some
-      const int front = max(0, seen0 - m0);
-      const int back = m0 + BLK > s.qlen && s.q0 + s.qlen < a.Sq ? s.qlen - m0 : BLK;
+      // the block has rows that nothing may be read from (it is masked then): before
+      // the first query that sees a key, or past the sequence's end where memory does
+      // hold some
+      const bool dead = m0 < seen0 || (m0 + BLK > s.qlen && s.q0 + s.qlen < a.Sq);
+      auto clear = [&](unsigned char* tile) {
+        if (m0 < seen0) zero_rows<D>(tile, 0, seen0 - m0);
+        if (m0 + BLK > s.qlen) zero_rows<D>(tile, s.qlen - m0, BLK);
+      };
       // the query that sees one key only; INT_MAX: all do, -1: none of the block
       const int alone = s.klen == 1 || a.window == 1 ? INT_MAX : a.causal ? -off - m0 : -1;
       if (masked) {
 #pragma unroll
         for (int i = 0; i < BLK; ++i)
           if (i < from || i >= to) x[i] = 0.f;
-        if (DV && (front > 0 || back < BLK)) {  // of dO; the block is masked then
+        if (DV && dead) {
           ok = __all_sync(0xffffffffu, bar_wait(bar.b_full + 8 * ost.at, ost.phase, waits));
           if (!ok) break;
-          zero_rows<D>(smem + C::B_OFF + ost.at * C::STRB, 0, front);
-          zero_rows<D>(smem + C::B_OFF + ost.at * C::STRB, back, BLK);
+          clear(smem + C::B_OFF + ost.at * C::STRB);
         }
       }
       if (DV) {
@@ -433,10 +436,7 @@ __global__ void __launch_bounds__(352, 1)
 #pragma unroll
           for (int i = 0; i < BLK; ++i)
             if (i < from || i >= to || i == alone || alone == INT_MAX) y[i] = 0.f;
-          if (front > 0 || back < BLK) {
-            zero_rows<D>(smem + C::A_OFF + st.at * C::STRB, 0, front);
-            zero_rows<D>(smem + C::A_OFF + st.at * C::STRB, back, BLK);
-          }
+          if (dead) clear(smem + C::A_OFF + st.at * C::STRB);
         }
         store64<T>(dp_at, y);
         if (FINE) store64_rest<T>(dp_at + 32, y);
@@ -673,9 +673,11 @@ __global__ void __launch_bounds__(352, 1)
 #pragma unroll
         for (int i = 0; i < BLK; ++i)
           if (i < from || i >= to) y[i] = 0.f;
-        // rows of K past the sequence's end that memory does hold
-        if (n0 + BLK > s.klen && s.k0 + s.klen < a.Sk)
-          zero_rows<D>(smem + C::A_OFF + (it % NA) * C::STRB, s.klen - n0, BLK);
+        // rows of K that nothing may be read from: before the first key that a query
+        // sees, and past the sequence's end where memory does hold some
+        unsigned char* kt = smem + C::A_OFF + (it % NA) * C::STRB;
+        if (n0 < first_key(a, s)) zero_rows<D>(kt, 0, first_key(a, s) - n0);
+        if (n0 + BLK > s.klen && s.k0 + s.klen < a.Sk) zero_rows<D>(kt, s.klen - n0, BLK);
       }
       store64<T>(dp_at, y);
       if (FINE) store64_rest<T>(dp_at + 32, y);

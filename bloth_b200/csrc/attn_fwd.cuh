@@ -26,10 +26,10 @@
 // Rows that see few keys (kFineKeys) have P as two terms, which take both
 // buffers: P of a block then waits for the product of the block before.
 //
-// Keys past the sequence's end are masked in S; their rows of V, which a
-// probability of 0 would turn into NaN if they hold an infinity, are zeroed
-// in shared memory by the groups (rows past the tensor's end are zero-filled
-// by the copy).
+// Keys past the sequence's end, or below every query's window, are masked in S;
+// their rows of V, which a probability of 0 would turn into NaN if they hold an
+// infinity, are zeroed in shared memory by the groups (rows past the tensor's
+// end are zero-filled by the copy).
 //
 // Bound at head_dim 128: the products. A block's for one tile take 392 cycles
 // with K (a step reads 6 KB of shared memory for 32 cycles of arithmetic) and
@@ -286,12 +286,16 @@ __global__ void __launch_bounds__(352, 1)
 #pragma unroll
         for (int i = 0; i < BLK; ++i)
           if (i >= hi || i < lo) x[i] = -INFINITY;
-        // rows of V past the sequence's end that memory does hold
-        if (n0 + BLK > s.klen && s.k0 + s.klen < a.Sk) {
+        // rows of V that nothing may be read from: before the first key that a query
+        // sees, and past the sequence's end where memory does hold some
+        const int seen0 = first_key(a, s);
+        if (n0 < seen0 || (n0 + BLK > s.klen && s.k0 + s.klen < a.Sk)) {
           const int it = j - b0, st = it % NST;
           ok = __all_sync(0xffffffffu, bar_wait(v_full + 8 * st, (uint32_t)(it / NST) & 1u, waits));
           if (!ok) break;
-          zero_rows<D>(smem + C::V_OFF + st * C::KB, s.klen - n0, BLK);
+          unsigned char* vt = smem + C::V_OFF + st * C::KB;
+          if (n0 < seen0) zero_rows<D>(vt, 0, seen0 - n0);
+          if (n0 + BLK > s.klen) zero_rows<D>(vt, s.klen - n0, BLK);
         }
       }
       float top[4] = {x[0], x[1], x[2], x[3]};

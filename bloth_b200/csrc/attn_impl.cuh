@@ -200,11 +200,14 @@ __device__ __forceinline__ void query_range(const AttnArgs& a, const AttnSeq& s,
   if (n1 <= n0 || hi <= lo) lo = hi = 0;
 }
 
-// The first query of a sequence that sees a key. The ones before it are used by
-// nobody: where a tile holds some beside others, they are cleared in shared
-// memory, since a probability of 0 times a NaN is a NaN.
+// The first query of a sequence that sees a key, and the first key that a query
+// sees. The ones before are used by nobody: where a tile holds some beside others,
+// they are cleared in shared memory, since a probability of 0 times a NaN is a NaN.
 __device__ __forceinline__ int first_query(const AttnArgs& a, const AttnSeq& s) {
   return a.causal ? max(0, s.qlen - s.klen) : 0;
+}
+__device__ __forceinline__ int first_key(const AttnArgs& a, const AttnSeq& s) {
+  return a.window ? max(0, s.klen - s.qlen - a.window + 1) : 0;
 }
 
 // CW columns of a warp's 32 rows, thread = row, as 16-bit pairs w, to global

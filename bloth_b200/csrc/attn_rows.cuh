@@ -14,7 +14,8 @@
 // of them, while the strip's share of HBM time is 0.2 us of an SM. Bound: HBM,
 // K and V once.
 //
-// Rows of K and V past the sequence's end are not read (zeros stand for them).
+// Rows of K and V past the sequence's end, or below every query's window, are
+// not read (zeros stand for them).
 #pragma once
 
 #include "attn_impl.cuh"
@@ -120,6 +121,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32)
   const int off = s.klen - s.qlen, rows = a.Sq * a.G;
   int lo, hi;
   key_range(a, s, 0, s.qlen, lo, hi);
+  const int seen0 = lo;  // the first key that a query sees
   lo = max(lo, split * pl.chunk) / kStrip * kStrip;
   hi = min(hi, (split + 1) * pl.chunk);
   const int strips = hi > lo ? (hi - lo + kStrip - 1) / kStrip : 0;
@@ -137,7 +139,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32)
 #pragma unroll
       for (int u = 0; u < kStrip * NC / 32; ++u) {
         const int x = u * 32 + lane, r = x / NC, c = x % NC;
-        const bool in = j0 + r < s.klen;
+        const bool in = j0 + r < s.klen && j0 + r >= seen0;
         const int64_t row = in ? j0 + r : j0;  // j0 < klen: a row of this sequence
         const uint32_t d = at + r * (D * 2) + ((c ^ (r & 7)) * 16);
         cp16(d, kb + row * a.k.ss + c * 8, in);

@@ -7,7 +7,8 @@
 // 4*ty.., streamed rows tx, tx + 16, ... Rows are padded by 4 floats, so the
 // 16-byte reads of eight neighbouring rows fall in different banks. Rows past
 // the sequence's end are zero in shared memory, whatever memory holds there, and
-// so are queries before the first that sees a key.
+// so are queries before the first that sees a key, and keys before the first
+// that a query sees.
 //
 // OWN is 64 where that gives a CTA for every SM, else 32: half the threads and
 // half the work of a CTA (100 rows of 4 heads of 64: dK and dV 35 us with
@@ -151,12 +152,12 @@ constexpr size_t simt_fwd_smem() {
 
 // One tile of keys for the own rows in qs: scores, running maximum m (natural
 // logarithm's units) and sum l, and acc += p V. `sees(i, j)`: whether own row i
-// sees key j of the tile.
+// sees key j of the tile; no query sees the first `front` (if positive).
 template <typename T, int D, int THREADS, typename Sees>
 __device__ __forceinline__ void simt_fwd_tile(const AttnArgs& a, const float* qs, float* ks,
-                                              float* ps, int b, int h, int r0, int nk, int ty,
-                                              int tx, float (&acc)[4][D / 16], float (&m)[4],
-                                              float (&l)[4], Sees sees) {
+                                              float* ps, int b, int h, int r0, int nk, int front,
+                                              int ty, int tx, float (&acc)[4][D / 16],
+                                              float (&m)[4], float (&l)[4], Sees sees) {
   constexpr int N = kSimtKeys, LP = N + 4;
   __syncthreads();
   simt_load<T, D, THREADS>(ks, N, a.k, b, h, r0, nk);
@@ -165,6 +166,7 @@ __device__ __forceinline__ void simt_fwd_tile(const AttnArgs& a, const float* qs
   simt_dot<D, 4>(qs, ks, ty, tx, x);
   __syncthreads();
   simt_load<T, D, THREADS>(ks, N, a.v, b, h, r0, nk);
+  if (front > 0) simt_clear<T, D, THREADS>(ks, front);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     float top = -INFINITY;
@@ -215,6 +217,7 @@ __global__ void __launch_bounds__(4 * OWN) attn_simt_fwd_kernel(const AttnArgs a
   const int rows = max(0, min(N, s.qlen - m0));
   int lo, hi;
   key_range(a, s, m0, m0 + rows, lo, hi);
+  const int seen0 = first_key(a, s);
   simt_load<T, D, THREADS>(qs, N, a.q, s.b, h, s.q0 + m0, rows);
   float acc[4][D / 16], m[4], l[4];
 #pragma unroll
@@ -226,7 +229,8 @@ __global__ void __launch_bounds__(4 * OWN) attn_simt_fwd_kernel(const AttnArgs a
   }
   for (int n0 = lo / kSimtKeys * kSimtKeys; n0 < hi; n0 += kSimtKeys)
     simt_fwd_tile<T, D, THREADS>(
-        a, qs, ks, ps, s.b, h / a.G, s.k0 + n0, min(kSimtKeys, s.klen - n0), ty, tx, acc, m, l,
+        a, qs, ks, ps, s.b, h / a.G, s.k0 + n0, min(kSimtKeys, s.klen - n0), seen0 - n0, ty,
+        tx, acc, m, l,
         [&](int i, int j) { return see_keys(a, s, m0 + i, n0 + j); });
   float f[4];
 #pragma unroll
@@ -264,6 +268,7 @@ __global__ void __launch_bounds__(4 * kSimtRows)
   const int rows = a.Sq * a.G;
   int lo, hi;
   key_range(a, s, 0, s.qlen, lo, hi);
+  const int seen0 = lo;  // the first key that a query sees
   lo = max(lo, split * pl.chunk) / kSimtKeys * kSimtKeys;
   hi = min(hi, (split + 1) * pl.chunk);
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
@@ -282,7 +287,7 @@ __global__ void __launch_bounds__(4 * kSimtRows)
   }
   for (int n0 = lo; n0 < hi; n0 += kSimtKeys)
     simt_fwd_tile<T, D, THREADS>(
-        a, qs, ks, ps, b, h, n0, min(kSimtKeys, s.klen - n0), ty, tx, acc, m, l,
+        a, qs, ks, ps, b, h, n0, min(kSimtKeys, s.klen - n0), seen0 - n0, ty, tx, acc, m, l,
         [&](int i, int j) { return i < rows && see_keys(a, s, i / a.G, n0 + j); });
   const int64_t part = ((int64_t)split * a.B * a.Hk + bh) * N;
 #pragma unroll
@@ -360,7 +365,7 @@ __global__ void __launch_bounds__(4 * OWN) attn_simt_bwd_kernel(const AttnArgs a
       acc1[i][c] = 0.f;
       if (DKV) acc2[i][c] = 0.f;
     }
-  const int seen0 = DKV ? first_query(a, s) : 0;
+  const int seen0 = DKV ? first_query(a, s) : first_key(a, s);
   const int h1 = !DKV ? h / a.G : SPLIT ? h : h * a.G;
   for (int g = 0; g < (DKV && !SPLIT ? a.G : 1); ++g) {
     const int64_t stat = (int64_t)(DKV ? h1 + g : h) * a.R + s.stat0;
@@ -369,7 +374,7 @@ __global__ void __launch_bounds__(4 * OWN) attn_simt_bwd_kernel(const AttnArgs a
       __syncthreads();
       simt_load<T, D, THREADS>(str1, M, DKV ? a.q : a.k, s.b, h1 + g, strb + t0, nt);
       simt_load<T, D, THREADS>(str2, M, DKV ? a.dout : a.v, s.b, h1 + g, strb + t0, nt);
-      if (DKV && t0 < seen0) {
+      if (t0 < seen0) {
         simt_clear<T, D, THREADS>(str1, seen0 - t0);
         simt_clear<T, D, THREADS>(str2, seen0 - t0);
       }

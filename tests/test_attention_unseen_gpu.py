@@ -1,5 +1,6 @@
 """What fused_attention must never use, though it lies inside a sequence: the
-query rows that see no key (causal, more queries than keys)."""
+query rows that see no key (causal, more queries than keys) and the keys that
+no query sees (below every row's window)."""
 import pytest
 import torch
 
@@ -58,3 +59,22 @@ def test_queries_before_the_first_key(cuda, dtype, D, bad, Sq, Sk):
 def test_queries_before_the_first_key_of_some_sequences(cuda, dtype, D):
     _run(cuda, dtype, D, 4, 200, 200, q_lens=[200, 150, 70, 5], k_lens=[137, 200, 1, 0])
     _run(cuda, dtype, D, 1, 300, 300, cu=[0, 100, 170, 300], cu_k=[0, 33, 200, 300])
+
+
+@pytest.mark.parametrize("dtype,D", TYPES)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("Sq,Sk,window", [(150, 333, 50), (300, 700, 5), (129, 200, 70),
+                                          (40, 500, 300)])
+def test_keys_below_every_window(cuda, dtype, D, bad, Sq, Sk, window):
+    _run(cuda, dtype, D, 2, Sq, Sk, window, bad=bad)
+
+
+@pytest.mark.parametrize("dtype,D", TYPES)
+@pytest.mark.parametrize("Sq,window", [(1, 7), (1, 300), (3, 100), (7, 1)])
+def test_cached_keys_below_the_window_of_a_few_rows(cuda, dtype, D, Sq, window):
+    _run(cuda, dtype, D, 3, Sq, 900, window, k_lens=[900, 333, 650], backward=Sq == 3)
+
+
+@pytest.mark.parametrize("dtype,D", TYPES)
+def test_keys_below_every_window_of_packed_sequences(cuda, dtype, D):
+    _run(cuda, dtype, D, 1, 400, 900, 30, cu=[0, 10, 200, 400], cu_k=[0, 200, 600, 900])
