@@ -16,7 +16,7 @@
 // P^T, dS^T and dS are rounded to the tensors' type and stay in tensor memory,
 // where S^T and dP lay, as the products' first operand; the streamed tiles are
 // read by the products both by rows and by columns, so nothing is transposed
-// or stored again. (Rows that see few keys, kFineKeys: as two terms, in the two
+// or stored again. (Tiles of few keys, kFineKeys: as two terms, in the two
 // halves of where S^T and dP lay.) Blocks alternate between two buffers of S and of dP in
 // tensor memory and two groups of four warps (thread = row of the kept tile,
 // 64 columns): a group has two blocks' time for its own, so neither the
@@ -161,7 +161,7 @@ __device__ __forceinline__ void store_sums(uint32_t at, float f, T* dst, int64_t
 }
 
 // ------------------------------------------------------------------ dK, dV
-template <typename T, int D, int SUMS, bool FINE>
+template <typename T, int D, int SUMS>
 __global__ void __launch_bounds__(352, 1)
     attn_dkv_kernel(const AttnArgs a, const __grid_constant__ BwdMaps maps) {
   using C = BwdCfg<D, SUMS>;
@@ -189,6 +189,7 @@ __global__ void __launch_bounds__(352, 1)
   query_range(a, s, n0, min(n0 + N, s.klen), lo, hi);
   const int mb = lo / BLK, nm = hi > lo ? (hi + BLK - 1) / BLK - mb : 0;  // blocks per head
   const int total = nm * a.G;
+  const bool fine = few_keys(a, s, hi);
 
   if (warp == 8) {
     tmem_alloc(tmem_ptr, C::COLS);
@@ -244,40 +245,45 @@ __global__ void __launch_bounds__(352, 1)
       Ring<2> buf, pbuf;
       bool ok = bar_wait(OWN_TMEM ? bar.there : bar.own, 0, waits);
       tc_fence_after();
-      for (int j = 0; ok && j < total + 2; ++j) {
-        if (j >= 2) {
-          ok = (!DV || bar_wait(bar.b_full + 8 * ost.at, ost.phase, waits)) &&
-               bar_wait(bar.p_full + 8 * pbuf.at, pbuf.phase, waits);
-          if (!ok) break;
-          tc_fence_after();
-          if (DV && lead) {
-            const uint32_t p = tmem + C::S_COL + pbuf.at * BLK;
-            const uint32_t ot = base + C::B_OFF + ost.at * C::STRB;
-            product_cols<T, D>(tmem + DV_COL, p, ot, j > 2);
-            if (FINE) product_cols<T, D>(tmem + DV_COL, p + 32, ot, true);
-            mma_commit(bar.b_free + 8 * ost.at);
-            // Q and the statistics went into P^T, which this product has read
-            if (!DK) mma_commit(bar.a_free + 8 * qold.at);
+      auto steps = [&](auto few) {
+        constexpr bool FINE = decltype(few)::value;
+        for (int j = 0; ok && j < total + 2; ++j) {
+          if (j >= 2) {
+            ok = (!DV || bar_wait(bar.b_full + 8 * ost.at, ost.phase, waits)) &&
+                 bar_wait(bar.p_full + 8 * pbuf.at, pbuf.phase, waits);
+            if (!ok) break;
+            tc_fence_after();
+            if (DV && lead) {
+              const uint32_t p = tmem + C::S_COL + pbuf.at * BLK;
+              const uint32_t ot = base + C::B_OFF + ost.at * C::STRB;
+              product_cols<T, D>(tmem + DV_COL, p, ot, j > 2);
+              if (FINE) product_cols<T, D>(tmem + DV_COL, p + 32, ot, true);
+              mma_commit(bar.b_free + 8 * ost.at);
+              // Q and the statistics went into P^T, which this product has read
+              if (!DK) mma_commit(bar.a_free + 8 * qold.at);
+            }
+            ost.next();
+            qold.next();
+            pbuf.next();
           }
-          ost.next();
-          qold.next();
-          pbuf.next();
-        }
-        if (j < total) {
-          ok = bar_wait(bar.a_full + 8 * qst.at, qst.phase, waits);
-          if (!ok) break;
-          if (lead) {
-            const uint32_t qt = base + C::A_OFF + qst.at * C::STRB;
-            if constexpr (OWN_TMEM)
-              product_rows_ts<T, D>(tmem + C::S_COL + buf.at * BLK, tmem + K_COL, qt);
-            else
-              product_rows<T, D>(tmem + C::S_COL + buf.at * BLK, ka, qt);
-            mma_commit(bar.s_full + 8 * buf.at);
+          if (j < total) {
+            ok = bar_wait(bar.a_full + 8 * qst.at, qst.phase, waits);
+            if (!ok) break;
+            if (lead) {
+              const uint32_t qt = base + C::A_OFF + qst.at * C::STRB;
+              if constexpr (OWN_TMEM)
+                product_rows_ts<T, D>(tmem + C::S_COL + buf.at * BLK, tmem + K_COL, qt);
+              else
+                product_rows<T, D>(tmem + C::S_COL + buf.at * BLK, ka, qt);
+              mma_commit(bar.s_full + 8 * buf.at);
+            }
+            qst.next();
+            buf.next();
           }
-          qst.next();
-          buf.next();
         }
-      }
+      };
+      if (fine) steps(std::true_type{});
+      else steps(std::false_type{});
       if (lead && (DV || !ok)) {
         mma_commit(ok ? bar.acc : bar.drained);
         if (!ok) bar_drain(bar.drained, 0, waits);
@@ -294,38 +300,43 @@ __global__ void __launch_bounds__(352, 1)
       Ring<2> buf, dbuf;
       bool ok = bar_wait(OWN_TMEM ? bar.there : bar.own, 0, waits);
       tc_fence_after();
-      for (int j = 0; ok && j < total + 2; ++j) {
-        if (j >= 2) {
-          ok = bar_wait(bar.a_full + 8 * qst.at, qst.phase, waits) &&
-               bar_wait(bar.ds_full + 8 * dbuf.at, dbuf.phase, waits);
-          if (!ok) break;
-          tc_fence_after();
-          if (lead) {
-            const uint32_t ds = tmem + C::DP_COL + dbuf.at * BLK;
-            const uint32_t qt = base + C::A_OFF + qst.at * C::STRB;
-            product_cols<T, D>(tmem + DK_COL, ds, qt, j > 2);
-            if (FINE) product_cols<T, D>(tmem + DK_COL, ds + 32, qt, true);
-            mma_commit(bar.a_free + 8 * qst.at);
+      auto steps = [&](auto few) {
+        constexpr bool FINE = decltype(few)::value;
+        for (int j = 0; ok && j < total + 2; ++j) {
+          if (j >= 2) {
+            ok = bar_wait(bar.a_full + 8 * qst.at, qst.phase, waits) &&
+                 bar_wait(bar.ds_full + 8 * dbuf.at, dbuf.phase, waits);
+            if (!ok) break;
+            tc_fence_after();
+            if (lead) {
+              const uint32_t ds = tmem + C::DP_COL + dbuf.at * BLK;
+              const uint32_t qt = base + C::A_OFF + qst.at * C::STRB;
+              product_cols<T, D>(tmem + DK_COL, ds, qt, j > 2);
+              if (FINE) product_cols<T, D>(tmem + DK_COL, ds + 32, qt, true);
+              mma_commit(bar.a_free + 8 * qst.at);
+            }
+            qst.next();
+            dbuf.next();
           }
-          qst.next();
-          dbuf.next();
-        }
-        if (j < total) {
-          ok = bar_wait(bar.b_full + 8 * ost.at, ost.phase, waits);
-          if (!ok) break;
-          if (lead) {
-            const uint32_t ot = base + C::B_OFF + ost.at * C::STRB;
-            if constexpr (OWN_TMEM)
-              product_rows_ts<T, D>(tmem + C::DP_COL + buf.at * BLK, tmem + V_COL, ot);
-            else
-              product_rows<T, D>(tmem + C::DP_COL + buf.at * BLK, va, ot);
-            mma_commit(bar.dp_full + 8 * buf.at);
-            mma_commit(bar.b_free + 8 * ost.at);
+          if (j < total) {
+            ok = bar_wait(bar.b_full + 8 * ost.at, ost.phase, waits);
+            if (!ok) break;
+            if (lead) {
+              const uint32_t ot = base + C::B_OFF + ost.at * C::STRB;
+              if constexpr (OWN_TMEM)
+                product_rows_ts<T, D>(tmem + C::DP_COL + buf.at * BLK, tmem + V_COL, ot);
+              else
+                product_rows<T, D>(tmem + C::DP_COL + buf.at * BLK, va, ot);
+              mma_commit(bar.dp_full + 8 * buf.at);
+              mma_commit(bar.b_free + 8 * ost.at);
+            }
+            ost.next();
+            buf.next();
           }
-          ost.next();
-          buf.next();
         }
-      }
+      };
+      if (fine) steps(std::true_type{});
+      else steps(std::false_type{});
       if (lead) {
         mma_commit(ok ? bar.acc : bar.drained + 8);
         if (!ok) bar_drain(bar.drained + 8, 0, waits);
@@ -362,97 +373,103 @@ __global__ void __launch_bounds__(352, 1)
         if (lane == 0) bar_arrive(bar.there);
       }
     }
-    for (int it = group; ok && it < total; it += 2, ph ^= 1u) {
-      const int m0 = (mb + mi) * BLK;
-      const float* stat = reinterpret_cast<const float*>(smem + C::STAT_OFF + st.at * 512);
-      ok = bar_wait(bar.a_full + 8 * st.at, st.phase, waits) &&
-           bar_wait(bar.s_full + 8 * group, ph, waits);
-      if (!(ok = __all_sync(0xffffffffu, ok))) break;
-      tc_fence_after();
-      float x[BLK];
-      load64(s_at, x);
-#pragma unroll
-      for (int i = 0; i < BLK; i += 4) {
-        const float4 l = *reinterpret_cast<const float4*>(stat + i);
-        const float2 u = f2_fma(f2(x[i], x[i + 1]), sc, f2(-l.x, -l.y));
-        const float2 w = f2_fma(f2(x[i + 2], x[i + 3]), sc, f2(-l.z, -l.w));
-        x[i] = ex2(u.x);
-        x[i + 1] = ex2(u.y);
-        x[i + 2] = ex2(w.x);
-        x[i + 3] = ex2(w.y);
-      }
-      // the block's columns that see this thread's key: [from, to)
-      const int from = a.causal ? key - off - m0 : 0;
-      const int to = min(s.qlen, a.window ? key - off + a.window : s.qlen) - m0;
-      const bool masked = m0 + BLK > s.qlen || s.klen == 1 || (a.causal && n0 + N - 1 - off > m0) ||
-                          (a.window && n0 - off + a.window < m0 + BLK);
-      // the block has rows that nothing may be read from (it is masked then): before
-      // the first query that sees a key, or past the sequence's end where memory does
-      // hold some
-      const bool dead = m0 < seen0 || (m0 + BLK > s.qlen && s.q0 + s.qlen < a.Sq);
-      auto clear = [&](unsigned char* tile) {
-        if (m0 < seen0) zero_rows<D>(tile, 0, seen0 - m0);
-        if (m0 + BLK > s.qlen) zero_rows<D>(tile, s.qlen - m0, BLK);
-      };
-      // the query that sees one key only; INT_MAX: all do, -1: none of the block
-      const int alone = s.klen == 1 || a.window == 1 ? INT_MAX : a.causal ? -off - m0 : -1;
-      if (masked) {
-#pragma unroll
-        for (int i = 0; i < BLK; ++i)
-          if (i < from || i >= to) x[i] = 0.f;
-        if (DV && dead) {
-          ok = __all_sync(0xffffffffu, bar_wait(bar.b_full + 8 * ost.at, ost.phase, waits));
-          if (!ok) break;
-          clear(smem + C::B_OFF + ost.at * C::STRB);
-        }
-      }
-      if (DV) {
-        store64<T>(s_at, x);
-        if (FINE) store64_rest<T>(s_at + 32, x);
-      }
-      const bool there = !DK || bar_test(bar.dp_full + 8 * group, ph);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) bar_arrive(bar.p_full + 8 * group);
-      ok = __all_sync(0xffffffffu, there || bar_wait(bar.dp_full + 8 * group, ph, waits));
-      if (!ok) break;
-      tc_fence_after();
-      if constexpr (DK) {
-        float y[BLK];
-        load64(dp_at, y);
+    auto blocks = [&](auto few) {  // two loops: as in the forward
+      constexpr bool FINE = decltype(few)::value;
+      for (int it = group; ok && it < total; it += 2, ph ^= 1u) {
+        const int m0 = (mb + mi) * BLK;
+        const float* stat = reinterpret_cast<const float*>(smem + C::STAT_OFF + st.at * 512);
+        ok = bar_wait(bar.a_full + 8 * st.at, st.phase, waits) &&
+             bar_wait(bar.s_full + 8 * group, ph, waits);
+        if (!(ok = __all_sync(0xffffffffu, ok))) break;
+        tc_fence_after();
+        float x[BLK];
+        load64(s_at, x);
 #pragma unroll
         for (int i = 0; i < BLK; i += 4) {
-          const float4 d = *reinterpret_cast<const float4*>(stat + 64 + i);
-          const float2 u = f2_mul(f2(x[i], x[i + 1]), f2_add(f2(y[i], y[i + 1]), f2(-d.x, -d.y)));
-          const float2 w =
-              f2_mul(f2(x[i + 2], x[i + 3]), f2_add(f2(y[i + 2], y[i + 3]), f2(-d.z, -d.w)));
-          y[i] = u.x;
-          y[i + 1] = u.y;
-          y[i + 2] = w.x;
-          y[i + 3] = w.y;
+          const float4 l = *reinterpret_cast<const float4*>(stat + i);
+          const float2 u = f2_fma(f2(x[i], x[i + 1]), sc, f2(-l.x, -l.y));
+          const float2 w = f2_fma(f2(x[i + 2], x[i + 3]), sc, f2(-l.z, -l.w));
+          x[i] = ex2(u.x);
+          x[i + 1] = ex2(u.y);
+          x[i + 2] = ex2(w.x);
+          x[i + 3] = ex2(w.y);
         }
+        // the block's columns that see this thread's key: [from, to)
+        const int from = a.causal ? key - off - m0 : 0;
+        const int to = min(s.qlen, a.window ? key - off + a.window : s.qlen) - m0;
+        const bool masked = m0 + BLK > s.qlen || s.klen == 1 ||
+                            (a.causal && n0 + N - 1 - off > m0) ||
+                            (a.window && n0 - off + a.window < m0 + BLK);
+        // the block has rows that nothing may be read from (it is masked then): before
+        // the first query that sees a key, or past the sequence's end where memory does
+        // hold some
+        const bool dead = m0 < seen0 || (m0 + BLK > s.qlen && s.q0 + s.qlen < a.Sq);
+        auto clear = [&](unsigned char* tile) {
+          if (m0 < seen0) zero_rows<D>(tile, 0, seen0 - m0);
+          if (m0 + BLK > s.qlen) zero_rows<D>(tile, s.qlen - m0, BLK);
+        };
+        // the query that sees one key only; INT_MAX: all do, -1: none of the block
+        const int alone = s.klen == 1 || a.window == 1 ? INT_MAX : a.causal ? -off - m0 : -1;
         if (masked) {
 #pragma unroll
           for (int i = 0; i < BLK; ++i)
-            if (i < from || i >= to || i == alone || alone == INT_MAX) y[i] = 0.f;
-          if (dead) clear(smem + C::A_OFF + st.at * C::STRB);
+            if (i < from || i >= to) x[i] = 0.f;
+          if (DV && dead) {
+            ok = __all_sync(0xffffffffu, bar_wait(bar.b_full + 8 * ost.at, ost.phase, waits));
+            if (!ok) break;
+            clear(smem + C::B_OFF + ost.at * C::STRB);
+          }
         }
-        store64<T>(dp_at, y);
-        if (FINE) store64_rest<T>(dp_at + 32, y);
+        if (DV) {
+          store64<T>(s_at, x);
+          if (FINE) store64_rest<T>(s_at + 32, x);
+        }
+        const bool there = !DK || bar_test(bar.dp_full + 8 * group, ph);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) bar_arrive(bar.ds_full + 8 * group);
+        if (lane == 0) bar_arrive(bar.p_full + 8 * group);
+        ok = __all_sync(0xffffffffu, there || bar_wait(bar.dp_full + 8 * group, ph, waits));
+        if (!ok) break;
+        tc_fence_after();
+        if constexpr (DK) {
+          float y[BLK];
+          load64(dp_at, y);
+#pragma unroll
+          for (int i = 0; i < BLK; i += 4) {
+            const float4 d = *reinterpret_cast<const float4*>(stat + 64 + i);
+            const float2 u = f2_mul(f2(x[i], x[i + 1]), f2_add(f2(y[i], y[i + 1]), f2(-d.x, -d.y)));
+            const float2 w =
+                f2_mul(f2(x[i + 2], x[i + 3]), f2_add(f2(y[i + 2], y[i + 3]), f2(-d.z, -d.w)));
+            y[i] = u.x;
+            y[i + 1] = u.y;
+            y[i + 2] = w.x;
+            y[i + 3] = w.y;
+          }
+          if (masked) {
+#pragma unroll
+            for (int i = 0; i < BLK; ++i)
+              if (i < from || i >= to || i == alone || alone == INT_MAX) y[i] = 0.f;
+            if (dead) clear(smem + C::A_OFF + st.at * C::STRB);
+          }
+          store64<T>(dp_at, y);
+          if (FINE) store64_rest<T>(dp_at + 32, y);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) bar_arrive(bar.ds_full + 8 * group);
+        }
+        st.next();
+        st.next();
+        ost.next();
+        ost.next();
+        mi += 2;
+        if (mi >= nm) mi -= nm;
+        if (mi >= nm) mi -= nm;  // nm == 1
       }
-      st.next();
-      st.next();
-      ost.next();
-      ost.next();
-      mi += 2;
-      if (mi >= nm) mi -= nm;
-      if (mi >= nm) mi -= nm;  // nm == 1
-    }
+    };
+    if (fine) blocks(std::true_type{});
+    else blocks(std::false_type{});
     if (ok && total > 0) {
       ok = __all_sync(0xffffffffu, bar_wait(bar.acc, 0, waits));
       tc_fence_after();
@@ -479,7 +496,7 @@ __global__ void __launch_bounds__(352, 1)
 }
 
 // ---------------------------------------------------------------------- dQ
-template <typename T, int D, bool FINE>
+template <typename T, int D>
 __global__ void __launch_bounds__(352, 1)
     attn_dq_kernel(const AttnArgs a, const __grid_constant__ BwdMaps maps) {
   using C = BwdCfg<D, kSumDQ>;
@@ -505,6 +522,7 @@ __global__ void __launch_bounds__(352, 1)
   int lo, hi;
   key_range(a, s, m0, min(m0 + N, s.qlen), lo, hi);
   const int b0 = lo / BLK, total = hi > lo ? (hi + BLK - 1) / BLK - b0 : 0;
+  const bool fine = few_keys(a, s, min(m0 + N, s.qlen));
 
   if (warp == 8) {
     tmem_alloc(tmem_ptr, C::COLS);
@@ -581,38 +599,44 @@ __global__ void __launch_bounds__(352, 1)
       Ring<2> buf, dbuf;
       bool ok = bar_wait(OWN_TMEM ? bar.there : bar.own, 0, waits);
       tc_fence_after();
-      for (int j = 0; ok && j < total + 2; ++j) {
-        if (j >= 2) {
-          ok = bar_wait(bar.a_full + 8 * kst.at, kst.phase, waits) &&
-               bar_wait(bar.ds_full + 8 * dbuf.at, dbuf.phase, waits);
-          if (!ok) break;
-          tc_fence_after();
-          if (lead) {
-            const uint32_t ds = tmem + C::DP_COL + dbuf.at * BLK;
-            const uint32_t kt = base + C::A_OFF + kst.at * C::STRB;
-            product_cols<T, D>(tmem + C::ACC_COL, ds, kt, j > 2);
-            if (FINE) product_cols<T, D>(tmem + C::ACC_COL, ds + 32, kt, true);
-            mma_commit(bar.a_free + 8 * kst.at);
+      auto steps = [&](auto few) {
+        constexpr bool FINE = decltype(few)::value;
+        for (int j = 0; ok && j < total + 2; ++j) {
+          if (j >= 2) {
+            ok = bar_wait(bar.a_full + 8 * kst.at, kst.phase, waits) &&
+                 bar_wait(bar.ds_full + 8 * dbuf.at, dbuf.phase, waits);
+            if (!ok) break;
+            tc_fence_after();
+            if (lead) {
+              const uint32_t ds = tmem + C::DP_COL + dbuf.at * BLK;
+              const uint32_t kt = base + C::A_OFF + kst.at * C::STRB;
+              product_cols<T, D>(tmem + C::ACC_COL, ds, kt, j > 2);
+              if (FINE) product_cols<T, D>(tmem + C::ACC_COL, ds + 32, kt, true);
+              mma_commit(bar.a_free + 8 * kst.at);
+            }
+            kst.next();
+            dbuf.next();
           }
-          kst.next();
-          dbuf.next();
-        }
-        if (j < total) {
-          ok = bar_wait(bar.b_full + 8 * vst.at, vst.phase, waits);
-          if (!ok) break;
-          if (lead) {
-            const uint32_t vt = base + C::B_OFF + vst.at * C::STRB;
-            if constexpr (OWN_TMEM)
-              product_rows_ts<T, D>(tmem + C::DP_COL + buf.at * BLK, tmem + O_COL, vt);
-            else
-              product_rows<T, D>(tmem + C::DP_COL + buf.at * BLK, base + C::OWN_OFF + C::OWNB, vt);
-            mma_commit(bar.dp_full + 8 * buf.at);
-            mma_commit(bar.b_free + 8 * vst.at);
+          if (j < total) {
+            ok = bar_wait(bar.b_full + 8 * vst.at, vst.phase, waits);
+            if (!ok) break;
+            if (lead) {
+              const uint32_t vt = base + C::B_OFF + vst.at * C::STRB;
+              if constexpr (OWN_TMEM)
+                product_rows_ts<T, D>(tmem + C::DP_COL + buf.at * BLK, tmem + O_COL, vt);
+              else
+                product_rows<T, D>(tmem + C::DP_COL + buf.at * BLK, base + C::OWN_OFF + C::OWNB,
+                                   vt);
+              mma_commit(bar.dp_full + 8 * buf.at);
+              mma_commit(bar.b_free + 8 * vst.at);
+            }
+            vst.next();
+            buf.next();
           }
-          vst.next();
-          buf.next();
         }
-      }
+      };
+      if (fine) steps(std::true_type{});
+      else steps(std::false_type{});
       if (lead) {
         mma_commit(ok ? bar.acc : bar.drained + 8);
         if (!ok) bar_drain(bar.drained + 8, 0, waits);
@@ -641,51 +665,56 @@ __global__ void __launch_bounds__(352, 1)
         if (lane == 0) bar_arrive(bar.there);
       }
     }
-    for (int it = group; ok && it < total; it += 2, ph ^= 1u) {
-      const int n0 = (b0 + it) * BLK;
-      ok = __all_sync(0xffffffffu, bar_wait(bar.s_full + 8 * group, ph, waits));
-      if (!ok) break;
-      tc_fence_after();
-      float x[BLK], y[BLK];
-      load64(s_at, x);
-      const bool there = bar_test(bar.dp_full + 8 * group, ph);
+    auto blocks = [&](auto few) {  // two loops: as in the forward
+      constexpr bool FINE = decltype(few)::value;
+      for (int it = group; ok && it < total; it += 2, ph ^= 1u) {
+        const int n0 = (b0 + it) * BLK;
+        ok = __all_sync(0xffffffffu, bar_wait(bar.s_full + 8 * group, ph, waits));
+        if (!ok) break;
+        tc_fence_after();
+        float x[BLK], y[BLK];
+        load64(s_at, x);
+        const bool there = bar_test(bar.dp_full + 8 * group, ph);
 #pragma unroll
-      for (int i = 0; i < BLK; i += 2) {
-        const float2 u = f2_fma(f2(x[i], x[i + 1]), sc, lse2);
-        x[i] = ex2(u.x);
-        x[i + 1] = ex2(u.y);
-      }
-      ok = __all_sync(0xffffffffu, there || bar_wait(bar.dp_full + 8 * group, ph, waits));
-      if (!ok) break;
-      tc_fence_after();
-      load64(dp_at, y);
+        for (int i = 0; i < BLK; i += 2) {
+          const float2 u = f2_fma(f2(x[i], x[i + 1]), sc, lse2);
+          x[i] = ex2(u.x);
+          x[i + 1] = ex2(u.y);
+        }
+        ok = __all_sync(0xffffffffu, there || bar_wait(bar.dp_full + 8 * group, ph, waits));
+        if (!ok) break;
+        tc_fence_after();
+        load64(dp_at, y);
 #pragma unroll
-      for (int i = 0; i < BLK; i += 2) {
-        const float2 d = f2_mul(f2(x[i], x[i + 1]), f2_add(f2(y[i], y[i + 1]), delta));
-        y[i] = d.x;
-        y[i + 1] = d.y;
-      }
-      if (n0 + BLK > s.klen || (a.causal && n0 + BLK - 1 > m0 + off) ||
-          (a.window && n0 <= m0 + N - 1 + off - a.window)) {
-        const int to = (a.causal ? min(s.klen, row + off + 1) : s.klen) - n0;
-        int from = a.window ? row + off - a.window + 1 - n0 : 0;
-        if (sees_one(a, s, row)) from = BLK;
+        for (int i = 0; i < BLK; i += 2) {
+          const float2 d = f2_mul(f2(x[i], x[i + 1]), f2_add(f2(y[i], y[i + 1]), delta));
+          y[i] = d.x;
+          y[i + 1] = d.y;
+        }
+        if (n0 + BLK > s.klen || (a.causal && n0 + BLK - 1 > m0 + off) ||
+            (a.window && n0 <= m0 + N - 1 + off - a.window)) {
+          const int to = (a.causal ? min(s.klen, row + off + 1) : s.klen) - n0;
+          int from = a.window ? row + off - a.window + 1 - n0 : 0;
+          if (sees_one(a, s, row)) from = BLK;
 #pragma unroll
-        for (int i = 0; i < BLK; ++i)
-          if (i < from || i >= to) y[i] = 0.f;
-        // rows of K that nothing may be read from: before the first key that a query
-        // sees, and past the sequence's end where memory does hold some
-        unsigned char* kt = smem + C::A_OFF + (it % NA) * C::STRB;
-        if (n0 < first_key(a, s)) zero_rows<D>(kt, 0, first_key(a, s) - n0);
-        if (n0 + BLK > s.klen && s.k0 + s.klen < a.Sk) zero_rows<D>(kt, s.klen - n0, BLK);
+          for (int i = 0; i < BLK; ++i)
+            if (i < from || i >= to) y[i] = 0.f;
+          // rows of K that nothing may be read from: before the first key that a query
+          // sees, and past the sequence's end where memory does hold some
+          unsigned char* kt = smem + C::A_OFF + (it % NA) * C::STRB;
+          if (n0 < first_key(a, s)) zero_rows<D>(kt, 0, first_key(a, s) - n0);
+          if (n0 + BLK > s.klen && s.k0 + s.klen < a.Sk) zero_rows<D>(kt, s.klen - n0, BLK);
+        }
+        store64<T>(dp_at, y);
+        if (FINE) store64_rest<T>(dp_at + 32, y);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(bar.ds_full + 8 * group);
       }
-      store64<T>(dp_at, y);
-      if (FINE) store64_rest<T>(dp_at + 32, y);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) bar_arrive(bar.ds_full + 8 * group);
-    }
+    };
+    if (fine) blocks(std::true_type{});
+    else blocks(std::false_type{});
     if (ok && total > 0) {
       ok = __all_sync(0xffffffffu, bar_wait(bar.acc, 0, waits));
       tc_fence_after();
@@ -706,7 +735,7 @@ __global__ void __launch_bounds__(352, 1)
   if (warp == 8) tmem_free(tmem, C::COLS);
 }
 
-template <typename T, int D, bool FINE>
+template <typename T, int D>
 int launch_attn_bwd(const AttnArgs& a0, cudaStream_t st) {
   AttnArgs a = a0;
   a.fault = fault_word();
@@ -736,7 +765,7 @@ int launch_attn_bwd(const AttnArgs& a0, cudaStream_t st) {
   auto keys = [&](auto sums) {
     constexpr int S = decltype(sums)::value;
     using C = BwdCfg<D, S>;
-    return run(attn_dkv_kernel<T, D, S, FINE>, C::SMEM, C::THREADS,
+    return run(attn_dkv_kernel<T, D, S>, C::SMEM, C::THREADS,
                attn_tiles(a.Sk, a.packed, C::TILE) * a.Hk * a.B);
   };
   if (a.dk.p != nullptr) {
@@ -749,7 +778,7 @@ int launch_attn_bwd(const AttnArgs& a0, cudaStream_t st) {
   }
   if (rc == BLOTH_OK && a.dq.p != nullptr) {
     using C = BwdCfg<D, kSumDQ>;
-    rc = run(attn_dq_kernel<T, D, FINE>, C::SMEM, C::THREADS,
+    rc = run(attn_dq_kernel<T, D>, C::SMEM, C::THREADS,
              attn_tiles(a.Sq, a.packed, C::TILE) * a.Hq * a.B);
   }
   return rc;

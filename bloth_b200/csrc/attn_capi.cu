@@ -72,7 +72,6 @@ int fill_common(AttnArgs& a, const void* q_seq, const void* k_seq, int seq_dtype
   a.scale_log2 = scale * kLog2e;
   a.causal = causal ? 1 : 0;
   a.window = window > kMaxSeq ? 0 : (int)window;  // wider than any sequence: no window
-  a.fine = a.Sk <= kFineKeys || (a.window > 0 && a.window <= kFineKeys);
   a.fault = nullptr;
   return BLOTH_OK;
 }

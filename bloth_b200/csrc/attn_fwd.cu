@@ -7,7 +7,7 @@ template <typename T>
 int attn_tc_fwd(const AttnArgs& a, int D, cudaStream_t st) {
   return attn_head_dim(D, [&](auto dd) {
     constexpr int DD = decltype(dd)::value;
-    return a.fine ? launch_attn_fwd<T, DD, true>(a, st) : launch_attn_fwd<T, DD, false>(a, st);
+    return launch_attn_fwd<T, DD>(a, st);
   });
 }
 template int attn_tc_fwd<__nv_bfloat16>(const AttnArgs&, int, cudaStream_t);

@@ -23,7 +23,7 @@
 // product). Until then p is at most 2^8, which costs no precision: p is
 // rounded relative to its own size, and sums are fp32.
 //
-// Rows that see few keys (kFineKeys) have P as two terms, which take both
+// Tiles whose rows see few keys (kFineKeys) have P as two terms, which take both
 // buffers: P of a block then waits for the product of the block before.
 //
 // Keys past the sequence's end, or below every query's window, are masked in S;
@@ -73,7 +73,7 @@ struct FwdMaps {
   CUtensorMap q, k, v;
 };
 
-template <typename T, int D, bool FINE>
+template <typename T, int D>
 __global__ void __launch_bounds__(352, 1)
     attn_fwd_kernel(const AttnArgs a, const __grid_constant__ FwdMaps maps) {
   using C = FwdCfg<D>;
@@ -195,46 +195,52 @@ __global__ void __launch_bounds__(352, 1)
       tc_fence_after();
       // step j: S of block j, then O of block j - 1; of the CTA's blocks [f, e)
       // are this tile's
-      for (int j = 0; ok && j <= nb; ++j) {
-        if (j < nb) {
-          const bool mine = j >= f && j < e;
-          ok = bar_wait(k_full + 8 * kst.at, kst.phase, waits);
-          if (ok && mine && j > f) ok = bar_wait(s_read + 8 * t, (uint32_t)(j - f - 1) & 1u, waits);
-          if (!ok) break;
-          tc_fence_after();
-          if (lead) {
-            if (mine) {
-              const uint32_t kt = base + C::K_OFF + kst.at * C::KB;
-              if constexpr (C::Q_TMEM)
-                product_rows_ts<T, D>(s_at, tmem + C::Q_COL + t * (D / 2), kt);
-              else
-                product_rows<T, D>(s_at, qa, kt);
-              mma_commit(s_full + 8 * t);
+      auto steps = [&](auto few) {
+        constexpr bool FINE = decltype(few)::value;
+        for (int j = 0; ok && j <= nb; ++j) {
+          if (j < nb) {
+            const bool mine = j >= f && j < e;
+            ok = bar_wait(k_full + 8 * kst.at, kst.phase, waits);
+            if (ok && mine && j > f)
+              ok = bar_wait(s_read + 8 * t, (uint32_t)(j - f - 1) & 1u, waits);
+            if (!ok) break;
+            tc_fence_after();
+            if (lead) {
+              if (mine) {
+                const uint32_t kt = base + C::K_OFF + kst.at * C::KB;
+                if constexpr (C::Q_TMEM)
+                  product_rows_ts<T, D>(s_at, tmem + C::Q_COL + t * (D / 2), kt);
+                else
+                  product_rows<T, D>(s_at, qa, kt);
+                mma_commit(s_full + 8 * t);
+              }
+              // (a commit completes with the products before it, if there are any)
+              mma_commit(k_free + 8 * kst.at);
             }
-            // (a commit completes with the products before it, if there are any)
-            mma_commit(k_free + 8 * kst.at);
+            kst.next();
           }
-          kst.next();
-        }
-        if (j > 0) {
-          const bool mine = j - 1 >= f && j - 1 < e;
-          ok = bar_wait(v_full + 8 * vst.at, vst.phase, waits);
-          if (ok && mine) ok = bar_wait(p_full + 16 * t + 8 * pb.at, pb.phase, waits);
-          if (!ok) break;
-          tc_fence_after();
-          if (lead) {
-            if (mine) {
-              const uint32_t vt = base + C::V_OFF + vst.at * C::KB;
-              product_cols<T, D>(o_at, s_at + BLK + (FINE ? 0 : pb.at * 32), vt, j - 1 > f);
-              if (FINE) product_cols<T, D>(o_at, s_at + BLK + 32, vt, true);
-              mma_commit((j - 1 < e - 1 ? o_done : o_last) + 8 * t);
+          if (j > 0) {
+            const bool mine = j - 1 >= f && j - 1 < e;
+            ok = bar_wait(v_full + 8 * vst.at, vst.phase, waits);
+            if (ok && mine) ok = bar_wait(p_full + 16 * t + 8 * pb.at, pb.phase, waits);
+            if (!ok) break;
+            tc_fence_after();
+            if (lead) {
+              if (mine) {
+                const uint32_t vt = base + C::V_OFF + vst.at * C::KB;
+                product_cols<T, D>(o_at, s_at + BLK + (FINE ? 0 : pb.at * 32), vt, j - 1 > f);
+                if (FINE) product_cols<T, D>(o_at, s_at + BLK + 32, vt, true);
+                mma_commit((j - 1 < e - 1 ? o_done : o_last) + 8 * t);
+              }
+              mma_commit(v_free + 8 * vst.at);
             }
-            mma_commit(v_free + 8 * vst.at);
+            vst.next();
+            if (mine) pb.next();
           }
-          vst.next();
-          if (mine) pb.next();
         }
-      }
+      };
+      if (few_keys(a, s, min(m0 + t * N + N, s.qlen))) steps(std::true_type{});
+      else steps(std::false_type{});
       if (!ok && lead) {  // given up: not before the products in flight have completed
         mma_commit(drained + 8 * t);
         bar_drain(drained + 8 * t, 0, waits);
@@ -271,93 +277,103 @@ __global__ void __launch_bounds__(352, 1)
     }
     float x[BLK];
     const uint32_t s_at = tmem + lanes + C::S_COL + t * N;
-    for (int j = f; j < e; ++j) {
-      if (!there) there = ok && bar_wait(s_full + 8 * t, (uint32_t)(j - f) & 1u, waits);
-      ok = __all_sync(0xffffffffu, there);
-      if (!ok) break;
-      tc_fence_after();
-      load64(s_at, x);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) bar_arrive(s_read + 8 * t);
-      const int n0 = j * BLK;
-      if (n0 > clear1 || n0 < clear0) {
-        const int hi = row_hi - n0, lo = row_lo - n0;
-#pragma unroll
-        for (int i = 0; i < BLK; ++i)
-          if (i >= hi || i < lo) x[i] = -INFINITY;
-        // rows of V that nothing may be read from: before the first key that a query
-        // sees, and past the sequence's end where memory does hold some
-        const int seen0 = first_key(a, s);
-        if (n0 < seen0 || (n0 + BLK > s.klen && s.k0 + s.klen < a.Sk)) {
-          const int it = j - b0, st = it % NST;
-          ok = __all_sync(0xffffffffu, bar_wait(v_full + 8 * st, (uint32_t)(it / NST) & 1u, waits));
-          if (!ok) break;
-          unsigned char* vt = smem + C::V_OFF + st * C::KB;
-          if (n0 < seen0) zero_rows<D>(vt, 0, seen0 - n0);
-          if (n0 + BLK > s.klen) zero_rows<D>(vt, s.klen - n0, BLK);
-        }
-      }
-      float top[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-      for (int i = 4; i + 8 <= BLK; i += 8)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) top[u] = max3(top[u], x[i + u], x[i + 4 + u]);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) top[u] = fmaxf(top[u], x[BLK - 4 + u]);
-      const float mb = max3(fmaxf(top[0], top[1]), top[2], top[3]) * a.scale_log2;
-      if (j == f) {
-        m = mb;
-      } else if (__any_sync(0xffffffffu, mb > m + 8.f)) {
-        const float mn = mb > m + 8.f ? mb : m;
-        const float w = mn == m ? 1.f : ex2(m - mn);
-        m = mn;
-        l *= w;
-        // O_t, after the product of the block before; the one before that has
-        // completed, since S of this block was issued after it
-        ok = __all_sync(0xffffffffu, bar_wait(o_done + 8 * t, (uint32_t)(j - f - 1) & 1u, waits));
+    // Two loops, and two of the products: with a flag inside of them instead, the
+    // softmax took 881 us for 727 (8192 full rows of 32/8 heads of 64), the products
+    // 983 for 922 (of 128).
+    auto blocks = [&](auto few) {
+      constexpr bool FINE = decltype(few)::value;
+      for (int j = f; j < e; ++j) {
+        if (!there) there = ok && bar_wait(s_full + 8 * t, (uint32_t)(j - f) & 1u, waits);
+        ok = __all_sync(0xffffffffu, there);
         if (!ok) break;
         tc_fence_after();
-#pragma unroll 1
-        for (int c = 0; c < D / 16; ++c) {
-          uint32_t o[16];
-          tmem_ld16(o_at + c * 16, o);
-          tmem_wait_ld();
+        load64(s_at, x);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(s_read + 8 * t);
+        const int n0 = j * BLK;
+        if (n0 > clear1 || n0 < clear0) {
+          const int hi = row_hi - n0, lo = row_lo - n0;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * w);
-          tmem_st16(o_at + c * 16, o);
+          for (int i = 0; i < BLK; ++i)
+            if (i >= hi || i < lo) x[i] = -INFINITY;
+          // rows of V that nothing may be read from: before the first key that a query
+          // sees, and past the sequence's end where memory does hold some
+          const int seen0 = first_key(a, s);
+          if (n0 < seen0 || (n0 + BLK > s.klen && s.k0 + s.klen < a.Sk)) {
+            const int it = j - b0, st = it % NST;
+            ok = __all_sync(0xffffffffu,
+                            bar_wait(v_full + 8 * st, (uint32_t)(it / NST) & 1u, waits));
+            if (!ok) break;
+            unsigned char* vt = smem + C::V_OFF + st * C::KB;
+            if (n0 < seen0) zero_rows<D>(vt, 0, seen0 - n0);
+            if (n0 + BLK > s.klen) zero_rows<D>(vt, s.klen - n0, BLK);
+          }
         }
-      }
-      // whether the next block's S is there: asked before the exponentials, so
-      // that the answer (200 cycles) comes during them
-      there = j + 1 < e && bar_test(s_full + 8 * t, (uint32_t)(j + 1 - f) & 1u);
-      // a row that has seen nothing (m = -inf) is masked everywhere: 2^(-inf - 0) = 0
-      const float2 from = f2s(m == -INFINITY ? 0.f : -m);
-      float2 sum[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
+        float top[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-      for (int i = 0; i < BLK; i += 2) {
-        const float2 y = f2_fma(f2(x[i], x[i + 1]), sc, from);
-        x[i] = ex2(y.x);
-        x[i + 1] = ex2(y.y);
-        sum[(i / 2) & 1] = f2_add(sum[(i / 2) & 1], f2(x[i], x[i + 1]));
-      }
-      if constexpr (FINE) {
-        if (j > f) {
+        for (int i = 4; i + 8 <= BLK; i += 8)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) top[u] = max3(top[u], x[i + u], x[i + 4 + u]);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) top[u] = fmaxf(top[u], x[BLK - 4 + u]);
+        const float mb = max3(fmaxf(top[0], top[1]), top[2], top[3]) * a.scale_log2;
+        if (j == f) {
+          m = mb;
+        } else if (__any_sync(0xffffffffu, mb > m + 8.f)) {
+          const float mn = mb > m + 8.f ? mb : m;
+          const float w = mn == m ? 1.f : ex2(m - mn);
+          m = mn;
+          l *= w;
+          // O_t, after the product of the block before; the one before that has
+          // completed, since S of this block was issued after it
           ok = __all_sync(0xffffffffu, bar_wait(o_done + 8 * t, (uint32_t)(j - f - 1) & 1u, waits));
           if (!ok) break;
           tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld16(o_at + c * 16, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * w);
+            tmem_st16(o_at + c * 16, o);
+          }
         }
-        store64<T>(s_at + BLK, x);
-        store64_rest<T>(s_at + BLK + 32, x);
-      } else {
-        store64<T>(s_at + BLK + ((j - f) & 1) * 32, x);
+        // whether the next block's S is there: asked before the exponentials, so
+        // that the answer (200 cycles) comes during them
+        there = j + 1 < e && bar_test(s_full + 8 * t, (uint32_t)(j + 1 - f) & 1u);
+        // a row that has seen nothing (m = -inf) is masked everywhere: 2^(-inf - 0) = 0
+        const float2 from = f2s(m == -INFINITY ? 0.f : -m);
+        float2 sum[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
+#pragma unroll
+        for (int i = 0; i < BLK; i += 2) {
+          const float2 y = f2_fma(f2(x[i], x[i + 1]), sc, from);
+          x[i] = ex2(y.x);
+          x[i + 1] = ex2(y.y);
+          sum[(i / 2) & 1] = f2_add(sum[(i / 2) & 1], f2(x[i], x[i + 1]));
+        }
+        if constexpr (FINE) {
+          if (j > f) {
+            ok = __all_sync(0xffffffffu,
+                            bar_wait(o_done + 8 * t, (uint32_t)(j - f - 1) & 1u, waits));
+            if (!ok) break;
+            tc_fence_after();
+          }
+          store64<T>(s_at + BLK, x);
+          store64_rest<T>(s_at + BLK + 32, x);
+        } else {
+          store64<T>(s_at + BLK + ((j - f) & 1) * 32, x);
+        }
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(p_full + 16 * t + 8 * ((j - f) & 1));
       }
-      l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) bar_arrive(p_full + 16 * t + 8 * ((j - f) & 1));
-    }
+    };
+    if (few_keys(a, s, min(m0 + t * N + N, s.qlen))) blocks(std::true_type{});
+    else blocks(std::false_type{});
     if (ok && e > f) {
       ok = __all_sync(0xffffffffu, bar_wait(o_last + 8 * t, 0, waits));
       tc_fence_after();
@@ -399,7 +415,7 @@ __global__ void __launch_bounds__(352, 1)
   if (warp == 8) tmem_free(tmem, C::COLS);
 }
 
-template <typename T, int D, bool FINE>
+template <typename T, int D>
 int launch_attn_fwd(const AttnArgs& a0, cudaStream_t st) {
   using C = FwdCfg<D>;
   AttnArgs a = a0;
@@ -415,7 +431,7 @@ int launch_attn_fwd(const AttnArgs& a0, cudaStream_t st) {
   if (rc == BLOTH_OK)
     rc = head_map(&m.v, a.v.p, a.v.sb, a.v.ss, a.v.sh, a.B, Sk, a.Hk, D, 64, dt);
   if (rc != BLOTH_OK) return rc;
-  auto kern = attn_fwd_kernel<T, D, FINE>;
+  auto kern = attn_fwd_kernel<T, D>;
   if ((rc = prepare_smem((const void*)kern, C::SMEM)) != BLOTH_OK) return rc;
   const int64_t grid = attn_tiles(a.Sq, a.packed, C::TILES * C::TILE) * a.Hq * a.B;
   if (grid > 0x7fffffff) return BLOTH_ERR_SHAPE;

@@ -39,17 +39,20 @@ struct AttnArgs {
   float scale, scale_log2;
   int causal;
   int window;         // 0: none
-  int fine;           // P and dS at twice the tensors' precision (16-bit tensors)
   unsigned int* fault;
 };
 
-// Rows that see at most this many keys have P and dS as two terms of 16 bits:
-// where few terms are summed, a gradient of two nearly equal ones lost up to
-// six times what rounding the result takes (bf16, two keys); with two terms no
-// more than that rounding. It costs a product for each of P and dS: 4 x 8192
-// rows of 32/8 heads of 128, forward and backward, 1720 us with a window of 128,
-// 1575 us with one of 129; 64 x 128 rows, 435 us, and 536 us for 64 x 129.
-// Sequences packed into more rows count as longer.
+// Tiles whose rows see at most this many keys each have P and dS as two terms of
+// 16 bits: where few terms are summed, a gradient of two nearly equal ones lost up
+// to six times what rounding the result takes (bf16, two keys); with two terms no
+// more than that rounding. A tile is what a CTA or a group of warps works on, in
+// the rows of one sequence: 128 query rows for o and dq, 128 keys with every query
+// that sees them for dk and dv, the call's few rows over a cache. The tensors'
+// extents do not count.
+// It costs a product for each of P and dS: 4 x 8192 rows of 32/8 heads of 128 (bf16),
+// forward and backward, 1447 us with a window of 128, 1302 us with one of 129; 8192
+// rows as 128 sequences 617 us, with one term 582; 64 x 129 rows, of which the first
+// 128 have two terms in o and dq, 489 us, with one term 463.
 constexpr int kFineKeys = 128;
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -165,6 +168,12 @@ __device__ __forceinline__ AttnSeq find_seq(const AttnArgs& a, int b, int t, int
     last_k = __shfl_sync(0xffffffffu, k1, 31);
   }
   return s;
+}
+
+// Whether every query of a sequence before row m1 sees at most kFineKeys keys.
+__device__ __forceinline__ bool few_keys(const AttnArgs& a, const AttnSeq& s, int m1) {
+  const int n = a.causal ? min(s.klen, m1 + s.klen - s.qlen) : s.klen;
+  return (a.window ? min(n, a.window) : n) <= kFineKeys;
 }
 
 // Query i of a sequence sees key j when j < klen and, causal, j <= i + klen -

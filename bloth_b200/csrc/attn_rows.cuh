@@ -185,104 +185,109 @@ __global__ void __launch_bounds__(kRowsWarps * 32)
       for (int e = 0; e < 4; ++e) acc[mt][n][e] = 0.f;
   }
 
-  for (int i = 0; i < mine; ++i) {
-    issue(i + C::ST - 1);
-    cp_wait<C::ST - 1>();
-    __syncwarp();
-    const int j0 = lo + (warp + i * kRowsWarps) * kStrip;
-    const uint32_t at = ring + (i % C::ST) * 2 * C::STRIPB;
-    float x[MT][2][4];
+  auto strip_loop = [&](auto few) {  // P as one term or two: see attn_fwd.cuh
+    constexpr bool FINE = decltype(few)::value;
+    for (int i = 0; i < mine; ++i) {
+      issue(i + C::ST - 1);
+      cp_wait<C::ST - 1>();
+      __syncwarp();
+      const int j0 = lo + (warp + i * kRowsWarps) * kStrip;
+      const uint32_t at = ring + (i % C::ST) * 2 * C::STRIPB;
+      float x[MT][2][4];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[mt][n][e] = 0.f;
-    {
-      const int id = lane >> 3, r = (lane & 7) + 8 * (id >> 1);
-#pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        uint32_t kf[4];
-        ldm4(at + r * (D * 2) + (((kk * 2 + (id & 1)) ^ (r & 7)) * 16), kf);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          mma16<T>(x[mt][0], qf[mt][kk], kf[0], kf[1]);
-          mma16<T>(x[mt][1], qf[mt][kk], kf[2], kf[3]);
-        }
-      }
-    }
-    const bool masked = j0 + kStrip > all_to || j0 < all_from || s.qlen < a.Sq;
-    uint32_t pf[MT][4], rest[MT][4];
-    bool move = false;
-    float top[MT][2];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        float mx = -INFINITY;
+      for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float& y = x[mt][n][2 * u + e];
-            const int j = j0 + n * 8 + 2 * t + e;
-            y = masked && (j >= to[mt][u] || j < from[mt][u]) ? -INFINITY : y * a.scale_log2;
-            mx = fmaxf(mx, y);
+          for (int e = 0; e < 4; ++e) x[mt][n][e] = 0.f;
+      {
+        const int id = lane >> 3, r = (lane & 7) + 8 * (id >> 1);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          uint32_t kf[4];
+          ldm4(at + r * (D * 2) + (((kk * 2 + (id & 1)) ^ (r & 7)) * 16), kf);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            mma16<T>(x[mt][0], qf[mt][kk], kf[0], kf[1]);
+            mma16<T>(x[mt][1], qf[mt][kk], kf[2], kf[3]);
           }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        top[mt][u] = mx;
-        move = move || mx > m[mt][u] + 8.f;  // as in the tile kernel: see attn_fwd.cuh
+        }
       }
-    if (__any_sync(0xffffffffu, move)) {
+      const bool masked = j0 + kStrip > all_to || j0 < all_from || s.qlen < a.Sq;
+      uint32_t pf[MT][4], rest[MT][4];
+      bool move = false;
+      float top[MT][2];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const float mn = fmaxf(m[mt][u], top[mt][u]);
-          const float w = mn == m[mt][u] ? 1.f : ex2(m[mt][u] - mn);
-          m[mt][u] = mn;
-          l[mt][u] *= w;
+          float mx = -INFINITY;
 #pragma unroll
-          for (int n = 0; n < D / 8; ++n) {
-            acc[mt][n][2 * u] *= w;
-            acc[mt][n][2 * u + 1] *= w;
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float& y = x[mt][n][2 * u + e];
+              const int j = j0 + n * 8 + 2 * t + e;
+              y = masked && (j >= to[mt][u] || j < from[mt][u]) ? -INFINITY : y * a.scale_log2;
+              mx = fmaxf(mx, y);
+            }
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          top[mt][u] = mx;
+          move = move || mx > m[mt][u] + 8.f;  // as in the tile kernel: see attn_fwd.cuh
+        }
+      if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const float mn = fmaxf(m[mt][u], top[mt][u]);
+            const float w = mn == m[mt][u] ? 1.f : ex2(m[mt][u] - mn);
+            m[mt][u] = mn;
+            l[mt][u] *= w;
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n) {
+              acc[mt][n][2 * u] *= w;
+              acc[mt][n][2 * u + 1] *= w;
+            }
+          }
+      }
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float base = m[mt][u] == -INFINITY ? 0.f : m[mt][u];
+          float p[4];
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) p[2 * n + e] = ex2(x[mt][n][2 * u + e] - base);
+          l[mt][u] += (p[0] + p[1]) + (p[2] + p[3]);
+          split2<T>(p[0], p[1], pf[mt][u], rest[mt][u]);
+          split2<T>(p[2], p[3], pf[mt][u + 2], rest[mt][u + 2]);
+        }
+      {
+        const int id = lane >> 3, r = (lane & 7) + 8 * (id & 1);
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt) {
+          uint32_t vf[4];
+          ldm4t(at + C::STRIPB + r * (D * 2) + (((dt * 2 + (id >> 1)) ^ (r & 7)) * 16), vf);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            mma16<T>(acc[mt][2 * dt], pf[mt], vf[0], vf[1]);
+            mma16<T>(acc[mt][2 * dt + 1], pf[mt], vf[2], vf[3]);
+            if (FINE) {
+              mma16<T>(acc[mt][2 * dt], rest[mt], vf[0], vf[1]);
+              mma16<T>(acc[mt][2 * dt + 1], rest[mt], vf[2], vf[3]);
+            }
           }
         }
-    }
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const float base = m[mt][u] == -INFINITY ? 0.f : m[mt][u];
-        float p[4];
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) p[2 * n + e] = ex2(x[mt][n][2 * u + e] - base);
-        l[mt][u] += (p[0] + p[1]) + (p[2] + p[3]);
-        split2<T>(p[0], p[1], pf[mt][u], rest[mt][u]);
-        split2<T>(p[2], p[3], pf[mt][u + 2], rest[mt][u + 2]);
       }
-    {
-      const int id = lane >> 3, r = (lane & 7) + 8 * (id & 1);
-#pragma unroll
-      for (int dt = 0; dt < D / 16; ++dt) {
-        uint32_t vf[4];
-        ldm4t(at + C::STRIPB + r * (D * 2) + (((dt * 2 + (id >> 1)) ^ (r & 7)) * 16), vf);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          mma16<T>(acc[mt][2 * dt], pf[mt], vf[0], vf[1]);
-          mma16<T>(acc[mt][2 * dt + 1], pf[mt], vf[2], vf[3]);
-          if (a.fine) {
-            mma16<T>(acc[mt][2 * dt], rest[mt], vf[0], vf[1]);
-            mma16<T>(acc[mt][2 * dt + 1], rest[mt], vf[2], vf[3]);
-          }
-        }
-      }
+      __syncwarp();  // the slot is free for the copy issued next
     }
-    __syncwarp();  // the slot is free for the copy issued next
-  }
+  };
+  if (few_keys(a, s, s.qlen)) strip_loop(std::true_type{});
+  else strip_loop(std::false_type{});
   cp_wait<0>();
 
   // the four warps' rows through shared memory: [warp][row][D], then
