@@ -435,6 +435,15 @@ __global__ void __launch_bounds__(352, 1)
         if constexpr (DK) {
           float y[BLK];
           load64(dp_at, y);
+          if constexpr (kBwdShift<T> != 0.f) {
+            const float2 down = f2s(exp2f(-kBwdShift<T>));
+#pragma unroll
+            for (int i = 0; i < BLK; i += 2) {
+              const float2 p = f2_mul(f2(x[i], x[i + 1]), down);
+              x[i] = p.x;
+              x[i + 1] = p.y;
+            }
+          }
 #pragma unroll
           for (int i = 0; i < BLK; i += 4) {
             const float4 d = *reinterpret_cast<const float4*>(stat + 64 + i);
@@ -484,9 +493,9 @@ __global__ void __launch_bounds__(352, 1)
       T* dst = reinterpret_cast<T*>(const_cast<void*>(t.p)) + (int64_t)s.b * t.sb +
                (int64_t)h * t.sh + (int64_t)(s.k0 + key0) * t.ss + c0;
       // through the kept tiles, which every product has read
-      store_sums<COLS>(tmem + lanes + (is_k ? DK_COL : DV_COL) + c0, is_k ? a.scale : 1.f, dst,
-                       t.ss, limit - key0, key < s.klen, total > 0,
-                       smem + C::OWN_OFF + warp * 4096);
+      store_sums<COLS>(tmem + lanes + (is_k ? DK_COL : DV_COL) + c0,
+                       is_k ? a.scale : exp2f(-kBwdShift<T>), dst, t.ss, limit - key0,
+                       key < s.klen, total > 0, smem + C::OWN_OFF + warp * 4096);
     }
   }
   tc_fence_before();
@@ -649,7 +658,8 @@ __global__ void __launch_bounds__(352, 1)
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const int row = m0 + r, off = s.klen - s.qlen;
     const int64_t stat = (int64_t)h * a.R + s.stat0 + row;
-    const float2 lse2 = f2s(-__ldg(a.lse2 + stat)), delta = f2s(-__ldg(a.delta + stat));
+    const float2 lse2 = f2s(-__ldg(a.lse2 + stat) - kBwdShift<T>);
+    const float2 delta = f2s(-__ldg(a.delta + stat));
     const float2 sc = f2s(a.scale_log2);
     const uint32_t s_at = tmem + lanes + C::S_COL + group * BLK;
     const uint32_t dp_at = tmem + lanes + C::DP_COL + group * BLK;

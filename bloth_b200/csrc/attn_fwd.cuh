@@ -21,7 +21,7 @@
 // The running maximum moves only when a block's maximum exceeds it by more
 // than 2^8 (then the group rescales O_t in tensor memory, after its last
 // product). Until then p is at most 2^8, which costs no precision: p is
-// rounded relative to its own size, and sums are fp32.
+// rounded relative to its own size (fp16: times kFwdShift), and sums are fp32.
 //
 // Tiles whose rows see few keys (kFineKeys) have P as two terms, which take both
 // buffers: P of a block then waits for the product of the block before.
@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(352, 1)
         // that the answer (200 cycles) comes during them
         there = j + 1 < e && bar_test(s_full + 8 * t, (uint32_t)(j + 1 - f) & 1u);
         // a row that has seen nothing (m = -inf) is masked everywhere: 2^(-inf - 0) = 0
-        const float2 from = f2s(m == -INFINITY ? 0.f : -m);
+        const float2 from = f2s(m == -INFINITY ? 0.f : kFwdShift<T> - m);
         float2 sum[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
 #pragma unroll
         for (int i = 0; i < BLK; i += 2) {
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(352, 1)
       }
       if (row < limit && a.lse != nullptr)
         a.lse[((int64_t)s.b * a.Hq + h) * a.Sq + s.q0 + row] =
-            inv != 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+            inv != 0.f ? (m - kFwdShift<T> + log2f(l)) * kLn2 : -INFINITY;
     }
   }
   tc_fence_before();

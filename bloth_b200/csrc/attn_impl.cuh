@@ -28,7 +28,8 @@ struct AttnArgs {
   HT q, k, v, o, dout, dq, dk, dv;
   void* rest;         // what rounding took off o, laid out as o (16-bit tensors), or NULL
   float* lse;         // [B, Hq, Sq] natural logarithm (forward writes, backward reads)
-  float* lse2;        // backward workspace: [Hq, R] lse * log2(e), +inf where nothing is seen
+  float* lse2;        // backward workspace: [Hq, R] lse * log2(e) - kBwdShift, +inf where
+                      // nothing is seen
   float* delta;       // backward workspace: [Hq, R]
   int64_t R;          // rows per head of lse2 and delta (attn_stat_rows)
   const void* qseq;   // dense: [B] query lengths or NULL; packed: [n + 1] offsets
@@ -54,6 +55,15 @@ struct AttnArgs {
 // rows as 128 sequences 617 us, with one term 582; 64 x 129 rows, of which the first
 // 128 have two terms in o and dq, 489 us, with one term 463.
 constexpr int kFineKeys = 128;
+
+// Powers of two that probabilities are held times where they enter a product, so
+// that fp16 holds small ones: its normal range starts at 2^-14. In the forward they
+// are at most 2^8 (attn_fwd.cuh), in the backward at most 1. They cost nothing: they
+// are added to the exponent, and leave with the sum of exponentials or the store.
+template <typename T>
+constexpr float kFwdShift = std::is_same<T, __half>::value ? 7.f : 0.f;
+template <typename T>
+constexpr float kBwdShift = std::is_same<T, __half>::value ? 15.f : 0.f;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;

@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32)
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const float base = m[mt][u] == -INFINITY ? 0.f : m[mt][u];
+          const float base = m[mt][u] == -INFINITY ? 0.f : m[mt][u] - kFwdShift<T>;
           float p[4];
 #pragma unroll
           for (int n = 0; n < 2; ++n)
@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32)
         *reinterpret_cast<float2*>(row + n * 8 + 2 * t) =
             f2(acc[mt][n][2 * u], acc[mt][n][2 * u + 1]);
       if (t == 0) {
-        stat[(warp * C::ROWS + r) * 2] = m[mt][u];
+        stat[(warp * C::ROWS + r) * 2] = m[mt][u] - kFwdShift<T>;
         stat[(warp * C::ROWS + r) * 2 + 1] = q;
       }
     }

@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(256) attn_stats_kernel(const AttnArgs a) {
     if (lane % LPR == 0) {
       const float l = in ? a.lse[((int64_t)s.b * a.Hq + h) * a.Sq + row] : -INFINITY;
       const bool none = l == -INFINITY;
-      a.lse2[stat + r] = none ? INFINITY : l * kLog2e;
+      a.lse2[stat + r] = none ? INFINITY : l * kLog2e - kBwdShift<T>;
       a.delta[stat + r] = none ? 0.f : sum;
     }
   }
