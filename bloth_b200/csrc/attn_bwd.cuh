@@ -17,7 +17,8 @@
 // where S^T and dP lay, as the products' first operand; the streamed tiles are
 // read by the products both by rows and by columns, so nothing is transposed
 // or stored again. (Tiles of few keys, kFineKeys: as two terms, in the two
-// halves of where S^T and dP lay.) Blocks alternate between two buffers of S and of dP in
+// halves of where S^T and dP lay. fp16: times powers of two that keep them in its
+// range, kBwdShift and ds_scale.) Blocks alternate between two buffers of S and of dP in
 // tensor memory and two groups of four warps (thread = row of the kept tile,
 // 64 columns): a group has two blocks' time for its own, so neither the
 // hand-over between warps nor its own latencies stop the tensor core. Warps 8
@@ -352,6 +353,22 @@ __global__ void __launch_bounds__(352, 1)
     const uint32_t dp_at = tmem + lanes + C::DP_COL + group * BLK;
     const float2 sc = f2s(a.scale_log2);
     const int seen0 = first_query(a, s);
+    // fp16: dS times a power of two, by the largest bound of the CTA's
+    float ds_up = 1.f;
+    if constexpr (DK && kBwdShift<T> != 0.f) {
+      if (total > 0) {
+        const float2* top = a.qtop + (int64_t)h * a.G * stat_tiles(a.R) + s.stat0 / 128 + lo / 128;
+        const int n = (hi + 127) / 128 - lo / 128;
+        float2 most = f2(0.f, 0.f);
+        for (int g = 0; g < a.G; ++g)
+          for (int i = lane; i < n; i += 32) {
+            const float2 u = __ldg(top + (int64_t)g * stat_tiles(a.R) + i);
+            most = f2(fmaxf(most.x, u.x), fmaxf(most.y, u.y));
+          }
+        const float v = __ldg(a.vtop + (int64_t)h * stat_tiles(a.RK) + s.kstat0 / 128 + s.tile);
+        ds_up = ds_scale(warp_top(most.x) * v + warp_top(most.y));
+      }
+    }
     Ring<NA> st;
     Ring<NB> ost;
     int mi = 0;
@@ -436,7 +453,7 @@ __global__ void __launch_bounds__(352, 1)
           float y[BLK];
           load64(dp_at, y);
           if constexpr (kBwdShift<T> != 0.f) {
-            const float2 down = f2s(exp2f(-kBwdShift<T>));
+            const float2 down = f2s(ds_up * exp2f(-kBwdShift<T>));
 #pragma unroll
             for (int i = 0; i < BLK; i += 2) {
               const float2 p = f2_mul(f2(x[i], x[i + 1]), down);
@@ -494,7 +511,7 @@ __global__ void __launch_bounds__(352, 1)
                (int64_t)h * t.sh + (int64_t)(s.k0 + key0) * t.ss + c0;
       // through the kept tiles, which every product has read
       store_sums<COLS>(tmem + lanes + (is_k ? DK_COL : DV_COL) + c0,
-                       is_k ? a.scale : exp2f(-kBwdShift<T>), dst, t.ss, limit - key0,
+                       is_k ? a.scale / ds_up : exp2f(-kBwdShift<T>), dst, t.ss, limit - key0,
                        key < s.klen, total > 0, smem + C::OWN_OFF + warp * 4096);
     }
   }
@@ -658,8 +675,19 @@ __global__ void __launch_bounds__(352, 1)
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const int row = m0 + r, off = s.klen - s.qlen;
     const int64_t stat = (int64_t)h * a.R + s.stat0 + row;
-    const float2 lse2 = f2s(-__ldg(a.lse2 + stat) - kBwdShift<T>);
     const float2 delta = f2s(-__ldg(a.delta + stat));
+    // fp16: dS times a power of two, by the row's bound, which is part of its p's
+    // exponent
+    float ds_up = 1.f, up = -kBwdShift<T>;
+    if constexpr (kBwdShift<T> != 0.f) {
+      const int hk = h / a.G;
+      const float* top = a.vtop + (int64_t)hk * stat_tiles(a.RK) + s.kstat0 / 128;
+      float v = 0.f;
+      for (int i = lo / 128 + lane; i < (hi + 127) / 128; i += 32) v = fmaxf(v, __ldg(top + i));
+      ds_up = ds_scale(__ldg(a.donorm + stat) * warp_top(v) + fabsf(delta.x));
+      up += (float)((__float_as_int(ds_up) >> 23) - 127);
+    }
+    const float2 lse2 = f2s(up - __ldg(a.lse2 + stat));
     const float2 sc = f2s(a.scale_log2);
     const uint32_t s_at = tmem + lanes + C::S_COL + group * BLK;
     const uint32_t dp_at = tmem + lanes + C::DP_COL + group * BLK;
@@ -735,7 +763,7 @@ __global__ void __launch_bounds__(352, 1)
                (int64_t)h * a.dq.sh + (int64_t)(s.q0 + row0) * a.dq.ss + group * (D / 2);
       // queries past the sequence's end (dense tensors) get zeros; through the
       // kept tiles, which every product has read
-      store_sums<D / 2>(tmem + lanes + C::ACC_COL + group * (D / 2), a.scale, dst, a.dq.ss,
+      store_sums<D / 2>(tmem + lanes + C::ACC_COL + group * (D / 2), a.scale / ds_up, dst, a.dq.ss,
                         limit - row0, row < s.qlen, total > 0, smem + C::OWN_OFF + warp * 4096);
     }
   }

@@ -136,6 +136,7 @@ size_t bloth_attention_bwd_workspace_bytes(int64_t B, int64_t Sq, int64_t Sk, in
                                            int64_t Hk, int64_t D, int64_t packed, int dtype) {
   if (check_sizes(B, Sq, Sk, Hq, Hk, D, packed, dtype)) return 0;
   int64_t n = 2 * Hq * attn_stat_rows(B, Sq, packed);
+  if (dtype == BLOTH_F16) n += attn_top_floats(B, Sq, Sk, Hq, Hk, packed);
   if (dtype == BLOTH_F32 && simt_split(B, Sk, Hk, Hq / Hk, packed)) n += 2 * B * Hq * Sk * D;
   return (size_t)n * sizeof(float);
 }
@@ -181,6 +182,12 @@ int bloth_attention_bwd(const void* dout, const int64_t* dout_strides, const voi
   a.R = attn_stat_rows(B, Sq, packed);
   a.lse2 = reinterpret_cast<float*>(workspace);
   a.delta = a.lse2 + Hq * a.R;
+  if (dtype == BLOTH_F16) {
+    a.RK = attn_stat_rows(B, Sk, packed);
+    a.donorm = a.delta + Hq * a.R;
+    a.qtop = reinterpret_cast<float2*>(a.donorm + Hq * a.R);
+    a.vtop = reinterpret_cast<float*>(a.qtop + Hq * stat_tiles(a.R));
+  }
   return by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     if (Sq > 0) {

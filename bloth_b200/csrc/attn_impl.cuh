@@ -32,6 +32,11 @@ struct AttnArgs {
                       // nothing is seen
   float* delta;       // backward workspace: [Hq, R]
   int64_t R;          // rows per head of lse2 and delta (attn_stat_rows)
+  // backward workspace of fp16 tensors, what bounds ds (ds_scale):
+  float* donorm;      // [Hq, R] |do_i|
+  float2* qtop;       // [Hq, stat_tiles(R)] of 128 query rows, largest |do_i| and |delta_i|
+  float* vtop;        // [Hk, stat_tiles(RK)] of 128 key rows, largest |v_j|
+  int64_t RK;         // as R, for key rows
   const void* qseq;   // dense: [B] query lengths or NULL; packed: [n + 1] offsets
   const void* kseq;   // the same for keys
   int seq_dt;
@@ -65,6 +70,18 @@ constexpr float kFwdShift = std::is_same<T, __half>::value ? 7.f : 0.f;
 template <typename T>
 constexpr float kBwdShift = std::is_same<T, __half>::value ? 15.f : 0.f;
 
+// The power of two that ds, at most `bound` in size, is held times in fp16, whose
+// largest number is 65504: it brings the bound to between 2^14 and 2^15. What it
+// leaves above fp16's normal range is 2^29 below the bound.
+__device__ __forceinline__ float ds_scale(float bound) {
+  const int x = max((__float_as_int(bound) >> 23) - 127, -100);  // floor(log2(bound)), or -100
+  return __int_as_float((127 + 14 - x) << 23);
+}
+// The largest of non-negative numbers, over the lanes of a warp.
+__device__ __forceinline__ float warp_top(float x) {
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(x)));
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -74,6 +91,7 @@ struct AttnSeq {
   int q0, qlen;    // first query row and their number
   int k0, klen;
   int64_t stat0;   // first row of its lse2 and delta rows
+  int64_t kstat0;  // the same for rows of keys
   int tile;        // tile of the sequence this CTA works on; < 0: none
 };
 
@@ -91,6 +109,9 @@ __host__ __device__ __forceinline__ int64_t attn_stat_base(int64_t cu, int64_t s
 inline int64_t attn_stat_rows(int64_t B, int64_t Sq, int64_t packed) {
   return packed ? attn_stat_base(Sq, packed + 2) + 128 : B * ((Sq + 127) / 128 * 128);
 }
+// Tile t of 128 rows of a sequence is entry stat0 / 128 + t of an array with an
+// entry for each tile; sequences start more than 128 rows apart.
+__host__ __device__ __forceinline__ int64_t stat_tiles(int64_t R) { return R / 128 + 1; }
 // Tiles of `tile` rows that cover every sequence, at most (the offsets of
 // packed sequences are known on the device only). The rows before the first
 // sequence and those past the last are two more, which see nothing.
@@ -114,6 +135,7 @@ __device__ __forceinline__ AttnSeq find_seq(const AttnArgs& a, int b, int t, int
     s.qlen = a.qseq ? seq_at(a.qseq, a.seq_dt, b, a.Sq) : a.Sq;
     s.klen = a.kseq ? seq_at(a.kseq, a.seq_dt, b, a.Sk) : a.Sk;
     s.stat0 = (int64_t)b * ((a.Sq + 127) / 128 * 128);
+    s.kstat0 = (int64_t)b * ((a.Sk + 127) / 128 * 128);
     s.tile = t;
     return s;
   }
@@ -169,6 +191,7 @@ __device__ __forceinline__ AttnSeq find_seq(const AttnArgs& a, int b, int t, int
       s.klen = __shfl_sync(0xffffffffu, k1, src) - s.k0;
       s.tile = t - before - __shfl_sync(0xffffffffu, upto - tiles, src);
       s.stat0 = attn_stat_base(s.q0, base + src);
+      s.kstat0 = attn_stat_base(s.k0, base + src);
       // rows outside of the sequences: nothing is seen from or by them
       if (base + src == 0 || base + src == n + 1) (BY_Q ? s.klen : s.qlen) = 0;
       return s;
@@ -281,6 +304,12 @@ template <typename T>
 int attn_simt_bwd(const AttnArgs& a, int D, void* partial, cudaStream_t st);
 template <typename T>
 int attn_stats(const AttnArgs& a, int D, cudaStream_t st);
+// Floats of workspace that fp16's bounds of ds take.
+inline int64_t attn_top_floats(int64_t B, int64_t Sq, int64_t Sk, int64_t Hq, int64_t Hk,
+                               int64_t packed) {
+  const int64_t R = attn_stat_rows(B, Sq, packed);
+  return Hq * (R + 2 * stat_tiles(R)) + Hk * stat_tiles(attn_stat_rows(B, Sk, packed));
+}
 
 template <typename F>
 int attn_head_dim(int D, F&& f) {
