@@ -421,10 +421,6 @@ __global__ void __launch_bounds__(352, 1)
         // the first query that sees a key, or past the sequence's end where memory does
         // hold some
         const bool dead = m0 < seen0 || (m0 + BLK > s.qlen && s.q0 + s.qlen < a.Sq);
-        auto clear = [&](unsigned char* tile) {
-          if (m0 < seen0) zero_rows<D>(tile, 0, seen0 - m0);
-          if (m0 + BLK > s.qlen) zero_rows<D>(tile, s.qlen - m0, BLK);
-        };
         // the query that sees one key only; INT_MAX: all do, -1: none of the block
         const int alone = s.klen == 1 || a.window == 1 ? INT_MAX : a.causal ? -off - m0 : -1;
         if (masked) {
@@ -434,7 +430,7 @@ __global__ void __launch_bounds__(352, 1)
           if (DV && dead) {
             ok = __all_sync(0xffffffffu, bar_wait(bar.b_full + 8 * ost.at, ost.phase, waits));
             if (!ok) break;
-            clear(smem + C::B_OFF + ost.at * C::STRB);
+            keep_rows<D>(smem + C::B_OFF + ost.at * C::STRB, seen0 - m0, s.qlen - m0);
           }
         }
         if (DV) {
@@ -476,7 +472,7 @@ __global__ void __launch_bounds__(352, 1)
 #pragma unroll
             for (int i = 0; i < BLK; ++i)
               if (i < from || i >= to || i == alone || alone == INT_MAX) y[i] = 0.f;
-            if (dead) clear(smem + C::A_OFF + st.at * C::STRB);
+            if (dead) keep_rows<D>(smem + C::A_OFF + st.at * C::STRB, seen0 - m0, s.qlen - m0);
           }
           store64<T>(dp_at, y);
           if (FINE) store64_rest<T>(dp_at + 32, y);
@@ -739,9 +735,9 @@ __global__ void __launch_bounds__(352, 1)
             if (i < from || i >= to) y[i] = 0.f;
           // rows of K that nothing may be read from: before the first key that a query
           // sees, and past the sequence's end where memory does hold some
-          unsigned char* kt = smem + C::A_OFF + (it % NA) * C::STRB;
-          if (n0 < first_key(a, s)) zero_rows<D>(kt, 0, first_key(a, s) - n0);
-          if (n0 + BLK > s.klen && s.k0 + s.klen < a.Sk) zero_rows<D>(kt, s.klen - n0, BLK);
+          if (n0 < first_key(a, s) || (n0 + BLK > s.klen && s.k0 + s.klen < a.Sk))
+            keep_rows<D>(smem + C::A_OFF + (it % NA) * C::STRB, first_key(a, s) - n0,
+                         s.klen - n0);
         }
         store64<T>(dp_at, y);
         if (FINE) store64_rest<T>(dp_at + 32, y);
