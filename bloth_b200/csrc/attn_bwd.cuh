@@ -34,11 +34,12 @@
 // or dK. With the kept tiles in tensor memory, where the sums leave room for
 // them (dQ up to head_dim 128; dK and dV at head_dim 64), S and dP take 256 as
 // well. Beside them 512 cycles a block for its exponentials.
-// Measured at 8192 rows of 32/8 heads of 128 (bf16): causal, dK and dV 835 us
-// (four products, 1320 TFLOP/s), dQ 585 us (three, 1410); full rows, dQ 1125 us,
-// with the kept tiles in shared memory 1370, and dK and dV 1700 to 1840 us, in
-// blocks of 128 queries in single buffers 1826. Sixteen softmax warps in place of
-// eight were no faster.
+// Measured at 8192 rows of 32/8 heads of 128 (bf16), from idle, at 1965 MHz: causal,
+// dK and dV 830 us (four products, 1320 TFLOP/s), dQ 582 us (three, 1410); full rows,
+// dQ 1120 us, with the kept tiles in shared memory 1370, and dK and dV 1700 to 1840 us,
+// in blocks of 128 queries in single buffers 1826. In seconds of calls the 1 kW cap
+// leaves 1470 to 1690 MHz: dQ 980 cycles a block and 11,500 a CTA beside them, dK and
+// dV 1650 and 6,400. Sixteen softmax warps in place of eight were no faster.
 #pragma once
 
 #include <climits>
@@ -671,19 +672,14 @@ __global__ void __launch_bounds__(352, 1)
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const int row = m0 + r, off = s.klen - s.qlen;
     const int64_t stat = (int64_t)h * a.R + s.stat0 + row;
-    const float2 delta = f2s(-__ldg(a.delta + stat));
-    // fp16: dS times a power of two, by the row's bound, which is part of its p's
-    // exponent
-    float ds_up = 1.f, up = -kBwdShift<T>;
+    const float delta1 = __ldg(a.delta + stat), lse1 = __ldg(a.lse2 + stat);
+    float v_top = 0.f, do_norm = 0.f;  // fp16; reduced below, while the tiles are on their way
     if constexpr (kBwdShift<T> != 0.f) {
-      const int hk = h / a.G;
-      const float* top = a.vtop + (int64_t)hk * stat_tiles(a.RK) + s.kstat0 / 128;
-      float v = 0.f;
-      for (int i = lo / 128 + lane; i < (hi + 127) / 128; i += 32) v = fmaxf(v, __ldg(top + i));
-      ds_up = ds_scale(__ldg(a.donorm + stat) * warp_top(v) + fabsf(delta.x));
-      up += (float)((__float_as_int(ds_up) >> 23) - 127);
+      const float* top = a.vtop + (int64_t)(h / a.G) * stat_tiles(a.RK) + s.kstat0 / 128;
+      for (int i = lo / 128 + lane; i < (hi + 127) / 128; i += 32)
+        v_top = fmaxf(v_top, __ldg(top + i));
+      do_norm = __ldg(a.donorm + stat);
     }
-    const float2 lse2 = f2s(up - __ldg(a.lse2 + stat));
     const float2 sc = f2s(a.scale_log2);
     const uint32_t s_at = tmem + lanes + C::S_COL + group * BLK;
     const uint32_t dp_at = tmem + lanes + C::DP_COL + group * BLK;
@@ -699,6 +695,14 @@ __global__ void __launch_bounds__(352, 1)
         if (lane == 0) bar_arrive(bar.there);
       }
     }
+    // fp16: dS times a power of two, by the row's bound, which is part of its p's
+    // exponent
+    float ds_up = 1.f, up = -kBwdShift<T>;
+    if constexpr (kBwdShift<T> != 0.f) {
+      ds_up = ds_scale(do_norm * warp_top(v_top) + fabsf(delta1));
+      up += (float)((__float_as_int(ds_up) >> 23) - 127);
+    }
+    const float2 lse2 = f2s(up - lse1), delta = f2s(-delta1);
     auto blocks = [&](auto few) {  // two loops: as in the forward
       constexpr bool FINE = decltype(few)::value;
       for (int it = group; ok && it < total; it += 2, ph ^= 1u) {

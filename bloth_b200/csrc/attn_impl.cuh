@@ -56,9 +56,9 @@ struct AttnArgs {
 // that sees them for dk and dv, the call's few rows over a cache. The tensors'
 // extents do not count.
 // It costs a product for each of P and dS: 4 x 8192 rows of 32/8 heads of 128 (bf16),
-// forward and backward, 1447 us with a window of 128, 1302 us with one of 129; 8192
-// rows as 128 sequences 617 us, with one term 582; 64 x 129 rows, of which the first
-// 128 have two terms in o and dq, 489 us, with one term 463.
+// forward and backward, 1405 us with a window of 128, 1272 us with one of 129; 8192
+// rows as 128 sequences 606 us, with one term 575; 64 x 129 rows, of which the first
+// 128 have two terms in o and dq, 480 us, with one term 459.
 constexpr int kFineKeys = 128;
 
 // Powers of two that probabilities are held times where they enter a product, so
