@@ -15,8 +15,9 @@ its q/k normalisation and rotary embedding through the sm_100a kernels:
 
 With ``fuse_attention=True`` the attention itself is ``fused_attention`` too,
 where HF passes no mask tensor (unpadded batches under ``sdpa`` or
-``flash_attention_2`` kwargs, whose ``cu_seq_lens_q`` / ``_k`` are passed on)
-and no dropout; other calls keep HF's attention, and so do flattened batches
+``flash_attention_*``; the ``cu_seq_lens_q`` / ``_k`` of one flattened row are
+passed on) and no dropout. Other calls keep HF's attention: other
+implementations, paged caches, offsets over several rows, and flattened rows
 whose documents HF's flash attention finds from ``position_ids`` alone.
 
 The rest of the forward is HuggingFace's own code path, restated for the

@@ -15,13 +15,15 @@
 // instructions, one after the other. At 8192 full rows of 32/8 heads of 128
 // (bf16): blocks of 128 keys in one buffer, P over S, and one issuing thread
 // 1050 us; blocks of 64 in two buffers of S, P over S, and two issuing warps
-// that run converged on uniform addresses 850 us; S freed when it has been read
-// 831 us (1323 TFLOP/s, 80% of cuBLAS's burst rate of 1660).
+// that run converged on uniform addresses 850 us; one buffer of S, freed when it
+// has been read, and two of P 831 us (1323 TFLOP/s, 80% of cuBLAS's burst rate of
+// 1660). These are from idle, at 1965 MHz; in seconds of calls the 1 kW cap leaves
+// 1570 MHz, and 950 us.
 //
 // The running maximum moves only when a block's maximum exceeds it by more
 // than 2^8 (then the group rescales O_t in tensor memory, after its last
 // product). Until then p is at most 2^8, which costs no precision: p is
-// rounded relative to its own size (fp16: times kFwdShift), and sums are fp32.
+// rounded relative to its own size (fp16: times 2^7, kFwdShift), and sums are fp32.
 //
 // Tiles whose rows see few keys (kFineKeys) have P as two terms, which take both
 // buffers: P of a block then waits for the product of the block before.
@@ -33,10 +35,11 @@
 //
 // Bound at head_dim 128: the products. A block's for one tile take 392 cycles
 // with K (a step reads 6 KB of shared memory for 32 cycles of arithmetic) and
-// 263 with V, 1310 for both tiles; a block takes 1760. At head_dim 64 the
-// groups: 1480 cycles a block, of them 730 for the exponentials (512 alone, at
-// 16 a cycle and SM), 320 for maximum and mask, 130 for the wait for S and 130
-// to store P. A quarter of the exponentials as polynomials on the FMA units
+// 263 with V, 1310 for both tiles; a block takes 1510 (at 1570 to 1690 MHz). At
+// head_dim 64 the groups: 1460 to 1480 cycles a block (1920 to 1965 MHz), of them
+// 730 for the exponentials (512 alone, at 16 a cycle and SM), 320 for maximum and
+// mask, 130 for the wait for S and 130 to store P. A CTA takes 19,000 and 12,000
+// beside its blocks. A quarter of the exponentials as polynomials on the FMA units
 // made it slower (700 to 860 us at 8192 full rows), as did leaving the maximum
 // out until a block's sum shows that it is needed.
 #pragma once
@@ -62,8 +65,8 @@ struct FwdCfg {
   // barriers, the tensor-memory address and the stop flag
   static constexpr int SMEM = BAR_OFF + BARS * 8 + 16;
   static_assert(SMEM <= 227 * 1024, "shared memory");
-  // tensor-memory columns: the tiles' S (two buffers of 64 each), their O, and
-  // where there is room their Q
+  // tensor-memory columns: for each tile 64 of S and two buffers of 32 of P, its O,
+  // and where there is room its Q
   static constexpr bool Q_TMEM = D != 128;
   static constexpr uint32_t COLS = 512;
   static constexpr uint32_t S_COL = 0, O_COL = TILES * 128, Q_COL = 384;

@@ -184,9 +184,18 @@ def fused_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: b
     ``cu_seqlens_k`` where the keys have their own. Lengths and offsets are
     read on the device and clamped to the tensors. Rows outside of every
     sequence and rows that see no key get zeros, and no gradient; their inputs
-    are never used, whatever they hold. A key that some rows of its sequence
-    see has to be finite for all of them (a probability of 0 times an infinity
-    is not a number).
+    are never used, whatever they hold, nor are keys that no row sees. A key
+    that some rows of its sequence see has to be finite for all of them (a
+    probability of 0 times an infinity is not a number).
+
+    Scores, statistics and sums are fp32. With 16-bit tensors the probabilities
+    and their gradient are rounded to the tensors' type where they enter a
+    product (as two terms where rows see at most 128 keys), which puts results
+    of many keys about 1.4 times as far off as rounding the result alone; fp32
+    tensors have none of it. For the backward of 16-bit tensors the forward
+    keeps, beside q, k, v, out and lse, what rounding took off out: a second
+    tensor of out's size until the backward. First derivatives in reverse mode
+    only; others are refused.
 
     Returns out, shaped as q; with ``return_lse`` also the fp32 logarithms of
     the rows' sums of exponentials [B, Hq, Sq] ([Hq, S] for 3-D tensors), -inf

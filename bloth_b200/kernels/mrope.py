@@ -104,8 +104,8 @@ def _check_pair(q4, k4):
 
 
 def _needs_grad(inv_freq, *tensors) -> bool:
-    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or \
-        _lib.has_tangent(inv_freq, *tensors)
+    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    return grad or _lib.has_tangent(inv_freq, *tensors)
 
 
 def _weight(w, D: int, dtype, device):

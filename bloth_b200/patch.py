@@ -97,8 +97,9 @@ def patch_model(model: nn.Module, patch_norms: bool = True, patch_attention: boo
         post_attention_layernorm (fused_add_rms_norm). Not in the reference.
     fuse_attention: as patch_attention, with the attention itself on
         fused_attention wherever HuggingFace passes it no mask tensor
-        (unpadded batches with attn_implementation="sdpa"). Not in the
-        reference.
+        (unpadded batches with attn_implementation="sdpa" or
+        "flash_attention_*"); also for layers that patch_attention bound
+        before. Not in the reference.
     """
     if verbose:
         print(f"\n[Bloth] Patching: {type(model).__name__}")

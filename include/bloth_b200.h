@@ -17,7 +17,8 @@
  * normalised vector of N elements; x[row, col] is at x + row*ldx + col.
  * Head convention (per-head q/k kernels): element [b, s, h, d] of a
  * [B, S, H, D] head tensor is at ptr + b*strides[0] + s*strides[1] +
- * h*strides[2] + d, i.e. the head dimension is contiguous.
+ * h*strides[2] + d, i.e. the head dimension is contiguous. The stride of a
+ * dimension of one element is not looked at.
  *
  * Weight offset: every normalising entry point takes w_offset, a constant
  * added in fp32 to each weight element before it multiplies the normalised
@@ -319,11 +320,16 @@ int bloth_mrope(const void* q, const int64_t* q_strides, void* q_out, const int6
  * causal, j <= i + klen - qlen (the last query sees the last key) and, with
  * window > 0 (causal only), also j > i + klen - qlen - window. A row that sees
  * nothing, and every row outside of the sequences, has out = 0, lse = -inf and
- * zero gradients; what memory holds outside of the sequences is never used.
+ * zero gradients. Queries that see nothing, keys that no query sees, and what
+ * memory holds outside of the sequences are never used.
  *
  * Scores, row statistics, probabilities and all sums are fp32; with 16-bit
  * tensors probabilities and ds are rounded to the tensors' type where they
- * enter a matrix product. Results do not depend on scheduling.
+ * enter a matrix product: as two terms, to twice its precision, where every row
+ * of a tile sees at most 128 keys (128 query rows of a sequence for out and dq,
+ * 128 keys with all the queries that see them for dk and dv), else as one. With
+ * fp16 they are held times powers of two that keep them in its range. Results do
+ * not depend on scheduling.
  * No counterpart in the reference, whose path ends at RoPE.
  * ---------------------------------------------------------------------- */
 size_t bloth_attention_fwd_workspace_bytes(int64_t B, int64_t Sq, int64_t Sk, int64_t Hq,
@@ -335,10 +341,10 @@ size_t bloth_attention_fwd_workspace_bytes(int64_t B, int64_t Sq, int64_t Sk, in
 int bloth_attention_fwd(const void* q, const int64_t* q_strides, const void* k,
                         const int64_t* k_strides, const void* v, const int64_t* v_strides,
                         void* out, const int64_t* out_strides, void* out_rest, float* lse,
-                        const void* q_seq, const void* k_seq, int seq_dtype, int64_t packed, int64_t B, int64_t Sq,
-                        int64_t Sk, int64_t Hq, int64_t Hk, int64_t D, float scale, int causal,
-                        int64_t window, int dtype, void* workspace, size_t workspace_bytes,
-                        void* stream);
+                        const void* q_seq, const void* k_seq, int seq_dtype, int64_t packed,
+                        int64_t B, int64_t Sq, int64_t Sk, int64_t Hq, int64_t Hk, int64_t D,
+                        float scale, int causal, int64_t window, int dtype, void* workspace,
+                        size_t workspace_bytes, void* stream);
 size_t bloth_attention_bwd_workspace_bytes(int64_t B, int64_t Sq, int64_t Sk, int64_t Hq,
                                            int64_t Hk, int64_t D, int64_t packed, int dtype);
 /* out, out_rest and lse are the forward's; with out_rest NULL the row sums
