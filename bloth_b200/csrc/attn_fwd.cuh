@@ -399,7 +399,7 @@ __global__ void __launch_bounds__(352, 1)
           load64(o_at + c, x);
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
-            split2<T>(x[2 * i] * inv, x[2 * i + 1] * inv, w[i], v[i]);
+            split2<T, kRestUp<T>>(x[2 * i] * inv, x[2 * i + 1] * inv, w[i], v[i]);
             if (inv == 0.f) w[i] = v[i] = 0u;
           }
         }

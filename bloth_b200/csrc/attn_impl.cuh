@@ -26,7 +26,8 @@ namespace bloth {
 
 struct AttnArgs {
   HT q, k, v, o, dout, dq, dk, dv;
-  void* rest;         // what rounding took off o, laid out as o (16-bit tensors), or NULL
+  void* rest;         // what rounding took off o, times kRestUp, laid out as o (16-bit
+                      // tensors), or NULL
   float* lse;         // [B, Hq, Sq] natural logarithm (forward writes, backward reads)
   float* lse2;        // backward workspace: [Hq, R] lse * log2(e) - kBwdShift, +inf where
                       // nothing is seen
@@ -81,6 +82,11 @@ __device__ __forceinline__ float ds_scale(float bound) {
 __device__ __forceinline__ float warp_top(float x) {
   return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(x)));
 }
+
+// What rounding takes off o is 2^-11 of it in fp16, or less: as it is it would leave
+// fp16's range where o is small.
+template <typename T>
+constexpr int kRestUp = std::is_same<T, __half>::value ? 2048 : 1;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;

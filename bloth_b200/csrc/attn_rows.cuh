@@ -95,7 +95,7 @@ __device__ __forceinline__ void rows_out(const AttnArgs& a, int b, int h, int r,
     *reinterpret_cast<float2*>(out) = f2(y0, y1);
   } else {
     uint32_t hi, lo;
-    split2<T>(y0, y1, hi, lo);
+    split2<T, kRestUp<T>>(y0, y1, hi, lo);
     *reinterpret_cast<uint32_t*>(out) = hi;
     if (a.rest != nullptr) *reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(a.rest) + at) = lo;
   }

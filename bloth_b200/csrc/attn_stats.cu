@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(256) attn_stats_kernel(const AttnArgs a, int q
           float e[VEC];
           unpack(ldg_pack<T, VEC>(rp + row * a.o.ss + x), e);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) f[i] += e[i];
+          for (int i = 0; i < VEC; ++i) f[i] = fmaf(e[i], 1.f / kRestUp<T>, f[i]);
         }
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {

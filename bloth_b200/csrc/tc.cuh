@@ -39,16 +39,17 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return r;
 }
 
-// Two floats y rounded to T, and what that took off them rounded to T.
-template <typename T>
+// Two floats y rounded to T, and what that took off them, times UP, rounded to T.
+template <typename T, int UP = 1>
 __device__ __forceinline__ void split2(float y0, float y1, uint32_t& hi, uint32_t& lo) {
   hi = pack2<T>(y0, y1);
   if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-    lo = pack2<T>(y0 - __uint_as_float(hi << 16), y1 - __uint_as_float(hi & 0xffff0000u));
+    lo = pack2<T>((y0 - __uint_as_float(hi << 16)) * UP,
+                  (y1 - __uint_as_float(hi & 0xffff0000u)) * UP);
   } else {
     __half2 h;
     memcpy(&h, &hi, 4);
-    lo = pack2<T>(y0 - __half2float(h.x), y1 - __half2float(h.y));
+    lo = pack2<T>((y0 - __half2float(h.x)) * UP, (y1 - __half2float(h.y)) * UP);
   }
 }
 

@@ -335,9 +335,9 @@ int bloth_mrope(const void* q, const int64_t* q_strides, void* q_out, const int6
 size_t bloth_attention_fwd_workspace_bytes(int64_t B, int64_t Sq, int64_t Sk, int64_t Hq,
                                            int64_t Hk, int64_t D, int64_t packed, int dtype);
 /* lse may be NULL when no backward follows. out_rest, for the backward of
-   16-bit tensors: what rounding took off out, with out's type and strides, or
-   NULL. The workspace may be NULL when the
-   function above reports 0 bytes; its base is aligned to 16 bytes. */
+   16-bit tensors: what rounding took off out (fp16: times 2048), with out's type
+   and strides, or NULL. The workspace may be NULL when the function above
+   reports 0 bytes; its base is aligned to 16 bytes. */
 int bloth_attention_fwd(const void* q, const int64_t* q_strides, const void* k,
                         const int64_t* k_strides, const void* v, const int64_t* v_strides,
                         void* out, const int64_t* out_strides, void* out_rest, float* lse,

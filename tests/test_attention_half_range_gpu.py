@@ -108,3 +108,10 @@ def test_dq_of_rows_of_different_sizes(cuda, D):
     # a row's ds have a range of their own in dq
     rows = 2.0 ** torch.randint(-10, 20, (400,), device=cuda).float()
     _run(cuda, D, 1, 400, 400, (1e-4, 300.0, 0.01, 1e-3), rows=rows, names=("dq",))
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("Sq,Sk,few", [(5, 5, True), (300, 300, False), (4, 700, False)])
+def test_delta_of_small_outputs(cuda, D, Sq, Sk, few):
+    # o below fp16's normal range: what its rounding takes off is at most 2^-25
+    _run(cuda, D, 1, Sq, Sk, (1.0, 1.0, 2e-6, 3000.0), few=few, names=("dq", "dk"))
